@@ -8,6 +8,8 @@ from __future__ import annotations
 import ctypes
 import os
 
+import torch
+
 from .build import LIB_PATH
 
 ABI_VERSION = 2
@@ -17,6 +19,7 @@ FA_OK = 0
 FA_DTYPE_BF16 = 0
 FA_DTYPE_FP8_E4M3 = 1
 FA_DTYPE_F16 = 2
+FA_DTYPE_F32 = 3
 FA_KSTATUS_SPIN_TIMEOUT = 1
 FA_KSTATUS_XCD_MAP = 2
 FA_KSTATUS_RANGE = 4
@@ -78,6 +81,16 @@ class PrefillArgs(ctypes.Structure):
     ]
 
 
+class W4Args(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int), ("out_dtype", ctypes.c_int),
+        ("x", ctypes.c_void_p), ("x_stride", ctypes.c_longlong), ("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+        ("rows", ctypes.c_int), ("n", ctypes.c_int), ("k", ctypes.c_int), ("group", ctypes.c_int),
+        ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("gate", ctypes.c_int), ("out", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class DeviceInfo(ctypes.Structure):
     _fields_ = [("cus", ctypes.c_int), ("xcds", ctypes.c_int), ("lds_bytes", ctypes.c_int),
                 ("coop_launch", ctypes.c_int), ("coop_max_blocks", ctypes.c_int), ("arch", ctypes.c_char * 64)]
@@ -100,6 +113,8 @@ SYMBOLS = [
     ("fa_ma2_max_batch", ctypes.c_int, []),
     ("fa_pi05_prefill", ctypes.c_int, [ctypes.POINTER(PrefillArgs), ctypes.c_void_p]),
     ("fa_pi05_prefill_workspace_bytes", ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    ("fa_w4_linear", ctypes.c_int, [ctypes.POINTER(W4Args), ctypes.c_void_p]),
+    ("fa_w4_workspace_bytes", ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     ("fa_device_query", ctypes.c_int, [ctypes.c_int, ctypes.POINTER(DeviceInfo)]),
     ("fa_last_error", ctypes.c_char_p, []),
     ("fa_abi_version", ctypes.c_int, []),
@@ -130,3 +145,14 @@ def check(rc: int, what: str) -> None:
     if rc != FA_OK:
         msg = lib().fa_last_error()
         raise FlashActError(f"{what} failed (status {rc}): {msg.decode() if msg else ''}")
+
+
+def run_on(index: int, fn, args, what: str) -> None:
+    """Enqueues the C entry point `fn` on the current stream of GPU `index`, which need not be the current device."""
+    if index == torch.cuda.current_device():
+        rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+    if rc != FA_OK:
+        check(rc, what)

@@ -1,6 +1,10 @@
 // Library-wide C-ABI entry points: error text, ABI version, device query, launch checks.
-#include <mutex>
 #include <string.h>
+
+#include <atomic>
+#include <mutex>
+#include <set>
+#include <utility>
 
 #include "../../include/flashact_mi355x.h"
 #include "fa_host.h"
@@ -28,6 +32,8 @@ struct KernelAttr {
 };
 KernelAttr g_attr[64];
 int g_nattr = 0;
+std::atomic<int> g_gfx950[64];                    // 0 unknown, 1 yes
+std::set<std::pair<const void*, int>> g_lds_set;  // (kernel, device) whose dynamic-LDS limit is raised
 }  // namespace
 
 int check_device(const void* kernel, int threads, unsigned lds_bytes, int nwg, const char* who) {
@@ -64,6 +70,39 @@ int check_device(const void* kernel, int threads, unsigned lds_bytes, int nwg, c
       return fail(FA_ERR_DEVICE, "%s: only %d x %d workgroups can be co-resident, need %d", who, per_cu,
                   d.prop.multiProcessorCount, nwg);
     if (g_nattr < 64) g_attr[g_nattr++] = KernelAttr{kernel, dev, lds_bytes};
+  }
+  return FA_OK;
+}
+
+int check_gfx950(const char* who) {
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return fail(FA_ERR_DEVICE, "%s: hipGetDevice failed: %s", who, hipGetErrorString(e));
+  if (dev < 0 || dev >= 64) return fail(FA_ERR_DEVICE, "%s: device ordinal %d out of range", who, dev);
+  if (g_gfx950[dev].load(std::memory_order_relaxed)) return FA_OK;
+  hipDeviceProp_t prop;
+  e = hipGetDeviceProperties(&prop, dev);
+  if (e != hipSuccess) return fail(FA_ERR_DEVICE, "%s: hipGetDeviceProperties: %s", who, hipGetErrorString(e));
+  if (strncmp(prop.gcnArchName, "gfx950", 6) != 0)
+    return fail(FA_ERR_DEVICE, "%s: device %d is %s; this library is built for gfx950 (MI355X)", who, dev,
+                prop.gcnArchName);
+  g_gfx950[dev].store(1, std::memory_order_relaxed);
+  return FA_OK;
+}
+
+int allow_lds(const void* kernel, unsigned lds_bytes, const char* who) {
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return fail(FA_ERR_DEVICE, "%s: hipGetDevice failed: %s", who, hipGetErrorString(e));
+  try {
+    std::lock_guard<std::mutex> lk(g_mu);
+    if (g_lds_set.count({kernel, dev})) return FA_OK;
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes);
+    if (e != hipSuccess)
+      return fail(FA_ERR_DEVICE, "%s: hipFuncSetAttribute(LDS=%u): %s", who, lds_bytes, hipGetErrorString(e));
+    g_lds_set.insert({kernel, dev});
+  } catch (...) {
+    return fail(FA_ERR_DEVICE, "%s: out of host memory", who);
   }
   return FA_OK;
 }

@@ -32,6 +32,11 @@ int coop_launch(const void* kernel, int nwg, int threads, void** args, unsigned 
 // workgroups of `threads` threads can be co-resident.
 int check_device(const void* kernel, int threads, unsigned lds_bytes, int nwg, const char* who);
 
+// For kernels launched without the cooperative machinery: the current device is a gfx950 (asked once per device).
+int check_gfx950(const char* who);
+// Raises a kernel's dynamic-LDS limit to `lds_bytes` (once per device and kernel).
+int allow_lds(const void* kernel, unsigned lds_bytes, const char* who);
+
 }  // namespace host
 
 // Batched pi0.5 launch (batch >= 2), dispatched from fa_pi05_denoise after the shared checks.

@@ -19,6 +19,7 @@
  *                            (src/pi05/binding.cpp:34-36, src/molmoact2/binding.cpp:33-34)
  *   fa_last_error ......... TORCH_CHECK on the launch status (src/pi05/binding.cpp:67)
  *   fa_device_query ....... the occupancy clamp / diagnostics of src/molmoact2/binding.cpp:65-79
+ *   fa_w4_linear .......... no counterpart (the backbone's token by token decoding)
  *   fa_abi_version ........ no counterpart (ABI guard for the Python and C++ callers)
  */
 #ifndef FLASHACT_MI355X_H
@@ -49,7 +50,7 @@ enum fa_status {
   FA_ERR_LAUNCH = 4        /* the HIP launch itself failed */
 };
 
-enum fa_dtype { FA_DTYPE_BF16 = 0, FA_DTYPE_FP8_E4M3 = 1, FA_DTYPE_F16 = 2 };
+enum fa_dtype { FA_DTYPE_BF16 = 0, FA_DTYPE_FP8_E4M3 = 1, FA_DTYPE_F16 = 2, FA_DTYPE_F32 = 3 };
 
 /* Kernel-side status bits (read back from the workspace by fa_*_read_status). */
 #define FA_KSTATUS_SPIN_TIMEOUT 1u /* a grid/XCD barrier wait hit its cap: results invalid */
@@ -277,6 +278,42 @@ typedef struct fa_prefill_args {
 /* All layers of the prefix prefill as ONE cooperative launch (256 workgroups). */
 int fa_pi05_prefill(const fa_prefill_args* args, fa_stream_t stream);
 size_t fa_pi05_prefill_workspace_bytes(int batch, int Lp, int Lmax);
+
+/* ---------------------------------------------------------------- 4-bit weights, few rows
+ * out[m][n] = sum_k x[m][k] e2m1(code[n][k]) scale[n][k / group] (+ bias[n]), m < rows <= FA_W4_MAX_ROWS.
+ * Codes are OCP e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), with one bf16 scale for each group of
+ * 32, 64 or 128 columns. Laid out in tiles of 16 rows x 128 columns, both padded with zeros:
+ *   codes  [ceil(n / 16)][ceil(k / 128)][4 q][16 r][16 bytes]: byte j holds columns 32 (j / 4) + 8 q + 2 (j % 4)
+ *          (lower nibble) and the next one of row r of the tile;
+ *   scales [ceil(n / 16)][ceil(k / 128) * 128 / group][16 rows] bf16.
+ * x is bf16 or fp16, [rows][k] with a row stride of x_stride elements (a multiple of 8; k % 8 == 0); out is
+ * contiguous, bf16, fp16 or fp32. Sums are fp32: within a group the unscaled products are added first.
+ * gate != 0: rows 2f, 2f + 1 of the weights are a gate and its input, out[m][f] = gelu_tanh(y[2f]) y[2f + 1]
+ * of width n / 2. residual (fp32, shaped like out, may be out itself) is added last.
+ * workspace: fa_w4_workspace_bytes(rows, n, k) bytes, 16-byte aligned, for the sums of a k that is split across
+ * workgroups (often 0: then NULL). It needs no initialisation and holds nothing between calls.
+ */
+#define FA_W4_MAX_ROWS 64
+typedef struct fa_w4_args {
+  int dtype;     /* of x: FA_DTYPE_BF16 or FA_DTYPE_F16 */
+  int out_dtype; /* FA_DTYPE_BF16, FA_DTYPE_F16 or FA_DTYPE_F32 */
+  const void* x;
+  long long x_stride;
+  const void* codes;
+  const void* scales;
+  int rows;
+  int n;
+  int k;
+  int group;
+  const float* bias;     /* [n] or NULL */
+  const float* residual; /* [rows][n or n / 2] or NULL */
+  int gate;
+  void* out;
+  void* workspace;
+  size_t workspace_bytes;
+} fa_w4_args;
+int fa_w4_linear(const fa_w4_args* args, fa_stream_t stream);
+size_t fa_w4_workspace_bytes(int rows, int n, int k);
 
 /* ---------------------------------------------------------------- common */
 int fa_device_query(int device, fa_device_info* info);

@@ -1,0 +1,153 @@
+"""``w4.linear`` on the MI355X against the product of the dequantised weights in 64 bits.
+
+Tolerance, element by element. The products x * code are exact in fp32; summing K of them with the groups' scales
+rounds each step by at most 2^-24 of the running magnitude, so |error| <= (K + K / 32 + 20) 2^-24 sum_k |x W| =: d,
+bias and residual among the 20. The result's own rounding adds eps / 2 |y| of its type. Gated: with g and u off by
+dg, du and |gelu'| <= 1.13, the error is at most 1.13 dg |u| + |gelu(g)| du + 2^-17 |gelu(g) u|: the device's gelu takes
+2^t with t = g (c1 + c3 g^2), three roundings of t (3 2^-24 |t|) and two approximate instructions; where the result
+is not lost (|t| < 60) that is below 2^-17 relative.
+"""
+import math
+
+import pytest
+import torch
+
+from flashact_amd import w4
+
+pytestmark = pytest.mark.gpu
+
+GELU_C = math.sqrt(2 / math.pi)
+
+
+def _gelu(g):
+    return 0.5 * g * (1 + torch.tanh(GELU_C * (g + 0.044715 * g ** 3)))
+
+
+def _reference(x, w, bias=None, residual=None, gate=None):
+    """(result, bound of the fp32 error) in fp64."""
+    wd, xd = w4.dequantize(w).double().t().contiguous(), x.double()
+    y, k = xd @ wd, w["k"]
+    d = (k + k / 32 + 20) * 2.0 ** -24 * (xd.abs() @ wd.abs())
+    if bias is not None:
+        y, d = y + bias.double(), d + 2.0 ** -24 * bias.double().abs()
+    if gate:
+        g, u, dg, du = y[..., 0::2], y[..., 1::2], d[..., 0::2], d[..., 1::2]
+        y = _gelu(g) * u
+        d = 1.13 * dg * u.abs() + _gelu(g).abs() * du + 1.13 * dg * du + 2.0 ** -17 * y.abs()
+    if residual is not None:
+        y = y + residual.double()
+        d = d + 2.0 ** -23 * (y.abs() + residual.double().abs())
+    return y, d
+
+
+def _check(out, ref, bound):
+    half = torch.finfo(out.dtype).eps / 2 * (ref.abs() + bound) + torch.finfo(out.dtype).tiny
+    err = (out.double() - ref).abs()
+    assert bool((err <= bound + half).all()), float((err - bound - half).max())
+
+
+SHAPES = [(16, 128), (2, 8), (34, 136), (1022, 1000), (2560, 2048), (64, 4104), (4096, 264), (17000, 64)]
+
+
+@pytest.mark.parametrize("rows", [1, 2, 4, 5, 16, 17, 32, 33, 64])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_products(gpu, rows, dtype):
+    gen = torch.Generator(device=gpu).manual_seed(rows)
+    for i, (n, k) in enumerate(SHAPES):
+        w = w4.quantize(torch.randn(n, k, generator=gen, device=gpu) * 0.02, w4.GROUPS[(i + rows) % 3])
+        x = torch.randn(rows, k, generator=gen, device=gpu).to(dtype)
+        bias = torch.randn(n, generator=gen, device=gpu)
+        res, half = torch.randn(rows, n, generator=gen, device=gpu), torch.randn(rows, n // 2, generator=gen, device=gpu)
+        for kw in (dict(), dict(bias=bias), dict(residual=res), dict(gate="gelu"), dict(bias=bias, gate="gelu", residual=half)):
+            ref, bound = _reference(x, w, **kw)
+            for t in (None, torch.float32):
+                out = w4.linear(x, w, out_dtype=t, **kw)
+                assert out.dtype == (t or (torch.float32 if "residual" in kw else dtype)) and out.shape == ref.shape
+                _check(out, ref, bound)
+
+
+@pytest.mark.parametrize("group", w4.GROUPS)
+def test_odd_rows_of_weights(gpu, group):
+    """An odd number of weight rows, and one."""
+    for n, k, rows in ((1, 128, 3), (33, 136, 1), (1023, 520, 7), (15, 2048, 20)):
+        w = w4.quantize(torch.randn(n, k, device=gpu), group)
+        x = torch.randn(rows, k, device=gpu).bfloat16()
+        _check(w4.linear(x, w), *_reference(x, w))
+
+
+def test_long_sums_split_across_workgroups(gpu):
+    """K long enough to be split, with and without an epilogue; twice the same bits."""
+    for rows, n, k in ((16, 2048, 16384), (1, 48, 16384), (64, 40, 8200), (3, 100, 30000)):
+        w = w4.quantize(torch.randn(n, k, device=gpu) * 0.02, 32)
+        x, res = torch.randn(rows, k, device=gpu).bfloat16(), torch.randn(rows, n, device=gpu)
+        out = w4.linear(x, w, residual=res)
+        _check(out, *_reference(x, w, residual=res))
+        assert torch.equal(out, w4.linear(x, w, residual=res))
+
+
+def test_views_in_place_and_single_rows(gpu):
+    w = w4.quantize(torch.randn(96, 256, device=gpu), 64)
+    wide = torch.randn(5, 1024, device=gpu).bfloat16()
+    x = wide[:, 512:768]  # rows with a stride
+    assert torch.equal(w4.linear(x, w), w4.linear(x.contiguous(), w))
+    assert torch.equal(w4.linear(x[2], w), w4.linear(x, w)[2])  # two chunks: one order of sums
+    res = torch.randn(5, 96, device=gpu)
+    ref = w4.linear(x, w, residual=res)
+    assert w4.linear(x, w, residual=res, out=res) is res and torch.equal(res, ref)
+    assert w4.linear(x[:0], w).shape == (0, 96)
+    out = torch.full((6, 96), 7.0, device=gpu)
+    w4.linear(x, w, out=out[:5])
+    assert torch.equal(out[:5], w4.linear(x, w, out_dtype=torch.float32)) and (out[5] == 7).all()
+
+
+def test_values_that_are_not_numbers_stay_in_their_row(gpu):
+    w = w4.quantize(torch.randn(48, 256, device=gpu), 32)
+    x = torch.randn(4, 256, device=gpu).bfloat16()
+    ref = w4.linear(x, w)
+    x[1, 5], x[2, 7] = float("nan"), float("inf")
+    out = w4.linear(x, w)
+    assert out[1].isnan().all() and not out[2].isfinite().any()
+    assert torch.equal(out[0], ref[0]) and torch.equal(out[3], ref[3])
+
+
+def test_streams_and_graphs(gpu):
+    """On a stream of its own, and captured: every replay equals the eager result on the inputs of that time."""
+    w = w4.quantize(torch.randn(64, 16384, device=gpu) * 0.02, 32)  # a split sum: two kernels and a workspace
+    x = torch.randn(8, 16384, device=gpu).bfloat16()
+    ref = w4.linear(x, w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = w4.linear(x, w)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, ref)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = w4.linear(x, w)
+    for i in range(4):
+        x.copy_(torch.randn(8, 16384, device=gpu))
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, w4.linear(x, w))
+
+
+def test_refuses_on_the_gpu(gpu):
+    w = w4.quantize(torch.randn(32, 64, device=gpu))
+    x = torch.randn(2, 72, device=gpu).bfloat16()
+    y = x[:, :64].contiguous()
+    for kw, err, text in (
+            (dict(x=torch.randn(130, device=gpu).bfloat16()[1:65]), ValueError, "aligned"),
+            (dict(x=torch.randn(64, 2, device=gpu).bfloat16().t()), ValueError, "contiguous"),
+            (dict(x=y[:1].expand(2, 64)), ValueError, "overlap"),
+            (dict(bias=torch.randn(32, device=gpu).half()), TypeError, "float32"),
+            (dict(bias=torch.randn(31, device=gpu)), ValueError, "bias"),
+            (dict(bias=torch.randn(32)), ValueError, "bias"),
+            (dict(residual=torch.randn(2, 16, device=gpu)), ValueError, "residual"),
+            (dict(out=torch.empty(2, 31, device=gpu)), ValueError, "out must be"),
+            (dict(out=torch.empty(2, 32, device=gpu, dtype=torch.int32)), TypeError, "out must be"),
+            (dict(out=torch.empty(2, 32, device=gpu), out_dtype=torch.float16), TypeError, "agree"),
+            (dict(out_dtype=torch.float64), TypeError, "out_dtype"),
+            (dict(w={k: v.cpu() if torch.is_tensor(v) else v for k, v in w.items()}), ValueError, "same GPU"),
+    ):
+        with pytest.raises(err, match=text):
+            w4.linear(**{"x": y, "w": w, **kw})
