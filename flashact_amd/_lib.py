@@ -91,6 +91,29 @@ class W4Args(ctypes.Structure):
     ]
 
 
+class Kv8RowsArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int),
+        ("k", ctypes.c_void_p), ("k_stride", ctypes.c_longlong * 4), ("v", ctypes.c_void_p), ("v_stride", ctypes.c_longlong * 4),
+        ("cache_k", ctypes.c_void_p), ("cache_v", ctypes.c_void_p), ("cache_ks", ctypes.c_void_p), ("cache_vs", ctypes.c_void_p),
+        ("start", ctypes.c_void_p), ("count", ctypes.c_void_p),
+        ("batch", ctypes.c_int), ("tokens", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+        ("blocks", ctypes.c_int), ("zero_rest", ctypes.c_int),
+    ]
+
+
+class Kv8AttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int), ("q", ctypes.c_void_p), ("q_stride", ctypes.c_longlong * 3),
+        ("cache_k", ctypes.c_void_p), ("cache_v", ctypes.c_void_p), ("cache_ks", ctypes.c_void_p), ("cache_vs", ctypes.c_void_p),
+        ("lens", ctypes.c_void_p), ("count", ctypes.c_void_p), ("slopes", ctypes.c_void_p),
+        ("batch", ctypes.c_int), ("tokens", ctypes.c_int), ("heads", ctypes.c_int), ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int), ("blocks", ctypes.c_int), ("causal", ctypes.c_int),
+        ("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("out", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class DeviceInfo(ctypes.Structure):
     _fields_ = [("cus", ctypes.c_int), ("xcds", ctypes.c_int), ("lds_bytes", ctypes.c_int),
                 ("coop_launch", ctypes.c_int), ("coop_max_blocks", ctypes.c_int), ("arch", ctypes.c_char * 64)]
@@ -115,10 +138,17 @@ SYMBOLS = [
     ("fa_pi05_prefill_workspace_bytes", ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     ("fa_w4_linear", ctypes.c_int, [ctypes.POINTER(W4Args), ctypes.c_void_p]),
     ("fa_w4_workspace_bytes", ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    ("fa_kv8_store", ctypes.c_int, [ctypes.POINTER(Kv8RowsArgs), ctypes.c_void_p]),
+    ("fa_kv8_load", ctypes.c_int, [ctypes.POINTER(Kv8RowsArgs), ctypes.c_void_p]),
+    ("fa_kv8_attention", ctypes.c_int, [ctypes.POINTER(Kv8AttnArgs), ctypes.c_void_p]),
+    ("fa_kv8_attention_workspace_bytes", ctypes.c_size_t, [ctypes.c_int] * 6),
     ("fa_device_query", ctypes.c_int, [ctypes.c_int, ctypes.POINTER(DeviceInfo)]),
     ("fa_last_error", ctypes.c_char_p, []),
     ("fa_abi_version", ctypes.c_int, []),
 ]
+
+# FA_DTYPE_* of a tensor's type
+DTYPES = {torch.bfloat16: FA_DTYPE_BF16, torch.float16: FA_DTYPE_F16, torch.float32: FA_DTYPE_F32}
 
 _lib = None
 

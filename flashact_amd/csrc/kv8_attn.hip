@@ -1,0 +1,450 @@
+// Attention of each sample's newest tokens over the 8-bit cache (fa_kv8_attention); the cache's layout is in kv8.hip.
+//
+// Row (t, h) of sample b is the query of token t < n at position i = len - n + t. It sees keys j < i + 1 (causal)
+// or j < len:  s_j = q . k_j scale, capped to cap tanh(s_j / cap), less slope_h |i - j|;  o = sum_j softmax(s)_j v_j.
+//
+// What bounds it is reading the cache once: 2 hd bytes a key and K/V head. The rows that share a K/V head (G heads of
+// each token) are the 16 columns of the MFMAs, so a key is read and converted once for all of them. A wave takes
+// blocks of 32 keys on its own with a running maximum and sum: S^T = K Q^T (16x16x32, two tiles of 16 keys), softmax
+// down the columns, O^T += V^T P^T. The tiles' rows are dealt so that the softmax leaves P exactly where the next
+// product wants it: row m of key tile t is key 8 (m / 4) + 4 t + m % 4, so lane quarter q ends with keys 8 q .. 8 q + 7.
+// The keys' next block is fetched as soon as the products with this one are done, the values' likewise: one
+// of the two is always under way, without a second set of registers. Keys are split over the waves of a workgroup and,
+// where rows are few, over workgroups (the sums then go through the workspace to join_kernel).
+//
+// Codes are exact in bf16 and fp16. Q K^T runs in q's type; P is rounded to fp16 (2^-12, half the step of an fp16
+// result, a sixteenth of bf16's) for the product with the values' codes; scales, softmax and sums are fp32.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "../../include/flashact_mi355x.h"
+#include "fa_device.h"
+#include "fa_host.h"
+
+namespace fa {
+namespace kv8 {
+
+constexpr int BT = 32;
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct AttnArgs {
+  const unsigned char* q;
+  int64_t qb, qt, qh;  // strides in elements
+  const unsigned char *k, *v;
+  const float *ks, *vs;
+  const int *lens, *count;
+  const float* slopes;
+  unsigned char* out;
+  float* part;  // [sample][head][row tile][split] {O[16][hd], m[16], l[16]}
+  int B, T, H, G, nblk, RT, S, causal;
+  float scale, cap;
+};
+
+// The row tile's share of what its sample has cached.
+struct Span {
+  int len, n;
+};
+__device__ __forceinline__ Span span_of(const AttnArgs& a, int b) {
+  const int cap = (int)min((int64_t)a.nblk * BT, (int64_t)0x7fffffff - 31);
+  Span s;
+  s.len = max(0, min(a.lens[b], cap));
+  s.n = a.count ? max(0, min(a.count[b], a.T)) : a.T;
+  return s;
+}
+// Splits that a sample uses: at least MINB blocks a wave.
+constexpr int MINB = 1;
+__device__ __forceinline__ int splits_used(int nb, int waves, int S) {
+  return max(1, min(S, (nb + waves * MINB - 1) / (waves * MINB)));
+}
+
+template <bool F16>
+__device__ __forceinline__ u32x4 cvt8(unsigned lo, unsigned hi) {  // eight e4m3 codes -> eight bf16 / fp16, exact
+  if constexpr (F16) {
+    return u32x4{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true))};
+  } else {
+    return u32x4{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true))};
+  }
+}
+
+// 0xff in the bytes below n (n <= 0: none, n >= 4: all)
+__device__ __forceinline__ unsigned bytes_below(int n) { return n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u; }
+// bit 7 of each byte that is the NaN code of either sign
+__device__ __forceinline__ unsigned nan_bytes(unsigned c) { return ((c & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+template <bool F16>
+__device__ __forceinline__ void store_row4(unsigned char* out, size_t at, f32x4 v) {
+  if constexpr (F16)
+    *reinterpret_cast<u32x2*>(out + at * 2) = u32x2{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3])};
+  else
+    *reinterpret_cast<u32x2*>(out + at * 2) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+}
+
+// 1 / l of a row: no keys give zeros, NaN stays.
+__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
+
+template <bool F16, int HD, int W, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(64 * W) attn_kernel(AttnArgs a) {
+  constexpr int KS = (HD + 63) / 64, NJ = HD / 32;
+  constexpr int DC = HD < 128 ? HD : 128, PITCH = DC + 4;  // dims a round of the waves' sum in LDS
+  __shared__ float osum[W * 16 * PITCH];
+  __shared__ float wm[W * 16], wl[W * 16];
+
+  // row tiles of one (sample, head, split) share their keys: neighbours on one XCD
+  const int xcd = blockIdx.x & 7, y = blockIdx.x >> 3, rt = y % a.RT, u = (y / a.RT) * 8 + xcd;
+  if (u >= a.B * a.H * a.S) return;
+  const int split = u % a.S, bh = u / a.S, h = bh % a.H, b = bh / a.H;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const Span sp = span_of(a, b);
+
+  const int rr = rt * 16 + r, t = rr / a.G, head = h * a.G + rr % a.G, pos = sp.len - sp.n + t;
+  const bool valid = rr < a.T * a.G && t < sp.n && pos >= 0;
+  int limit = valid ? (a.causal ? pos + 1 : sp.len) : 0;
+  int hi = limit, lo = valid ? limit : 0x7fffffff;
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    hi = max(hi, __shfl_xor(hi, o));
+    lo = min(lo, __shfl_xor(lo, o));
+  }
+  hi = __builtin_amdgcn_readfirstlane(hi);  // keys that any row sees
+  lo = __builtin_amdgcn_readfirstlane(lo);  // keys that every row sees (rows that are not there do not count)
+  if (!valid) limit = hi;
+  const int nb = (hi + BT - 1) / BT;
+  const int used = splits_used(nb, W, a.S);
+  if (split >= used) return;
+  const int at = split * W + wave, all = used * W;
+  const int b0 = (int)((int64_t)nb * at / all), b1 = (int)((int64_t)nb * (at + 1) / all);
+
+  u32x4 qf[KS][2];
+#pragma unroll
+  for (int i = 0; i < KS; i++)
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      const int d = 64 * i + 16 * q + 8 * s;
+      qf[i][s] = u32x4{0, 0, 0, 0};
+      if (valid && d < HD)
+        qf[i][s] = *reinterpret_cast<const u32x4*>(a.q + (b * a.qb + t * a.qt + head * a.qh + d) * 2);
+    }
+  const float slope = BIAS && valid ? a.slopes[head] * LOG2E : 0.f;
+
+  const size_t unit = ((size_t)b * a.H + h) * a.nblk;
+  const unsigned char* kp = a.k + unit * (BT * HD) + (q * BT + 8 * (r >> 2) + (r & 3)) * 16;
+  const unsigned char* vp = a.v + unit * (BT * HD) + (2 * r + (q & 1)) * BT + (q >> 1) * 16;
+  u32x4 kc[2][KS], vc[NJ];
+  float ksc = 0.f, vsc = 0.f, ksn = 0.f, vsn = 0.f;
+  auto load_k = [&](int blk) {
+    const unsigned char* p = kp + (size_t)blk * (BT * HD);
+#pragma unroll
+    for (int i = 0; i < KS; i++)
+#pragma unroll
+      for (int s = 0; s < 2; s++) {
+        kc[s][i] = u32x4{0, 0, 0, 0};
+        if (HD % 64 == 0 || 64 * i + 16 * q < HD)
+          kc[s][i] = *reinterpret_cast<const u32x4*>(p + i * (4 * BT * 16) + s * 64);
+      }
+    ksn = a.ks[unit + blk];
+  };
+  auto load_v = [&](int blk) {
+    const unsigned char* p = vp + (size_t)blk * (BT * HD);
+#pragma unroll
+    for (int j = 0; j < NJ; j++) vc[j] = *reinterpret_cast<const u32x4*>(p + j * (32 * BT));
+    vsn = a.vs[unit + blk];
+  };
+
+  f32x4 O[NJ][2];
+#pragma unroll
+  for (int j = 0; j < NJ; j++) O[j][0] = O[j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;  // l: this lane's keys only
+  if (b0 < b1) {
+    load_k(b0);
+    load_v(b0);
+  }
+  for (int blk = b0; blk < b1; blk++) {
+    f32x4 s[2];
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      s[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KS; i++) {
+        const u32x4 c = kc[x][i], c0 = cvt8<F16>(c[0], c[1]), c1 = cvt8<F16>(c[2], c[3]);
+        s[x] = F16 ? mfma16h(c0, qf[i][0], s[x]) : mfma16(c0, qf[i][0], s[x]);
+        s[x] = F16 ? mfma16h(c1, qf[i][1], s[x]) : mfma16(c1, qf[i][1], s[x]);
+      }
+    }
+    ksc = ksn;
+    if (blk + 1 < b1) load_k(blk + 1);
+    // scores in base 2
+    const int key0 = blk * BT + 8 * q;
+    const float f = ksc * a.scale;
+    const bool mixed = blk * BT + BT > lo;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        float v = s[x][i] * f;
+        if constexpr (CAP) {
+          // cap tanh(v / cap) = cap - 2 cap / (1 + e^(2 v / cap)); scale and cap are passed so that v is 2 log2(e) q.k / cap
+          v = a.cap - 2.f * a.cap * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v));
+        }
+        if constexpr (BIAS) v -= slope * fabsf((float)(pos - (key0 + 4 * x + i)));
+        if (mixed && key0 + 4 * x + i >= limit) v = -INFINITY;
+        s[x][i] = v;
+        mx = fmaxf(mx, v);
+      }
+    const float mn = fmaxf(m, cols_max(mx));
+    const float ms = mn == -INFINITY ? 0.f : mn;
+    if (__builtin_amdgcn_ballot_w64(mn != m)) {
+      const float al = exp2_w(m - ms);  // 0 where there was nothing yet
+      l *= al;
+#pragma unroll
+      for (int j = 0; j < NJ; j++) {
+        O[j][0] *= al;
+        O[j][1] *= al;
+      }
+      m = mn;
+    }
+    u32x4 P;
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        s[x][i] = exp2_w(s[x][i] - ms);
+        l += s[x][i];
+      }
+      P[2 * x] = pack_f16x2(s[x][0], s[x][1]);
+      P[2 * x + 1] = pack_f16x2(s[x][2], s[x][3]);
+    }
+    vsc = vsn;
+    const f32x4 zero = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (!mixed) {
+#pragma unroll
+      for (int j = 0; j < NJ; j++) {
+        const LanePair w0 = swap16(vc[j][0], vc[j][2]), w1 = swap16(vc[j][1], vc[j][3]);
+        O[j][0] += vsc * mfma16h(cvt8<true>(w0.lo, w1.lo), P, zero);
+        O[j][1] += vsc * mfma16h(cvt8<true>(w0.hi, w1.hi), P, zero);
+      }
+    } else {
+      // Values of keys that a row does not see must not reach it: its P is 0 there, but 0 x NaN is NaN. Keys behind the
+      // last that any row sees are cleared; where one between lo and hi is NaN, each column has its own product.
+      bool bad = false;
+      const unsigned k0 = bytes_below(hi - key0), k1 = bytes_below(hi - key0 - 4);
+      const unsigned n0 = k0 & ~bytes_below(lo - key0), n1 = k1 & ~bytes_below(lo - key0 - 4);
+      u32x2 w[NJ][2];
+#pragma unroll
+      for (int j = 0; j < NJ; j++) {
+        const LanePair w0 = swap16(vc[j][0], vc[j][2]), w1 = swap16(vc[j][1], vc[j][3]);
+        w[j][0] = u32x2{w0.lo & k0, w1.lo & k1};
+        w[j][1] = u32x2{w0.hi & k0, w1.hi & k1};
+        bad = bad || ((nan_bytes(w[j][0][0]) | nan_bytes(w[j][1][0])) & n0) || ((nan_bytes(w[j][0][1]) | nan_bytes(w[j][1][1])) & n1);
+      }
+      if (!__builtin_amdgcn_ballot_w64(bad)) {
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+          O[j][0] += vsc * mfma16h(cvt8<true>(w[j][0][0], w[j][0][1]), P, zero);
+          O[j][1] += vsc * mfma16h(cvt8<true>(w[j][1][0], w[j][1][1]), P, zero);
+        }
+      } else {
+        for (int c = 0; c < 16; c++) {
+          const int lc = __builtin_amdgcn_readlane(limit, c);
+          const unsigned m0 = bytes_below(lc - key0), m1 = bytes_below(lc - key0 - 4);
+#pragma unroll
+          for (int j = 0; j < NJ; j++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+              const f32x4 o = mfma16h(cvt8<true>(w[j][x][0] & m0, w[j][x][1] & m1), P, zero);
+              if (r == c) O[j][x] += vsc * o;
+            }
+        }
+      }
+    }
+    if (blk + 1 < b1) load_v(blk + 1);
+  }
+
+  // the waves' sums
+  l = cols_sum(l);
+  if (q == 0) {
+    wm[wave * 16 + r] = m;
+    wl[wave * 16 + r] = l;
+  }
+  __syncthreads();
+  float M = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < W; w++) M = fmaxf(M, wm[w * 16 + r]);
+  const float mine = m == -INFINITY ? 0.f : exp2_w(m - M);
+  float* part = a.part + (((size_t)bh * a.RT + rt) * a.S + split) * (16 * HD + 32);
+#pragma unroll
+  for (int d0 = 0; d0 < HD; d0 += DC) {
+    if (d0) __syncthreads();
+#pragma unroll
+    for (int j = d0 / 32; j < (d0 + DC) / 32; j++) {
+      float* o = osum + (wave * 16 + r) * PITCH + 32 * j - d0 + 8 * q;
+      *reinterpret_cast<f32x4*>(o) = mine * f32x4{O[j][0][0], O[j][1][0], O[j][0][1], O[j][1][1]};
+      *reinterpret_cast<f32x4*>(o + 4) = mine * f32x4{O[j][0][2], O[j][1][2], O[j][0][3], O[j][1][3]};
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 16 * DC / 4; e += 64 * W) {
+      const int row = e / (DC / 4), d = e % (DC / 4) * 4, g = rt * 16 + row;
+      if (g >= a.T * a.G) continue;
+      float rm = -INFINITY, rl = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; w++) rm = fmaxf(rm, wm[w * 16 + row]);
+#pragma unroll
+      for (int w = 0; w < W; w++) rl += wm[w * 16 + row] == -INFINITY ? 0.f : wl[w * 16 + row] * exp2_w(wm[w * 16 + row] - rm);
+      f32x4 o = *reinterpret_cast<const f32x4*>(osum + row * PITCH + d);
+#pragma unroll
+      for (int w = 1; w < W; w++) o += *reinterpret_cast<const f32x4*>(osum + (w * 16 + row) * PITCH + d);
+      if (used > 1) {
+        *reinterpret_cast<f32x4*>(part + row * HD + d0 + d) = o;
+        if (d0 + d == 0) {
+          part[16 * HD + row] = rm;
+          part[16 * HD + 16 + row] = rl;
+        }
+      } else {
+        const int tt = g / a.G;
+        if (tt >= sp.n || sp.len - sp.n + tt < 0) o = f32x4{0.f, 0.f, 0.f, 0.f}, rl = 0.f;
+        store_row4<F16>(a.out, ((size_t)b * a.T + tt) * a.H * a.G * HD + (size_t)(h * a.G + g % a.G) * HD + d0 + d,
+                        o * inverse(rl));
+      }
+    }
+  }
+}
+
+// The splits' sums, in their order. One workgroup: one row tile; nothing to do where its sample used one split.
+template <bool F16, int HD, int W>
+__global__ void __launch_bounds__(256) join_kernel(AttnArgs a) {
+  const int rt = blockIdx.x % a.RT, bh = blockIdx.x / a.RT, h = bh % a.H, b = bh / a.H;
+  const Span sp = span_of(a, b);
+  int hi = 0;  // as the attention found it: the keys that the tile's last row sees
+  const int last = min(rt * 16 + 15, a.T * a.G - 1) / a.G, first = rt * 16 / a.G;
+  if (first < sp.n && sp.len > 0) {
+    const int t = min(last, sp.n - 1);
+    hi = a.causal ? max(0, sp.len - sp.n + t + 1) : (sp.len - sp.n + t >= 0 ? sp.len : 0);
+  }
+  const int used = splits_used((hi + BT - 1) / BT, W, a.S);
+  if (used == 1) return;
+  const float* part = a.part + ((size_t)bh * a.RT + rt) * a.S * (16 * HD + 32);
+  for (int e = blockIdx.y * 256 + threadIdx.x; e < 16 * HD / 4; e += 256 * gridDim.y) {
+    const int row = e / (HD / 4), d = e % (HD / 4) * 4, g = rt * 16 + row;
+    if (g >= a.T * a.G) continue;
+    const int t = g / a.G;
+    float M = -INFINITY, L = 0.f;
+    for (int s = 0; s < used; s++) M = fmaxf(M, part[(size_t)s * (16 * HD + 32) + 16 * HD + row]);
+    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < used; s++) {
+      const float* p = part + (size_t)s * (16 * HD + 32);
+      const float ms = p[16 * HD + row], f = ms == -INFINITY ? 0.f : exp2_w(ms - M);
+      L += f * p[16 * HD + 16 + row];
+      o += f * *reinterpret_cast<const f32x4*>(p + row * HD + d);
+    }
+    if (t >= sp.n || sp.len - sp.n + t < 0) o = f32x4{0.f, 0.f, 0.f, 0.f}, L = 0.f;
+    store_row4<F16>(a.out, ((size_t)b * a.T + t) * a.H * a.G * HD + (size_t)(h * a.G + g % a.G) * HD + d, o * inverse(L));
+  }
+}
+
+constexpr int WAVES = 4;
+
+// Splits of the keys across workgroups: enough for about eight waves a CU, at most one a block of keys and wave.
+int splits_for(int batch, int tokens, int heads, int kv_heads, int blocks) {
+  const int64_t rt = ((int64_t)tokens * (heads / kv_heads) + 15) / 16, units = rt * batch * kv_heads;
+  const int64_t most = std::max<int64_t>(1, blocks / (WAVES * MINB));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({2048 / (WAVES * units), most, 64}));
+}
+
+size_t attn_workspace(int batch, int tokens, int heads, int kv_heads, int hd, int blocks) {
+  const int S = splits_for(batch, tokens, heads, kv_heads, blocks);
+  if (S == 1) return 0;
+  const size_t rt = ((size_t)tokens * (heads / kv_heads) + 15) / 16;
+  return rt * batch * kv_heads * S * (16 * hd + 32) * sizeof(float);
+}
+
+template <bool F16, int HD>
+int launch_attn(const AttnArgs& a, hipStream_t s) {
+  const int64_t units = ((int64_t)a.B * a.H * a.S + 7) / 8 * 8, grid = units * a.RT;
+  if (grid > 0x7fffffff) return host::fail(FA_ERR_INVALID_ARG, "fa_kv8_attention: too many rows for one call");
+  const bool cap = a.cap > 0.f, bias = a.slopes != nullptr;
+  void (*k)(AttnArgs) = cap ? (bias ? attn_kernel<F16, HD, WAVES, true, true> : attn_kernel<F16, HD, WAVES, true, false>)
+                            : (bias ? attn_kernel<F16, HD, WAVES, false, true> : attn_kernel<F16, HD, WAVES, false, false>);
+  hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * WAVES), 0, s, a);
+  if (a.S > 1)
+    hipLaunchKernelGGL((join_kernel<F16, HD, WAVES>), dim3((unsigned)(a.B * a.H * a.RT), HD / 64), dim3(256), 0, s, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return host::fail(FA_ERR_LAUNCH, "fa_kv8_attention: %s", hipGetErrorString(e));
+  return FA_OK;
+}
+
+template <bool F16>
+int launch_attn(const AttnArgs& a, int hd, hipStream_t s) {
+  if (hd == 64) return launch_attn<F16, 64>(a, s);
+  if (hd == 96) return launch_attn<F16, 96>(a, s);
+  if (hd == 128) return launch_attn<F16, 128>(a, s);
+  return launch_attn<F16, 256>(a, s);
+}
+
+int check_cache(const void* k, const void* v, const void* ks, const void* vs, int batch, int heads, int hd, int blocks,
+                const char* who);  // kv8.hip
+
+}  // namespace kv8
+}  // namespace fa
+
+extern "C" size_t fa_kv8_attention_workspace_bytes(int batch, int tokens, int heads, int kv_heads, int head_dim, int blocks) {
+  if (batch < 1 || tokens < 1 || kv_heads < 1 || heads < kv_heads || heads % kv_heads || head_dim < 1 || blocks < 1) return 0;
+  return fa::kv8::attn_workspace(batch, tokens, heads, kv_heads, head_dim, blocks);
+}
+
+extern "C" int fa_kv8_attention(const fa_kv8_attn_args* a, fa_stream_t stream) {
+  using namespace fa;
+  const char* who = "fa_kv8_attention";
+  if (!a) return host::fail(FA_ERR_INVALID_ARG, "%s: args is NULL", who);
+  int rc = kv8::check_cache(a->cache_k, a->cache_v, a->cache_ks, a->cache_vs, a->batch, a->kv_heads, a->head_dim, a->blocks, who);
+  if (rc != FA_OK) return rc;
+  if (a->dtype != FA_DTYPE_BF16 && a->dtype != FA_DTYPE_F16)
+    return host::fail(FA_ERR_INVALID_ARG, "%s: dtype %d: q is bf16 or fp16", who, a->dtype);
+  if (a->heads < 1 || a->heads > (1 << 16) || a->heads % a->kv_heads)
+    return host::fail(FA_ERR_INVALID_ARG, "%s: heads=%d is no multiple of kv_heads=%d", who, a->heads, a->kv_heads);
+  if (a->tokens < 0 || (int64_t)a->tokens * a->heads > (1 << 24))
+    return host::fail(FA_ERR_INVALID_ARG, "%s: tokens=%d x heads=%d outside [0, 2^24]", who, a->tokens, a->heads);
+  if (!(a->softcap >= 0.f) || !(a->softcap < INFINITY) || !(fabsf(a->scale) < INFINITY))
+    return host::fail(FA_ERR_INVALID_ARG, "%s: scale=%g and softcap=%g must be finite, softcap >= 0", who, a->scale,
+                      a->softcap);
+  if (a->tokens == 0) return FA_OK;
+  if (!a->q || !a->out || !a->lens) return host::fail(FA_ERR_INVALID_ARG, "%s: q, out or lens is NULL", who);
+  if (reinterpret_cast<uintptr_t>(a->q) % 16 || reinterpret_cast<uintptr_t>(a->out) % 16)
+    return host::fail(FA_ERR_INVALID_ARG, "%s: q or out is not 16-byte aligned", who);
+  if (reinterpret_cast<uintptr_t>(a->lens) % 4 || reinterpret_cast<uintptr_t>(a->count) % 4 ||
+      reinterpret_cast<uintptr_t>(a->slopes) % 4)
+    return host::fail(FA_ERR_INVALID_ARG, "%s: lens, count or slopes is not 4-byte aligned", who);
+  for (int i = 0; i < 3; i++)
+    if (a->q_stride[i] % 8)
+      return host::fail(FA_ERR_INVALID_ARG, "%s: q_stride[%d]=%lld is no multiple of 8", who, i, a->q_stride[i]);
+  const size_t need = kv8::attn_workspace(a->batch, a->tokens, a->heads, a->kv_heads, a->head_dim, a->blocks);
+  if (need && (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16))
+    return host::fail(FA_ERR_INVALID_ARG, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, need,
+                      a->workspace ? a->workspace_bytes : (size_t)0);
+  rc = host::check_gfx950(who);
+  if (rc != FA_OK) return rc;
+  kv8::AttnArgs p{};
+  p.q = static_cast<const unsigned char*>(a->q);
+  p.qb = a->q_stride[0], p.qt = a->q_stride[1], p.qh = a->q_stride[2];
+  p.k = static_cast<const unsigned char*>(a->cache_k), p.v = static_cast<const unsigned char*>(a->cache_v);
+  p.ks = a->cache_ks, p.vs = a->cache_vs;
+  p.lens = a->lens, p.count = a->count, p.slopes = a->slopes;
+  p.out = static_cast<unsigned char*>(a->out), p.part = static_cast<float*>(a->workspace);
+  p.B = a->batch, p.T = a->tokens, p.H = a->kv_heads, p.G = a->heads / a->kv_heads, p.nblk = a->blocks;
+  p.RT = (p.T * p.G + 15) / 16;
+  p.S = kv8::splits_for(a->batch, a->tokens, a->heads, a->kv_heads, a->blocks);
+  p.causal = a->causal;
+  // in base 2: s log2(e); capped, the exponent 2 log2(e) s / cap of the tanh, and cap log2(e)
+  p.scale = a->softcap > 0.f ? 2.f * kv8::LOG2E * a->scale / a->softcap : a->scale * kv8::LOG2E;
+  p.cap = a->softcap * kv8::LOG2E;
+  return a->dtype == FA_DTYPE_F16 ? kv8::launch_attn<true>(p, a->head_dim, (hipStream_t)stream)
+                                  : kv8::launch_attn<false>(p, a->head_dim, (hipStream_t)stream);
+}

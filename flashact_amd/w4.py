@@ -14,7 +14,7 @@ from . import _lib
 MAX_ROWS = 64
 GROUPS = (32, 64, 128)
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
-_DT = {torch.bfloat16: _lib.FA_DTYPE_BF16, torch.float16: _lib.FA_DTYPE_F16, torch.float32: _lib.FA_DTYPE_F32}
+_DT = _lib.DTYPES
 
 
 def quantize(w: torch.Tensor, group: int = 32) -> dict:

@@ -19,7 +19,8 @@
  *                            (src/pi05/binding.cpp:34-36, src/molmoact2/binding.cpp:33-34)
  *   fa_last_error ......... TORCH_CHECK on the launch status (src/pi05/binding.cpp:67)
  *   fa_device_query ....... the occupancy clamp / diagnostics of src/molmoact2/binding.cpp:65-79
- *   fa_w4_linear .......... no counterpart (the backbone's token by token decoding)
+ *   fa_w4_linear,
+ *   fa_kv8_* .............. no counterpart (the backbone's token by token decoding)
  *   fa_abi_version ........ no counterpart (ABI guard for the Python and C++ callers)
  */
 #ifndef FLASHACT_MI355X_H
@@ -314,6 +315,81 @@ typedef struct fa_w4_args {
 } fa_w4_args;
 int fa_w4_linear(const fa_w4_args* args, fa_stream_t stream);
 size_t fa_w4_workspace_bytes(int rows, int n, int k);
+
+/* ---------------------------------------------------------------- 8-bit K/V cache
+ * One layer's cache of `batch` samples and `kv_heads` heads of 64, 96, 128 or 256 dims, `blocks` blocks of 32 tokens,
+ * contiguous:
+ *   cache_k [batch][kv_heads][blocks][head_dim / 16][32 tokens][16 dims] and
+ *   cache_v [batch][kv_heads][blocks][head_dim][32 tokens] OCP e4m3 codes (16-byte aligned);
+ *   cache_ks, cache_vs [batch][kv_heads][blocks] fp32, each a power of two; value = code * scale.
+ * fa_kv8_store puts row i < count[b] (tokens where count is NULL) of sample b at token start[b] + i. A block's scale is
+ * the smallest power of two s with max|x| <= 448 s over its new rows (2^-100 .. 2^120), or the scale of the block's
+ * earlier tokens (those before start[b]) if that is larger; if it grows, they are recoded. Codes are rounded to
+ * nearest even; infinities and NaN become NaN and set no scale. Tokens behind the new ones keep their codes. Rows
+ * that do not fit into the cache are dropped, as is a sample with a negative start.
+ * fa_kv8_load writes the values of tokens i < min(count[b], tokens) to row i of k and v; rows behind them become
+ * zero with zero_rest, else they are left as they are.
+ * k and v rows are bf16, fp16 or fp32 with strides (sample, token, head, dim) in elements; rows whose dims are
+ * contiguous and 16-byte aligned are moved 16 bytes a lane.
+ */
+typedef struct fa_kv8_rows_args {
+  int dtype; /* of the rows: FA_DTYPE_BF16, FA_DTYPE_F16 or FA_DTYPE_F32 */
+  void* k;
+  long long k_stride[4];
+  void* v;
+  long long v_stride[4];
+  void* cache_k;
+  void* cache_v;
+  float* cache_ks;
+  float* cache_vs;
+  const int* start; /* [batch], store only */
+  const int* count; /* [batch] */
+  int batch;
+  int tokens;
+  int kv_heads;
+  int head_dim;
+  int blocks;
+  int zero_rest; /* load only */
+} fa_kv8_rows_args;
+int fa_kv8_store(const fa_kv8_rows_args* args, fa_stream_t stream);
+int fa_kv8_load(const fa_kv8_rows_args* args, fa_stream_t stream);
+
+/* Attention of the newest n = count[b] <= tokens tokens (tokens where count is NULL) of each sample over its lens[b]
+ * cached ones, themselves among them: query t is at position i = lens[b] - n + t and sees keys j <= i (causal) or all
+ * j < lens[b]. Query heads h share K/V head h / (heads / kv_heads). Scores are s = q . k * scale, with softcap > 0
+ * softcap * tanh(s / softcap), less slopes[h] * |i - j| (slopes [heads] fp32 or NULL). Rows without keys (t >= n, or
+ * i < 0) become zero. lens beyond the cache count as its end.
+ * q bf16 or fp16 with strides (sample, token, head) in elements, multiples of 8, dims contiguous, 16-byte aligned;
+ * out [batch][tokens][heads][head_dim] contiguous, of q's type, 16-byte aligned. workspace:
+ * fa_kv8_attention_workspace_bytes(...) bytes, 16-byte aligned (0: may be NULL); it needs no initialisation and holds
+ * nothing between calls, but calls that may overlap need one each.
+ */
+typedef struct fa_kv8_attn_args {
+  int dtype; /* of q and out */
+  const void* q;
+  long long q_stride[3];
+  const void* cache_k;
+  const void* cache_v;
+  const float* cache_ks;
+  const float* cache_vs;
+  const int* lens;  /* [batch] */
+  const int* count; /* [batch] or NULL */
+  const float* slopes;
+  int batch;
+  int tokens;
+  int heads;
+  int kv_heads;
+  int head_dim;
+  int blocks;
+  int causal;
+  float scale;
+  float softcap;
+  void* out;
+  void* workspace;
+  size_t workspace_bytes;
+} fa_kv8_attn_args;
+int fa_kv8_attention(const fa_kv8_attn_args* args, fa_stream_t stream);
+size_t fa_kv8_attention_workspace_bytes(int batch, int tokens, int heads, int kv_heads, int head_dim, int blocks);
 
 /* ---------------------------------------------------------------- common */
 int fa_device_query(int device, fa_device_info* info);
