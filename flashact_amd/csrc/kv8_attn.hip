@@ -8,9 +8,11 @@
 // blocks of 32 keys on its own with a running maximum and sum: S^T = K Q^T (16x16x32, two tiles of 16 keys), softmax
 // down the columns, O^T += V^T P^T. The tiles' rows are dealt so that the softmax leaves P exactly where the next
 // product wants it: row m of key tile t is key 8 (m / 4) + 4 t + m % 4, so lane quarter q ends with keys 8 q .. 8 q + 7.
-// The keys' next block is fetched as soon as the products with this one are done, the values' likewise: one
-// of the two is always under way, without a second set of registers. Keys are split over the waves of a workgroup and,
-// where rows are few, over workgroups (the sums then go through the workspace to join_kernel).
+// Each wave copies its blocks to LDS on its own (no registers, no barrier): the keys' next block is asked for as soon as
+// this one's codes are in registers, the values' likewise, so a whole block is on its way at any time. Keys are split
+// over the waves of a workgroup and, where rows are few, over workgroups (the sums then go through the workspace to
+// join_kernel). They are dealt block by block, so that the waves read one contiguous stretch of memory together: with a
+// stretch for each wave, equally far apart, all of them met in the same memory channels (2 x 131072 keys: 35.8 us instead of 33.0).
 //
 // Codes are exact in bf16 and fp16. Q K^T runs in q's type; P is rounded to fp16 (2^-12, half the step of an fp16
 // result, a sixteenth of bf16's) for the product with the values' codes; scales, softmax and sums are fp32.
@@ -37,7 +39,7 @@ struct AttnArgs {
   const float* slopes;
   unsigned char* out;
   float* part;  // [sample][head][row tile][split] {O[16][hd], m[16], l[16]}
-  int B, T, H, G, nblk, RT, S, causal;
+  int B, T, H, G, nblk, RT, S, least, causal;
   float scale, cap;
 };
 
@@ -52,10 +54,11 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int b) {
   s.n = a.count ? max(0, min(a.count[b], a.T)) : a.T;
   return s;
 }
-// Splits that a sample uses: at least MINB blocks a wave.
-constexpr int MINB = 1;
-__device__ __forceinline__ int splits_used(int nb, int waves, int S) {
-  return max(1, min(S, (nb + waves * MINB - 1) / (waves * MINB)));
+// Splits that a row tile of nb blocks uses: each wave of each has a.least blocks or more.
+constexpr int MAX_SPLITS = 256;
+__device__ __forceinline__ int splits_used(const AttnArgs& a, int nb, int waves) {
+  const unsigned per = waves * a.least;
+  return max(1, min(a.S, (int)((nb + per - 1) / per)));
 }
 
 template <bool F16>
@@ -89,17 +92,50 @@ __device__ __forceinline__ void store_row4(unsigned char* out, size_t at, f32x4 
 // 1 / l of a row: no keys give zeros, NaN stays.
 __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
-template <bool F16, int HD, int W, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(64 * W) attn_kernel(AttnArgs a) {
-  constexpr int KS = (HD + 63) / 64, NJ = HD / 32;
-  constexpr int DC = HD < 128 ? HD : 128, PITCH = DC + 4;  // dims a round of the waves' sum in LDS
-  __shared__ float osum[W * 16 * PITCH];
-  __shared__ float wm[W * 16], wl[W * 16];
+// 1 KB from global memory to LDS: lane i brings 16 bytes from base + 16 i to lds + 16 i. Inline asm, so that the compiler
+// does not drain these copies at waits of its own; vm_wait<N> waits until at most N are outstanding.
+__device__ __forceinline__ void copy1k(const unsigned char* base, unsigned lane16, unsigned lds) {
+  unsigned saved;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+               : "=&s"(saved)
+               : "v"(lane16), "s"(base), "s"(lds)
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void vm_wait() {
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+  asm volatile("" ::: "memory");
+}
+// this wave's LDS reads have returned
+__device__ __forceinline__ void lds_wait() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-  // row tiles of one (sample, head, split) share their keys: neighbours on one XCD
-  const int xcd = blockIdx.x & 7, y = blockIdx.x >> 3, rt = y % a.RT, u = (y / a.RT) * 8 + xcd;
-  if (u >= a.B * a.H * a.S) return;
-  const int split = u % a.S, bh = u / a.S, h = bh % a.H, b = bh / a.H;
+template <int HD, int W>
+struct Lds {
+  static constexpr int DC = W == 4 || HD < 128 ? HD : 128, PITCH = DC + 4;  // dims a round of the waves' sum
+  static constexpr int WAVE = 2 * BT * HD;                           // a block of keys and one of values
+  static constexpr int SUM = W * 16 * PITCH * 4 > W * WAVE ? W * 16 * PITCH * 4 : W * WAVE;
+  static constexpr int BYTES = SUM + 2 * W * 16 * 4;
+};
+
+template <bool F16, int HD, int W, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) attn_kernel(AttnArgs a) {
+  constexpr int KS = (HD + 63) / 64, NT = HD / 16, NC = BT * HD / 1024;  // NC: copies of a block
+  constexpr int DC = Lds<HD, W>::DC, PITCH = Lds<HD, W>::PITCH;
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  float* osum = reinterpret_cast<float*>(lds);
+  float* wm = reinterpret_cast<float*>(lds + Lds<HD, W>::SUM);
+  float* wl = wm + W * 16;
+
+  // Row tiles of one (split, sample, head) share their keys: neighbours on one XCD. Splits are the slowest index: samples
+  // that leave the later ones unused would else leave XCDs unused (64 samples of 1050 keys on 16 splits: 72 us instead
+  // of 21); within a split the samples are turned, so that the splits of one meet on different XCDs.
+  const unsigned xcd = blockIdx.x & 7, y = blockIdx.x >> 3, yr = y / (unsigned)a.RT, u = yr * 8 + xcd;
+  const unsigned heads = a.B * a.H;
+  const int rt = y - yr * a.RT, split = u / heads;
+  unsigned turned = u - split * heads + (heads >= 8 ? (split * (heads - 1)) & 7 : 0);
+  if (turned >= heads) turned -= heads;
+  const int bh = turned, b = bh / (unsigned)a.H, h = bh - b * a.H;
+  if (split >= a.S) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
   const Span sp = span_of(a, b);
@@ -117,10 +153,9 @@ __global__ void __launch_bounds__(64 * W) attn_kernel(AttnArgs a) {
   lo = __builtin_amdgcn_readfirstlane(lo);  // keys that every row sees (rows that are not there do not count)
   if (!valid) limit = hi;
   const int nb = (hi + BT - 1) / BT;
-  const int used = splits_used(nb, W, a.S);
+  const int used = splits_used(a, nb, W);
   if (split >= used) return;
   const int at = split * W + wave, all = used * W;
-  const int b0 = (int)((int64_t)nb * at / all), b1 = (int)((int64_t)nb * (at + 1) / all);
 
   u32x4 qf[KS][2];
 #pragma unroll
@@ -135,38 +170,38 @@ __global__ void __launch_bounds__(64 * W) attn_kernel(AttnArgs a) {
   const float slope = BIAS && valid ? a.slopes[head] * LOG2E : 0.f;
 
   const size_t unit = ((size_t)b * a.H + h) * a.nblk;
-  const unsigned char* kp = a.k + unit * (BT * HD) + (q * BT + 8 * (r >> 2) + (r & 3)) * 16;
-  const unsigned char* vp = a.v + unit * (BT * HD) + (2 * r + (q & 1)) * BT + (q >> 1) * 16;
-  u32x4 kc[2][KS], vc[NJ];
-  float ksc = 0.f, vsc = 0.f, ksn = 0.f, vsn = 0.f;
-  auto load_k = [&](int blk) {
-    const unsigned char* p = kp + (size_t)blk * (BT * HD);
+  unsigned char* kl = lds + wave * Lds<HD, W>::WAVE;
+  unsigned char* vl = kl + BT * HD;
+  const unsigned at_k = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)kl), at_v = at_k + BT * HD;
+  auto copy = [&](const unsigned char* from, int blk, unsigned to) {
+    const unsigned char* p = from + (unit + blk) * (BT * HD);
+#pragma unroll
+    for (int i = 0; i < NC; i++) copy1k(p + i * 1024, lane * 16, to + i * 1024);
+  };
+
+  f32x4 O[NT];
+#pragma unroll
+  for (int j = 0; j < NT; j++) O[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;  // l: this lane's keys only
+  if (at < nb) {
+    copy(a.k, at, at_k);
+    copy(a.v, at, at_v);
+  }
+  for (int blk = at; blk < nb; blk += all) {
+    const bool more = blk + all < nb;
+    vm_wait<NC>();  // the keys; the values are still on their way
+    u32x4 kc[2][KS];
 #pragma unroll
     for (int i = 0; i < KS; i++)
 #pragma unroll
-      for (int s = 0; s < 2; s++) {
-        kc[s][i] = u32x4{0, 0, 0, 0};
+      for (int x = 0; x < 2; x++) {
+        kc[x][i] = u32x4{0, 0, 0, 0};
         if (HD % 64 == 0 || 64 * i + 16 * q < HD)
-          kc[s][i] = *reinterpret_cast<const u32x4*>(p + i * (4 * BT * 16) + s * 64);
+          kc[x][i] = *reinterpret_cast<const u32x4*>(kl + ((4 * i + q) * BT + 8 * (r >> 2) + 4 * x + (r & 3)) * 16);
       }
-    ksn = a.ks[unit + blk];
-  };
-  auto load_v = [&](int blk) {
-    const unsigned char* p = vp + (size_t)blk * (BT * HD);
-#pragma unroll
-    for (int j = 0; j < NJ; j++) vc[j] = *reinterpret_cast<const u32x4*>(p + j * (32 * BT));
-    vsn = a.vs[unit + blk];
-  };
-
-  f32x4 O[NJ][2];
-#pragma unroll
-  for (int j = 0; j < NJ; j++) O[j][0] = O[j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;  // l: this lane's keys only
-  if (b0 < b1) {
-    load_k(b0);
-    load_v(b0);
-  }
-  for (int blk = b0; blk < b1; blk++) {
+    const float ksc = a.ks[unit + blk], vsc = a.vs[unit + blk];
+    lds_wait();
+    if (more) copy(a.k, blk + all, at_k);
     f32x4 s[2];
 #pragma unroll
     for (int x = 0; x < 2; x++) {
@@ -178,8 +213,6 @@ __global__ void __launch_bounds__(64 * W) attn_kernel(AttnArgs a) {
         s[x] = F16 ? mfma16h(c1, qf[i][1], s[x]) : mfma16(c1, qf[i][1], s[x]);
       }
     }
-    ksc = ksn;
-    if (blk + 1 < b1) load_k(blk + 1);
     // scores in base 2
     const int key0 = blk * BT + 8 * q;
     const float f = ksc * a.scale;
@@ -205,10 +238,7 @@ __global__ void __launch_bounds__(64 * W) attn_kernel(AttnArgs a) {
       const float al = exp2_w(m - ms);  // 0 where there was nothing yet
       l *= al;
 #pragma unroll
-      for (int j = 0; j < NJ; j++) {
-        O[j][0] *= al;
-        O[j][1] *= al;
-      }
+      for (int j = 0; j < NT; j++) O[j] *= al;
       m = mn;
     }
     u32x4 P;
@@ -222,54 +252,49 @@ __global__ void __launch_bounds__(64 * W) attn_kernel(AttnArgs a) {
       P[2 * x] = pack_f16x2(s[x][0], s[x][1]);
       P[2 * x + 1] = pack_f16x2(s[x][2], s[x][3]);
     }
-    vsc = vsn;
+    if (more) vm_wait<NC>();
+    else vm_wait<0>();
+    u32x2 vc[NT];  // keys key0 .. key0 + 7 of dim 16 j + r
+#pragma unroll
+    for (int j = 0; j < NT; j++) vc[j] = *reinterpret_cast<const u32x2*>(vl + (16 * j + r) * BT + 8 * q);
+    lds_wait();
+    if (more) copy(a.v, blk + all, at_v);
+    // Values of keys that a row does not see must not reach it: its P is 0 there, but 0 x NaN is NaN. Codes behind the
+    // last key that any row sees are cleared; where one between lo and hi is NaN, each column has its own product.
+    bool apart = false;
+    if (mixed) {
+      const u32x2 some = u32x2{bytes_below(hi - key0), bytes_below(hi - key0 - 4)};
+      const u32x2 each = u32x2{bytes_below(lo - key0), bytes_below(lo - key0 - 4)};
+      unsigned bad = 0;
+#pragma unroll
+      for (int j = 0; j < NT; j++) {
+        vc[j] &= some;
+        bad |= (nan_bytes(vc[j][0]) & ~each[0]) | (nan_bytes(vc[j][1]) & ~each[1]);
+      }
+      apart = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+    }
     const f32x4 zero = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (!mixed) {
+    if (!apart) {
 #pragma unroll
-      for (int j = 0; j < NJ; j++) {
-        const LanePair w0 = swap16(vc[j][0], vc[j][2]), w1 = swap16(vc[j][1], vc[j][3]);
-        O[j][0] += vsc * mfma16h(cvt8<true>(w0.lo, w1.lo), P, zero);
-        O[j][1] += vsc * mfma16h(cvt8<true>(w0.hi, w1.hi), P, zero);
-      }
+      for (int j = 0; j < NT; j++) O[j] += vsc * mfma16h(cvt8<true>(vc[j][0], vc[j][1]), P, zero);
     } else {
-      // Values of keys that a row does not see must not reach it: its P is 0 there, but 0 x NaN is NaN. Keys behind the
-      // last that any row sees are cleared; where one between lo and hi is NaN, each column has its own product.
-      bool bad = false;
-      const unsigned k0 = bytes_below(hi - key0), k1 = bytes_below(hi - key0 - 4);
-      const unsigned n0 = k0 & ~bytes_below(lo - key0), n1 = k1 & ~bytes_below(lo - key0 - 4);
-      u32x2 w[NJ][2];
+#pragma unroll 1
+      for (int c = 0; c < 16; c++) {
+        const int n = __builtin_amdgcn_readlane(limit, c) - key0;
+        const unsigned own0 = bytes_below(n), own1 = bytes_below(n - 4);
 #pragma unroll
-      for (int j = 0; j < NJ; j++) {
-        const LanePair w0 = swap16(vc[j][0], vc[j][2]), w1 = swap16(vc[j][1], vc[j][3]);
-        w[j][0] = u32x2{w0.lo & k0, w1.lo & k1};
-        w[j][1] = u32x2{w0.hi & k0, w1.hi & k1};
-        bad = bad || ((nan_bytes(w[j][0][0]) | nan_bytes(w[j][1][0])) & n0) || ((nan_bytes(w[j][0][1]) | nan_bytes(w[j][1][1])) & n1);
-      }
-      if (!__builtin_amdgcn_ballot_w64(bad)) {
-#pragma unroll
-        for (int j = 0; j < NJ; j++) {
-          O[j][0] += vsc * mfma16h(cvt8<true>(w[j][0][0], w[j][0][1]), P, zero);
-          O[j][1] += vsc * mfma16h(cvt8<true>(w[j][1][0], w[j][1][1]), P, zero);
-        }
-      } else {
-        for (int c = 0; c < 16; c++) {
-          const int lc = __builtin_amdgcn_readlane(limit, c);
-          const unsigned m0 = bytes_below(lc - key0), m1 = bytes_below(lc - key0 - 4);
-#pragma unroll
-          for (int j = 0; j < NJ; j++)
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-              const f32x4 o = mfma16h(cvt8<true>(w[j][x][0] & m0, w[j][x][1] & m1), P, zero);
-              if (r == c) O[j][x] += vsc * o;
-            }
+        for (int j = 0; j < NT; j++) {
+          const f32x4 o = mfma16h(cvt8<true>(vc[j][0] & own0, vc[j][1] & own1), P, zero);
+          if (r == c) O[j] += vsc * o;
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
-    if (blk + 1 < b1) load_v(blk + 1);
   }
 
   // the waves' sums
   l = cols_sum(l);
+  __syncthreads();  // the blocks in LDS are done with
   if (q == 0) {
     wm[wave * 16 + r] = m;
     wl[wave * 16 + r] = l;
@@ -284,11 +309,8 @@ __global__ void __launch_bounds__(64 * W) attn_kernel(AttnArgs a) {
   for (int d0 = 0; d0 < HD; d0 += DC) {
     if (d0) __syncthreads();
 #pragma unroll
-    for (int j = d0 / 32; j < (d0 + DC) / 32; j++) {
-      float* o = osum + (wave * 16 + r) * PITCH + 32 * j - d0 + 8 * q;
-      *reinterpret_cast<f32x4*>(o) = mine * f32x4{O[j][0][0], O[j][1][0], O[j][0][1], O[j][1][1]};
-      *reinterpret_cast<f32x4*>(o + 4) = mine * f32x4{O[j][0][2], O[j][1][2], O[j][0][3], O[j][1][3]};
-    }
+    for (int j = d0 / 16; j < (d0 + DC) / 16; j++)
+      *reinterpret_cast<f32x4*>(osum + (wave * 16 + r) * PITCH + 16 * j - d0 + 4 * q) = mine * O[j];
     __syncthreads();
     for (int e = threadIdx.x; e < 16 * DC / 4; e += 64 * W) {
       const int row = e / (DC / 4), d = e % (DC / 4) * 4, g = rt * 16 + row;
@@ -317,68 +339,104 @@ __global__ void __launch_bounds__(64 * W) attn_kernel(AttnArgs a) {
   }
 }
 
-// The splits' sums, in their order. One workgroup: one row tile; nothing to do where its sample used one split.
+// The splits' sums, in a fixed order. One workgroup: one row; nothing to do where its sample used one split. Threads are
+// (hd / 4) dims x groups of splits, so many splits are read side by side.
 template <bool F16, int HD, int W>
 __global__ void __launch_bounds__(256) join_kernel(AttnArgs a) {
-  const int rt = blockIdx.x % a.RT, bh = blockIdx.x / a.RT, h = bh % a.H, b = bh / a.H;
+  constexpr int SLOTS = HD / 4, GROUPS = 256 / SLOTS;
+  __shared__ float wt[MAX_SPLITS], red[8];
+  __shared__ f32x4 sums[GROUPS][SLOTS];
+  const int rows = a.T * a.G, g = blockIdx.x % rows, bh = blockIdx.x / rows, h = bh % a.H, b = bh / a.H;
+  const int rt = g >> 4, row = g & 15, t = g / a.G;
   const Span sp = span_of(a, b);
   int hi = 0;  // as the attention found it: the keys that the tile's last row sees
-  const int last = min(rt * 16 + 15, a.T * a.G - 1) / a.G, first = rt * 16 / a.G;
-  if (first < sp.n && sp.len > 0) {
-    const int t = min(last, sp.n - 1);
-    hi = a.causal ? max(0, sp.len - sp.n + t + 1) : (sp.len - sp.n + t >= 0 ? sp.len : 0);
+  if (rt * 16 / a.G < sp.n) {
+    const int last = min(min(rt * 16 + 15, rows - 1) / a.G, sp.n - 1), pos = sp.len - sp.n + last;
+    hi = pos < 0 ? 0 : a.causal ? pos + 1 : sp.len;
   }
-  const int used = splits_used((hi + BT - 1) / BT, W, a.S);
+  const int used = splits_used(a, (hi + BT - 1) / BT, W);
   if (used == 1) return;
-  const float* part = a.part + ((size_t)bh * a.RT + rt) * a.S * (16 * HD + 32);
-  for (int e = blockIdx.y * 256 + threadIdx.x; e < 16 * HD / 4; e += 256 * gridDim.y) {
-    const int row = e / (HD / 4), d = e % (HD / 4) * 4, g = rt * 16 + row;
-    if (g >= a.T * a.G) continue;
-    const int t = g / a.G;
-    float M = -INFINITY, L = 0.f;
-    for (int s = 0; s < used; s++) M = fmaxf(M, part[(size_t)s * (16 * HD + 32) + 16 * HD + row]);
-    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int s = 0; s < used; s++) {
-      const float* p = part + (size_t)s * (16 * HD + 32);
-      const float ms = p[16 * HD + row], f = ms == -INFINITY ? 0.f : exp2_w(ms - M);
-      L += f * p[16 * HD + 16 + row];
-      o += f * *reinterpret_cast<const f32x4*>(p + row * HD + d);
-    }
-    if (t >= sp.n || sp.len - sp.n + t < 0) o = f32x4{0.f, 0.f, 0.f, 0.f}, L = 0.f;
-    store_row4<F16>(a.out, ((size_t)b * a.T + t) * a.H * a.G * HD + (size_t)(h * a.G + g % a.G) * HD + d, o * inverse(L));
+  constexpr int ONE = 16 * HD + 32;
+  const float* part = a.part + ((size_t)bh * a.RT + rt) * a.S * ONE;
+  const int i = threadIdx.x, wave = i >> 6;
+  const float ms = i < used ? part[(size_t)i * ONE + 16 * HD + row] : -INFINITY;
+  const float ls = i < used ? part[(size_t)i * ONE + 16 * HD + 16 + row] : 0.f;
+  float x = wave_max(ms);
+  if ((i & 63) == 0) red[wave] = x;
+  __syncthreads();
+  const float M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float w = ms == -INFINITY ? 0.f : exp2_w(ms - M);
+  wt[i] = w;
+  x = wave_sum(w * ls);
+  if ((i & 63) == 0) red[4 + wave] = x;
+  __syncthreads();
+  float L = red[4] + red[5] + red[6] + red[7];
+  const int d = (i % SLOTS) * 4, grp = i / SLOTS;
+  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (grp < GROUPS) {
+#pragma unroll 8
+    for (int s = grp; s < used; s += GROUPS) o += wt[s] * *reinterpret_cast<const f32x4*>(part + (size_t)s * ONE + row * HD + d);
+    sums[grp][i % SLOTS] = o;
   }
+  __syncthreads();
+  if (i >= SLOTS) return;
+  o = sums[0][i];
+#pragma unroll
+  for (int s = 1; s < GROUPS; s++) o += sums[s][i];
+  if (t >= sp.n || sp.len - sp.n + t < 0) o = f32x4{0.f, 0.f, 0.f, 0.f}, L = 0.f;
+  store_row4<F16>(a.out, ((size_t)b * a.T + t) * a.H * a.G * HD + (size_t)(h * a.G + g % a.G) * HD + d, o * inverse(L));
 }
 
-constexpr int WAVES = 4;
+constexpr int WAVES = 4;  // of a workgroup
 
-// Splits of the keys across workgroups: enough for about eight waves a CU, at most one a block of keys and wave.
-int splits_for(int batch, int tokens, int heads, int kv_heads, int blocks) {
+// Splits of the keys across workgroups. A wave takes about 2.3 us for a block of 256 dims that comes from memory (1.2 of 128
+// and less), more than one (four) workgroups a CU share its bandwidth, and joining the splits costs 3 us: the number with
+// the least estimate, for samples that fill the cache (their lengths are on the GPU), is taken. Shorter ones use fewer.
+int splits_for(int batch, int tokens, int heads, int kv_heads, int hd, int blocks) {
   const int64_t rt = ((int64_t)tokens * (heads / kv_heads) + 15) / 16, units = rt * batch * kv_heads;
-  const int64_t most = std::max<int64_t>(1, blocks / (WAVES * MINB));
-  return (int)std::max<int64_t>(1, std::min<int64_t>({2048 / (WAVES * units), most, 64}));
+  const double block = hd == 256 ? 2.3 : 1.2, resident = hd == 256 ? 1.0 : 4.0;
+  const int64_t most = std::min<int64_t>((blocks + WAVES - 1) / WAVES, MAX_SPLITS);
+  int best = 1;
+  double least = 1e300;
+  auto consider = [&](int64_t S) {
+    if (S < 1 || S > most) return;
+    const int64_t each = (blocks + WAVES * S - 1) / (WAVES * S);
+    const double t = block * each * std::max(1.0, (units * S + 255) / 256 / resident) + (S > 1 ? 3.0 : 0.0);
+    if (t < least) best = (int)S, least = t;
+  };
+  for (int64_t S = 1; S <= most; S += std::max<int64_t>(1, S / 4)) consider(S);
+  for (int64_t n = 1; n <= 4; n *= 2) consider(256 * n / units);  // whole rounds of workgroups
+  return best;
 }
 
 size_t attn_workspace(int batch, int tokens, int heads, int kv_heads, int hd, int blocks) {
-  const int S = splits_for(batch, tokens, heads, kv_heads, blocks);
+  const int S = splits_for(batch, tokens, heads, kv_heads, hd, blocks);
   if (S == 1) return 0;
   const size_t rt = ((size_t)tokens * (heads / kv_heads) + 15) / 16;
   return rt * batch * kv_heads * S * (16 * hd + 32) * sizeof(float);
 }
 
-template <bool F16, int HD>
-int launch_attn(const AttnArgs& a, hipStream_t s) {
+template <bool F16, int HD, int W>
+int launch_waves(const AttnArgs& a, hipStream_t s) {
   const int64_t units = ((int64_t)a.B * a.H * a.S + 7) / 8 * 8, grid = units * a.RT;
   if (grid > 0x7fffffff) return host::fail(FA_ERR_INVALID_ARG, "fa_kv8_attention: too many rows for one call");
   const bool cap = a.cap > 0.f, bias = a.slopes != nullptr;
-  void (*k)(AttnArgs) = cap ? (bias ? attn_kernel<F16, HD, WAVES, true, true> : attn_kernel<F16, HD, WAVES, true, false>)
-                            : (bias ? attn_kernel<F16, HD, WAVES, false, true> : attn_kernel<F16, HD, WAVES, false, false>);
-  hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * WAVES), 0, s, a);
+  void (*k)(AttnArgs) = cap ? (bias ? attn_kernel<F16, HD, W, true, true> : attn_kernel<F16, HD, W, true, false>)
+                            : (bias ? attn_kernel<F16, HD, W, false, true> : attn_kernel<F16, HD, W, false, false>);
+  const unsigned lds = Lds<HD, W>::BYTES;
+  const int rc = host::allow_lds(reinterpret_cast<const void*>(k), lds, "fa_kv8_attention");
+  if (rc != FA_OK) return rc;
+  hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * W), lds, s, a);
   if (a.S > 1)
-    hipLaunchKernelGGL((join_kernel<F16, HD, WAVES>), dim3((unsigned)(a.B * a.H * a.RT), HD / 64), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((join_kernel<F16, HD, W>), dim3((unsigned)(a.B * a.H * a.T * a.G)), dim3(256), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return host::fail(FA_ERR_LAUNCH, "fa_kv8_attention: %s", hipGetErrorString(e));
   return FA_OK;
+}
+
+template <bool F16, int HD>
+int launch_attn(const AttnArgs& a, hipStream_t s) {
+  return launch_waves<F16, HD, WAVES>(a, s);
 }
 
 template <bool F16>
@@ -440,7 +498,8 @@ extern "C" int fa_kv8_attention(const fa_kv8_attn_args* a, fa_stream_t stream) {
   p.out = static_cast<unsigned char*>(a->out), p.part = static_cast<float*>(a->workspace);
   p.B = a->batch, p.T = a->tokens, p.H = a->kv_heads, p.G = a->heads / a->kv_heads, p.nblk = a->blocks;
   p.RT = (p.T * p.G + 15) / 16;
-  p.S = kv8::splits_for(a->batch, a->tokens, a->heads, a->kv_heads, a->blocks);
+  p.S = kv8::splits_for(a->batch, a->tokens, a->heads, a->kv_heads, a->head_dim, a->blocks);
+  p.least = (int64_t)p.RT * p.B * p.H >= 64 ? 4 : 1;
   p.causal = a->causal;
   // in base 2: s log2(e); capped, the exponent 2 log2(e) s / cap of the tanh, and cap log2(e)
   p.scale = a->softcap > 0.f ? 2.f * kv8::LOG2E * a->scale / a->softcap : a->scale * kv8::LOG2E;
