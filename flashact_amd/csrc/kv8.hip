@@ -95,16 +95,11 @@ __device__ __forceinline__ float scale_for(float amax) {
   return as_f32((unsigned)(e + 127) << 23);
 }
 
-// Two values, already divided by the scale -> two codes (round to nearest even) in the low 16 bits. What is not finite
-// becomes the NaN code: e4m3 has no infinity.
-__device__ __forceinline__ unsigned codes2(float a, float b) {
-  unsigned c = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu;
-  if (!(fabsf(a) <= 448.f)) c = (c & 0xff00u) | 0x7fu;
-  if (!(fabsf(b) <= 448.f)) c = (c & 0x00ffu) | 0x7f00u;
-  return c;
-}
+// Four values, already divided by the scale -> four codes, rounded to nearest even. What is not finite becomes a NaN
+// code (e4m3 has no infinity, and the instruction does not saturate).
 __device__ __forceinline__ unsigned codes4(float a, float b, float c, float d) {
-  return codes2(a, b) | (codes2(c, d) << 16);
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
 }
 __device__ __forceinline__ void values4(unsigned c, float (&x)[4]) {
   const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
@@ -148,7 +143,21 @@ __global__ void __launch_bounds__(256) store_kernel(CacheArgs a) {
   float* scale = (val ? a.vs : a.ks) + unit;
   const int c8 = threadIdx.x % (a.hd / 8), rg = threadIdx.x / (a.hd / 8);
   const bool mine = rg < 8;
+  const float old = lo > 0 ? *scale : 0.f;
 
+  // what the block holds and keeps is asked for together with the new rows: two words a token of keys, one a dim of values
+  unsigned held[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (mine && val && (4 * rg < lo || 4 * rg + 4 > hi)) {
+#pragma unroll
+    for (int d = 0; d < 8; d++) held[d] = *reinterpret_cast<const unsigned*>(code + (8 * c8 + d) * BT + 4 * rg);
+  } else if (mine && !val) {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (4 * rg + j < lo) {
+        const u32x2 c = *reinterpret_cast<const u32x2*>(code + ((c8 >> 1) * BT + 4 * rg + j) * 16 + (c8 & 1) * 8);
+        held[2 * j] = c[0], held[2 * j + 1] = c[1];
+      }
+  }
   float x[4][8], amax = 0.f;
 #pragma unroll
   for (int j = 0; j < 4; j++) {
@@ -165,7 +174,6 @@ __global__ void __launch_bounds__(256) store_kernel(CacheArgs a) {
   }
   amax = wave_max(amax);
   if ((threadIdx.x & 63) == 0) wmax[threadIdx.x >> 6] = amax;
-  const float old = lo > 0 ? *scale : 0.f;
   __syncthreads();
   amax = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
   const float to = lo > 0 ? fmaxf(scale_for(amax), old) : scale_for(amax);
@@ -183,8 +191,7 @@ __global__ void __launch_bounds__(256) store_kernel(CacheArgs a) {
         *p = u32x2{codes4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv),
                    codes4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv)};
       } else if (row < lo && to != old) {
-        const u32x2 c = *p;
-        *p = u32x2{recode4(c[0], ratio), recode4(c[1], ratio)};
+        *p = u32x2{recode4(held[2 * j], ratio), recode4(held[2 * j + 1], ratio)};
       }
     }
     return;
@@ -194,8 +201,7 @@ __global__ void __launch_bounds__(256) store_kernel(CacheArgs a) {
     for (int d = 0; d < 8; d++) {
       unsigned c = codes4(x[0][d] * inv, x[1][d] * inv, x[2][d] * inv, x[3][d] * inv);
       if (4 * rg < lo || 4 * rg + 4 > hi) {  // tokens of the word that are not new
-        unsigned was = *reinterpret_cast<const unsigned*>(code + (8 * c8 + d) * BT + 4 * rg);
-        const unsigned again = to != old ? recode4(was, ratio) : was;
+        const unsigned was = held[d], again = to != old ? recode4(was, ratio) : was;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const unsigned m = 0xffu << (8 * j);
