@@ -114,6 +114,17 @@ class Kv8AttnArgs(ctypes.Structure):
     ]
 
 
+class SpanArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int), ("q", ctypes.c_void_p), ("q_stride", ctypes.c_longlong * 3),
+        ("k", ctypes.c_void_p), ("k_stride", ctypes.c_longlong * 3), ("v", ctypes.c_void_p), ("v_stride", ctypes.c_longlong * 3),
+        ("spans", ctypes.c_void_p), ("slopes", ctypes.c_void_p),
+        ("batch", ctypes.c_int), ("queries", ctypes.c_int), ("keys", ctypes.c_int), ("heads", ctypes.c_int),
+        ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
+        ("out", ctypes.c_void_p),
+    ]
+
+
 class DeviceInfo(ctypes.Structure):
     _fields_ = [("cus", ctypes.c_int), ("xcds", ctypes.c_int), ("lds_bytes", ctypes.c_int),
                 ("coop_launch", ctypes.c_int), ("coop_max_blocks", ctypes.c_int), ("arch", ctypes.c_char * 64)]
@@ -142,6 +153,7 @@ SYMBOLS = [
     ("fa_kv8_load", ctypes.c_int, [ctypes.POINTER(Kv8RowsArgs), ctypes.c_void_p]),
     ("fa_kv8_attention", ctypes.c_int, [ctypes.POINTER(Kv8AttnArgs), ctypes.c_void_p]),
     ("fa_kv8_attention_workspace_bytes", ctypes.c_size_t, [ctypes.c_int] * 6),
+    ("fa_span_attention", ctypes.c_int, [ctypes.POINTER(SpanArgs), ctypes.c_void_p]),
     ("fa_device_query", ctypes.c_int, [ctypes.c_int, ctypes.POINTER(DeviceInfo)]),
     ("fa_last_error", ctypes.c_char_p, []),
     ("fa_abi_version", ctypes.c_int, []),

@@ -1,0 +1,393 @@
+// Attention in which every query has its own span of keys (fa_span_attention): packed prompts, prefixes, windows.
+//
+//   s_ij = q_i . k_j scale, capped to cap tanh(s / cap), less slope_h |i + Tk - Tq - j|;  o_i = sum_j softmax_j(s_ij) v_j
+//   over the keys first_i <= j < last_i; a query whose span is empty gets zeros.
+//
+// One pass over the keys with a running maximum and sum. A workgroup of four waves takes 64 QB queries of one head (16 QB a
+// wave) and walks over the tiles of KT keys between the first key that any of them sees and the last; tiles that all of
+// them see whole skip the masks. S^T = K Q^T and O^T += V^T P^T on the 16x16x32 MFMA: a lane holds one query's column, the
+// softmax needs two cross-lane steps, and P^T is already the second product's operand (slot 8 q + j of a 32-key step is key
+// 4 q + j of its first 16 for j < 4, key 16 + 4 q + j - 4 beyond), which the values' transposing LDS read matches.
+// Keys and values of the next tile are copied to LDS (no registers) while this one is worked on, one barrier a tile; two
+// workgroups share a CU, so one's softmax runs under the other's products.
+//
+// Rounding: the scores' products are exact in fp32, softmax and sums are fp32, P is rounded to the values' type for the
+// second product (bf16 values have a range that fp16 weights times fp16 values would not hold), the result once.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "../../include/flashact_mi355x.h"
+#include "fa_device.h"
+#include "fa_host.h"
+
+namespace fa {
+namespace attn {
+
+struct Params {
+  const unsigned char *q, *k, *v;
+  int64_t qb, qt, qh, kb, vb, kh, vh;  // strides in elements; the token strides of k and v fit 32 bits
+  int kt, vt;
+  const int* spans;  // [B][Tq][2] or NULL: all keys
+  const float* slopes;
+  unsigned char* out;  // [B][Tq][H][hd]
+  int B, Tq, Tk, H, G, hd, ntile;
+  float scale, cap;
+};
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int NW = 4;
+
+// LDS slot of chunk c (16 bytes) of row `row`: rows of CH chunks whose chunks are exchanged so that 16 rows' equal chunks
+// lie in different banks.
+template <int CH>
+__device__ __forceinline__ int turn(int row) {
+  if constexpr (CH == 8) return (row >> 1) & 7;
+  else if constexpr (CH == 12) return (row >> 2) & 3;
+  else return row & 15;
+}
+
+__device__ __forceinline__ void copy16(const unsigned char* base, unsigned off, unsigned lds) {
+  unsigned saved;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+               : "=&s"(saved)
+               : "v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds))
+               : "memory");
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+// Four rows of 16 two-byte elements, held by 16 lanes as 8-byte pieces (lane 4 a + p: row a, elements 4 p .. 4 p + 3) ->
+// lane i gets element i of the four rows.
+__device__ __forceinline__ u32x2 read_turned(const unsigned char* p) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) s16x4*)(const_cast<unsigned char*>(p))));
+}
+
+template <bool F16>
+__device__ __forceinline__ unsigned pack2(float a, float b) {
+  return F16 ? pack_f16x2(a, b) : pack_bf16x2(a, b);
+}
+template <bool F16>
+__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+  return F16 ? mfma16h(a, b, c) : mfma16(a, b, c);
+}
+// sign bit of each half that is an infinity or NaN
+template <bool F16>
+__device__ __forceinline__ unsigned not_finite(unsigned x) {
+  return F16 ? ((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u : ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+}
+// sign bit of each half whose fraction is not zero
+template <bool F16>
+__device__ __forceinline__ unsigned fraction(unsigned x) {
+  return F16 ? ((x & 0x03ff03ffu) + 0x7fff7fffu) & 0x80008000u : ((x & 0x007f007fu) + 0x7fff7fffu) & 0x80008000u;
+}
+// the halves whose sign bit is set, whole
+__device__ __forceinline__ unsigned spread(unsigned sign) { return sign | (sign - (sign >> 15)); }
+
+template <bool F16, int HD, int QB, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
+  constexpr int KT = HD == 256 ? 32 : 64, CH = HD / 8, NK = HD / 32, NT = HD / 16, MT = KT / 16;
+  constexpr int TILE = KT * HD * 2, PER = KT * CH / (64 * NW);  // bytes of a tile of keys, copies a wave issues for it
+  constexpr unsigned ONE = F16 ? 0x3c00u : 0x3f80u;
+  static_assert(KT * CH % (64 * NW) == 0, "whole copies");
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // two buffers of {keys, values}
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, q = lane >> 4;
+
+  // Heads (of all samples) go to XCDs in runs where they divide evenly, so that those that share keys meet in one L2;
+  // the last tiles, which see most under a causal span, start first.
+  const unsigned heads = p.B * p.H, id = blockIdx.x;
+  unsigned bh, tile;
+  if (heads % 8 == 0) {
+    const unsigned per = heads / 8, j = id >> 3;
+    tile = j / per;
+    bh = (id & 7) * per + (j - tile * per);
+  } else {
+    tile = id / heads;
+    bh = id - tile * heads;
+  }
+  const int b = bh / (unsigned)p.H, h = bh - b * p.H, kvh = h / p.G;
+  const int row0 = (p.ntile - 1 - (int)tile) * (16 * QB * NW) + wave * 16 * QB;
+
+  // this lane's queries and the tile's extent
+  int first[QB], last[QB], lo = 0x7fffffff, hi = 0, all_lo = 0, all_hi = 0x7fffffff;
+#pragma unroll
+  for (int x = 0; x < QB; x++) {
+    const int row = row0 + 16 * x + r;
+    first[x] = 0, last[x] = 0;
+    if (row < p.Tq) {
+      if (p.spans) {
+        const int* s = p.spans + ((size_t)b * p.Tq + row) * 2;
+        first[x] = max(s[0], 0);
+        last[x] = min(s[1], p.Tk);
+      } else {
+        last[x] = p.Tk;
+      }
+      if (first[x] < last[x]) {
+        lo = min(lo, first[x]), hi = max(hi, last[x]);
+        all_lo = max(all_lo, first[x]), all_hi = min(all_hi, last[x]);
+      } else {
+        first[x] = last[x] = 0;
+        all_hi = 0;  // a row that sees nothing: every tile is masked
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    lo = min(lo, __shfl_xor(lo, o));
+    hi = max(hi, __shfl_xor(hi, o));
+    all_lo = max(all_lo, __shfl_xor(all_lo, o));
+    all_hi = min(all_hi, __shfl_xor(all_hi, o));
+  }
+  int* ext = reinterpret_cast<int*>(lds + 4 * TILE);  // the workgroup walks over the keys of all its waves
+  if (lane == 0) {
+    ext[2 * wave] = lo;
+    ext[2 * wave + 1] = hi;
+  }
+  // dims behind hd are zero in LDS: the copies never write them
+  if (p.hd < HD)
+    for (int i = threadIdx.x; i < 4 * TILE / 16; i += 64 * NW) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
+  __syncthreads();
+  int k0 = 0x7fffffff, k1 = 0;
+#pragma unroll
+  for (int w = 0; w < NW; w++) k0 = min(k0, ext[2 * w]), k1 = max(k1, ext[2 * w + 1]);
+  k0 = __builtin_amdgcn_readfirstlane(k0);
+  k1 = __builtin_amdgcn_readfirstlane(k1);
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  hi = __builtin_amdgcn_readfirstlane(hi);
+  all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+  all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+
+  u32x4 qf[QB][NK];
+#pragma unroll
+  for (int x = 0; x < QB; x++)
+#pragma unroll
+    for (int i = 0; i < NK; i++) {
+      const int row = row0 + 16 * x + r, d = 32 * i + 8 * q;
+      qf[x][i] = u32x4{0, 0, 0, 0};
+      if (row < p.Tq && d < p.hd)
+        qf[x][i] = *reinterpret_cast<const u32x4*>(p.q + (b * p.qb + row * p.qt + h * p.qh + d) * 2);
+    }
+  const float slope = BIAS ? p.slopes[h] * LOG2E : 0.f;
+
+  const unsigned char* kg = p.k + (b * p.kb + kvh * p.kh) * 2;
+  const unsigned char* vg = p.v + (b * p.vb + kvh * p.vh) * 2;
+  const unsigned lbase = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)lds);
+  auto copy_tile = [&](int key, int buf) {  // keys [key, key + KT), those behind the last one repeat it
+    const unsigned char* kp = kg + (int64_t)key * p.kt * 2;
+    const unsigned char* vp = vg + (int64_t)key * p.vt * 2;
+#pragma unroll
+    for (int n = 0; n < PER; n++) {
+      const int slot = (wave * PER + n) * 64 + lane, row = slot / CH, c = (slot % CH) ^ turn<CH>(row);
+      const unsigned at = min(row, p.Tk - 1 - key), to = lbase + buf * 2 * TILE + (wave * PER + n) * 1024;
+      if (c * 8 < p.hd) {
+        copy16(kp, at * (unsigned)(p.kt * 2) + c * 16, to);
+        copy16(vp, at * (unsigned)(p.vt * 2) + c * 16, to + TILE);
+      }
+    }
+  };
+
+  f32x4 O[QB][NT];
+  float m[QB], l[QB];
+#pragma unroll
+  for (int x = 0; x < QB; x++) {
+    m[x] = -INFINITY, l[x] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NT; j++) O[x][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  int buf = 0;
+  if (k0 < k1) copy_tile(k0, 0);
+  for (int key = k0; key < k1; key += KT, buf ^= 1) {
+    __builtin_amdgcn_s_waitcnt(0);  // this wave's share of the tile has landed
+    __syncthreads();                // everyone's has, and the other buffer is no longer read
+    if (key + KT < k1) copy_tile(key + KT, buf ^ 1);
+    if (key + KT <= lo || key >= hi) continue;  // nothing in it for this wave
+    const unsigned char* kl = lds + buf * 2 * TILE;
+    const unsigned char* vl = kl + TILE;
+    const bool mixed = key < all_lo || key + KT > all_hi;
+
+    f32x4 s[QB][MT];
+#pragma unroll
+    for (int t = 0; t < MT; t++) {
+      u32x4 kf[NK];
+#pragma unroll
+      for (int i = 0; i < NK; i++)
+        kf[i] = *reinterpret_cast<const u32x4*>(kl + ((16 * t + r) * CH + ((4 * i + q) ^ turn<CH>(16 * t + r))) * 16);
+#pragma unroll
+      for (int x = 0; x < QB; x++) {
+        s[x][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NK; i++) s[x][t] = mma<F16>(kf[i], qf[x][i], s[x][t]);
+      }
+    }
+    u32x4 P[QB][KT / 32];
+#pragma unroll
+    for (int x = 0; x < QB; x++) {
+      // relative to the lane's first key of the tile
+      const int f = first[x] - key - 4 * q, e = last[x] - key - 4 * q;
+      const float away = BIAS ? (float)(row0 + 16 * x + r + p.Tk - p.Tq - key - 4 * q) : 0.f;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < MT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int j = 16 * t + i;
+          float v = s[x][t][i];
+          if constexpr (CAP) {
+            // cap tanh(s / cap) = cap - 2 cap / (1 + e^(2 s / cap)); scale is 2 log2(e) / cap of the scores', cap in base 2
+            v = p.cap - 2.f * p.cap * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * p.scale));
+            if constexpr (BIAS) v -= slope * fabsf(away - j);
+          } else if constexpr (BIAS) {
+            v = v * p.scale - slope * fabsf(away - j);
+          }
+          if (mixed && (j < f || j >= e)) v = -INFINITY;
+          s[x][t][i] = v;
+          mx = fmaxf(mx, v);
+        }
+      // without a cap or bias the scale (>= 0) joins the exponent's subtraction
+      constexpr bool RAW = !CAP && !BIAS;
+      mx = cols_max(mx);
+      if constexpr (RAW) mx *= p.scale;
+      const float mn = fmaxf(m[x], mx), ms = mn == -INFINITY ? 0.f : mn;
+      if (__builtin_amdgcn_ballot_w64(mn != m[x])) {
+        const float al = exp2_w(m[x] - ms);  // 0 where there was nothing yet
+        l[x] *= al;
+#pragma unroll
+        for (int j = 0; j < NT; j++) O[x][j] *= al;
+        m[x] = mn;
+      }
+#pragma unroll
+      for (int t = 0; t < MT; t++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          s[x][t][i] = exp2_w(RAW ? s[x][t][i] * p.scale - ms : s[x][t][i] - ms);
+          l[x] += s[x][t][i];
+        }
+        P[x][t >> 1][2 * (t & 1)] = pack2<F16>(s[x][t][0], s[x][t][1]);
+        P[x][t >> 1][2 * (t & 1) + 1] = pack2<F16>(s[x][t][2], s[x][t][3]);
+      }
+    }
+    // value operand of step u (32 keys), dims 16 j ..: two turned reads of four keys each
+    auto value = [&](int u, int j, int half, int ln) {
+      const int row = 32 * u + 16 * half + (ln >> 2), c = 2 * j + ((ln & 3) >> 1);  // ln >> 2 = 4 q + r / 4
+      return read_turned(vl + (row * CH + (c ^ turn<CH>(row))) * 16 + (ln & 1) * 8);
+    };
+    bool apart = false;
+    if (mixed) {
+      // A value that a query does not see must not reach it, but 0 x NaN is NaN: where a masked tile holds values that are
+      // not finite, they are left out of the product, and counted for the queries that see them.
+      unsigned bad = 0;
+      int ln = lane;
+      asm volatile("" : "+v"(ln));
+#pragma unroll
+      for (int u = 0; u < KT / 32; u++)
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+          for (int half = 0; half < 2; half++) {
+            const u32x2 w = value(u, j, half, ln);
+            bad |= not_finite<F16>(w[0]) | not_finite<F16>(w[1]);
+            if (half && j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+          }
+      apart = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+      asm volatile("" ::: "memory");  // read again below: a tile of values does not fit the registers
+    }
+    if (!apart) {
+#pragma unroll
+      for (int u = 0; u < KT / 32; u++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+          const u32x2 a = value(u, j, 0, lane), c = value(u, j, 1, lane);
+          const u32x4 vf = u32x4{a[0], a[1], c[0], c[1]};
+#pragma unroll
+          for (int x = 0; x < QB; x++) O[x][j] = mma<F16>(vf, P[x][u], O[x][j]);
+        }
+    } else {
+#pragma unroll
+      for (int ux = 0; ux < KT / 32 * QB; ux++) {
+        const int u = ux / QB, x = ux % QB;
+        int at = 32 * u + 4 * q, ln = lane;
+        asm volatile("" : "+v"(at), "+v"(ln));  // nothing of this rare path is worked out ahead of the loop and kept
+        u32x4 seen;                             // one for each key that the lane's query sees
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          const int j = key + at + 16 * (w >> 1) + 2 * (w & 1);
+          seen[w] = (j >= first[x] && j < last[x] ? ONE : 0u) | (j + 1 >= first[x] && j + 1 < last[x] ? ONE << 16 : 0u);
+        }
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+          const u32x2 a = value(u, j, 0, ln), c = value(u, j, 1, ln);
+          u32x4 clean, nan, up, down;
+#pragma unroll
+          for (int w = 0; w < 4; w++) {
+            const unsigned v = w < 2 ? a[w] : c[w - 2];
+            const unsigned odd = spread(not_finite<F16>(v)), ones = odd & (ONE * 0x10001u);
+            const unsigned is_nan = spread(fraction<F16>(v)), minus = spread(v & 0x80008000u);
+            clean[w] = v & ~odd;
+            nan[w] = ones & is_nan;
+            up[w] = ones & ~is_nan & ~minus;
+            down[w] = ones & ~is_nan & minus;
+          }
+          O[x][j] = mma<F16>(clean, P[x][u], O[x][j]);
+          auto add = [&](u32x4 which, float what) {
+            const f32x4 n = mma<F16>(which, seen, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int i = 0; i < 4; i++) O[x][j][i] += n[i] > 0.f ? what : 0.f;
+            __builtin_amdgcn_sched_barrier(0);
+          };
+          add(nan, NAN);
+          add(up, INFINITY);
+          add(down, -INFINITY);
+        }
+      }
+    }
+  }
+
+#pragma unroll
+  for (int x = 0; x < QB; x++) {
+    const int row = row0 + 16 * x + r;
+    const float sum = cols_sum(l[x]), inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (row >= p.Tq) continue;
+    unsigned char* o = p.out + (((size_t)b * p.Tq + row) * p.H + h) * p.hd * 2;
+#pragma unroll
+    for (int j = 0; j < NT; j++)
+      if (16 * j + 4 * q < p.hd)
+        *reinterpret_cast<u32x2*>(o + (16 * j + 4 * q) * 2) =
+            u32x2{pack2<F16>(O[x][j][0] * inv, O[x][j][1] * inv), pack2<F16>(O[x][j][2] * inv, O[x][j][3] * inv)};
+  }
+}
+
+template <bool F16, int HD, int QB>
+int launch(Params p, hipStream_t s) {
+  constexpr int KT = HD == 256 ? 32 : 64, LDS = 4 * KT * HD * 2 + 2 * NW * 4;
+  p.ntile = (p.Tq + 16 * QB * NW - 1) / (16 * QB * NW);
+  const int64_t grid = (int64_t)p.ntile * p.B * p.H;
+  if (grid > 0x7fffffff) return host::fail(FA_ERR_INVALID_ARG, "fa_span_attention: too many rows for one call");
+  const bool cap = p.cap > 0.f, bias = p.slopes != nullptr;
+  void (*k)(Params) = cap ? (bias ? span_kernel<F16, HD, QB, true, true> : span_kernel<F16, HD, QB, true, false>)
+                          : (bias ? span_kernel<F16, HD, QB, false, true> : span_kernel<F16, HD, QB, false, false>);
+  const int rc = host::allow_lds(reinterpret_cast<const void*>(k), LDS, "fa_span_attention");
+  if (rc != FA_OK) return rc;
+  hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * NW), LDS, s, p);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return host::fail(FA_ERR_LAUNCH, "fa_span_attention: %s", hipGetErrorString(e));
+  return FA_OK;
+}
+
+template <bool F16>
+int launch_type(const Params& p, hipStream_t s) {
+  // Two blocks of queries a wave halve the LDS reads for each product; one where that would leave CUs without work.
+  const bool two = ((int64_t)p.Tq + 127) / 128 * p.B * p.H >= 512;
+  if (p.hd <= 64) return two ? launch<F16, 64, 2>(p, s) : launch<F16, 64, 1>(p, s);
+  if (p.hd <= 96) return two ? launch<F16, 96, 2>(p, s) : launch<F16, 96, 1>(p, s);
+  if (p.hd <= 128) return two ? launch<F16, 128, 2>(p, s) : launch<F16, 128, 1>(p, s);
+  return launch<F16, 256, 1>(p, s);
+}
+
+int run_bf16(const Params& p, hipStream_t s);
+int run_f16(const Params& p, hipStream_t s);
+
+}  // namespace attn
+}  // namespace fa

@@ -19,6 +19,7 @@
  *                            (src/pi05/binding.cpp:34-36, src/molmoact2/binding.cpp:33-34)
  *   fa_last_error ......... TORCH_CHECK on the launch status (src/pi05/binding.cpp:67)
  *   fa_device_query ....... the occupancy clamp / diagnostics of src/molmoact2/binding.cpp:65-79
+ *   fa_span_attention ..... no counterpart of its own (the attention inside openpi's forward of packed or padded prompts)
  *   fa_w4_linear,
  *   fa_kv8_* .............. no counterpart (the backbone's token by token decoding)
  *   fa_abi_version ........ no counterpart (ABI guard for the Python and C++ callers)
@@ -390,6 +391,39 @@ typedef struct fa_kv8_attn_args {
 } fa_kv8_attn_args;
 int fa_kv8_attention(const fa_kv8_attn_args* args, fa_stream_t stream);
 size_t fa_kv8_attention_workspace_bytes(int batch, int tokens, int heads, int kv_heads, int head_dim, int blocks);
+
+/* ---------------------------------------------------------------- attention over spans of keys
+ * Query i of sample b sees the keys spans[b][i][0] <= j < spans[b][i][1] (clamped to [0, keys); spans NULL: all): the
+ * documents of a packed batch, a prefix that all see with causal tokens behind it, windows, rows that see nothing (they
+ * become zero). Scores are s = q . k * scale, with softcap > 0 softcap * tanh(s / softcap), less
+ * slopes[h] * |i + keys - queries - j| (slopes [heads] fp32 or NULL). Query heads h share K/V head h / (heads / kv_heads).
+ * What a query does not see does not reach it, NaN and infinities included.
+ * q [batch][queries][heads][head_dim], k and v [batch][keys][kv_heads][head_dim], bf16 or fp16, head_dim a multiple of 8
+ * up to 256, dims contiguous, 16-byte aligned, with strides (sample, token, head) in elements, multiples of 8 (token
+ * strides of k and v at most 2^23). out [batch][queries][heads][head_dim] contiguous, of the same type, 16-byte aligned.
+ * No workspace.
+ */
+typedef struct fa_span_args {
+  int dtype;
+  const void* q;
+  long long q_stride[3];
+  const void* k;
+  long long k_stride[3];
+  const void* v;
+  long long v_stride[3];
+  const int* spans; /* [batch][queries][2] or NULL */
+  const float* slopes;
+  int batch;
+  int queries;
+  int keys;
+  int heads;
+  int kv_heads;
+  int head_dim;
+  float scale;
+  float softcap;
+  void* out;
+} fa_span_args;
+int fa_span_attention(const fa_span_args* args, fa_stream_t stream);
 
 /* ---------------------------------------------------------------- common */
 int fa_device_query(int device, fa_device_info* info);

@@ -1,0 +1,195 @@
+"""``attention.attend`` on the MI355X against attention in 64 bits (tests/span_case.py has the bound)."""
+import pytest
+import torch
+
+from flashact_amd import attention
+from tests import span_case as C
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16]
+
+
+def _qkv(gpu, b, tq, tk, h, hkv, hd, dtype, seed=0):
+    g = torch.Generator(device=gpu).manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device=gpu).to(dtype)  # noqa: E731
+    return r(b, tq, h, hd), r(b, tk, hkv, hd), r(b, tk, hkv, hd)
+
+
+def _random_spans(gpu, b, tq, tk, seed=0):
+    """Any spans: empty, reversed, past both ends, single keys."""
+    g = torch.Generator(device=gpu).manual_seed(seed)
+    a = torch.randint(-5, tk + 5, (b, tq), generator=g, device=gpu)
+    n = torch.randint(-3, tk + 8, (b, tq), generator=g, device=gpu)
+    n = torch.where(torch.rand(b, tq, generator=g, device=gpu) < 0.2, torch.randint(-1, 2, (b, tq), generator=g, device=gpu), n)
+    return torch.stack([a, a + n], -1).to(torch.int32)
+
+
+def _documents(gpu, lengths, prefix, behind=0):
+    t = lambda v: torch.tensor(v, device=gpu)  # noqa: E731
+    return attention.prefix_spans(t(lengths), t(prefix), sum(lengths) + behind)
+
+
+CASES = [
+    # b, tq, tk, heads, kv_heads, hd, spans, options
+    (1, 1, 1, 1, 1, 64, None, {}),
+    (2, 3, 70, 4, 2, 64, None, {}),
+    (1, 130, 130, 2, 1, 128, "causal", {}),
+    (2, 100, 100, 2, 2, 96, "random", {}),
+    (1, 333, 333, 4, 2, 72, "documents", dict(softcap=20.0)),
+    (1, 300, 300, 8, 1, 256, "documents", {}),
+    (2, 65, 257, 3, 3, 256, "random", dict(slopes=True)),
+    (1, 200, 129, 2, 1, 8, "random", {}),
+    (3, 77, 401, 6, 2, 104, "random", dict(softcap=5.0, slopes=True)),
+    (1, 64, 1000, 2, 2, 40, "causal", dict(slopes=True)),
+    (2, 1100, 1100, 32, 4, 64, "documents", {}),      # enough tiles for two blocks of queries a wave
+    (1, 1500, 1500, 48, 16, 128, "documents", dict(softcap=50.0)),
+    (1, 2100, 2100, 32, 8, 88, "window", dict(scale=0.5)),
+    (4, 1030, 515, 16, 4, 128, "random", dict(slopes=True)),
+]
+
+
+def _spans(gpu, kind, b, tq, tk):
+    if kind is None:
+        return None
+    if kind == "random":
+        return _random_spans(gpu, b, tq, tk, seed=tq)
+    i = torch.arange(tq, device=gpu) + tk - tq
+    if kind == "causal":
+        return torch.stack([torch.zeros_like(i), i + 1], -1).to(torch.int32)
+    if kind == "window":
+        return torch.stack([i - 129, i + 1], -1).to(torch.int32)
+    return _documents(gpu, [tq // 2 - 9, 1, tq // 3, 0], [tq // 3, 1, 0, 0], tq - (tq // 2 - 8 + tq // 3))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(str(x) for x in c[:7]))
+def test_attend(gpu, case, dtype):
+    b, tq, tk, h, hkv, hd, kind, opt = case
+    q, k, v = _qkv(gpu, b, tq, tk, h, hkv, hd, dtype, seed=tq + hd)
+    o = dict(opt)
+    if o.pop("slopes", False):
+        o["slopes"] = torch.rand(h, device=gpu) * 0.1
+    spans = _spans(gpu, kind, b, tq, tk)
+    out = attention.attend(q, k, v, spans, **o)
+    assert out.dtype == dtype and out.shape == q.shape
+    C.check(out, *C.attend(q, k, v, spans, **o))
+    assert torch.equal(out, attention.attend(q, k, v, spans, **o))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd,n,heads", [(64, 200, 2), (128, 300, 2), (256, 150, 2), (128, 1400, 48)])
+def test_what_a_query_does_not_see_does_not_reach_it(gpu, dtype, hd, n, heads):
+    """Two documents in one tile, one full of infinities and NaN; and causal rows ahead of a bad token."""
+    q, k, v = _qkv(gpu, 1, n, n, heads, heads, hd, dtype, seed=hd)
+    a = n // 2 + 3
+    spans = _documents(gpu, [a, n - a], [a, 0])
+    ref = attention.attend(q, k, v, spans)
+    k2, v2 = k.clone(), v.clone()
+    k2[0, a + 5, 0], k2[0, a + 40, 1, 3] = float("nan"), float("inf")
+    v2[0, a + 9, 0, 1], v2[0, a + 20, 1, 2], v2[0, a + 31, 1, 2] = float("nan"), float("inf"), float("-inf")
+    out = attention.attend(q, k2, v2, spans)
+    assert torch.equal(out[:, :a], ref[:, :a])
+    assert torch.equal(out[:, a:a + 5, 0], ref[:, a:a + 5, 0])
+    assert out[:, a + 5:, 0].isnan().all()
+    # without bad keys: infinities and NaN of values reach exactly the rows that see them, in their dims
+    out = attention.attend(q, k, v2, spans)
+    C.check(out, *C.attend(q, k, v2, spans))
+    assert out[:, a + 9:, 0, 1].isnan().all() and (out[:, a + 20:a + 31, 1, 2] == float("inf")).all()
+    assert out[:, a + 31:, 1, 2].isnan().all()
+
+
+def test_rows_that_see_nothing_are_zero(gpu):
+    q, k, v = _qkv(gpu, 2, 150, 60, 2, 1, 96, torch.bfloat16)
+    v[:] = float("nan")
+    for spans in (torch.zeros(150, 2), torch.full((150, 2), 60.0), torch.tensor([[50.0, 3.0]]).expand(150, 2),
+                  torch.tensor([[-9.0, 0.0]]).expand(150, 2)):
+        assert not attention.attend(q, k, v, spans.to(gpu, torch.int32)).any()
+    assert not attention.attend(q, k[:, :0], v[:, :0]).any()
+    assert attention.attend(q[:, :0], k, v).shape == (2, 0, 2, 96)
+    assert attention.attend(q[:0], k[:0], v[:0]).shape == (0, 150, 2, 96)
+
+
+def test_extreme_scores(gpu):
+    """Scores of thousands, equal and opposite: the running maximum moves with every tile; masks next to the lowest values."""
+    q, k, v = _qkv(gpu, 1, 70, 500, 2, 2, 128, torch.float16, seed=3)
+    k = (k * torch.linspace(0, 60, 500, device=gpu)[:, None, None]).half()
+    for spans in (None, _random_spans(gpu, 1, 70, 500)):
+        C.check(attention.attend(q, k, v, spans, scale=1.0), *C.attend(q, k, v, spans, scale=1.0))
+    big = torch.full_like(k, -240.0)
+    C.check(attention.attend(big[:, :70], big.neg(), v, None), *C.attend(big[:, :70], big.neg(), v, None))
+
+
+def test_views_of_one_projection(gpu):
+    """Strided views: heads of one projection, samples of a larger batch, every second token, a transposed layout."""
+    qkv = torch.randn(2, 90, 10, 128, device=gpu).bfloat16()
+    q, k, v = qkv[:, :, :6], qkv[:, :, 6:8], qkv[:, :, 8:]
+    ref = attention.attend(q.contiguous(), k.contiguous(), v.contiguous())
+    assert torch.equal(attention.attend(q, k, v), ref)
+    assert torch.equal(attention.attend(q[1:], k[1:], v[1:]), ref[1:])
+    every = attention.attend(q[:, ::2], k[:, ::2], v[:, ::2])
+    assert torch.equal(every, attention.attend(q[:, ::2].contiguous(), k[:, ::2].contiguous(), v[:, ::2].contiguous()))
+    t = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v)]  # [B][H][T][hd] behind the view
+    assert torch.equal(attention.attend(*t), ref)
+    one = k[:, :, :1].expand(2, 90, 2, 128)  # a head shared by stride 0
+    assert torch.equal(attention.attend(q, one, v), attention.attend(q, one.contiguous(), v.contiguous()))
+    out = torch.empty_like(ref)
+    assert attention.attend(q, k, v, out=out) is out and torch.equal(out, ref)
+
+
+def test_prefix_spans(gpu):
+    for dev in ("cpu", gpu):
+        t = lambda *v: torch.tensor(v, device=dev)  # noqa: E731
+        s = attention.prefix_spans(t(3, 0, 4), t(2, 0, 9), 9)
+        assert s.dtype == torch.int32
+        assert s.tolist() == [[0, 2], [0, 2], [0, 3], [3, 7], [3, 7], [3, 7], [3, 7], [0, 0], [0, 0]]
+        assert attention.prefix_spans(t(3, 4), t(0, 4), 5).tolist() == [[0, 1], [0, 2], [0, 3], [3, 5], [3, 5]]  # cut off
+        assert attention.prefix_spans(t(5)[:0], t(5)[:0], 2).tolist() == [[0, 0], [0, 0]]
+
+
+def test_streams_and_graphs(gpu):
+    q, k, v = _qkv(gpu, 1, 200, 200, 4, 2, 128, torch.bfloat16)
+    spans = _documents(gpu, [120, 80], [50, 80])
+    ref = attention.attend(q, k, v, spans)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = attention.attend(q, k, v, spans)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other, ref)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = attention.attend(q, k, v, spans)
+    for i in range(4):
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, device=gpu))
+        spans.copy_(_documents(gpu, [60 + 30 * i, 140 - 30 * i], [10 * i, 140 - 30 * i]))
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, attention.attend(q, k, v, spans))
+
+
+def test_offsets_past_32_bits(gpu):
+    """Keys and values in one tensor of more than 2^32 bytes: a token stride of 2^20 elements, 2100 tokens, bytes past 4 GiB."""
+    wide = torch.zeros(1, 2100, 1 << 20, dtype=torch.bfloat16, device=gpu)
+    k, v = wide[:, :, :128].unflatten(2, (1, 128)), wide[:, :, 128:256].unflatten(2, (1, 128))
+    k.copy_(torch.randn(1, 2100, 1, 128, device=gpu))
+    v.copy_(torch.randn(1, 2100, 1, 128, device=gpu))
+    q = torch.randn(1, 70, 2, 128, device=gpu).bfloat16()
+    assert torch.equal(attention.attend(q, k, v), attention.attend(q, k.contiguous(), v.contiguous()))
+
+
+def test_refuses_on_the_gpu(gpu):
+    q, k, v = _qkv(gpu, 2, 8, 8, 4, 2, 64, torch.bfloat16)
+    spans = torch.zeros(8, 2, dtype=torch.int32, device=gpu)
+    bad = torch.randn(2, 8, 2, 68, device=gpu).bfloat16()[..., :64]
+    for kw, err, text in (
+            (dict(k=k.half()), TypeError, "like q"), (dict(q=q.float()), TypeError, "q must be"),
+            (dict(k=bad), ValueError, "multiples of 8"), (dict(k=k.cpu()), ValueError, "same GPU"),
+            (dict(spans=spans.long()), ValueError, "int32"), (dict(spans=spans[:7]), ValueError, "spans"),
+            (dict(spans=spans.cpu()), ValueError, "spans"), (dict(slopes=torch.ones(2, device=gpu)), ValueError, "slopes"),
+            (dict(out=torch.empty(2, 8, 4, 64, device=gpu)), ValueError, "out must"),
+            (dict(softcap=-1.0), ValueError, "softcap"), (dict(scale=-0.1), ValueError, "scale"),
+            (dict(scale=float("nan")), ValueError, "scale")):
+        with pytest.raises(err, match=text):
+            attention.attend(**{"q": q, "k": k, "v": v, **kw})
