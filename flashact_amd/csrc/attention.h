@@ -32,7 +32,7 @@ struct Params {
   const int* spans;  // [B][Tq][2] or NULL: all keys
   const float* slopes;
   unsigned char* out;  // [B][Tq][H][hd]
-  int B, Tq, Tk, H, G, hd, ntile;
+  int B, Tq, Tk, H, G, hd, ntile, stages;
   float scale, cap;
 };
 
@@ -54,6 +54,12 @@ __device__ __forceinline__ void copy16(const unsigned char* base, unsigned off, 
                : "=&s"(saved)
                : "v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds))
                : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void vm_wait() {  // until at most N copies (or loads) of this wave are outstanding
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+  asm volatile("" ::: "memory");
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -90,8 +96,11 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
   constexpr int KT = HD == 256 ? 32 : 64, CH = HD / 8, NK = HD / 32, NT = HD / 16, MT = KT / 16;
   constexpr int TILE = KT * HD * 2, PER = KT * CH / (64 * NW);  // bytes of a tile of keys, copies a wave issues for it
   constexpr unsigned ONE = F16 ? 0x3c00u : 0x3f80u;
+  // 4096 for a NaN, 64 for an infinity, 1 for a negative one: the 32 keys of a step sum up without mixing
+  constexpr unsigned NANS = (F16 ? 0x6c00u : 0x4580u) * 0x10001u, UPS = (F16 ? 0x5400u : 0x4280u) * 0x10001u;
+  constexpr unsigned DOWNS = ONE * 0x10001u;
   static_assert(KT * CH % (64 * NW) == 0, "whole copies");
-  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // two buffers of {keys, values}
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // p.stages buffers of {keys, values}
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
 
@@ -140,20 +149,20 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
     all_lo = max(all_lo, __shfl_xor(all_lo, o));
     all_hi = min(all_hi, __shfl_xor(all_hi, o));
   }
-  int* ext = reinterpret_cast<int*>(lds + 4 * TILE);  // the workgroup walks over the keys of all its waves
+  int* ext = reinterpret_cast<int*>(lds + p.stages * 2 * TILE);  // the workgroup walks over the keys of all its waves
   if (lane == 0) {
     ext[2 * wave] = lo;
     ext[2 * wave + 1] = hi;
   }
   // dims behind hd are zero in LDS: the copies never write them
   if (p.hd < HD)
-    for (int i = threadIdx.x; i < 4 * TILE / 16; i += 64 * NW) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
+    for (int i = threadIdx.x; i < p.stages * 2 * TILE / 16; i += 64 * NW) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
   __syncthreads();
   int k0 = 0x7fffffff, k1 = 0;
 #pragma unroll
   for (int w = 0; w < NW; w++) k0 = min(k0, ext[2 * w]), k1 = max(k1, ext[2 * w + 1]);
-  k0 = __builtin_amdgcn_readfirstlane(k0);
   k1 = __builtin_amdgcn_readfirstlane(k1);
+  k0 = min(__builtin_amdgcn_readfirstlane(k0), k1);  // a workgroup whose queries see nothing: 0, 0
   lo = __builtin_amdgcn_readfirstlane(lo);
   hi = __builtin_amdgcn_readfirstlane(hi);
   all_lo = __builtin_amdgcn_readfirstlane(all_lo);
@@ -177,9 +186,11 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
   auto copy_tile = [&](int key, int buf) {  // keys [key, key + KT), those behind the last one repeat it
     const unsigned char* kp = kg + (int64_t)key * p.kt * 2;
     const unsigned char* vp = vg + (int64_t)key * p.vt * 2;
+    int ln = lane;
+    if (HD == 128 && QB == 2) asm volatile("" : "+v"(ln));  // worked out here each time: no registers to keep it in
 #pragma unroll
     for (int n = 0; n < PER; n++) {
-      const int slot = (wave * PER + n) * 64 + lane, row = slot / CH, c = (slot % CH) ^ turn<CH>(row);
+      const int slot = (wave * PER + n) * 64 + ln, row = slot / CH, c = (slot % CH) ^ turn<CH>(row);
       const unsigned at = min(row, p.Tk - 1 - key), to = lbase + buf * 2 * TILE + (wave * PER + n) * 1024;
       if (c * 8 < p.hd) {
         copy16(kp, at * (unsigned)(p.kt * 2) + c * 16, to);
@@ -197,15 +208,23 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
     for (int j = 0; j < NT; j++) O[x][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  int buf = 0;
-  if (k0 < k1) copy_tile(k0, 0);
-  for (int key = k0; key < k1; key += KT, buf ^= 1) {
-    __builtin_amdgcn_s_waitcnt(0);  // this wave's share of the tile has landed
-    __syncthreads();                // everyone's has, and the other buffer is no longer read
-    if (key + KT < k1) copy_tile(key + KT, buf ^ 1);
-    if (key + KT <= lo || key >= hi) continue;  // nothing in it for this wave
+  // p.stages - 1 tiles are on their way
+  const int ahead = (p.stages - 1) * KT;
+  for (int i = 0; i < p.stages - 1; i++)
+    if (k0 + i * KT < k1) copy_tile(k0 + i * KT, i);
+  int buf = 0, free = p.stages - 1;
+  for (int key = k0; key < k1; key += KT) {
+    const int later = min(p.stages - 2, (k1 - 1 - key) / KT);  // tiles behind this one that are on their way
+    if (later <= 0) vm_wait<0>();                              // this wave's share of this one has landed
+    else if (later == 1) vm_wait<2 * PER>();
+    else vm_wait<4 * PER>();
+    __syncthreads();  // everyone's has, and the tile before is no longer read
+    if (key + ahead < k1) copy_tile(key + ahead, free);
     const unsigned char* kl = lds + buf * 2 * TILE;
     const unsigned char* vl = kl + TILE;
+    free = buf;
+    buf = buf + 1 == p.stages ? 0 : buf + 1;
+    if (key + KT <= lo || key >= hi) continue;  // nothing in it for this wave
     const bool mixed = key < all_lo || key + KT > all_hi;
 
     f32x4 s[QB][MT];
@@ -319,27 +338,22 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
 #pragma unroll
         for (int j = 0; j < NT; j++) {
           const u32x2 a = value(u, j, 0, ln), c = value(u, j, 1, ln);
-          u32x4 clean, nan, up, down;
+          const u32x4 v = u32x4{a[0], a[1], c[0], c[1]};
+          u32x4 clean, odd;
 #pragma unroll
           for (int w = 0; w < 4; w++) {
-            const unsigned v = w < 2 ? a[w] : c[w - 2];
-            const unsigned odd = spread(not_finite<F16>(v)), ones = odd & (ONE * 0x10001u);
-            const unsigned is_nan = spread(fraction<F16>(v)), minus = spread(v & 0x80008000u);
-            clean[w] = v & ~odd;
-            nan[w] = ones & is_nan;
-            up[w] = ones & ~is_nan & ~minus;
-            down[w] = ones & ~is_nan & minus;
+            const unsigned not_fin = spread(not_finite<F16>(v[w])), nan = spread(fraction<F16>(v[w]));
+            clean[w] = v[w] & ~not_fin;
+            odd[w] = not_fin & ((nan & NANS) | (~nan & ((spread(v[w] & 0x80008000u) & DOWNS) | (~spread(v[w] & 0x80008000u) & UPS))));
           }
           O[x][j] = mma<F16>(clean, P[x][u], O[x][j]);
-          auto add = [&](u32x4 which, float what) {
-            const f32x4 n = mma<F16>(which, seen, f32x4{0.f, 0.f, 0.f, 0.f});
+          const f32x4 n = mma<F16>(odd, seen, f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-            for (int i = 0; i < 4; i++) O[x][j][i] += n[i] > 0.f ? what : 0.f;
-            __builtin_amdgcn_sched_barrier(0);
-          };
-          add(nan, NAN);
-          add(up, INFINITY);
-          add(down, -INFINITY);
+          for (int i = 0; i < 4; i++) {
+            const float rest = n[i] - 64.f * floorf(n[i] * (1.f / 64));
+            O[x][j][i] += n[i] >= 4096.f ? NAN : (n[i] >= 64.f ? INFINITY : 0.f) - (rest >= 1.f ? INFINITY : 0.f);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
@@ -361,14 +375,19 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
 
 template <bool F16, int HD, int QB>
 int launch(Params p, hipStream_t s) {
-  constexpr int KT = HD == 256 ? 32 : 64, LDS = 4 * KT * HD * 2 + 2 * NW * 4;
+  constexpr int KT = HD == 256 ? 32 : 64, STAGE = 2 * KT * HD * 2, MOST = 4;
   p.ntile = (p.Tq + 16 * QB * NW - 1) / (16 * QB * NW);
   const int64_t grid = (int64_t)p.ntile * p.B * p.H;
   if (grid > 0x7fffffff) return host::fail(FA_ERR_INVALID_ARG, "fa_span_attention: too many rows for one call");
   const bool cap = p.cap > 0.f, bias = p.slopes != nullptr;
   void (*k)(Params) = cap ? (bias ? span_kernel<F16, HD, QB, true, true> : span_kernel<F16, HD, QB, true, false>)
                           : (bias ? span_kernel<F16, HD, QB, false, true> : span_kernel<F16, HD, QB, false, false>);
-  const int rc = host::allow_lds(reinterpret_cast<const void*>(k), LDS, "fa_span_attention");
+  // As many tiles on their way as the LDS holds next to the workgroups that share a CU (at most two): a few workgroups
+  // have nothing else to hide the copies' latency behind.
+  const int share = grid > 256 ? 2 : 1;
+  p.stages = std::max(2, std::min({MOST, 160 * 1024 / share / (STAGE + 64)}));
+  const unsigned LDS = p.stages * STAGE + 2 * NW * 4;
+  const int rc = host::allow_lds(reinterpret_cast<const void*>(k), std::min(MOST * STAGE + 2 * NW * 4, 160 * 1024), "fa_span_attention");
   if (rc != FA_OK) return rc;
   hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * NW), LDS, s, p);
   const hipError_t e = hipGetLastError();
