@@ -37,15 +37,14 @@ struct Params {
 };
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int NW = 4;
 
-// LDS slot of chunk c (16 bytes) of row `row`: rows of CH chunks whose chunks are exchanged so that 16 rows' equal chunks
-// lie in different banks.
+// Chunk c (16 bytes) of row `row` lies in LDS slot c ^ turn of the row's CH slots: the same chunk of 16 rows (a key operand)
+// and the same pair of chunks of 8 rows (a value operand) meet in different banks.
 template <int CH>
 __device__ __forceinline__ int turn(int row) {
-  if constexpr (CH == 8) return (row >> 1) & 7;
-  else if constexpr (CH == 12) return (row >> 2) & 3;
-  else return row & 15;
+  if constexpr (CH == 8) return (row & 6) | ((row >> 3) & 1);
+  else if constexpr (CH == 12) return ((row >> 1) & 2) | ((row >> 3) & 1);
+  else return ((row & 7) << 1) | ((row >> 3) & 1);
 }
 
 __device__ __forceinline__ void copy16(const unsigned char* base, unsigned off, unsigned lds) {
@@ -56,9 +55,15 @@ __device__ __forceinline__ void copy16(const unsigned char* base, unsigned off, 
                : "memory");
 }
 
-template <int N>
-__device__ __forceinline__ void vm_wait() {  // until at most N copies (or loads) of this wave are outstanding
-  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+#define ATTN_VMCNT(n) (((n) & 15) | (((n) >> 4) << 14) | (7 << 4) | (15 << 8))
+// Waits until at most n (wave-uniform: 2, 4, 6, 8, 16, or else 0) copies or loads of this wave are outstanding.
+__device__ __forceinline__ void vm_wait(int n) {
+  if (n == 16) __builtin_amdgcn_s_waitcnt(ATTN_VMCNT(16));
+  else if (n == 8) __builtin_amdgcn_s_waitcnt(ATTN_VMCNT(8));
+  else if (n == 6) __builtin_amdgcn_s_waitcnt(ATTN_VMCNT(6));
+  else if (n == 4) __builtin_amdgcn_s_waitcnt(ATTN_VMCNT(4));
+  else if (n == 2) __builtin_amdgcn_s_waitcnt(ATTN_VMCNT(2));
+  else __builtin_amdgcn_s_waitcnt(ATTN_VMCNT(0));
   asm volatile("" ::: "memory");
 }
 
@@ -91,15 +96,15 @@ __device__ __forceinline__ unsigned fraction(unsigned x) {
 // the halves whose sign bit is set, whole
 __device__ __forceinline__ unsigned spread(unsigned sign) { return sign | (sign - (sign >> 15)); }
 
-template <bool F16, int HD, int QB, bool CAP, bool BIAS>
+template <bool F16, int HD, int QB, int NW, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
   constexpr int KT = HD == 256 ? 32 : 64, CH = HD / 8, NK = HD / 32, NT = HD / 16, MT = KT / 16;
-  constexpr int TILE = KT * HD * 2, PER = KT * CH / (64 * NW);  // bytes of a tile of keys, copies a wave issues for it
+  constexpr int TILE = KT * HD * 2, COPIES = KT * CH / 64, PER = (COPIES + NW - 1) / NW;  // bytes, copies of a tile of keys
   constexpr unsigned ONE = F16 ? 0x3c00u : 0x3f80u;
   // 4096 for a NaN, 64 for an infinity, 1 for a negative one: the 32 keys of a step sum up without mixing
   constexpr unsigned NANS = (F16 ? 0x6c00u : 0x4580u) * 0x10001u, UPS = (F16 ? 0x5400u : 0x4280u) * 0x10001u;
   constexpr unsigned DOWNS = ONE * 0x10001u;
-  static_assert(KT * CH % (64 * NW) == 0, "whole copies");
+  static_assert(KT * CH % 64 == 0, "whole copies");
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // p.stages buffers of {keys, values}
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
@@ -190,8 +195,10 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
     if (HD == 128 && QB == 2) asm volatile("" : "+v"(ln));  // worked out here each time: no registers to keep it in
 #pragma unroll
     for (int n = 0; n < PER; n++) {
-      const int slot = (wave * PER + n) * 64 + ln, row = slot / CH, c = (slot % CH) ^ turn<CH>(row);
-      const unsigned at = min(row, p.Tk - 1 - key), to = lbase + buf * 2 * TILE + (wave * PER + n) * 1024;
+      const int copy = n * NW + wave;
+      if (COPIES % NW && copy >= COPIES) break;
+      const int slot = copy * 64 + ln, row = slot / CH, c = (slot % CH) ^ turn<CH>(row);
+      const unsigned at = min(row, p.Tk - 1 - key), to = lbase + buf * 2 * TILE + copy * 1024;
       if (c * 8 < p.hd) {
         copy16(kp, at * (unsigned)(p.kt * 2) + c * 16, to);
         copy16(vp, at * (unsigned)(p.vt * 2) + c * 16, to + TILE);
@@ -209,15 +216,18 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
   }
 
   // p.stages - 1 tiles are on their way
-  const int ahead = (p.stages - 1) * KT;
+  const int ahead = (p.stages - 1) * KT, mine = (COPIES - wave + NW - 1) / NW;
   for (int i = 0; i < p.stages - 1; i++)
     if (k0 + i * KT < k1) copy_tile(k0 + i * KT, i);
+  // The queries are waited for here: left to the compiler, that wait (for everything under way) stands in the loop.
+#pragma unroll
+  for (int x = 0; x < QB; x++)
+#pragma unroll
+    for (int i = 0; i < NK; i++) asm volatile("" : "+v"(qf[x][i]));
   int buf = 0, free = p.stages - 1;
   for (int key = k0; key < k1; key += KT) {
     const int later = min(p.stages - 2, (k1 - 1 - key) / KT);  // tiles behind this one that are on their way
-    if (later <= 0) vm_wait<0>();                              // this wave's share of this one has landed
-    else if (later == 1) vm_wait<2 * PER>();
-    else vm_wait<4 * PER>();
+    vm_wait(later * 2 * mine);  // this wave's share of this one has landed
     __syncthreads();  // everyone's has, and the tile before is no longer read
     if (key + ahead < k1) copy_tile(key + ahead, free);
     const unsigned char* kl = lds + buf * 2 * TILE;
@@ -227,20 +237,42 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
     if (key + KT <= lo || key >= hi) continue;  // nothing in it for this wave
     const bool mixed = key < all_lo || key + KT > all_hi;
 
-    f32x4 s[QB][MT];
-#pragma unroll
-    for (int t = 0; t < MT; t++) {
-      u32x4 kf[NK];
+    // LDS reads are asked for a step ahead of the products that use them, and kept there (sched_barrier): left alone, the
+    // compiler saves registers by reading just before each use, and every product waits for the LDS.
+    auto key_operand = [&](int t, u32x4(&kf)[NK]) {
 #pragma unroll
       for (int i = 0; i < NK; i++)
         kf[i] = *reinterpret_cast<const u32x4*>(kl + ((16 * t + r) * CH + ((4 * i + q) ^ turn<CH>(16 * t + r))) * 16);
+    };
+    // dims 16 j .. of 32 keys from 32 u: two turned reads of four keys each (lane >> 2 = 4 q + r / 4)
+    auto value = [&](int u, int j, int ln) {
+      u32x2 w[2];
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        const int row = 32 * u + 16 * half + (ln >> 2), c = 2 * j + ((ln & 3) >> 1);
+        w[half] = read_turned(vl + (row * CH + (c ^ turn<CH>(row))) * 16 + (ln & 1) * 8);
+      }
+      return u32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
+    };
+    f32x4 s[QB][MT];
+    u32x4 kf[2][NK];
+    key_operand(0, kf[0]);
+#pragma unroll
+    for (int t = 0; t < MT; t++) {
+      if (t + 1 < MT) key_operand(t + 1, kf[(t + 1) & 1]);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int x = 0; x < QB; x++) {
         s[x][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < NK; i++) s[x][t] = mma<F16>(kf[i], qf[x][i], s[x][t]);
+        for (int i = 0; i < NK; i++) s[x][t] = mma<F16>(kf[t & 1][i], qf[x][i], s[x][t]);
       }
     }
+    constexpr int NG = HD == 128 && QB == 2 ? 2 : NT % 4 ? 3 : 4, STEPS = KT / 32 * (NT / NG);  // value operands a step
+    u32x4 vf[2][NG];
+#pragma unroll
+    for (int n = 0; n < NG; n++) vf[0][n] = value(0, n, lane);
+    __builtin_amdgcn_sched_barrier(0);
     u32x4 P[QB][KT / 32];
 #pragma unroll
     for (int x = 0; x < QB; x++) {
@@ -261,10 +293,20 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
           } else if constexpr (BIAS) {
             v = v * p.scale - slope * fabsf(away - j);
           }
-          if (mixed && (j < f || j >= e)) v = -INFINITY;
           s[x][t][i] = v;
-          mx = fmaxf(mx, v);
         }
+      if (mixed) {
+        asm volatile("");  // a branch: as selects the masks cost every tile
+#pragma unroll
+        for (int t = 0; t < MT; t++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (16 * t + i < f || 16 * t + i >= e) s[x][t][i] = -INFINITY;
+      }
+#pragma unroll
+      for (int t = 0; t < MT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[x][t][i]);
       // without a cap or bias the scale (>= 0) joins the exponent's subtraction
       constexpr bool RAW = !CAP && !BIAS;
       mx = cols_max(mx);
@@ -288,11 +330,6 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
         P[x][t >> 1][2 * (t & 1) + 1] = pack2<F16>(s[x][t][2], s[x][t][3]);
       }
     }
-    // value operand of step u (32 keys), dims 16 j ..: two turned reads of four keys each
-    auto value = [&](int u, int j, int half, int ln) {
-      const int row = 32 * u + 16 * half + (ln >> 2), c = 2 * j + ((ln & 3) >> 1);  // ln >> 2 = 4 q + r / 4
-      return read_turned(vl + (row * CH + (c ^ turn<CH>(row))) * 16 + (ln & 1) * 8);
-    };
     bool apart = false;
     if (mixed) {
       // A value that a query does not see must not reach it, but 0 x NaN is NaN: where a masked tile holds values that are
@@ -303,59 +340,56 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
 #pragma unroll
       for (int u = 0; u < KT / 32; u++)
 #pragma unroll
-        for (int j = 0; j < NT; j++)
+        for (int j = 0; j < NT; j++) {
+          const u32x4 w = value(u, j, ln);
 #pragma unroll
-          for (int half = 0; half < 2; half++) {
-            const u32x2 w = value(u, j, half, ln);
-            bad |= not_finite<F16>(w[0]) | not_finite<F16>(w[1]);
-            if (half && j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-          }
+          for (int n = 0; n < 4; n++) bad |= not_finite<F16>(w[n]);
+          if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
       apart = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
-      asm volatile("" ::: "memory");  // read again below: a tile of values does not fit the registers
     }
-    if (!apart) {
 #pragma unroll
-      for (int u = 0; u < KT / 32; u++)
+    for (int st = 0; st < STEPS; st++) {
+      const int u = st / (NT / NG), j0 = st % (NT / NG) * NG;
+      if (st + 1 < STEPS) {
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
-          const u32x2 a = value(u, j, 0, lane), c = value(u, j, 1, lane);
-          const u32x4 vf = u32x4{a[0], a[1], c[0], c[1]};
+        for (int n = 0; n < NG; n++) vf[(st + 1) & 1][n] = value((st + 1) / (NT / NG), (st + 1) % (NT / NG) * NG + n, lane);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (apart) {
 #pragma unroll
-          for (int x = 0; x < QB; x++) O[x][j] = mma<F16>(vf, P[x][u], O[x][j]);
-        }
-    } else {
-#pragma unroll
-      for (int ux = 0; ux < KT / 32 * QB; ux++) {
-        const int u = ux / QB, x = ux % QB;
-        int at = 32 * u + 4 * q, ln = lane;
-        asm volatile("" : "+v"(at), "+v"(ln));  // nothing of this rare path is worked out ahead of the loop and kept
-        u32x4 seen;                             // one for each key that the lane's query sees
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-          const int j = key + at + 16 * (w >> 1) + 2 * (w & 1);
-          seen[w] = (j >= first[x] && j < last[x] ? ONE : 0u) | (j + 1 >= first[x] && j + 1 < last[x] ? ONE << 16 : 0u);
-        }
-#pragma unroll
-        for (int j = 0; j < NT; j++) {
-          const u32x2 a = value(u, j, 0, ln), c = value(u, j, 1, ln);
-          const u32x4 v = u32x4{a[0], a[1], c[0], c[1]};
-          u32x4 clean, odd;
+        for (int x = 0; x < QB; x++) {
+          int at = 32 * u + 4 * q;
+          asm volatile("" : "+v"(at));  // nothing of this rare path is worked out ahead of the loop and kept
+          u32x4 seen;                   // one for each key that the lane's query sees
 #pragma unroll
           for (int w = 0; w < 4; w++) {
-            const unsigned not_fin = spread(not_finite<F16>(v[w])), nan = spread(fraction<F16>(v[w]));
-            clean[w] = v[w] & ~not_fin;
-            odd[w] = not_fin & ((nan & NANS) | (~nan & ((spread(v[w] & 0x80008000u) & DOWNS) | (~spread(v[w] & 0x80008000u) & UPS))));
+            const int j = key + at + 16 * (w >> 1) + 2 * (w & 1);
+            seen[w] = (j >= first[x] && j < last[x] ? ONE : 0u) | (j + 1 >= first[x] && j + 1 < last[x] ? ONE << 16 : 0u);
           }
-          O[x][j] = mma<F16>(clean, P[x][u], O[x][j]);
-          const f32x4 n = mma<F16>(odd, seen, f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const float rest = n[i] - 64.f * floorf(n[i] * (1.f / 64));
-            O[x][j][i] += n[i] >= 4096.f ? NAN : (n[i] >= 64.f ? INFINITY : 0.f) - (rest >= 1.f ? INFINITY : 0.f);
+          for (int n = 0; n < NG; n++) {
+            u32x4 odd;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+              const unsigned v = vf[st & 1][n][w], nan = spread(fraction<F16>(v)), minus = spread(v & 0x80008000u);
+              odd[w] = spread(not_finite<F16>(v)) & ((nan & NANS) | (~nan & ((minus & DOWNS) | (~minus & UPS))));
+              if (x == QB - 1) vf[st & 1][n][w] = v & ~spread(not_finite<F16>(v));
+            }
+            const f32x4 c = mma<F16>(odd, seen, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const float rest = c[i] - 64.f * floorf(c[i] * (1.f / 64));
+              O[x][j0 + n][i] += c[i] >= 4096.f ? NAN : (c[i] >= 64.f ? INFINITY : 0.f) - (rest >= 1.f ? INFINITY : 0.f);
+            }
+            __builtin_amdgcn_sched_barrier(0);
           }
-          __builtin_amdgcn_sched_barrier(0);
         }
       }
+#pragma unroll
+      for (int n = 0; n < NG; n++)
+#pragma unroll
+        for (int x = 0; x < QB; x++) O[x][j0 + n] = mma<F16>(vf[st & 1][n], P[x][u], O[x][j0 + n]);
     }
   }
 
@@ -373,23 +407,24 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
   }
 }
 
-template <bool F16, int HD, int QB>
+template <bool F16, int HD, int QB, int NW>
 int launch(Params p, hipStream_t s) {
-  constexpr int KT = HD == 256 ? 32 : 64, STAGE = 2 * KT * HD * 2, MOST = 4;
+  constexpr int KT = HD == 256 ? 32 : 64, STAGE = 2 * KT * HD * 2, EXTRA = 2 * NW * 4;
   p.ntile = (p.Tq + 16 * QB * NW - 1) / (16 * QB * NW);
   const int64_t grid = (int64_t)p.ntile * p.B * p.H;
   if (grid > 0x7fffffff) return host::fail(FA_ERR_INVALID_ARG, "fa_span_attention: too many rows for one call");
   const bool cap = p.cap > 0.f, bias = p.slopes != nullptr;
-  void (*k)(Params) = cap ? (bias ? span_kernel<F16, HD, QB, true, true> : span_kernel<F16, HD, QB, true, false>)
-                          : (bias ? span_kernel<F16, HD, QB, false, true> : span_kernel<F16, HD, QB, false, false>);
-  // As many tiles on their way as the LDS holds next to the workgroups that share a CU (at most two): a few workgroups
-  // have nothing else to hide the copies' latency behind.
-  const int share = grid > 256 ? 2 : 1;
-  p.stages = std::max(2, std::min({MOST, 160 * 1024 / share / (STAGE + 64)}));
-  const unsigned LDS = p.stages * STAGE + 2 * NW * 4;
-  const int rc = host::allow_lds(reinterpret_cast<const void*>(k), std::min(MOST * STAGE + 2 * NW * 4, 160 * 1024), "fa_span_attention");
+  void (*k)(Params) =
+      cap ? (bias ? span_kernel<F16, HD, QB, NW, true, true> : span_kernel<F16, HD, QB, NW, true, false>)
+          : (bias ? span_kernel<F16, HD, QB, NW, false, true> : span_kernel<F16, HD, QB, NW, false, false>);
+  // Up to four tiles in LDS: workgroups of eight waves have a CU to themselves, two of four waves share one.
+  constexpr int STAGES = std::min(4, (NW == 8 ? 160 : 80) * 1024 / (STAGE + EXTRA));
+  static_assert(STAGES >= 2, "LDS");
+  p.stages = STAGES;
+  const unsigned lds = STAGES * STAGE + EXTRA;
+  const int rc = host::allow_lds(reinterpret_cast<const void*>(k), lds, "fa_span_attention");
   if (rc != FA_OK) return rc;
-  hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * NW), LDS, s, p);
+  hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * NW), lds, s, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return host::fail(FA_ERR_LAUNCH, "fa_span_attention: %s", hipGetErrorString(e));
   return FA_OK;
@@ -397,12 +432,14 @@ int launch(Params p, hipStream_t s) {
 
 template <bool F16>
 int launch_type(const Params& p, hipStream_t s) {
-  // Two blocks of queries a wave halve the LDS reads for each product; one where that would leave CUs without work.
-  const bool two = ((int64_t)p.Tq + 127) / 128 * p.B * p.H >= 512;
-  if (p.hd <= 64) return two ? launch<F16, 64, 2>(p, s) : launch<F16, 64, 1>(p, s);
-  if (p.hd <= 96) return two ? launch<F16, 96, 2>(p, s) : launch<F16, 96, 1>(p, s);
-  if (p.hd <= 128) return two ? launch<F16, 128, 2>(p, s) : launch<F16, 128, 1>(p, s);
-  return launch<F16, 256, 1>(p, s);
+  // Workgroups of 128 queries either way. Many: four waves with two blocks of queries each, which halves the LDS reads for
+  // each product, two workgroups a CU. Few: eight waves with one block each, a CU to themselves, so that a lone workgroup
+  // has twice the waves and more tiles under way. 256 dims leave registers for one block only.
+  const bool many = ((int64_t)p.Tq + 127) / 128 * p.B * p.H > 256;
+  if (p.hd <= 64) return many ? launch<F16, 64, 2, 4>(p, s) : launch<F16, 64, 1, 8>(p, s);
+  if (p.hd <= 96) return many ? launch<F16, 96, 2, 4>(p, s) : launch<F16, 96, 1, 8>(p, s);
+  if (p.hd <= 128) return many ? launch<F16, 128, 2, 4>(p, s) : launch<F16, 128, 1, 8>(p, s);
+  return launch<F16, 256, 1, 8>(p, s);
 }
 
 int run_bf16(const Params& p, hipStream_t s);

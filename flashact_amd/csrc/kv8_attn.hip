@@ -187,6 +187,12 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) att
     copy(a.k, at, at_k);
     copy(a.v, at, at_v);
   }
+  // The queries are waited for here: left to the compiler, that wait (for everything under way) stands in the loop.
+#pragma unroll
+  for (int i = 0; i < KS; i++) {
+    asm volatile("" : "+v"(qf[i][0]));
+    asm volatile("" : "+v"(qf[i][1]));
+  }
   for (int blk = at; blk < nb; blk += all) {
     const bool more = blk + all < nb;
     vm_wait<NC>();  // the keys; the values are still on their way
@@ -228,10 +234,20 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) att
           v = a.cap - 2.f * a.cap * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v));
         }
         if constexpr (BIAS) v -= slope * fabsf((float)(pos - (key0 + 4 * x + i)));
-        if (mixed && key0 + 4 * x + i >= limit) v = -INFINITY;
         s[x][i] = v;
-        mx = fmaxf(mx, v);
       }
+    if (mixed) {
+      asm volatile("");  // a branch: as selects the masks cost every block
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (key0 + 4 * x + i >= limit) s[x][i] = -INFINITY;
+    }
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[x][i]);
     const float mn = fmaxf(m, cols_max(mx));
     const float ms = mn == -INFINITY ? 0.f : mn;
     if (__builtin_amdgcn_ballot_w64(mn != m)) {
