@@ -56,9 +56,10 @@ __device__ __forceinline__ void copy16(const unsigned char* base, unsigned off, 
 }
 
 #define ATTN_VMCNT(n) (((n) & 15) | (((n) >> 4) << 14) | (7 << 4) | (15 << 8))
-// Waits until at most n (wave-uniform: 2, 4, 6, 8, 16, or else 0) copies or loads of this wave are outstanding.
+// Waits until at most n (wave-uniform: 2, 4, 6, 8, 12, 16, or else 0) copies or loads of this wave are outstanding.
 __device__ __forceinline__ void vm_wait(int n) {
   if (n == 16) __builtin_amdgcn_s_waitcnt(ATTN_VMCNT(16));
+  else if (n == 12) __builtin_amdgcn_s_waitcnt(ATTN_VMCNT(12));
   else if (n == 8) __builtin_amdgcn_s_waitcnt(ATTN_VMCNT(8));
   else if (n == 6) __builtin_amdgcn_s_waitcnt(ATTN_VMCNT(6));
   else if (n == 4) __builtin_amdgcn_s_waitcnt(ATTN_VMCNT(4));
@@ -417,12 +418,13 @@ int launch(Params p, hipStream_t s) {
   void (*k)(Params) =
       cap ? (bias ? span_kernel<F16, HD, QB, NW, true, true> : span_kernel<F16, HD, QB, NW, true, false>)
           : (bias ? span_kernel<F16, HD, QB, NW, false, true> : span_kernel<F16, HD, QB, NW, false, false>);
-  // Up to four tiles in LDS: workgroups of eight waves have a CU to themselves, two of four waves share one.
-  constexpr int STAGES = std::min(4, (NW == 8 ? 160 : 80) * 1024 / (STAGE + EXTRA));
-  static_assert(STAGES >= 2, "LDS");
-  p.stages = STAGES;
-  const unsigned lds = STAGES * STAGE + EXTRA;
-  const int rc = host::allow_lds(reinterpret_cast<const void*>(k), lds, "fa_span_attention");
+  // Up to four tiles in LDS: a workgroup of eight waves has a CU to itself, as have those of four while there are no more
+  // than CUs; else two share one.
+  constexpr int ALONE = std::min(4, 160 * 1024 / (STAGE + EXTRA)), SHARED = std::min(4, 80 * 1024 / (STAGE + EXTRA));
+  static_assert(SHARED >= 2, "LDS");
+  p.stages = NW == 8 || grid <= 256 ? ALONE : SHARED;
+  const unsigned lds = p.stages * STAGE + EXTRA;
+  const int rc = host::allow_lds(reinterpret_cast<const void*>(k), ALONE * STAGE + EXTRA, "fa_span_attention");
   if (rc != FA_OK) return rc;
   hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * NW), lds, s, p);
   const hipError_t e = hipGetLastError();
@@ -432,14 +434,14 @@ int launch(Params p, hipStream_t s) {
 
 template <bool F16>
 int launch_type(const Params& p, hipStream_t s) {
-  // Workgroups of 128 queries either way. Many: four waves with two blocks of queries each, which halves the LDS reads for
-  // each product, two workgroups a CU. Few: eight waves with one block each, a CU to themselves, so that a lone workgroup
-  // has twice the waves and more tiles under way. 256 dims leave registers for one block only.
-  const bool many = ((int64_t)p.Tq + 127) / 128 * p.B * p.H > 256;
-  if (p.hd <= 64) return many ? launch<F16, 64, 2, 4>(p, s) : launch<F16, 64, 1, 8>(p, s);
-  if (p.hd <= 96) return many ? launch<F16, 96, 2, 4>(p, s) : launch<F16, 96, 1, 8>(p, s);
-  if (p.hd <= 128) return many ? launch<F16, 128, 2, 4>(p, s) : launch<F16, 128, 1, 8>(p, s);
-  return launch<F16, 256, 1, 8>(p, s);
+  // Few queries: workgroups of 64, one block a wave, so that every CU has one and each step is short (LDS reads bound it).
+  // Many: workgroups of 128; two blocks a wave halve the LDS reads for each product (8192 x 8192 of 16 heads of 128 dims: 631
+  // us instead of 843), while 256 dims leave registers for one block only (two, at one wave a SIMD: 2506 us instead of 1585).
+  const bool few = ((int64_t)p.Tq + 63) / 64 * p.B * p.H <= 512;
+  if (p.hd <= 64) return few ? launch<F16, 64, 1, 4>(p, s) : launch<F16, 64, 2, 4>(p, s);
+  if (p.hd <= 96) return few ? launch<F16, 96, 1, 4>(p, s) : launch<F16, 96, 2, 4>(p, s);
+  if (p.hd <= 128) return few ? launch<F16, 128, 1, 4>(p, s) : launch<F16, 128, 2, 4>(p, s);
+  return few ? launch<F16, 256, 1, 4>(p, s) : launch<F16, 256, 1, 8>(p, s);
 }
 
 int run_bf16(const Params& p, hipStream_t s);
