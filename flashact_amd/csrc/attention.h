@@ -255,19 +255,25 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
       }
       return u32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
     };
+    // One block of queries: two key operands a step, whose products do not wait for one another.
+    constexpr int KG = QB == 1 ? 2 : 1;
     f32x4 s[QB][MT];
-    u32x4 kf[2][NK];
-    key_operand(0, kf[0]);
+    u32x4 kf[2 * KG < MT ? 2 * KG : MT][NK];
 #pragma unroll
-    for (int t = 0; t < MT; t++) {
-      if (t + 1 < MT) key_operand(t + 1, kf[(t + 1) & 1]);
+    for (int t = 0; t < KG; t++) key_operand(t, kf[t]);
+#pragma unroll
+    for (int t = 0; t < MT; t += KG) {
+#pragma unroll
+      for (int n = 0; n < KG; n++)
+        if (t + KG + n < MT) key_operand(t + KG + n, kf[(t + KG + n) % (2 * KG)]);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int x = 0; x < QB; x++) {
-        s[x][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int n = 0; n < KG * QB; n++) s[n % QB][t + n / QB] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < NK; i++) s[x][t] = mma<F16>(kf[t & 1][i], qf[x][i], s[x][t]);
-      }
+      for (int i = 0; i < NK; i++)
+#pragma unroll
+        for (int n = 0; n < KG * QB; n++)
+          s[n % QB][t + n / QB] = mma<F16>(kf[(t + n / QB) % (2 * KG)][i], qf[n % QB][i], s[n % QB][t + n / QB]);
     }
     constexpr int NG = HD == 128 && QB == 2 ? 2 : NT % 4 ? 3 : 4, STEPS = KT / 32 * (NT / NG);  // value operands a step
     u32x4 vf[2][NG];
@@ -312,14 +318,16 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
       constexpr bool RAW = !CAP && !BIAS;
       mx = cols_max(mx);
       if constexpr (RAW) mx *= p.scale;
-      const float mn = fmaxf(m[x], mx), ms = mn == -INFINITY ? 0.f : mn;
-      if (__builtin_amdgcn_ballot_w64(mn != m[x])) {
-        const float al = exp2_w(m[x] - ms);  // 0 where there was nothing yet
+      // The reference that weights are taken against follows the maximum only where it is passed by more than 2^8: what
+      // counts is that no weight overflows, and most tiles leave the sums as they are.
+      if (__builtin_amdgcn_ballot_w64(mx > m[x] + 8.f)) {
+        const float mn = fmaxf(m[x], mx), al = m[x] == mn ? 1.f : exp2_w(m[x] - mn);  // 0 where there was nothing yet
         l[x] *= al;
 #pragma unroll
         for (int j = 0; j < NT; j++) O[x][j] *= al;
         m[x] = mn;
       }
+      const float ms = m[x] == -INFINITY ? 0.f : m[x];
 #pragma unroll
       for (int t = 0; t < MT; t++) {
 #pragma unroll
