@@ -3,13 +3,15 @@
 //   s_ij = q_i . k_j scale, capped to cap tanh(s / cap), less slope_h |i + Tk - Tq - j|;  o_i = sum_j softmax_j(s_ij) v_j
 //   over the keys first_i <= j < last_i; a query whose span is empty gets zeros.
 //
-// One pass over the keys with a running maximum and sum. A workgroup of four waves takes 64 QB queries of one head (16 QB a
-// wave) and walks over the tiles of KT keys between the first key that any of them sees and the last; tiles that all of
-// them see whole skip the masks. S^T = K Q^T and O^T += V^T P^T on the 16x16x32 MFMA: a lane holds one query's column, the
+// One pass over the keys with a running maximum and sum. The waves of a workgroup take 16 or 32 queries of one head each and
+// walk together over the tiles of KT keys between the first key that any of them sees and the last; tiles that all queries of
+// a wave see whole skip the masks. S^T = K Q^T and O^T += V^T P^T on the 16x16x32 MFMA: a lane holds one query's column, the
 // softmax needs two cross-lane steps, and P^T is already the second product's operand (slot 8 q + j of a 32-key step is key
 // 4 q + j of its first 16 for j < 4, key 16 + 4 q + j - 4 beyond), which the values' transposing LDS read matches.
-// Keys and values of the next tile are copied to LDS (no registers) while this one is worked on, one barrier a tile; two
-// workgroups share a CU, so one's softmax runs under the other's products.
+// Keys and values of the next tiles are copied to LDS (no registers) while this one is worked on, one barrier a tile. With
+// many queries the MFMAs are the bound, next to the LDS reads that feed them (each operand of 1 KB serves 16 or 32 queries)
+// and, capped, the three exponentials a score; with few it is one wave's chain of a tile's steps, about 3000 cycles.
+// 8191 tokens of 16 heads of 128 dims over 4 K/V heads, causal behind a tenth, capped: 389 us, 714 TFLOP/s.
 //
 // Rounding: the scores' products are exact in fp32, softmax and sums are fp32, P is rounded to the values' type for the
 // second product (bf16 values have a range that fp16 weights times fp16 values would not hold), the result once.
@@ -97,8 +99,8 @@ __device__ __forceinline__ unsigned fraction(unsigned x) {
 // the halves whose sign bit is set, whole
 __device__ __forceinline__ unsigned spread(unsigned sign) { return sign | (sign - (sign >> 15)); }
 
-template <bool F16, int HD, int QB, int NW, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
+template <bool F16, int HD, int QB, int NW, int SP, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
   constexpr int KT = HD == 256 ? 32 : 64, CH = HD / 8, NK = HD / 32, NT = HD / 16, MT = KT / 16;
   constexpr int TILE = KT * HD * 2, COPIES = KT * CH / 64, PER = (COPIES + NW - 1) / NW;  // bytes, copies of a tile of keys
   constexpr unsigned ONE = F16 ? 0x3c00u : 0x3f80u;
@@ -107,7 +109,8 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
   constexpr unsigned DOWNS = ONE * 0x10001u;
   static_assert(KT * CH % 64 == 0, "whole copies");
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // p.stages buffers of {keys, values}
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = SP > 1 ? all_waves % NW : all_waves, grp = SP > 1 ? all_waves / NW : 0;  // grp: whose tiles of keys
   const int r = lane & 15, q = lane >> 4;
 
   // Heads (of all samples) go to XCDs in runs where they divide evenly, so that those that share keys meet in one L2;
@@ -155,14 +158,14 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
     all_lo = max(all_lo, __shfl_xor(all_lo, o));
     all_hi = min(all_hi, __shfl_xor(all_hi, o));
   }
-  int* ext = reinterpret_cast<int*>(lds + p.stages * 2 * TILE);  // the workgroup walks over the keys of all its waves
-  if (lane == 0) {
+  int* ext = reinterpret_cast<int*>(lds + p.stages * SP * 2 * TILE);  // the workgroup walks over the keys of all its waves
+  if (lane == 0 && grp == 0) {
     ext[2 * wave] = lo;
     ext[2 * wave + 1] = hi;
   }
   // dims behind hd are zero in LDS: the copies never write them
   if (p.hd < HD)
-    for (int i = threadIdx.x; i < p.stages * 2 * TILE / 16; i += 64 * NW) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
+    for (int i = threadIdx.x; i < p.stages * SP * 2 * TILE / 16; i += 64 * NW * SP) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
   __syncthreads();
   int k0 = 0x7fffffff, k1 = 0;
 #pragma unroll
@@ -189,20 +192,37 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
   const unsigned char* kg = p.k + (b * p.kb + kvh * p.kh) * 2;
   const unsigned char* vg = p.v + (b * p.vb + kvh * p.vh) * 2;
   const unsigned lbase = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)lds);
-  auto copy_tile = [&](int key, int buf) {  // keys [key, key + KT), those behind the last one repeat it
+  // Keys [key, key + KT); behind the last one it is repeated, and dims behind hd are left out.
+  unsigned koff[PER], voff[PER];  // of the lane's chunks in a whole tile
+#pragma unroll
+  for (int n = 0; n < PER; n++) {
+    const int slot = (n * NW + wave) * 64 + lane, row = slot / CH, c = (slot % CH) ^ turn<CH>(row);
+    koff[n] = row * (unsigned)(p.kt * 2) + c * 16;
+    voff[n] = row * (unsigned)(p.vt * 2) + c * 16;
+  }
+  auto copy_tile = [&](int key, int buf) {
     const unsigned char* kp = kg + (int64_t)key * p.kt * 2;
     const unsigned char* vp = vg + (int64_t)key * p.vt * 2;
+    const unsigned to = lbase + (buf * SP + grp) * 2 * TILE + wave * 1024;
+    if (p.hd == HD && key + KT <= p.Tk) {
+#pragma unroll
+      for (int n = 0; n < PER; n++) {
+        if (COPIES % NW && n * NW + wave >= COPIES) break;
+        copy16(kp, koff[n], to + n * NW * 1024);
+        copy16(vp, voff[n], to + n * NW * 1024 + TILE);
+      }
+      return;
+    }
     int ln = lane;
-    if (HD == 128 && QB == 2) asm volatile("" : "+v"(ln));  // worked out here each time: no registers to keep it in
+    asm volatile("" : "+v"(ln));  // worked out here each time: no registers to keep it in
 #pragma unroll
     for (int n = 0; n < PER; n++) {
-      const int copy = n * NW + wave;
-      if (COPIES % NW && copy >= COPIES) break;
-      const int slot = copy * 64 + ln, row = slot / CH, c = (slot % CH) ^ turn<CH>(row);
-      const unsigned at = min(row, p.Tk - 1 - key), to = lbase + buf * 2 * TILE + copy * 1024;
+      if (COPIES % NW && n * NW + wave >= COPIES) break;
+      const int slot = (n * NW + wave) * 64 + ln, row = slot / CH, c = (slot % CH) ^ turn<CH>(row);
+      const unsigned at = min(row, p.Tk - 1 - key);
       if (c * 8 < p.hd) {
-        copy16(kp, at * (unsigned)(p.kt * 2) + c * 16, to);
-        copy16(vp, at * (unsigned)(p.vt * 2) + c * 16, to + TILE);
+        copy16(kp, at * (unsigned)(p.kt * 2) + c * 16, to + n * NW * 1024);
+        copy16(vp, at * (unsigned)(p.vt * 2) + c * 16, to + n * NW * 1024 + TILE);
       }
     }
   };
@@ -217,21 +237,23 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
   }
 
   // p.stages - 1 tiles are on their way
-  const int ahead = (p.stages - 1) * KT, mine = (COPIES - wave + NW - 1) / NW;
+  constexpr int STEP = KT * SP;
+  const int ahead = (p.stages - 1) * STEP, mine = (COPIES - wave + NW - 1) / NW;
   for (int i = 0; i < p.stages - 1; i++)
-    if (k0 + i * KT < k1) copy_tile(k0 + i * KT, i);
+    if (k0 + i * STEP + grp * KT < k1) copy_tile(k0 + i * STEP + grp * KT, i);
   // The queries are waited for here: left to the compiler, that wait (for everything under way) stands in the loop.
 #pragma unroll
   for (int x = 0; x < QB; x++)
 #pragma unroll
     for (int i = 0; i < NK; i++) asm volatile("" : "+v"(qf[x][i]));
   int buf = 0, free = p.stages - 1;
-  for (int key = k0; key < k1; key += KT) {
-    const int later = min(p.stages - 2, (k1 - 1 - key) / KT);  // tiles behind this one that are on their way
+  for (int step = k0; step < k1; step += STEP) {
+    const int key = step + grp * KT;
+    const int later = min(p.stages - 2, max(k1 - 1 - key, 0) / STEP);  // tiles behind this one that are on their way
     vm_wait(later * 2 * mine);  // this wave's share of this one has landed
     __syncthreads();  // everyone's has, and the tile before is no longer read
     if (key + ahead < k1) copy_tile(key + ahead, free);
-    const unsigned char* kl = lds + buf * 2 * TILE;
+    const unsigned char* kl = lds + (buf * SP + grp) * 2 * TILE;
     const unsigned char* vl = kl + TILE;
     free = buf;
     buf = buf + 1 == p.stages ? 0 : buf + 1;
@@ -402,6 +424,24 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
     }
   }
 
+  if constexpr (SP > 1) {  // the second group hands its sums, lane by lane, to the first
+    static_assert(QB == 1 && SP == 2, "one block of queries, two groups");
+    __syncthreads();
+    float* o = reinterpret_cast<float*>(lds) + (wave * (NT * 4 + 2)) * 64;
+    if (grp == 1) {
+#pragma unroll
+      for (int j = 0; j < NT; j++) *reinterpret_cast<f32x4*>(o + (j * 64 + lane) * 4) = O[0][j];
+      o[NT * 256 + lane] = m[0];
+      o[NT * 256 + 64 + lane] = l[0];
+    }
+    __syncthreads();
+    if (grp == 1) return;
+    const float m1 = o[NT * 256 + lane], l1 = o[NT * 256 + 64 + lane], mm = fmaxf(m[0], m1);
+    const float f0 = m[0] == -INFINITY ? 0.f : exp2_w(m[0] - mm), f1 = m1 == -INFINITY ? 0.f : exp2_w(m1 - mm);
+    l[0] = l[0] * f0 + l1 * f1;
+#pragma unroll
+    for (int j = 0; j < NT; j++) O[0][j] = O[0][j] * f0 + f1 * *reinterpret_cast<const f32x4*>(o + (j * 64 + lane) * 4);
+  }
 #pragma unroll
   for (int x = 0; x < QB; x++) {
     const int row = row0 + 16 * x + r;
@@ -416,40 +456,48 @@ __global__ void __launch_bounds__(64 * NW, 2) span_kernel(Params p) {
   }
 }
 
-template <bool F16, int HD, int QB, int NW>
+template <bool F16, int HD, int QB, int NW, int SP>
 int launch(Params p, hipStream_t s) {
-  constexpr int KT = HD == 256 ? 32 : 64, STAGE = 2 * KT * HD * 2, EXTRA = 2 * NW * 4;
+  constexpr int KT = HD == 256 ? 32 : 64, STAGE = SP * 2 * KT * HD * 2, EXTRA = 2 * NW * 4;
   p.ntile = (p.Tq + 16 * QB * NW - 1) / (16 * QB * NW);
   const int64_t grid = (int64_t)p.ntile * p.B * p.H;
   if (grid > 0x7fffffff) return host::fail(FA_ERR_INVALID_ARG, "fa_span_attention: too many rows for one call");
   const bool cap = p.cap > 0.f, bias = p.slopes != nullptr;
   void (*k)(Params) =
-      cap ? (bias ? span_kernel<F16, HD, QB, NW, true, true> : span_kernel<F16, HD, QB, NW, true, false>)
-          : (bias ? span_kernel<F16, HD, QB, NW, false, true> : span_kernel<F16, HD, QB, NW, false, false>);
-  // Up to four tiles in LDS: a workgroup of eight waves has a CU to itself, as have those of four while there are no more
-  // than CUs; else two share one.
-  constexpr int ALONE = std::min(4, 160 * 1024 / (STAGE + EXTRA)), SHARED = std::min(4, 80 * 1024 / (STAGE + EXTRA));
-  static_assert(SHARED >= 2, "LDS");
-  p.stages = NW == 8 || grid <= 256 ? ALONE : SHARED;
-  const unsigned lds = p.stages * STAGE + EXTRA;
-  const int rc = host::allow_lds(reinterpret_cast<const void*>(k), ALONE * STAGE + EXTRA, "fa_span_attention");
+      cap ? (bias ? span_kernel<F16, HD, QB, NW, SP, true, true> : span_kernel<F16, HD, QB, NW, SP, true, false>)
+          : (bias ? span_kernel<F16, HD, QB, NW, SP, false, true> : span_kernel<F16, HD, QB, NW, SP, false, false>);
+  // Up to four tiles in LDS: a workgroup of eight waves has a CU to itself, two of four waves share one.
+  constexpr int STAGES = std::min(4, (NW * SP == 8 ? 160 : 80) * 1024 / (STAGE + EXTRA));
+  static_assert(STAGES >= 2, "LDS");
+  p.stages = STAGES;
+  const unsigned lds = STAGES * STAGE + EXTRA;
+  const int rc = host::allow_lds(reinterpret_cast<const void*>(k), lds, "fa_span_attention");
   if (rc != FA_OK) return rc;
-  hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * NW), lds, s, p);
+  hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * NW * SP), lds, s, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return host::fail(FA_ERR_LAUNCH, "fa_span_attention: %s", hipGetErrorString(e));
   return FA_OK;
 }
 
+template <bool F16, int HD>
+int launch_dims(const Params& p, hipStream_t s) {
+  // Few queries: workgroups of 64, one block of queries a wave. While every one can have a CU to itself (and with 256 dims
+  // up to twice that: packed prompts of 2604 tokens 85 -> 63 us) two groups of waves share the keys, as a lone wave a SIMD
+  // waits for itself most of the time (2048 tokens of 8 heads of 128 dims 44 -> 33 us; 384 workgroups of 96 dims, though,
+  // 40 -> 45). Many: workgroups of 128; two blocks a wave halve the LDS reads for each product (8192 tokens of 16 heads of
+  // 128 dims: 631 us instead of 843), while 256 dims leave registers for one (two, at one wave a SIMD: 2506 instead of 1585).
+  const int64_t small = ((int64_t)p.Tq + 63) / 64 * p.B * p.H;
+  if (small <= (HD == 256 ? 512 : 256)) return launch<F16, HD, 1, 4, 2>(p, s);
+  if constexpr (HD == 256) return launch<F16, HD, 1, 8, 1>(p, s);
+  else return small <= 512 ? launch<F16, HD, 1, 4, 1>(p, s) : launch<F16, HD, 2, 4, 1>(p, s);
+}
+
 template <bool F16>
 int launch_type(const Params& p, hipStream_t s) {
-  // Few queries: workgroups of 64, one block a wave, so that every CU has one and each step is short (LDS reads bound it).
-  // Many: workgroups of 128; two blocks a wave halve the LDS reads for each product (8192 x 8192 of 16 heads of 128 dims: 631
-  // us instead of 843), while 256 dims leave registers for one block only (two, at one wave a SIMD: 2506 us instead of 1585).
-  const bool few = ((int64_t)p.Tq + 63) / 64 * p.B * p.H <= 512;
-  if (p.hd <= 64) return few ? launch<F16, 64, 1, 4>(p, s) : launch<F16, 64, 2, 4>(p, s);
-  if (p.hd <= 96) return few ? launch<F16, 96, 1, 4>(p, s) : launch<F16, 96, 2, 4>(p, s);
-  if (p.hd <= 128) return few ? launch<F16, 128, 1, 4>(p, s) : launch<F16, 128, 2, 4>(p, s);
-  return few ? launch<F16, 256, 1, 4>(p, s) : launch<F16, 256, 1, 8>(p, s);
+  if (p.hd <= 64) return launch_dims<F16, 64>(p, s);
+  if (p.hd <= 96) return launch_dims<F16, 96>(p, s);
+  if (p.hd <= 128) return launch_dims<F16, 128>(p, s);
+  return launch_dims<F16, 256>(p, s);
 }
 
 int run_bf16(const Params& p, hipStream_t s);
