@@ -7,6 +7,11 @@ cooperative launch (C ABI ``fa_pi05_prefill``) that writes the RoPE'd keys into 
 [0, Lp) and the transposed values into vtcache columns [0, Lp) of every layer, so the caches go
 straight to ``pi05.launch`` with no copy in between.
 
+``prefill_packed`` and ``extend`` run the same backbone where that launch does not reach: prompts of different lengths packed
+one behind the other, with tokens that are causal behind a prefix that all see, and further tokens one by one (or a few)
+behind what is cached. They keep keys and values in 8 bits (``kv8``), from where ``kv8.load`` fills the denoise loop's caches;
+``extend`` reads the weights in 4 bits (``w4``).
+
 Backbone shape: D = 2048, 8 query heads / 1 K/V head of 256, F = 16384 (GeLU-tanh gate), RMSNorm
 eps 1e-6 scaled by (1 + w), RoPE base 10000 at positions 0..Lp-1, no mask inside the prefix.
 """
@@ -16,9 +21,9 @@ import ctypes
 
 import torch
 
-from . import _lib, pi05
+from . import _lib, attention, kv8, pi05, w4
 
-D, F, HD = 2048, 16384, 256
+D, F, HD, H = 2048, 16384, 256, 8
 
 
 def pack_backbone(wq, wk, wv, wo, wg, wu, wd) -> dict:
@@ -26,6 +31,12 @@ def pack_backbone(wq, wk, wv, wo, wg, wu, wd) -> dict:
     RoPE pairs adjacent, gate/up rows interleaved): {"wqkv", "wo", "wgu", "wdn"}."""
     p = pi05.pack_weights(wq, wk, wv, wo, wg, wu, wd)
     return {"wqkv": p["w1"], "wo": p["wo"], "wgu": p["w2"], "wdn": p["w3"]}
+
+
+def pack_backbone_w4(packed: dict, group: int = 32) -> list:
+    """``pack_backbone`` buffers -> per layer {"wqkv", "wo", "wgu", "wdn"} in 4 bits (``w4.quantize``), for ``extend``."""
+    return [{k: w4.quantize(packed[k][l], group) for k in ("wqkv", "wo", "wgu", "wdn")}
+            for l in range(int(packed["wqkv"].shape[0]))]
 
 
 def rope_table(Lp: int, device=None):
@@ -125,3 +136,105 @@ def prefill(packed: dict, ln_in, ln_post, x, kcache, vtcache, rope_cos=None, rop
     _lib.check(L.fa_pi05_prefill(ctypes.byref(a), ctypes.c_void_p(stream)), "fa_pi05_prefill")
     if check_status:
         pi05.raise_on_status(wsp, torch.cuda.current_stream(dev), what="fa_pi05_prefill")
+
+
+# ---------------------------------------------------------------- packed prompts, further tokens
+def _norm(x, ln):
+    return torch.nn.functional.rms_norm(x, (D,), 1.0 + ln, 1e-6).to(torch.bfloat16)
+
+
+def _rope(pos, device):
+    """cos, sin [..][128] of the positions' angles (the table of ``rope_table``, at any positions)."""
+    inv = 1.0 / (10000.0 ** (torch.arange(0, HD, 2, dtype=torch.float32, device=device) / HD))
+    a = pos.float()[..., None] * inv
+    return a.cos()[..., None, :], a.sin()[..., None, :]
+
+
+def _qkv(y, rope):
+    """Rows [..][2560] of the packed projection (RoPE pairs adjacent) -> q [..][8][256], k and v [..][1][256], q and k turned
+    and in split halves."""
+    cos, sin = rope
+    qk = y[..., :9 * HD].unflatten(-1, (9, HD // 2, 2)).float()
+    a, b = qk[..., 0], qk[..., 1]
+    qk = torch.cat([a * cos - b * sin, b * cos + a * sin], -1).to(y.dtype)
+    return qk[..., :H, :], qk[..., H:, :], y[..., 9 * HD:].unflatten(-1, (1, HD))
+
+
+def _check_backbone(ln_in, ln_post, layers, x, caches):
+    if x.dtype is not torch.float32 or ln_in.dtype is not torch.float32 or ln_post.dtype is not torch.float32:
+        raise TypeError("x, ln_in and ln_post must be float32")
+    if x.shape[-1] != D or ln_in.shape != (layers, D) or ln_post.shape != (layers, D):
+        raise ValueError(f"shapes: x {tuple(x.shape)}, ln_in {tuple(ln_in.shape)}, ln_post {tuple(ln_post.shape)}: need "
+                         f"[..][{D}] and [{layers}][{D}]")
+    if len(caches) != layers or any(c["v"].shape[1] != 1 or c["v"].shape[3] != HD for c in caches):
+        raise ValueError(f"caches must be {layers} layers of kv8.make_caches with one K/V head of {HD}")
+
+
+def prefill_packed(packed: dict, ln_in, ln_post, x, lengths, caches: list, prefix=None) -> torch.Tensor:
+    """Runs the backbone over prompts of different lengths, packed one behind the other, into empty 8-bit caches.
+
+    packed: ``pack_backbone`` output. x [T][2048] fp32: the hidden states entering layer 0 of prompt 0, then of prompt 1, and
+    so on; lengths: their tokens (whole numbers, on the host; their sum is at most T, rows behind it are padding). prefix:
+    how many of its first tokens all of a prompt sees, the others being causal (None: all, no mask in a prompt). caches:
+    ``kv8.make_caches(layers, len(lengths), ...)``, filled from token 0 on. Returns the hidden states leaving the last
+    layer [T][2048] fp32 (undefined in padding). The matrix products are the library's; the attention and the cache are
+    ``attention.attend`` and ``kv8.store``.
+    """
+    layers = int(packed["wqkv"].shape[0])
+    _check_backbone(ln_in, ln_post, layers, x, caches)
+    lengths = [int(n) for n in lengths]
+    prefix = lengths if prefix is None else [int(n) for n in prefix]
+    if x.dim() != 2 or min(lengths, default=0) < 0 or sum(lengths) > x.shape[0] or len(prefix) != len(lengths):
+        raise ValueError(f"x {tuple(x.shape)} must be [T][{D}] with T >= the sum of lengths {lengths}, and prefix {prefix} "
+                         "as long as lengths")
+    cap = caches[0]["v"].shape[2] * kv8.BLOCK
+    if caches[0]["v"].shape[0] != len(lengths) or max(lengths, default=0) > cap:
+        raise ValueError(f"caches of {caches[0]['v'].shape[0]} samples x {cap} tokens do not hold prompts of {lengths}")
+    for k in ("wqkv", "wo", "wgu", "wdn"):
+        if packed[k].dtype is not torch.bfloat16:
+            raise TypeError(f"packed[{k!r}] must be bfloat16")
+    dev, T = x.device, x.shape[0]
+    t = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    spans = attention.prefix_spans(t(lengths), t(prefix), T)
+    rope = _rope(torch.arange(T, device=dev) - spans[:, 0], dev)
+    zero, at = t([0]), [sum(lengths[:i]) for i in range(len(lengths))]
+    for l in range(layers):
+        q, k, v = _qkv(_norm(x, ln_in[l]) @ packed["wqkv"][l].t(), rope)
+        for b, n in enumerate(lengths):
+            if n:
+                kv8.store({name: c[b:b + 1] for name, c in caches[l].items()}, k[None, at[b]:at[b] + n],
+                          v[None, at[b]:at[b] + n], zero)
+        o = attention.attend(q[None], k[None], v[None], spans)
+        x = x + (o.view(T, H * HD) @ packed["wo"][l].t()).float()
+        y = (_norm(x, ln_post[l]) @ packed["wgu"][l].t()).unflatten(-1, (F, 2)).float()
+        h = (torch.nn.functional.gelu(y[..., 0], approximate="tanh") * y[..., 1]).to(torch.bfloat16)
+        x = x + (h @ packed["wdn"][l].t()).float()
+    return x
+
+
+def extend(weights: list, ln_in, ln_post, x, caches: list, lens, count=None) -> torch.Tensor:
+    """Runs the backbone over T further tokens of each sample behind its cached ones (answers token by token: T = 1).
+
+    weights: ``pack_backbone_w4`` output. x [B][T][2048] fp32: the hidden states entering layer 0, B T <= 64. caches as
+    ``prefill_packed`` leaves them; lens int32 [B] on the GPU: tokens cached so far, the positions of the new ones follow
+    them; count int32 [B]: how many of the T are real (None: all). The tokens' keys and values are appended (the caller's
+    lens grow by T or count), each token sees all cached ones and the new ones up to itself. Returns the hidden states
+    leaving the last layer [B][T][2048] fp32 (undefined behind count). Nothing synchronises, and a captured graph serves
+    every length.
+    """
+    _check_backbone(ln_in, ln_post, len(weights), x, caches)
+    if x.dim() != 3 or x.shape[0] != caches[0]["v"].shape[0] or x.shape[0] * x.shape[1] > w4.MAX_ROWS:
+        raise ValueError(f"x must be [B={caches[0]['v'].shape[0]}][T][{D}] with B T <= {w4.MAX_ROWS}, got {tuple(x.shape)}")
+    B, T = int(x.shape[0]), int(x.shape[1])
+    dev = x.device
+    rope = _rope(lens[:, None] + torch.arange(T, device=dev), dev)
+    after = lens + (T if count is None else count)
+    x = x.reshape(B * T, D)
+    for l, w in enumerate(weights):
+        q, k, v = _qkv(w4.linear(_norm(x, ln_in[l]), w["wqkv"]).view(B, T, -1), rope)
+        kv8.store(caches[l], k, v, lens, count)
+        o = kv8.attend(q, caches[l], after, count=count)
+        x = w4.linear(o.view(B * T, H * HD), w["wo"], residual=x)
+        h = w4.linear(_norm(x, ln_post[l]), w["wgu"], gate="gelu")
+        x = w4.linear(h, w["wdn"], residual=x)
+    return x.view(B, T, D)
