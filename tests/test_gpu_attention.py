@@ -147,27 +147,6 @@ def test_prefix_spans(gpu):
         assert attention.prefix_spans(t(5)[:0], t(5)[:0], 2).tolist() == [[0, 0], [0, 0]]
 
 
-def test_streams_and_graphs(gpu):
-    q, k, v = _qkv(gpu, 1, 200, 200, 4, 2, 128, torch.bfloat16)
-    spans = _documents(gpu, [120, 80], [50, 80])
-    ref = attention.attend(q, k, v, spans)
-    side = torch.cuda.Stream()
-    side.wait_stream(torch.cuda.current_stream())
-    with torch.cuda.stream(side):
-        other = attention.attend(q, k, v, spans)
-    torch.cuda.current_stream().wait_stream(side)
-    assert torch.equal(other, ref)
-    g = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(g):
-        y = attention.attend(q, k, v, spans)
-    for i in range(4):
-        for x in (q, k, v):
-            x.copy_(torch.randn(x.shape, device=gpu))
-        spans.copy_(_documents(gpu, [60 + 30 * i, 140 - 30 * i], [10 * i, 140 - 30 * i]))
-        g.replay()
-        torch.cuda.synchronize()
-        assert torch.equal(y, attention.attend(q, k, v, spans))
-
 
 def test_offsets_past_32_bits(gpu):
     """Keys and values in one tensor of more than 2^32 bytes: a token stride of 2^20 elements, 2100 tokens, bytes past 4 GiB."""

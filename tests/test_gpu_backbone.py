@@ -158,28 +158,6 @@ def test_answers_behind_packed_prompts(gpu):
     assert lens.tolist() == [r.held for r in refs]
 
 
-def test_extend_in_a_graph(gpu):
-    """One captured step answers token after token: its replays equal the eager steps on a copy of the cache."""
-    _, _, w4s, ln = _weights(gpu, seed=1)
-    caches = [kv8.make_caches(NL, 3, 64, device=gpu) for _ in range(2)]
-    lens, x = _ints(gpu, 0, 5, 29), torch.randn(3, 1, 2048, device=gpu)
-    side = torch.cuda.Stream()
-    side.wait_stream(torch.cuda.current_stream())
-    with torch.cuda.stream(side):  # warm-up on a third cache: library handles are made outside the capture
-        prefill.extend(w4s, *ln, x, kv8.make_caches(NL, 3, 64, device=gpu), lens)
-    torch.cuda.current_stream().wait_stream(side)
-    g = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(g):
-        y = prefill.extend(w4s, *ln, x, caches[0], lens)
-    for _ in range(5):
-        x.copy_(torch.randn(3, 1, 2048, device=gpu))
-        g.replay()
-        torch.cuda.synchronize()
-        assert torch.equal(y, prefill.extend(w4s, *ln, x, caches[1], lens))
-        for a, b in zip(*caches):
-            assert all(torch.equal(a[n], b[n]) for n in a)
-        lens += 1
-
 
 def test_the_action_expert_reads_what_was_answered(gpu):
     """Prompt, answer, then the denoise loop on the cache's values: the same actions as from rows rounded by hand."""

@@ -201,7 +201,8 @@ def test_attend_over_scales_that_differ_widely(gpu):
         C.check(out, ref, bound)
 
 
-def test_attend_views_streams_and_graphs(gpu):
+
+def test_attend_views(gpu):
     cache = _filled(gpu, 2, 600, 2, 128, seed=6)
     qkv = torch.randn(2, 3, 12, 128, device=gpu).bfloat16()
     q, lens = qkv[:, :, 2:10], _ints(gpu, 600, 217)
@@ -209,29 +210,6 @@ def test_attend_views_streams_and_graphs(gpu):
     assert torch.equal(kv8.attend(q, cache, lens), ref)
     out = torch.empty_like(ref)
     assert kv8.attend(q, cache, lens, out=out) is out and torch.equal(out, ref)
-    side = torch.cuda.Stream()
-    side.wait_stream(torch.cuda.current_stream())
-    with torch.cuda.stream(side):
-        other = kv8.attend(q, cache, lens)
-    torch.cuda.current_stream().wait_stream(side)
-    assert torch.equal(other, ref)
-    # a captured step: store a token, attend, the length grows between replays
-    k, v = (torch.randn(2, 1, 2, 128, device=gpu).bfloat16() for _ in range(2))
-    start, qs = _ints(gpu, 300, 217), q[:, :1].contiguous()
-    copies = [{n: t.clone() for n, t in cache.items()} for _ in range(2)]
-    g = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(g):
-        kv8.store(copies[0], k, v, start)
-        y = kv8.attend(qs, copies[0], start + 1)
-    for i in range(5):
-        k.copy_(torch.randn(2, 1, 2, 128, device=gpu))
-        qs.copy_(torch.randn(2, 1, 8, 128, device=gpu))
-        g.replay()
-        torch.cuda.synchronize()
-        kv8.store(copies[1], k, v, start)
-        assert torch.equal(y, kv8.attend(qs, copies[1], start + 1))
-        assert all(torch.equal(copies[0][n], copies[1][n]) for n in cache)
-        start += 1
 
 
 def test_long_cache_past_32_bit_offsets(gpu):
