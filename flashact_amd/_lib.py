@@ -198,3 +198,23 @@ def run_on(index: int, fn, args, what: str) -> None:
             rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
     if rc != FA_OK:
         check(rc, what)
+
+
+def strides3(t) -> tuple:
+    """Strides of a tensor's first three dimensions; those of size one, which are never stepped, as 0."""
+    n, s = t.shape, t.stride()
+    return (s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
+
+
+def overlap(a, b) -> bool:
+    """Whether two tensors' memory ranges meet."""
+    def ends(t):
+        at = t.data_ptr()
+        if not t.numel():
+            return at, at
+        low = sum(s * (n - 1) for s, n in zip(t.stride(), t.shape) if s < 0)
+        high = sum(s * (n - 1) for s, n in zip(t.stride(), t.shape) if s > 0)
+        return at + low * t.element_size(), at + (high + 1) * t.element_size()
+    a0, a1 = ends(a)
+    b0, b1 = ends(b)
+    return a0 < b1 and b0 < a1

@@ -63,10 +63,11 @@ def attend(q, k, v, spans=None, *, scale=None, softcap: float = 0.0, slopes=None
     if k.shape[0] != b or k.shape[3] != hd or hkv < 1 or h < 1 or h % hkv or hd < 8 or hd % 8 or hd > 256:
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)}: need equal B and hd (a multiple of 8 up to 256), and H "
                          "a multiple of Hkv")
-    strides = q.stride(), k.stride(), v.stride()
+    strides = _lib.strides3(q), _lib.strides3(k), _lib.strides3(v)
     for s, x in zip(strides, (q, k, v)):
-        if s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 or x.data_ptr() % 16:
-            raise ValueError(f"q, k and v must have contiguous dims and strides that are multiples of 8, 16-byte aligned, got {s}")
+        if x.stride(3) != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 or x.data_ptr() % 16:
+            raise ValueError("q, k and v must have contiguous dims and strides that are multiples of 8, 16-byte aligned, got "
+                             f"{x.stride()}")
     scale = hd ** -0.5 if scale is None else float(scale)
     softcap = float(softcap)
     if not 0.0 <= softcap < float("inf") or not 0.0 <= scale < float("inf"):
@@ -87,8 +88,10 @@ def attend(q, k, v, spans=None, *, scale=None, softcap: float = 0.0, slopes=None
         out = q.new_empty((b, tq, h, hd))
     elif out.dtype is not t or out.shape != q.shape or not out.is_contiguous() or out.get_device() != index or out.data_ptr() % 16:
         raise ValueError(f"out must be contiguous, 16-byte aligned {t} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
-    a = _lib.SpanArgs(_lib.DTYPES[t], q.data_ptr(), _S3(*strides[0][:3]), k.data_ptr(), _S3(*strides[1][:3]), v.data_ptr(),
-                      _S3(*strides[2][:3]), None if spans is None else spans.data_ptr(),
+    elif _lib.overlap(out, k) or _lib.overlap(out, v):
+        raise ValueError("out must not share memory with k or v")
+    a = _lib.SpanArgs(_lib.DTYPES[t], q.data_ptr(), _S3(*strides[0]), k.data_ptr(), _S3(*strides[1]), v.data_ptr(),
+                      _S3(*strides[2]), None if spans is None else spans.data_ptr(),
                       None if slopes is None else slopes.data_ptr(), b, tq, tk, h, hkv, hd,
                       scale, softcap, out.data_ptr())
     _lib.run_on(index, _lib.lib().fa_span_attention, a, "fa_span_attention")

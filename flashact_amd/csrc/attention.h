@@ -35,7 +35,8 @@ struct Params {
   const float* slopes;
   unsigned char* out;  // [B][Tq][H][hd]
   int B, Tq, Tk, H, G, hd, ntile, stages;
-  float scale, cap;
+  // base 2: scale log2(e); capped, 2 log2(e) scale / cap for tanh_far, scale / cap for tanh_near, and cap log2(e)
+  float scale, over, cap;
 };
 
 constexpr float LOG2E = 1.4426950408889634f;
@@ -308,22 +309,34 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
       // relative to the lane's first key of the tile
       const int f = first[x] - key - 4 * q, e = last[x] - key - 4 * q;
       const float away = BIAS ? (float)(row0 + 16 * x + r + p.Tk - p.Tq - key - 4 * q) : 0.f;
-      float mx = -INFINITY;
+      // s becomes the score in units of `post`: as it is, capped the tanh, with a bias its base-2 logarithm's worth whole
+      const float post = BIAS ? 1.f : CAP ? p.cap : p.scale;
+      if constexpr (CAP) {
+        float most = 0.f;
 #pragma unroll
-      for (int t = 0; t < MT; t++)
+        for (int t = 0; t < MT; t++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int j = 16 * t + i;
-          float v = s[x][t][i];
-          if constexpr (CAP) {
-            // cap tanh(s / cap) = cap - 2 cap / (1 + e^(2 s / cap)); scale is 2 log2(e) / cap of the scores', cap in base 2
-            v = p.cap - 2.f * p.cap * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * p.scale));
-            if constexpr (BIAS) v -= slope * fabsf(away - j);
-          } else if constexpr (BIAS) {
-            v = v * p.scale - slope * fabsf(away - j);
-          }
-          s[x][t][i] = v;
+          for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(s[x][t][i]));
+        if (__builtin_amdgcn_ballot_w64(most * p.over > kTanhNear) == 0) {
+#pragma unroll
+          for (int t = 0; t < MT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[x][t][i] = tanh_near(s[x][t][i] * p.over);
+        } else {
+#pragma unroll
+          for (int t = 0; t < MT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[x][t][i] = tanh_far(s[x][t][i] * p.scale);
         }
+      }
+      if constexpr (BIAS) {
+        const float unit = CAP ? p.cap : p.scale;
+#pragma unroll
+        for (int t = 0; t < MT; t++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) s[x][t][i] = s[x][t][i] * unit - slope * fabsf(away - (16 * t + i));
+      }
+      float mx = -INFINITY;
       if (mixed) {
         asm volatile("");  // a branch: as selects the masks cost every tile
 #pragma unroll
@@ -336,10 +349,7 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
       for (int t = 0; t < MT; t++)
 #pragma unroll
         for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[x][t][i]);
-      // without a cap or bias the scale (>= 0) joins the exponent's subtraction
-      constexpr bool RAW = !CAP && !BIAS;
-      mx = cols_max(mx);
-      if constexpr (RAW) mx *= p.scale;
+      mx = cols_max(mx) * post;  // post >= 0
       // The reference that weights are taken against follows the maximum only where it is passed by more than 2^8: what
       // counts is that no weight overflows, and most tiles leave the sums as they are.
       if (__builtin_amdgcn_ballot_w64(mx > m[x] + 8.f)) {
@@ -354,7 +364,7 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
       for (int t = 0; t < MT; t++) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          s[x][t][i] = exp2_w(RAW ? s[x][t][i] * p.scale - ms : s[x][t][i] - ms);
+          s[x][t][i] = exp2_w(s[x][t][i] * post - ms);
           l[x] += s[x][t][i];
         }
         P[x][t >> 1][2 * (t & 1)] = pack2<F16>(s[x][t][0], s[x][t][1]);

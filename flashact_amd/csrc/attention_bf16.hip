@@ -33,8 +33,6 @@ extern "C" int fa_span_attention(const fa_span_args* a, fa_stream_t stream) {
   // a tile's rows are addressed with 32-bit offsets
   if (a->k_stride[1] < 0 || a->v_stride[1] < 0 || a->k_stride[1] > (1 << 23) || a->v_stride[1] > (1 << 23))
     return host::fail(FA_ERR_UNSUPPORTED, "%s: token strides of k and v must be in [0, 2^23]", who);
-  int rc = host::check_gfx950(who);
-  if (rc != FA_OK) return rc;
   attn::Params p{};
   p.q = static_cast<const unsigned char*>(a->q);
   p.k = static_cast<const unsigned char*>(a->k);
@@ -45,8 +43,12 @@ extern "C" int fa_span_attention(const fa_span_args* a, fa_stream_t stream) {
   p.spans = a->spans, p.slopes = a->slopes;
   p.out = static_cast<unsigned char*>(a->out);
   p.B = a->batch, p.Tq = a->queries, p.Tk = a->keys, p.H = a->heads, p.G = a->heads / a->kv_heads, p.hd = a->head_dim;
-  // in base 2: s log2(e); capped, the exponent 2 log2(e) s / cap of the tanh, and cap log2(e)
   p.scale = a->softcap > 0.f ? 2.f * attn::LOG2E * a->scale / a->softcap : a->scale * attn::LOG2E;
+  p.over = a->softcap > 0.f ? a->scale / a->softcap : 0.f;
   p.cap = a->softcap * attn::LOG2E;
+  if (!(p.scale < INFINITY) || !(p.cap < INFINITY))
+    return host::fail(FA_ERR_INVALID_ARG, "%s: scale=%g over softcap=%g leaves the fp32 range", who, a->scale, a->softcap);
+  const int rc = host::check_gfx950(who);
+  if (rc != FA_OK) return rc;
   return a->dtype == FA_DTYPE_F16 ? attn::run_f16(p, (hipStream_t)stream) : attn::run_bf16(p, (hipStream_t)stream);
 }

@@ -247,6 +247,18 @@ __device__ __forceinline__ float silu(float x) {
   return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
 }
 
+// tanh(x) of an attention score's cap, in two forms. Near zero the odd Taylor series up to x^9 (|x| <= kTanhNear: the next term
+// is 2^-22 of x); else 1 - 2 / (1 + e^2x) with e = 2 log2(e) x given, two instructions of about 1 ulp each: an error of 2^-23
+// absolute, which a large cap would multiply where x is small, so a tile takes the series if all its scores allow it.
+constexpr float kTanhNear = 0.35f;
+__device__ __forceinline__ float tanh_near(float x) {
+  const float u = x * x;
+  return x * (1.f + u * (-1.f / 3 + u * (2.f / 15 + u * (-17.f / 315 + u * (62.f / 2835)))));
+}
+__device__ __forceinline__ float tanh_far(float e) {
+  return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(e));
+}
+
 // 2^x as the bare v_exp_f32, for softmax weights and their rescale factors: a result below 2^-126
 // comes out as zero or a flushed value instead of an exact denormal (exp2f adds a range fix-up of
 // four more instructions per call for that case). Weights that small vanish against the row sum.

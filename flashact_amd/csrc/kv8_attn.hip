@@ -40,7 +40,7 @@ struct AttnArgs {
   unsigned char* out;
   float* part;  // [sample][head][row tile][split] {O[16][hd], m[16], l[16]}
   int B, T, H, G, nblk, RT, S, least, causal;
-  float scale, cap;
+  float scale, over, cap;  // base 2: scale log2(e); capped, scale / cap and cap log2(e)
 };
 
 // The row tile's share of what its sample has cached.
@@ -221,21 +221,34 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) att
     }
     // scores in base 2
     const int key0 = blk * BT + 8 * q;
-    const float f = ksc * a.scale;
     const bool mixed = blk * BT + BT > lo;
-    float mx = -INFINITY;
+    if constexpr (CAP) {
+      float most = 0.f;
 #pragma unroll
-    for (int x = 0; x < 2; x++)
+      for (int x = 0; x < 2; x++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        float v = s[x][i] * f;
-        if constexpr (CAP) {
-          // cap tanh(v / cap) = cap - 2 cap / (1 + e^(2 v / cap)); scale and cap are passed so that v is 2 log2(e) q.k / cap
-          v = a.cap - 2.f * a.cap * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v));
+        for (int i = 0; i < 4; i++) {
+          s[x][i] *= ksc * a.over;
+          most = fmaxf(most, fabsf(s[x][i]));
         }
-        if constexpr (BIAS) v -= slope * fabsf((float)(pos - (key0 + 4 * x + i)));
-        s[x][i] = v;
-      }
+      const bool near = __builtin_amdgcn_ballot_w64(most > kTanhNear) == 0;
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          s[x][i] = a.cap * (near ? tanh_near(s[x][i]) : tanh_far(s[x][i] * (2.f * LOG2E)));
+    } else {
+      const float f = ksc * a.scale;
+      s[0] *= f;
+      s[1] *= f;
+    }
+    float mx = -INFINITY;
+    if constexpr (BIAS) {
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[x][i] -= slope * fabsf((float)(pos - (key0 + 4 * x + i)));
+    }
     if (mixed) {
       asm volatile("");  // a branch: as selects the masks cost every block
 #pragma unroll
@@ -503,8 +516,6 @@ extern "C" int fa_kv8_attention(const fa_kv8_attn_args* a, fa_stream_t stream) {
   if (need && (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16))
     return host::fail(FA_ERR_INVALID_ARG, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, need,
                       a->workspace ? a->workspace_bytes : (size_t)0);
-  rc = host::check_gfx950(who);
-  if (rc != FA_OK) return rc;
   kv8::AttnArgs p{};
   p.q = static_cast<const unsigned char*>(a->q);
   p.qb = a->q_stride[0], p.qt = a->q_stride[1], p.qh = a->q_stride[2];
@@ -517,9 +528,13 @@ extern "C" int fa_kv8_attention(const fa_kv8_attn_args* a, fa_stream_t stream) {
   p.S = kv8::splits_for(a->batch, a->tokens, a->heads, a->kv_heads, a->head_dim, a->blocks);
   p.least = (int64_t)p.RT * p.B * p.H >= 64 ? 4 : 1;
   p.causal = a->causal;
-  // in base 2: s log2(e); capped, the exponent 2 log2(e) s / cap of the tanh, and cap log2(e)
-  p.scale = a->softcap > 0.f ? 2.f * kv8::LOG2E * a->scale / a->softcap : a->scale * kv8::LOG2E;
+  p.scale = a->scale * kv8::LOG2E;
+  p.over = a->softcap > 0.f ? a->scale / a->softcap : 0.f;
   p.cap = a->softcap * kv8::LOG2E;
+  if (!(fabsf(p.over) < INFINITY) || !(p.cap < INFINITY))
+    return host::fail(FA_ERR_INVALID_ARG, "%s: scale=%g over softcap=%g leaves the fp32 range", who, a->scale, a->softcap);
+  rc = host::check_gfx950(who);
+  if (rc != FA_OK) return rc;
   return a->dtype == FA_DTYPE_F16 ? kv8::launch_attn<true>(p, a->head_dim, (hipStream_t)stream)
                                   : kv8::launch_attn<false>(p, a->head_dim, (hipStream_t)stream);
 }

@@ -102,6 +102,8 @@ def load(cache: dict, lens, *, k=None, v=None, dtype=torch.bfloat16):
     if (k is None) != (v is None):
         raise ValueError("pass both of k and v or neither")
     fresh = k is None
+    if not fresh and any(s == 0 and n > 1 for t in (k, v) for s, n in zip(t.stride(), t.shape)):
+        raise ValueError("k and v are written: no two of their elements may be one")
     if fresh:
         if dtype not in _lib.DTYPES:
             raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
@@ -131,8 +133,8 @@ def attend(q, cache: dict, lens, *, count=None, scale=None, softcap: float = 0.0
     if q.dim() != 4 or q.shape[0] != b or q.shape[3] != hd or q.shape[2] < 1 or q.shape[2] % h:
         raise ValueError(f"q must be [{b}][tokens][a multiple of {h}][{hd}], got {tuple(q.shape)}")
     tokens, heads = q.shape[1], q.shape[2]
-    sb, st, sh, sd = q.stride()
-    if sd != 1 or sb % 8 or st % 8 or sh % 8 or q.data_ptr() % 16:
+    sb, st, sh = _lib.strides3(q)
+    if q.stride(3) != 1 or sb % 8 or st % 8 or sh % 8 or q.data_ptr() % 16:
         raise ValueError(f"q must have contiguous dims and strides that are multiples of 8, 16-byte aligned, got {q.stride()}")
     softcap = float(softcap)
     if not 0.0 <= softcap < float("inf"):

@@ -71,7 +71,7 @@ def _args(**kw):
     (dict(dtype=3), 1, "dtype"), (dict(batch=-1), 1, "batch=-1"), (dict(keys=-1), 1, "keys=-1"),
     (dict(heads=5), 1, "heads=5"), (dict(kv_heads=0), 1, "kv_heads=0"), (dict(head_dim=260), 1, "head_dim=260"),
     (dict(head_dim=12), 1, "head_dim=12"), (dict(softcap=-1.0), 1, "softcap"), (dict(scale=float("nan")), 1, "scale"),
-    (dict(scale=-1.0), 1, "scale"), (dict(v=None), 1, "NULL"), (dict(k=FAKE + 8), 1, "16-byte"),
+    (dict(scale=-1.0), 1, "scale"), (dict(scale=1.0, softcap=1e-39), 1, "fp32 range"), (dict(v=None), 1, "NULL"), (dict(k=FAKE + 8), 1, "16-byte"),
     (dict(spans=FAKE + 2), 1, "4-byte"), (dict(q_stride=(ctypes.c_longlong * 3)(0, 4, 8)), 1, "multiples of 8"),
     (dict(k_stride=(ctypes.c_longlong * 3)(0, 1 << 24, 8)), 2, "2^23"),
     (dict(v_stride=(ctypes.c_longlong * 3)(0, -8, 8)), 2, "2^23"),

@@ -120,6 +120,32 @@ def test_extreme_scores(gpu):
     C.check(attention.attend(big[:, :70], big.neg(), v, None), *C.attend(big[:, :70], big.neg(), v, None))
 
 
+@pytest.mark.parametrize("softcap", [1e-3, 0.5, 30.0, 1e4, 1e7])
+def test_caps_far_from_the_scores(gpu, softcap):
+    """Caps that leave nothing of the scores and caps that leave them as they are: a large one must not cost precision."""
+    q, k, v = _qkv(gpu, 1, 70, 300, 2, 2, 64, torch.float16, seed=11)
+    spans = _random_spans(gpu, 1, 70, 300)
+    for scale in (0.125, 4.0):  # within the near form, and past it
+        ref, bound = C.attend(q, k, v, spans, scale=scale, softcap=softcap)
+        # the tanh is off by 2^-22 of itself near zero and 2^-23 of one else, where it is 0.3 or more: 2^-21 of the score
+        plain = C.attend(q, k, v, spans, scale=scale)[1] + 2.0 ** -10 * ref.abs()
+        C.check(attention.attend(q, k, v, spans, scale=scale, softcap=softcap), ref, torch.minimum(bound, plain)
+                if softcap >= 1e4 else bound)
+
+
+def test_sizes_of_one_have_no_strides(gpu):
+    """A dimension of one element is never stepped, whatever stride its view carries; memory of its own for the output."""
+    q, k, v = (torch.randn(1, 5, 2, 64, device=gpu).bfloat16() for _ in range(3))
+    odd = [x.as_strided((1, 5, 2, 64), (3, 128, 64, 1)) for x in (q, k, v)]
+    assert torch.equal(attention.attend(*odd), attention.attend(q, k, v))
+    one = k[:, :1].as_strided((1, 1, 2, 64), (7, 9, 64, 1)), v[:, :1].as_strided((1, 1, 2, 64), (7, 9, 64, 1))
+    assert torch.equal(attention.attend(q, *one), attention.attend(q, k[:, :1], v[:, :1]))
+    ref = attention.attend(q, k, v)
+    assert attention.attend(q, k, v, out=q) is q and torch.equal(q, ref)  # each query is read before it is written
+    with pytest.raises(ValueError, match="share memory"):
+        attention.attend(q, k, v, out=k)
+
+
 def test_views_of_one_projection(gpu):
     """Strided views: heads of one projection, samples of a larger batch, every second token, a transposed layout."""
     qkv = torch.randn(2, 90, 10, 128, device=gpu).bfloat16()

@@ -212,6 +212,31 @@ def test_attend_views(gpu):
     assert kv8.attend(q, cache, lens, out=out) is out and torch.equal(out, ref)
 
 
+@pytest.mark.parametrize("softcap", [1e-3, 30.0, 1e7])
+def test_attend_caps_far_from_the_scores(gpu, softcap):
+    cache = _filled(gpu, 1, 200, 1, 64, seed=12)
+    q = torch.randn(1, 2, 4, 64, device=gpu).half()
+    kc, vc = C.rows_of(cache)
+    k, v = C.values(kc, cache["ks"]).to(gpu), C.values(vc, cache["vs"]).to(gpu)
+    for scale in (0.05, 2.0, -0.3):
+        ref, bound = C.attend(q, k, v, (200,), scale=scale, softcap=softcap)
+        plain = C.attend(q, k, v, (200,), scale=scale)[1] + 2.0 ** -10 * ref.abs()  # the tanh is off by 2^-21 of the score
+        out = kv8.attend(q, cache, _ints(gpu, 200), scale=scale, softcap=softcap)
+        C.check(out, ref, torch.minimum(bound, plain) if softcap >= 1e4 else bound)
+
+
+def test_sizes_of_one_and_shared_memory(gpu):
+    cache = _filled(gpu, 1, 64, 1, 128, seed=13)
+    q = torch.randn(1, 1, 4, 128, device=gpu).bfloat16()
+    lens = _ints(gpu, 50)
+    ref = kv8.attend(q, cache, lens)
+    assert torch.equal(kv8.attend(q.as_strided((1, 1, 4, 128), (3, 5, 128, 1)), cache, lens), ref)
+    assert kv8.attend(q, cache, lens, out=q) is q and torch.equal(q, ref)  # each query is read before it is written
+    rows = torch.zeros(1, 1, 1, 128, device=gpu).expand(1, 64, 1, 128)
+    with pytest.raises(ValueError, match="may be one"):
+        kv8.load(cache, lens, k=rows, v=rows)
+
+
 def test_long_cache_past_32_bit_offsets(gpu):
     """A cache of more than 4 GiB of codes: 9 samples of 2^20 + 64 tokens."""
     tokens = (1 << 20) + 64

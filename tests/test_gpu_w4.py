@@ -114,7 +114,7 @@ def test_values_that_are_not_numbers_stay_in_their_row(gpu):
 def test_refuses_on_the_gpu(gpu):
     w = w4.quantize(torch.randn(32, 64, device=gpu))
     x = torch.randn(2, 72, device=gpu).bfloat16()
-    y = x[:, :64].contiguous()
+    y, f32 = x[:, :64].contiguous(), torch.zeros(3, 32, device=gpu)
     for kw, err, text in (
             (dict(x=torch.randn(130, device=gpu).bfloat16()[1:65]), ValueError, "aligned"),
             (dict(x=torch.randn(64, 2, device=gpu).bfloat16().t()), ValueError, "contiguous"),
@@ -126,6 +126,8 @@ def test_refuses_on_the_gpu(gpu):
             (dict(out=torch.empty(2, 31, device=gpu)), ValueError, "out must be"),
             (dict(out=torch.empty(2, 32, device=gpu, dtype=torch.int32)), TypeError, "out must be"),
             (dict(out=torch.empty(2, 32, device=gpu), out_dtype=torch.float16), TypeError, "agree"),
+            (dict(out=y.view(-1)[:64].view(2, 32)), ValueError, "share memory"),
+            (dict(residual=f32[:2], out=f32[1:]), ValueError, "share memory"),
             (dict(out_dtype=torch.float64), TypeError, "out_dtype"),
             (dict(w={k: v.cpu() if torch.is_tensor(v) else v for k, v in w.items()}), ValueError, "same GPU"),
     ):

@@ -99,7 +99,7 @@ def _attn_args(**kw):
 @pytest.mark.parametrize("kw,text", [
     (dict(dtype=3), "dtype"), (dict(heads=7), "heads=7"), (dict(heads=0), "heads=0"), (dict(head_dim=32), "head_dim=32"),
     (dict(tokens=-1), "tokens=-1"), (dict(tokens=1 << 22), "2^24"), (dict(softcap=-1.0), "softcap"),
-    (dict(softcap=float("nan")), "softcap"), (dict(scale=float("inf")), "scale"), (dict(q=None), "NULL"),
+    (dict(softcap=float("nan")), "softcap"), (dict(scale=1.0, softcap=1e-39), "fp32 range"), (dict(scale=float("inf")), "scale"), (dict(q=None), "NULL"),
     (dict(out=FAKE + 8), "16-byte"), (dict(lens=FAKE + 2), "4-byte"), (dict(workspace=None), "workspace"),
     (dict(workspace_bytes=100), "workspace"), (dict(q_stride=(ctypes.c_longlong * 3)(1024, 1024, 100)), "q_stride"),
 ])
