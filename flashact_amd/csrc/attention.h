@@ -11,7 +11,7 @@
 // Keys and values of the next tiles are copied to LDS (no registers) while this one is worked on, one barrier a tile. With
 // many queries the MFMAs are the bound, next to the LDS reads that feed them (each operand of 1 KB serves 16 or 32 queries)
 // and, capped, the three exponentials a score; with few it is one wave's chain of a tile's steps, about 3000 cycles.
-// 8191 tokens of 16 heads of 128 dims over 4 K/V heads, causal behind a tenth, capped: 389 us, 714 TFLOP/s.
+// 8191 tokens of 16 heads of 128 dims over 4 K/V heads, causal behind a tenth, capped: 376 us, 738 TFLOP/s.
 //
 // Rounding: the scores' products are exact in fp32, softmax and sums are fp32, P is rounded to the values' type for the
 // second product (bf16 values have a range that fp16 weights times fp16 values would not hold), the result once.
@@ -290,6 +290,7 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
       for (int n = 0; n < KG; n++)
         if (t + KG + n < MT) key_operand(t + KG + n, kf[(t + KG + n) % (2 * KG)]);
       __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);  // products first: the other wave's softmax fills what they leave (397 -> 381 us)
 #pragma unroll
       for (int n = 0; n < KG * QB; n++) s[n % QB][t + n / QB] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -298,6 +299,7 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
         for (int n = 0; n < KG * QB; n++)
           s[n % QB][t + n / QB] = mma<F16>(kf[(t + n / QB) % (2 * KG)][i], qf[n % QB][i], s[n % QB][t + n / QB]);
     }
+    __builtin_amdgcn_s_setprio(0);
     constexpr int NG = HD == 128 && QB == 2 ? 2 : NT % 4 ? 3 : 4, STEPS = KT / 32 * (NT / NG);  // value operands a step
     u32x4 vf[2][NG];
 #pragma unroll
@@ -427,11 +429,13 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
           }
         }
       }
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int n = 0; n < NG; n++)
 #pragma unroll
         for (int x = 0; x < QB; x++) O[x][j0 + n] = mma<F16>(vf[st & 1][n], P[x][u], O[x][j0 + n]);
     }
+    __builtin_amdgcn_s_setprio(0);
   }
 
   if constexpr (SP > 1) {  // the second group hands its sums, lane by lane, to the first
