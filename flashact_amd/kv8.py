@@ -9,6 +9,7 @@ fp32. How many tokens of it count is the caller's, an int32 tensor on the GPU, s
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -16,7 +17,14 @@ from . import _lib
 
 BLOCK = 32
 HEAD_DIMS = (64, 96, 128, 256)
+_U8, _I32, _F32 = torch.uint8, torch.int32, torch.float32
 _S3, _S4 = ctypes.c_longlong * 3, ctypes.c_longlong * 4
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(b, tokens, heads, h, hd, nb) -> int:
+    """A function of the sizes alone."""
+    return _lib.lib().fa_kv8_attention_workspace_bytes(b, tokens, heads, h, hd, nb) if tokens else 0
 
 
 def make_caches(num_layers: int, batch: int, max_tokens: int, kv_heads: int = 1, head_dim: int = 256, device="cuda") -> list:
@@ -34,44 +42,43 @@ def make_caches(num_layers: int, batch: int, max_tokens: int, kv_heads: int = 1,
 def _cache(cache):
     """(k, v, ks, vs, batch, kv_heads, blocks, head_dim, GPU index) of a cache, checked."""
     k, v, ks, vs = cache["k"], cache["v"], cache["ks"], cache["vs"]
-    if v.dim() != 5 or v.shape[4] != BLOCK or v.shape[3] not in HEAD_DIMS:
-        raise ValueError(f"cache v must be [B][Hkv][blocks][hd in {HEAD_DIMS}][{BLOCK}], got {tuple(v.shape)}")
-    b, h, nb, hd, _ = v.shape
-    if k.shape != (b, h, nb, hd // 16, BLOCK, 16) or ks.shape != (b, h, nb) or vs.shape != (b, h, nb):
+    shape = v.shape
+    if len(shape) != 5 or shape[4] != BLOCK or shape[3] not in HEAD_DIMS:
+        raise ValueError(f"cache v must be [B][Hkv][blocks][hd in {HEAD_DIMS}][{BLOCK}], got {tuple(shape)}")
+    b, h, nb, hd, _ = shape
+    units = (b, h, nb)
+    if k.shape != (b, h, nb, hd // 16, BLOCK, 16) or ks.shape != units or vs.shape != units:
         raise ValueError(f"cache k {tuple(k.shape)}, ks {tuple(ks.shape)}, vs {tuple(vs.shape)} do not belong to v "
                          f"{tuple(v.shape)}")
-    if k.dtype is not torch.uint8 or v.dtype is not torch.uint8 or ks.dtype is not torch.float32 or vs.dtype is not torch.float32:
+    if k.dtype is not _U8 or v.dtype is not _U8 or ks.dtype is not _F32 or vs.dtype is not _F32:
         raise TypeError("cache k and v must be uint8, ks and vs float32")
     if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError("cache tensors must be contiguous")
     if not b * h * nb:
-        raise ValueError(f"the cache is empty: {tuple(v.shape)}")
-    return k, v, ks, vs, b, h, nb, hd
+        raise ValueError(f"the cache is empty: {tuple(shape)}")
+    index = v.get_device()
+    if k.get_device() != index or ks.get_device() != index or vs.get_device() != index:
+        raise ValueError("the cache's tensors must be on one GPU")
+    return k, v, ks, vs, b, h, nb, hd, index
 
 
 def _index(name, t, b, index):
-    if t.dtype is not torch.int32 or t.shape != (b,) or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous int32 [{b}], got {t.dtype} {tuple(t.shape)}")
-    if t.get_device() != index:
-        raise ValueError(f"{name} must be on the cache's GPU, got {t.device}")
+    if t.dtype is not _I32 or t.shape != (b,) or not t.is_contiguous() or t.get_device() != index:
+        raise ValueError(f"{name} must be contiguous int32 [{b}] on the cache's GPU, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _on_gpu(c, *tensors):
-    index = c[0].get_device()
-    if index < 0:
-        raise ValueError("the cache must be on a GPU")
-    for t in (*c[1:4], *tensors):
-        if t.get_device() != index:
-            raise ValueError(f"all tensors must be on the cache's GPU, got {t.device}")
-    return index
-
-
-def _rows(k, v, b, h, hd):
-    if k.dtype not in _lib.DTYPES or v.dtype is not k.dtype:
+def _rows(k, v, b, h, hd, index):
+    """The rows' tokens and FA_DTYPE, checked."""
+    t = _lib.DTYPES.get(k.dtype)
+    if t is None or v.dtype is not k.dtype:
         raise TypeError(f"k and v must both be bfloat16, float16 or float32, got {k.dtype} and {v.dtype}")
-    if k.dim() != 4 or k.shape[0] != b or k.shape[2] != h or k.shape[3] != hd or v.shape != k.shape:
-        raise ValueError(f"k and v must be [{b}][tokens][{h}][{hd}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    shape = k.shape
+    if len(shape) != 4 or shape[0] != b or shape[2] != h or shape[3] != hd or v.shape != shape:
+        raise ValueError(f"k and v must be [{b}][tokens][{h}][{hd}], got {tuple(shape)} and {tuple(v.shape)}")
+    if index < 0 or k.get_device() != index or v.get_device() != index:
+        raise ValueError(f"cache, k and v must be on the same GPU, got {k.device} and {v.device}")
+    return shape[1], t
 
 
 def store(cache: dict, k, v, start, count=None) -> None:
@@ -82,12 +89,11 @@ def store(cache: dict, k, v, start, count=None) -> None:
     is larger; if it grows they are recoded. Infinities and NaN are stored as NaN and set no scale. Tokens behind the
     new ones keep their codes; rows that do not fit into the cache are dropped, all of a sample whose start is negative.
     """
-    c = ck, cv, ks, vs, b, h, nb, hd = _cache(cache)
-    _rows(k, v, b, h, hd)
-    index = _on_gpu(c, k, v)
-    a = _lib.Kv8RowsArgs(_lib.DTYPES[k.dtype], k.data_ptr(), _S4(*k.stride()), v.data_ptr(), _S4(*v.stride()), ck.data_ptr(),
+    ck, cv, ks, vs, b, h, nb, hd, index = _cache(cache)
+    tokens, t = _rows(k, v, b, h, hd, index)
+    a = _lib.Kv8RowsArgs(t, k.data_ptr(), _S4(*k.stride()), v.data_ptr(), _S4(*v.stride()), ck.data_ptr(),
                          cv.data_ptr(), ks.data_ptr(), vs.data_ptr(), _index("start", start, b, index),
-                         None if count is None else _index("count", count, b, index), b, k.shape[1], h, hd, nb, 0)
+                         None if count is None else _index("count", count, b, index), b, tokens, h, hd, nb, 0)
     _lib.run_on(index, _lib.lib().fa_kv8_store, a, "fa_kv8_store")
 
 
@@ -98,7 +104,7 @@ def load(cache: dict, lens, *, k=None, v=None, dtype=torch.bfloat16):
     rows), they are written in place up to min(lens[b], T) and left as they are behind it: a view of
     ``pi05.make_caches`` caches takes a prefix to the denoise loop.
     """
-    c = ck, cv, ks, vs, b, h, nb, hd = _cache(cache)
+    ck, cv, ks, vs, b, h, nb, hd, index = _cache(cache)
     if (k is None) != (v is None):
         raise ValueError("pass both of k and v or neither")
     fresh = k is None
@@ -107,12 +113,12 @@ def load(cache: dict, lens, *, k=None, v=None, dtype=torch.bfloat16):
     if fresh:
         if dtype not in _lib.DTYPES:
             raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
-        k, v = (ck.new_empty((b, nb * BLOCK, h, hd), dtype=dtype) for _ in range(2))
-    _rows(k, v, b, h, hd)
-    index = _on_gpu(c, k, v)
-    a = _lib.Kv8RowsArgs(_lib.DTYPES[k.dtype], k.data_ptr(), _S4(*k.stride()), v.data_ptr(), _S4(*v.stride()), ck.data_ptr(),
-                         cv.data_ptr(), ks.data_ptr(), vs.data_ptr(), None, _index("lens", lens, b, index), b, k.shape[1],
-                         h, hd, nb, int(fresh))
+        shape = (b, nb * BLOCK, h, hd)
+        k, v = ck.new_empty(shape, dtype=dtype), ck.new_empty(shape, dtype=dtype)
+    tokens, t = _rows(k, v, b, h, hd, index)
+    a = _lib.Kv8RowsArgs(t, k.data_ptr(), _S4(*k.stride()), v.data_ptr(), _S4(*v.stride()), ck.data_ptr(),
+                         cv.data_ptr(), ks.data_ptr(), vs.data_ptr(), None, _index("lens", lens, b, index), b, tokens, h, hd,
+                         nb, int(fresh))
     _lib.run_on(index, _lib.lib().fa_kv8_load, a, "fa_kv8_load")
     return k, v
 
@@ -127,7 +133,7 @@ def attend(q, cache: dict, lens, *, count=None, scale=None, softcap: float = 0.0
     hd^-1/2), capped to softcap * tanh(s / softcap) where softcap > 0, less slopes[h] |i - j| where slopes (fp32 [H]) are
     given. Rows without keys become zero. Returns [B][T][H][hd] of q's type.
     """
-    c = ck, cv, ks, vs, b, h, nb, hd = _cache(cache)
+    ck, cv, ks, vs, b, h, nb, hd, index = _cache(cache)
     if q.dtype is not torch.bfloat16 and q.dtype is not torch.float16:
         raise TypeError(f"q must be bfloat16 or float16, got {q.dtype}")
     if q.dim() != 4 or q.shape[0] != b or q.shape[3] != hd or q.shape[2] < 1 or q.shape[2] % h:
@@ -139,7 +145,8 @@ def attend(q, cache: dict, lens, *, count=None, scale=None, softcap: float = 0.0
     softcap = float(softcap)
     if not 0.0 <= softcap < float("inf"):
         raise ValueError(f"softcap must be finite and >= 0, got {softcap}")
-    index = _on_gpu(c, q)
+    if index < 0 or q.get_device() != index:
+        raise ValueError(f"cache and q must be on the same GPU, got {q.device}")
     if slopes is not None and (slopes.dtype is not torch.float32 or slopes.shape != (heads,) or not slopes.is_contiguous()
                                or slopes.get_device() != index):
         raise ValueError(f"slopes must be contiguous float32 [{heads}] on q's GPU, got {slopes.dtype} {tuple(slopes.shape)}")
@@ -148,7 +155,7 @@ def attend(q, cache: dict, lens, *, count=None, scale=None, softcap: float = 0.0
     elif out.dtype is not q.dtype or out.shape != q.shape or not out.is_contiguous() or out.get_device() != index:
         raise ValueError(f"out must be contiguous {q.dtype} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
     lib = _lib.lib()
-    need = lib.fa_kv8_attention_workspace_bytes(b, tokens, heads, h, hd, nb) if tokens else 0
+    need = _workspace_bytes(b, tokens, heads, h, hd, nb)
     ws = q.new_empty(need, dtype=torch.uint8) if need else None
     a = _lib.Kv8AttnArgs(_lib.DTYPES[q.dtype], q.data_ptr(), _S3(sb, st, sh), ck.data_ptr(), cv.data_ptr(), ks.data_ptr(),
                          vs.data_ptr(), _index("lens", lens, b, index), None if count is None else _index("count", count, b, index),

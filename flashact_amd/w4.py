@@ -7,6 +7,8 @@ with one bf16 scale for each group of 32, 64 or 128 columns, 4.5 bits a weight a
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -15,6 +17,12 @@ MAX_ROWS = 64
 GROUPS = (32, 64, 128)
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 _DT = _lib.DTYPES
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(rows, n, k) -> int:
+    """A function of the sizes alone."""
+    return _lib.lib().fa_w4_workspace_bytes(rows, n, k)
 
 
 def quantize(w: torch.Tensor, group: int = 32) -> dict:
@@ -114,7 +122,7 @@ def linear(x: torch.Tensor, w: dict, *, bias=None, residual=None, gate=None, out
     if rows == 0:
         return out
     lib = _lib.lib()
-    need = lib.fa_w4_workspace_bytes(rows, n, k)
+    need = _workspace_bytes(rows, n, k)
     ws = x.new_empty(need, dtype=torch.uint8) if need else None
     a = _lib.W4Args(_DT[xt], _DT[t], x.data_ptr(), stride, codes.data_ptr(), scales.data_ptr(), rows, n, k, group,
                     None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(),
