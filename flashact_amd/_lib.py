@@ -121,7 +121,7 @@ class SpanArgs(ctypes.Structure):
         ("spans", ctypes.c_void_p), ("slopes", ctypes.c_void_p),
         ("batch", ctypes.c_int), ("queries", ctypes.c_int), ("keys", ctypes.c_int), ("heads", ctypes.c_int),
         ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
-        ("out", ctypes.c_void_p),
+        ("out", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -153,6 +153,7 @@ SYMBOLS = [
     ("fa_kv8_load", ctypes.c_int, [ctypes.POINTER(Kv8RowsArgs), ctypes.c_void_p]),
     ("fa_kv8_attention", ctypes.c_int, [ctypes.POINTER(Kv8AttnArgs), ctypes.c_void_p]),
     ("fa_kv8_attention_workspace_bytes", ctypes.c_size_t, [ctypes.c_int] * 6),
+    ("fa_span_attention_workspace_bytes", ctypes.c_size_t, [ctypes.c_int] * 5),
     ("fa_span_attention", ctypes.c_int, [ctypes.POINTER(SpanArgs), ctypes.c_void_p]),
     ("fa_device_query", ctypes.c_int, [ctypes.c_int, ctypes.POINTER(DeviceInfo)]),
     ("fa_last_error", ctypes.c_char_p, []),

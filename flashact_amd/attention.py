@@ -3,17 +3,24 @@
 The prompt's form of attention for what the prefill's fused kernel does not take: prompts of different lengths packed one
 behind the other, a prefix that all of a document sees with causal tokens behind it (the attention pattern of PaliGemma's
 prompts, where images and instruction see each other and the answer is causal), capped scores, a distance bias, rows that
-are padding. One HIP launch (C ABI ``fa_span_attention``), no workspace.
+are padding. One HIP launch (C ABI ``fa_span_attention``); a second joins the parts where few queries see many keys.
 """
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
 from . import _lib
 
 _S3 = ctypes.c_longlong * 3
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(b, tq, tk, heads, hd) -> int:
+    """A function of the sizes alone."""
+    return _lib.lib().fa_span_attention_workspace_bytes(b, tq, tk, heads, hd)
 
 
 def prefix_spans(lengths, prefix, total: int) -> torch.Tensor:
@@ -90,9 +97,11 @@ def attend(q, k, v, spans=None, *, scale=None, softcap: float = 0.0, slopes=None
         raise ValueError(f"out must be contiguous, 16-byte aligned {t} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
     elif _lib.overlap(out, k) or _lib.overlap(out, v):
         raise ValueError("out must not share memory with k or v")
+    need = _workspace_bytes(b, tq, tk, h, hd)
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
     a = _lib.SpanArgs(_lib.DTYPES[t], q.data_ptr(), _S3(*strides[0]), k.data_ptr(), _S3(*strides[1]), v.data_ptr(),
                       _S3(*strides[2]), None if spans is None else spans.data_ptr(),
                       None if slopes is None else slopes.data_ptr(), b, tq, tk, h, hkv, hd,
-                      scale, softcap, out.data_ptr())
+                      scale, softcap, out.data_ptr(), None if ws is None else ws.data_ptr(), need)
     _lib.run_on(index, _lib.lib().fa_span_attention, a, "fa_span_attention")
     return out

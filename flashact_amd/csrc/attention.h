@@ -8,6 +8,7 @@
 // a wave see whole skip the masks. S^T = K Q^T and O^T += V^T P^T on the 16x16x32 MFMA: a lane holds one query's column, the
 // softmax needs two cross-lane steps, and P^T is already the second product's operand (slot 8 q + j of a 32-key step is key
 // 4 q + j of its first 16 for j < 4, key 16 + 4 q + j - 4 beyond), which the values' transposing LDS read matches.
+// Where that leaves CUs idle, the keys are split over workgroups too, whose sums go through a workspace to join_kernel.
 // Keys and values of the next tiles are copied to LDS (no registers) while this one is worked on, one barrier a tile. With
 // many queries the MFMAs are the bound, next to the LDS reads that feed them (each operand of 1 KB serves 16 or 32 queries)
 // and, capped, the three exponentials a score; with few it is one wave's chain of a tile's steps, about 3000 cycles.
@@ -37,9 +38,15 @@ struct Params {
   int B, Tq, Tk, H, G, hd, ntile, stages;
   // base 2: scale log2(e); capped, 2 log2(e) scale / cap for tanh_far, scale / cap for tanh_near, and cap log2(e)
   float scale, over, cap;
+  // where keys are split over workgroups: into up to S parts of `least` steps or more; the parts that each (tile, sample,
+  // head) was split into, and their sums, 64 rows of {O[hd], m, l} each as a wave's lanes hold them
+  int S, least;
+  int* used;
+  float* part;
 };
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr int MAX_SPLITS = 256, LEAST = 8;
 
 // Chunk c (16 bytes) of row `row` lies in LDS slot c ^ turn of the row's CH slots: the same chunk of 16 rows (a key operand)
 // and the same pair of chunks of 8 rows (a value operand) meet in different banks.
@@ -100,6 +107,8 @@ __device__ __forceinline__ unsigned fraction(unsigned x) {
 // the halves whose sign bit is set, whole
 __device__ __forceinline__ unsigned spread(unsigned sign) { return sign | (sign - (sign >> 15)); }
 
+constexpr int part_floats(int nt) { return nt * 256 + 32; }  // of 16 rows
+
 template <bool F16, int HD, int QB, int NW, int SP, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
   constexpr int KT = HD == 256 ? 32 : 64, CH = HD / 8, NK = HD / 32, NT = HD / 16, MT = KT / 16;
@@ -116,7 +125,8 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
 
   // Heads (of all samples) go to XCDs in runs where they divide evenly, so that those that share keys meet in one L2;
   // the last tiles, which see most under a causal span, start first.
-  const unsigned heads = p.B * p.H, id = blockIdx.x;
+  const unsigned heads = p.B * p.H, units = heads * p.ntile, split = SP > 1 ? blockIdx.x / units : 0;
+  const unsigned id = SP > 1 ? blockIdx.x - split * units : blockIdx.x;
   unsigned bh, tile;
   if (heads % 8 == 0) {
     const unsigned per = heads / 8, j = id >> 3;
@@ -173,6 +183,18 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
   for (int w = 0; w < NW; w++) k0 = min(k0, ext[2 * w]), k1 = max(k1, ext[2 * w + 1]);
   k1 = __builtin_amdgcn_readfirstlane(k1);
   k0 = min(__builtin_amdgcn_readfirstlane(k0), k1);  // a workgroup whose queries see nothing: 0, 0
+  int used = 1;
+  if constexpr (SP > 1) {
+    if (p.S > 1) {
+      const int steps = (k1 - k0 + KT * SP - 1) / (KT * SP), parts = max(1, min(p.S, steps / p.least));
+      const int per = (steps + parts - 1) / parts;
+      used = steps > 0 ? (steps + per - 1) / per : 1;
+      if (split == 0 && threadIdx.x == 0) p.used[bh * p.ntile + tile] = used;
+      if ((int)split >= used) return;
+      k0 += (int)split * per * (KT * SP);
+      k1 = min(k1, k0 + per * (KT * SP));
+    }
+  }
   lo = __builtin_amdgcn_readfirstlane(lo);
   hi = __builtin_amdgcn_readfirstlane(hi);
   all_lo = __builtin_amdgcn_readfirstlane(all_lo);
@@ -355,7 +377,8 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
       // The reference that weights are taken against follows the maximum only where it is passed by more than 2^8: what
       // counts is that no weight overflows, and most tiles leave the sums as they are.
       if (__builtin_amdgcn_ballot_w64(mx > m[x] + 8.f)) {
-        const float mn = fmaxf(m[x], mx), al = m[x] == mn ? 1.f : exp2_w(m[x] - mn);  // 0 where there was nothing yet
+        // each row's by itself: another's keys do not change its roundings
+        const float mn = mx > m[x] + 8.f ? mx : m[x], al = m[x] == mn ? 1.f : exp2_w(m[x] - mn);  // 0 where there was nothing yet
         l[x] *= al;
 #pragma unroll
         for (int j = 0; j < NT; j++) O[x][j] *= al;
@@ -455,6 +478,17 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
     l[0] = l[0] * f0 + l1 * f1;
 #pragma unroll
     for (int j = 0; j < NT; j++) O[0][j] = O[0][j] * f0 + f1 * *reinterpret_cast<const f32x4*>(o + (j * 64 + lane) * 4);
+    if (used > 1) {
+      float* to = p.part + (((size_t)bh * p.ntile + tile) * p.S + split) * (NW * part_floats(NT)) + wave * part_floats(NT);
+#pragma unroll
+      for (int j = 0; j < NT; j++) *reinterpret_cast<f32x4*>(to + (j * 64 + lane) * 4) = O[0][j];
+      const float all = cols_sum(l[0]);
+      if (lane < 16) {
+        to[NT * 256 + lane] = fmaxf(m[0], m1);
+        to[NT * 256 + 16 + lane] = all;
+      }
+      return;
+    }
   }
 #pragma unroll
   for (int x = 0; x < QB; x++) {
@@ -470,11 +504,80 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
   }
 }
 
+// Joins the parts of 16 rows; a wave takes every fourth tile of 16 dims.
+template <bool F16, int HD>
+__global__ void __launch_bounds__(256) join_kernel(Params p) {
+  constexpr int NT = HD / 16, NJ = (NT + 3) / 4;
+  __shared__ float wt[MAX_SPLITS][16];
+  const unsigned unit = blockIdx.x >> 2, rows = blockIdx.x & 3, bh = unit / p.ntile, tile = unit - bh * p.ntile;
+  const int used = p.used[unit];
+  if (used == 1) return;
+  const float* from = p.part + (size_t)unit * p.S * (4 * part_floats(NT)) + rows * part_floats(NT);
+  const int stride = 4 * part_floats(NT), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, q = lane >> 4;
+  float mm = -INFINITY;
+  for (int s = 0; s < used; s++) mm = fmaxf(mm, from[(size_t)s * stride + NT * 256 + r]);
+  float sum = 0.f;
+  for (int s = 0; s < used; s++) {
+    const float m = from[(size_t)s * stride + NT * 256 + r], l = from[(size_t)s * stride + NT * 256 + 16 + r];
+    const float w = m == -INFINITY ? 0.f : exp2_w(m - mm);
+    sum += w * l;
+    if (tid < 16) wt[s][r] = w;
+  }
+  __syncthreads();
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  f32x4 O[NJ];
+#pragma unroll
+  for (int i = 0; i < NJ; i++) O[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < used; s++) {
+    const float w = wt[s][r];
+#pragma unroll
+    for (int i = 0; i < NJ; i++)
+      if (NT % 4 == 0 || 4 * i + wave < NT)
+        O[i] += w * *reinterpret_cast<const f32x4*>(from + (size_t)s * stride + ((4 * i + wave) * 64 + lane) * 4);
+  }
+  const int row = (p.ntile - 1 - (int)tile) * 64 + rows * 16 + r, b = bh / (unsigned)p.H, h = bh - b * p.H;
+  if (row >= p.Tq) return;
+  unsigned char* o = p.out + (((size_t)b * p.Tq + row) * p.H + h) * p.hd * 2;
+#pragma unroll
+  for (int i = 0; i < NJ; i++) {
+    const int d = 16 * (4 * i + wave) + 4 * q;
+    if (d < p.hd)
+      *reinterpret_cast<u32x2*>(o + d * 2) =
+          u32x2{pack2<F16>(O[i][0] * inv, O[i][1] * inv), pack2<F16>(O[i][2] * inv, O[i][3] * inv)};
+  }
+}
+
+// Parts that keys are split into, for workgroups of 64 queries with two groups of waves: the least of (rounds of
+// workgroups) x (steps of each, and two for its beginning and end), joining taken as three. A workgroup whose queries see
+// fewer keys makes fewer parts, of LEAST steps or more (packed prompts of 2604 tokens: 60 us with 8, 68 with 4, 62 with 16).
+// 64 queries over 65536 keys of 256 dims 1521 -> 107 us, one over 131072 of 128 dims 1534 -> 128, 1024 over 4096 56 -> 40;
+// of the counts 1 .. 16 the rule's was within 8 % of the best in all of 14 shapes between.
+inline int splits_for(int64_t units, int keys, int hd) {
+  const int step = hd > 128 ? 64 : 128;
+  const int64_t n = (keys + (int64_t)step - 1) / step, most = std::min<int64_t>({n / LEAST, MAX_SPLITS, 1024 / units});
+  int best = 1;
+  int64_t cost = (units + 255) / 256 * (n + 2);
+  for (int64_t S = 2; S <= most; S++) {
+    const int64_t t = (units * S + 255) / 256 * ((n + S - 1) / S + 2) + 3;
+    if (t < cost) best = (int)S, cost = t;
+  }
+  return best;
+}
+inline int64_t units_of(int batch, int queries, int heads) { return ((int64_t)queries + 63) / 64 * batch * heads; }
+// Few queries: see launch_dims.
+inline bool few(int64_t units, int hd) { return units <= (hd > 128 ? 384 : 256); }
+inline size_t workspace(int batch, int queries, int keys, int heads, int hd) {
+  const int64_t units = units_of(batch, queries, heads);
+  const int S = few(units, hd) ? splits_for(units, keys, hd) : 1, nt = (hd <= 64 ? 64 : hd <= 96 ? 96 : hd <= 128 ? 128 : 256) / 16;
+  return S == 1 ? 0 : ((size_t)units * 4 + 255) / 256 * 256 + (size_t)units * S * 4 * part_floats(nt) * 4;
+}
+
 template <bool F16, int HD, int QB, int NW, int SP>
 int launch(Params p, hipStream_t s) {
   constexpr int KT = HD == 256 ? 32 : 64, STAGE = SP * 2 * KT * HD * 2, EXTRA = 2 * NW * 4;
   p.ntile = (p.Tq + 16 * QB * NW - 1) / (16 * QB * NW);
-  const int64_t grid = (int64_t)p.ntile * p.B * p.H;
+  const int64_t units = (int64_t)p.ntile * p.B * p.H, grid = units * (SP > 1 ? p.S : 1);
   if (grid > 0x7fffffff) return host::fail(FA_ERR_INVALID_ARG, "fa_span_attention: too many rows for one call");
   const bool cap = p.cap > 0.f, bias = p.slopes != nullptr;
   void (*k)(Params) =
@@ -488,6 +591,7 @@ int launch(Params p, hipStream_t s) {
   const int rc = host::allow_lds(reinterpret_cast<const void*>(k), lds, "fa_span_attention");
   if (rc != FA_OK) return rc;
   hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * NW * SP), lds, s, p);
+  if (SP > 1 && p.S > 1) hipLaunchKernelGGL((join_kernel<F16, HD>), dim3((unsigned)(4 * units)), dim3(256), 0, s, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return host::fail(FA_ERR_LAUNCH, "fa_span_attention: %s", hipGetErrorString(e));
   return FA_OK;
@@ -495,14 +599,15 @@ int launch(Params p, hipStream_t s) {
 
 template <bool F16, int HD>
 int launch_dims(const Params& p, hipStream_t s) {
-  // Few queries: workgroups of 64, one block of queries a wave. While every one can have a CU to itself (and with 256 dims
-  // up to twice that: packed prompts of 2604 tokens 85 -> 63 us) two groups of waves share the keys, as a lone wave a SIMD
-  // waits for itself most of the time (2048 tokens of 8 heads of 128 dims 44 -> 33 us; 384 workgroups of 96 dims, though,
-  // 40 -> 45). Many: workgroups of 128; two blocks a wave halve the LDS reads for each product (8192 tokens of 16 heads of
-  // 128 dims: 631 us instead of 843), while 256 dims leave registers for one (two, at one wave a SIMD: 2506 instead of 1585).
-  const int64_t small = ((int64_t)p.Tq + 63) / 64 * p.B * p.H;
-  if (small <= (HD == 256 ? 512 : 256)) return launch<F16, HD, 1, 4, 2>(p, s);
-  if constexpr (HD == 256) return launch<F16, HD, 1, 8, 1>(p, s);
+  // Few queries: workgroups of 64 in which two groups of waves share the keys, as a lone wave a SIMD waits for itself most of
+  // the time (2048 tokens of 8 heads of 128 dims 44 -> 33 us; 384 workgroups of 96 dims, though, 40 -> 45; with 256 dims up to
+  // 384, where packed prompts of 2604 tokens gain, 86 -> 60 us, more than whole ones of 3000 lose, 140 -> 143). Many:
+  // workgroups of 128 with two blocks a wave, which halve the LDS reads for each product (8192 tokens of 16 heads of 128
+  // dims: 631 us instead of 843). 256 dims leave registers for one (two, at one wave a SIMD: 2374 instead of 1467), and two
+  // workgroups of 64 on a CU go better than one of 128 (1467 instead of 1511).
+  const int64_t small = units_of(p.B, p.Tq, p.H);
+  if (few(small, HD)) return launch<F16, HD, 1, 4, 2>(p, s);
+  if constexpr (HD == 256) return launch<F16, HD, 1, 4, 1>(p, s);
   else return small <= 512 ? launch<F16, HD, 1, 4, 1>(p, s) : launch<F16, HD, 2, 4, 1>(p, s);
 }
 

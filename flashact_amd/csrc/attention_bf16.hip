@@ -3,6 +3,11 @@
 
 int fa::attn::run_bf16(const Params& p, hipStream_t s) { return launch_type<false>(p, s); }
 
+extern "C" size_t fa_span_attention_workspace_bytes(int batch, int queries, int keys, int heads, int head_dim) {
+  if (batch < 1 || queries < 1 || keys < 1 || heads < 1 || head_dim < 1 || head_dim > 256) return 0;
+  return fa::attn::workspace(batch, queries, keys, heads, head_dim);
+}
+
 extern "C" int fa_span_attention(const fa_span_args* a, fa_stream_t stream) {
   using namespace fa;
   const char* who = "fa_span_attention";
@@ -48,6 +53,18 @@ extern "C" int fa_span_attention(const fa_span_args* a, fa_stream_t stream) {
   p.cap = a->softcap * attn::LOG2E;
   if (!(p.scale < INFINITY) || !(p.cap < INFINITY))
     return host::fail(FA_ERR_INVALID_ARG, "%s: scale=%g over softcap=%g leaves the fp32 range", who, a->scale, a->softcap);
+  const size_t need = attn::workspace(a->batch, a->queries, a->keys, a->heads, a->head_dim);
+  p.S = 1;
+  if (a->workspace && need) {
+    if (a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16)
+      return host::fail(FA_ERR_INVALID_ARG, "%s: workspace of %zu bytes at %p, needs %zu, 16-byte aligned", who,
+                        a->workspace_bytes, a->workspace, need);
+    const int64_t units = attn::units_of(a->batch, a->queries, a->heads);
+    p.S = attn::splits_for(units, a->keys, a->head_dim);
+    p.least = attn::LEAST;
+    p.used = static_cast<int*>(a->workspace);
+    p.part = reinterpret_cast<float*>(static_cast<unsigned char*>(a->workspace) + (units * 4 + 255) / 256 * 256);
+  }
   const int rc = host::check_gfx950(who);
   if (rc != FA_OK) return rc;
   return a->dtype == FA_DTYPE_F16 ? attn::run_f16(p, (hipStream_t)stream) : attn::run_bf16(p, (hipStream_t)stream);

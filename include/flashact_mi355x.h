@@ -401,7 +401,8 @@ size_t fa_kv8_attention_workspace_bytes(int batch, int tokens, int heads, int kv
  * q [batch][queries][heads][head_dim], k and v [batch][keys][kv_heads][head_dim], bf16 or fp16, head_dim a multiple of 8
  * up to 256, dims contiguous, 16-byte aligned, with strides (sample, token, head) in elements, multiples of 8 (token
  * strides of k and v at most 2^23). out [batch][queries][heads][head_dim] contiguous, of the same type, 16-byte aligned.
- * No workspace.
+ * workspace: with fa_span_attention_workspace_bytes of it (16-byte aligned, no initial contents) the keys of few queries are
+ * split over workgroups, whose sums meet in it; NULL: each workgroup of 64 queries takes all of its keys.
  */
 typedef struct fa_span_args {
   int dtype;
@@ -422,8 +423,12 @@ typedef struct fa_span_args {
   float scale;
   float softcap;
   void* out;
+  void* workspace; /* or NULL */
+  size_t workspace_bytes;
 } fa_span_args;
 int fa_span_attention(const fa_span_args* args, fa_stream_t stream);
+/* 0: a call of these sizes has no use for one */
+size_t fa_span_attention_workspace_bytes(int batch, int queries, int keys, int heads, int head_dim);
 
 /* ---------------------------------------------------------------- common */
 int fa_device_query(int device, fa_device_info* info);

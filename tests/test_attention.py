@@ -89,3 +89,17 @@ def test_c_entry_without_work_or_device():
     assert lib.fa_span_attention(ctypes.byref(_args(batch=0)), None) == 0
     if not torch.cuda.is_available():
         assert lib.fa_span_attention(ctypes.byref(_args()), None) == 3
+
+
+def test_c_entry_workspace():
+    """Few queries over many keys have a use for one, few keys or many queries none; one that is too small is refused."""
+    lib = _lib.lib()
+    need = lib.fa_span_attention_workspace_bytes
+    assert need(1, 1, 100000, 8, 128) > 0 and need(1, 64, 4096, 8, 256) > 0
+    assert need(1, 1, 100, 8, 128) == need(1, 8192, 8192, 16, 128) == need(0, 1, 1, 1, 1) == need(1, 0, 9, 1, 8) == 0
+    assert need(1, 1, 1 << 30, 1, 256) <= 80 << 20  # bounded: no more than 1024 parts of 64 rows
+    n = need(2, 8, 9000, 4, 128)
+    a = _args(keys=9000, workspace=FAKE, workspace_bytes=n - 1)
+    assert lib.fa_span_attention(ctypes.byref(a), None) == 1 and "workspace" in lib.fa_last_error().decode()
+    a = _args(keys=9000, workspace=FAKE + 8, workspace_bytes=n)
+    assert lib.fa_span_attention(ctypes.byref(a), None) == 1 and "16-byte" in lib.fa_last_error().decode()

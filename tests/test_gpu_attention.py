@@ -198,3 +198,52 @@ def test_refuses_on_the_gpu(gpu):
             (dict(scale=float("nan")), ValueError, "scale")):
         with pytest.raises(err, match=text):
             attention.attend(**{"q": q, "k": k, "v": v, **kw})
+
+
+SPLIT = [
+    # few queries over many keys: the keys are split over workgroups
+    (1, 1, 5000, 2, 1, 64, None, {}),
+    (2, 70, 3001, 4, 2, 128, "random", dict(slopes=True)),
+    (1, 64, 9001, 8, 1, 256, "causal", dict(softcap=30.0)),
+    (3, 130, 4099, 3, 3, 96, "window", {}),            # spans of few keys: one part each
+    (1, 200, 2600, 2, 2, 72, "random", dict(softcap=5.0, slopes=True)),
+    (1, 17, 40000, 16, 4, 128, "causal", {}),
+    (1, 1100, 2100, 8, 1, 256, "causal", {}),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", SPLIT, ids=lambda c: "-".join(str(x) for x in c[:7]))
+def test_few_queries_over_many_keys(gpu, monkeypatch, case, dtype):
+    b, tq, tk, h, hkv, hd, kind, opt = case
+    assert attention._workspace_bytes(b, tq, tk, h, hd) > 0
+    q, k, v = _qkv(gpu, b, tq, tk, h, hkv, hd, dtype, seed=tq + hd)
+    o = dict(opt)
+    if o.pop("slopes", False):
+        o["slopes"] = torch.rand(h, device=gpu) * 0.1
+    spans = _spans(gpu, kind, b, tq, tk)
+    ref, bound = C.attend(q, k, v, spans, **o)
+    out = attention.attend(q, k, v, spans, **o)
+    C.check(out, ref, bound)
+    assert torch.equal(out, attention.attend(q, k, v, spans, **o))
+    monkeypatch.setattr(attention, "_workspace_bytes", lambda *a: 0)  # no workspace, no parts
+    C.check(attention.attend(q, k, v, spans, **o), ref, bound)
+
+
+@pytest.mark.parametrize("hd", [64, 256])
+def test_parts_keep_what_is_not_finite(gpu, hd):
+    """A stretch of keys that is all NaN, infinities among the values of another, rows that see neither, either or both."""
+    tk = 6000
+    q, k, v = _qkv(gpu, 1, 40, tk, 2, 2, hd, torch.bfloat16, seed=hd)
+    spans = torch.tensor([[0, tk], [0, 2900], [4100, tk], [2900, 4100], [0, 5000], [7, 7]], device=gpu, dtype=torch.int32)
+    spans = spans.repeat(7, 1)[:40].contiguous()
+    ref = attention.attend(q, k, v, spans)
+    k2, v2 = k.clone(), v.clone()
+    k2[0, 2900:4100, 0] = float("nan")
+    v2[0, 5500, 1, 5], v2[0, 100, 1, 6] = float("inf"), float("-inf")
+    out = attention.attend(q, k2, v2, spans)
+    row = torch.arange(40, device=gpu) % 6
+    bad = (row == 0) | (row == 3) | (row == 4)  # see the NaN keys, of head 0
+    assert out[0, bad, 0].isnan().all() and torch.equal(out[0, ~bad, 0], ref[0, ~bad, 0])
+    C.check(out[:, :, 1:], *C.attend(q[:, :, 1:], k2[:, :, 1:], v2[:, :, 1:], spans))
+    assert (out[0, (row == 0) | (row == 2), 1, 5] == float("inf")).all() and not out[0, row == 5].any()
