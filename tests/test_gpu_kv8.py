@@ -282,3 +282,17 @@ def test_refusals_on_the_gpu(gpu):
         with pytest.raises(err, match=text):
             kv8.attend(**{"q": q, "cache": cache, "lens": at, **kw})
     assert kv8.attend(q[:, :0], cache, at).shape == (2, 0, 4, 128)
+
+
+@pytest.mark.parametrize("b,tokens,h,hkv,hd,length", [(1, 200, 8, 1, 64, 1100), (3, 45, 16, 1, 96, 333), (1, 33, 6, 3, 128, 90),
+                                                      (2, 70, 32, 4, 64, 5000)])
+def test_attend_many_rows(gpu, b, tokens, h, hkv, hd, length):
+    """Many row tiles of few samples and heads, which are dealt to the XCDs in runs: the last run is not full."""
+    cache = _filled(gpu, b, length, hkv, hd, seed=tokens)
+    q = torch.randn(b, tokens, h, hd, generator=torch.Generator(device=gpu).manual_seed(1), device=gpu).bfloat16()
+    lens = [length - 7 * i for i in range(b)]
+    kc, vc = C.rows_of(cache)
+    k, v = C.values(kc, cache["ks"]).to(gpu), C.values(vc, cache["vs"]).to(gpu)
+    for causal in (True, False):
+        out = kv8.attend(q, cache, _ints(gpu, *lens), causal=causal)
+        C.check(out, *C.attend(q, k, v, lens, causal=causal))
