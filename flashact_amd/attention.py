@@ -95,8 +95,9 @@ def attend(q, k, v, spans=None, *, scale=None, softcap: float = 0.0, slopes=None
         out = q.new_empty((b, tq, h, hd))
     elif out.dtype is not t or out.shape != q.shape or not out.is_contiguous() or out.get_device() != index or out.data_ptr() % 16:
         raise ValueError(f"out must be contiguous, 16-byte aligned {t} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
-    elif _lib.overlap(out, k) or _lib.overlap(out, v):
-        raise ValueError("out must not share memory with k or v")
+    elif (_lib.overlap(out, k) or _lib.overlap(out, v)
+          or _lib.overlap(out, q) and (out.data_ptr() != q.data_ptr() or not q.is_contiguous())):
+        raise ValueError("out must not share memory with k or v, nor with q but for being it")
     need = _workspace_bytes(b, tq, tk, h, hd)
     ws = q.new_empty(need, dtype=torch.uint8) if need else None
     a = _lib.SpanArgs(_lib.DTYPES[t], q.data_ptr(), _S3(*strides[0]), k.data_ptr(), _S3(*strides[1]), v.data_ptr(),

@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(256) load_kernel(CacheArgs a) {
 
 int check_cache(const void* k, const void* v, const void* ks, const void* vs, int batch, int heads, int hd, int blocks,
                 const char* who) {
-  if (batch < 1 || heads < 1 || blocks < 1 || batch > (1 << 20) || heads > (1 << 16) || blocks > (1 << 26))
+  if (batch < 1 || heads < 1 || blocks < 1 || batch > (1 << 20) || heads > (1 << 16) || blocks >= (1 << 26))
     return host::fail(FA_ERR_INVALID_ARG, "%s: batch=%d, kv_heads=%d, blocks=%d", who, batch, heads, blocks);
   if (hd != 64 && hd != 96 && hd != 128 && hd != 256)
     return host::fail(FA_ERR_INVALID_ARG, "%s: head_dim=%d is none of 64, 96, 128, 256", who, hd);

@@ -108,7 +108,8 @@ def load(cache: dict, lens, *, k=None, v=None, dtype=torch.bfloat16):
     if (k is None) != (v is None):
         raise ValueError("pass both of k and v or neither")
     fresh = k is None
-    if not fresh and any(s == 0 and n > 1 for t in (k, v) for s, n in zip(t.stride(), t.shape)):
+    if not fresh and (k.numel() and k.data_ptr() == v.data_ptr()
+                      or any(s == 0 and n > 1 for t in (k, v) for s, n in zip(t.stride(), t.shape))):
         raise ValueError("k and v are written: no two of their elements may be one")
     if fresh:
         if dtype not in _lib.DTYPES:
@@ -131,7 +132,7 @@ def attend(q, cache: dict, lens, *, count=None, scale=None, softcap: float = 0.0
     [B]: cached tokens; count int32 [B]: how many of the T are real (None: all). Query t < n is at position
     i = lens - n + t and sees keys j <= i, or all of the cached ones with causal=False. Scores are q . k * scale (default
     hd^-1/2), capped to softcap * tanh(s / softcap) where softcap > 0, less slopes[h] |i - j| where slopes (fp32 [H]) are
-    given. Rows without keys become zero. Returns [B][T][H][hd] of q's type.
+    given. Rows without keys become zero. Returns [B][T][H][hd] of q's type, in `out` where it is given (q itself may be).
     """
     ck, cv, ks, vs, b, h, nb, hd, index = _cache(cache)
     if q.dtype is not torch.bfloat16 and q.dtype is not torch.float16:
@@ -154,6 +155,8 @@ def attend(q, cache: dict, lens, *, count=None, scale=None, softcap: float = 0.0
         out = q.new_empty((b, tokens, heads, hd))
     elif out.dtype is not q.dtype or out.shape != q.shape or not out.is_contiguous() or out.get_device() != index:
         raise ValueError(f"out must be contiguous {q.dtype} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
+    elif _lib.overlap(out, q) and (out.data_ptr() != q.data_ptr() or not q.is_contiguous()):
+        raise ValueError("out must not share memory with q but for being it")
     lib = _lib.lib()
     need = _workspace_bytes(b, tokens, heads, h, hd, nb)
     ws = q.new_empty(need, dtype=torch.uint8) if need else None

@@ -217,7 +217,7 @@ def extend(weights: list, ln_in, ln_post, x, caches: list, lens, count=None) -> 
 
     weights: ``pack_backbone_w4`` output. x [B][T][2048] fp32: the hidden states entering layer 0, B T <= 64. caches as
     ``prefill_packed`` leaves them; lens int32 [B] on the GPU: tokens cached so far, the positions of the new ones follow
-    them; count int32 [B]: how many of the T are real (None: all); lens + T must fit the caches, which is
+    them; count int32 [B]: how many of the T are real (None: all, clamped to [0, T]); lens + T must fit the caches, which is
     not checked (tokens behind their end are dropped). The tokens' keys and values are appended (the caller's
     lens grow by T or count), each token sees all cached ones and the new ones up to itself. Returns the hidden states
     leaving the last layer [B][T][2048] fp32 (undefined behind count). Nothing synchronises, and a captured graph serves
@@ -229,6 +229,8 @@ def extend(weights: list, ln_in, ln_post, x, caches: list, lens, count=None) -> 
     B, T = int(x.shape[0]), int(x.shape[1])
     dev = x.device
     rope = _rope(lens[:, None] + torch.arange(T, device=dev), dev)
+    if count is not None:
+        count = count.clamp(0, T)
     after = lens + (T if count is None else count)
     x = x.reshape(B * T, D)
     for l, w in enumerate(weights):

@@ -247,3 +247,16 @@ def test_parts_keep_what_is_not_finite(gpu, hd):
     assert out[0, bad, 0].isnan().all() and torch.equal(out[0, ~bad, 0], ref[0, ~bad, 0])
     C.check(out[:, :, 1:], *C.attend(q[:, :, 1:], k2[:, :, 1:], v2[:, :, 1:], spans))
     assert (out[0, (row == 0) | (row == 2), 1, 5] == float("inf")).all() and not out[0, row == 5].any()
+
+
+@pytest.mark.parametrize("tk", [40, 9000])
+def test_out_is_q_or_apart_from_it(gpu, tk):
+    buf = torch.randn(40 * 4 * 64 + 64, device=gpu).bfloat16()
+    q = buf[:40 * 4 * 64].view(1, 40, 4, 64)
+    _, k, v = _qkv(gpu, 1, 1, tk, 4, 2, 64, torch.bfloat16)
+    ref = attention.attend(q, k, v)
+    with pytest.raises(ValueError, match="share memory"):
+        attention.attend(q, k, v, out=buf[64:].view(1, 40, 4, 64))
+    with pytest.raises(ValueError, match="share memory"):
+        attention.attend(q.view(1, 4, 40, 64).transpose(1, 2), k, v, out=q)
+    assert attention.attend(q, k, v, out=q) is q and torch.equal(q, ref)

@@ -205,3 +205,15 @@ def test_refusals(gpu):
     for bad in (torch.zeros(2, 33, 2048, device=gpu), torch.zeros(3, 1, 2048, device=gpu), x):
         with pytest.raises(ValueError, match="x must be"):
             prefill.extend(layers, *ln, bad, caches, _ints(gpu, 0, 0))
+
+
+def test_extend_clamps_counts(gpu):
+    """A count past T is T, one below zero is none: the caches come out the same."""
+    _, _, w4s, ln = _weights(gpu, seed=5)
+    x, lens = torch.randn(2, 2, 2048, device=gpu), _ints(gpu, 0, 0)
+    runs = []
+    for count in ((2, 0), (9, -3)):
+        caches = kv8.make_caches(NL, 2, 32, device=gpu)
+        runs.append((prefill.extend(w4s, *ln, x, caches, lens, _ints(gpu, *count)), caches))
+    assert torch.equal(runs[0][0][0], runs[1][0][0]) and runs[0][0][0].isfinite().all()
+    assert all(torch.equal(a[n], b[n]) for a, b in zip(runs[0][1], runs[1][1]) for n in a)

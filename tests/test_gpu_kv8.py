@@ -296,3 +296,23 @@ def test_attend_many_rows(gpu, b, tokens, h, hkv, hd, length):
     for causal in (True, False):
         out = kv8.attend(q, cache, _ints(gpu, *lens), causal=causal)
         C.check(out, *C.attend(q, k, v, lens, causal=causal))
+
+
+def test_shared_memory_is_refused_but_for_q_itself(gpu):
+    cache = _filled(gpu, 1, 500, 2, 64, seed=9)
+    lens = _ints(gpu, 500)
+    buf = torch.randn(4 * 8 * 64 + 64, device=gpu).bfloat16()
+    q = buf[:4 * 8 * 64].view(1, 4, 8, 64)
+    ref = kv8.attend(q, cache, lens)
+    with pytest.raises(ValueError, match="share memory"):
+        kv8.attend(q, cache, lens, out=buf[64:].view(1, 4, 8, 64))
+    with pytest.raises(ValueError, match="share memory"):
+        kv8.attend(q.view(1, 8, 4, 64).transpose(1, 2), cache, lens, out=q)
+    assert kv8.attend(q, cache, lens, out=q) is q and torch.equal(q, ref)
+    k = torch.empty(1, 500, 2, 64, device=gpu)
+    with pytest.raises(ValueError, match="no two"):
+        kv8.load(cache, lens, k=k, v=k)
+    both = torch.empty(1, 500, 2, 2, 64, device=gpu)  # interleaved: different elements
+    kv8.load(cache, lens, k=both[:, :, 0], v=both[:, :, 1])
+    want = kv8.load(cache, lens, dtype=torch.float32)
+    assert torch.equal(both[:, :, 0], want[0][:, :500]) and torch.equal(both[:, :, 1], want[1][:, :500])
