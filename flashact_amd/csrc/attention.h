@@ -12,7 +12,7 @@
 // Keys and values of the next tiles are copied to LDS (no registers) while this one is worked on, one barrier a tile. With
 // many queries the MFMAs are the bound, next to the LDS reads that feed them (each operand of 1 KB serves 16 or 32 queries)
 // and, capped, the three exponentials a score; with few it is one wave's chain of a tile's steps, about 3000 cycles.
-// 8191 tokens of 16 heads of 128 dims over 4 K/V heads, causal behind a tenth, capped: 376 us, 738 TFLOP/s.
+// 8191 tokens of 16 heads of 128 dims over 4 K/V heads, causal behind a tenth, capped: 374 us, 742 TFLOP/s.
 //
 // Rounding: the scores' products are exact in fp32, softmax and sums are fp32, P is rounded to the values' type for the
 // second product (bf16 values have a range that fp16 weights times fp16 values would not hold), the result once.
@@ -20,6 +20,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/flashact_mi355x.h"
 #include "fa_device.h"
@@ -107,6 +108,16 @@ __device__ __forceinline__ unsigned fraction(unsigned x) {
 // the halves whose sign bit is set, whole
 __device__ __forceinline__ unsigned spread(unsigned sign) { return sign | (sign - (sign >> 15)); }
 
+typedef int i32x2 __attribute__((ext_vector_type(2), aligned(4)));
+
+// The least of a row of 16 lanes, in each of them (DPP row_ror).
+__device__ __forceinline__ int rows_least(int v) {
+  v = min(v, __builtin_amdgcn_update_dpp(0, v, 0x128, 0xF, 0xF, false));
+  v = min(v, __builtin_amdgcn_update_dpp(0, v, 0x124, 0xF, 0xF, false));
+  v = min(v, __builtin_amdgcn_update_dpp(0, v, 0x122, 0xF, 0xF, false));
+  return min(v, __builtin_amdgcn_update_dpp(0, v, 0x121, 0xF, 0xF, false));
+}
+
 constexpr int part_floats(int nt) { return nt * 256 + 32; }  // of 16 rows
 
 template <bool F16, int HD, int QB, int NW, int SP, bool CAP, bool BIAS>
@@ -139,36 +150,30 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
   const int b = bh / (unsigned)p.H, h = bh - b * p.H, kvh = h / p.G;
   const int row0 = (p.ntile - 1 - (int)tile) * (16 * QB * NW) + wave * 16 * QB;
 
-  // this lane's queries and the tile's extent
+  // this lane's queries and the tile's extent; rows behind the last load what it loads and see nothing
   int first[QB], last[QB], lo = 0x7fffffff, hi = 0, all_lo = 0, all_hi = 0x7fffffff;
 #pragma unroll
-  for (int x = 0; x < QB; x++) {
-    const int row = row0 + 16 * x + r;
-    first[x] = 0, last[x] = 0;
-    if (row < p.Tq) {
-      if (p.spans) {
-        const int* s = p.spans + ((size_t)b * p.Tq + row) * 2;
-        first[x] = max(s[0], 0);
-        last[x] = min(s[1], p.Tk);
-      } else {
-        last[x] = p.Tk;
-      }
-      if (first[x] < last[x]) {
-        lo = min(lo, first[x]), hi = max(hi, last[x]);
-        all_lo = max(all_lo, first[x]), all_hi = min(all_hi, last[x]);
-      } else {
-        first[x] = last[x] = 0;
-        all_hi = 0;  // a row that sees nothing: every tile is masked
-      }
+  for (int x = 0; x < QB; x++) first[x] = 0, last[x] = p.Tk;
+  if (p.spans) {
+#pragma unroll
+    for (int x = 0; x < QB; x++) {
+      const i32x2 s = *reinterpret_cast<const i32x2*>(p.spans + ((size_t)b * p.Tq + min(row0 + 16 * x + r, p.Tq - 1)) * 2);
+      first[x] = s[0], last[x] = s[1];
     }
   }
 #pragma unroll
-  for (int o = 1; o < 16; o <<= 1) {
-    lo = min(lo, __shfl_xor(lo, o));
-    hi = max(hi, __shfl_xor(hi, o));
-    all_lo = max(all_lo, __shfl_xor(all_lo, o));
-    all_hi = min(all_hi, __shfl_xor(all_hi, o));
+  for (int x = 0; x < QB; x++) {
+    const bool there = row0 + 16 * x + r < p.Tq;
+    first[x] = max(first[x], 0), last[x] = there ? min(last[x], p.Tk) : 0;
+    if (first[x] < last[x]) {
+      lo = min(lo, first[x]), hi = max(hi, last[x]);
+      all_lo = max(all_lo, first[x]), all_hi = min(all_hi, last[x]);
+    } else {
+      first[x] = last[x] = 0;
+      if (there) all_hi = 0;  // a row that sees nothing: every tile is masked
+    }
   }
+  lo = rows_least(lo), hi = -rows_least(-hi), all_lo = -rows_least(-all_lo), all_hi = rows_least(all_hi);
   int* ext = reinterpret_cast<int*>(lds + p.stages * SP * 2 * TILE);  // the workgroup walks over the keys of all its waves
   if (lane == 0 && grp == 0) {
     ext[2 * wave] = lo;
@@ -177,6 +182,16 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
   // dims behind hd are zero in LDS: the copies never write them
   if (p.hd < HD)
     for (int i = threadIdx.x; i < p.stages * SP * 2 * TILE / 16; i += 64 * NW * SP) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
+  u32x4 qf[QB][NK];
+#pragma unroll
+  for (int x = 0; x < QB; x++)
+#pragma unroll
+    for (int i = 0; i < NK; i++) {
+      const int row = min(row0 + 16 * x + r, p.Tq - 1), d = 32 * i + 8 * q;
+      qf[x][i] = u32x4{0, 0, 0, 0};
+      if (d < p.hd) qf[x][i] = *reinterpret_cast<const u32x4*>(p.q + (b * p.qb + row * p.qt + h * p.qh + d) * 2);
+    }
+  const float slope = BIAS ? p.slopes[h] * LOG2E : 0.f;
   __syncthreads();
   int k0 = 0x7fffffff, k1 = 0;
 #pragma unroll
@@ -199,18 +214,6 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
   hi = __builtin_amdgcn_readfirstlane(hi);
   all_lo = __builtin_amdgcn_readfirstlane(all_lo);
   all_hi = __builtin_amdgcn_readfirstlane(all_hi);
-
-  u32x4 qf[QB][NK];
-#pragma unroll
-  for (int x = 0; x < QB; x++)
-#pragma unroll
-    for (int i = 0; i < NK; i++) {
-      const int row = row0 + 16 * x + r, d = 32 * i + 8 * q;
-      qf[x][i] = u32x4{0, 0, 0, 0};
-      if (row < p.Tq && d < p.hd)
-        qf[x][i] = *reinterpret_cast<const u32x4*>(p.q + (b * p.qb + row * p.qt + h * p.qh + d) * 2);
-    }
-  const float slope = BIAS ? p.slopes[h] * LOG2E : 0.f;
 
   const unsigned char* kg = p.k + (b * p.kb + kvh * p.kh) * 2;
   const unsigned char* vg = p.v + (b * p.vb + kvh * p.vh) * 2;
@@ -461,46 +464,72 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
     __builtin_amdgcn_s_setprio(0);
   }
 
-  if constexpr (SP > 1) {  // the second group hands its sums, lane by lane, to the first
-    static_assert(QB == 1 && SP == 2, "one block of queries, two groups");
-    __syncthreads();
-    float* o = reinterpret_cast<float*>(lds) + (wave * (NT * 4 + 2)) * 64;
-    if (grp == 1) {
+  __syncthreads();  // the tiles in LDS are done with
+  // Rows leave through LDS, 16 bytes a lane along a row: a lane holds four dims of its row, and stores of 8 bytes to 16 rows
+  // took the address unit 3500 cycles with 256 dims.
+  constexpr int PITCH = HD * 2 + 16;
+  static_assert(NW * SP * 16 * PITCH <= 2 * SP * 2 * TILE, "LDS");
+  unsigned char* turn_rows = lds + all_waves * (16 * PITCH);
+  auto put = [&](int j, f32x4 o) {
+    *reinterpret_cast<u32x2*>(turn_rows + r * PITCH + (16 * j + 4 * q) * 2) = u32x2{pack2<F16>(o[0], o[1]), pack2<F16>(o[2], o[3])};
+  };
+  auto leave = [&](int x, int j0, auto tiles) {  // dims of tiles j0 .. j0 + tiles - 1
+    constexpr int C = 2 * decltype(tiles)::value;
+    wave_fence();
 #pragma unroll
-      for (int j = 0; j < NT; j++) *reinterpret_cast<f32x4*>(o + (j * 64 + lane) * 4) = O[0][j];
-      o[NT * 256 + lane] = m[0];
-      o[NT * 256 + 64 + lane] = l[0];
+    for (int i = 0; i < (16 * C + 63) / 64; i++) {
+      const int at = i * 64 + lane, rr = at / C, d = 16 * j0 + at % C * 8, row = row0 + 16 * x + rr;
+      if ((16 * C % 64 == 0 || rr < 16) && row < p.Tq && d < p.hd)
+        *reinterpret_cast<u32x4*>(p.out + ((((size_t)b * p.Tq + row) * p.H + h) * p.hd + d) * 2) =
+            *reinterpret_cast<const u32x4*>(turn_rows + rr * PITCH + d * 2);
     }
-    __syncthreads();
-    if (grp == 1) return;
-    const float m1 = o[NT * 256 + lane], l1 = o[NT * 256 + 64 + lane], mm = fmaxf(m[0], m1);
-    const float f0 = m[0] == -INFINITY ? 0.f : exp2_w(m[0] - mm), f1 = m1 == -INFINITY ? 0.f : exp2_w(m1 - mm);
-    l[0] = l[0] * f0 + l1 * f1;
+    wave_fence();
+  };
+  if constexpr (SP > 1) {  // each of the two groups finishes half of the dims: it hands the sums of the others over, lane by lane
+    static_assert(QB == 1 && SP == 2 && NT % 2 == 0, "one block of queries, two groups");
+    constexpr int HALF = NT / 2, MINE = HALF * 256 + 128;
+    static_assert(NW * 2 * MINE * 4 <= 2 * SP * 2 * TILE, "LDS");
+    float* give = reinterpret_cast<float*>(lds) + (wave * 2 + grp) * MINE;
+    const float* take = reinterpret_cast<const float*>(lds) + (wave * 2 + 1 - grp) * MINE;
+    auto finish = [&](auto low) {  // low: this group's tiles start at 0
+      constexpr int J0 = decltype(low)::value ? 0 : HALF, J1 = HALF - J0;
 #pragma unroll
-    for (int j = 0; j < NT; j++) O[0][j] = O[0][j] * f0 + f1 * *reinterpret_cast<const f32x4*>(o + (j * 64 + lane) * 4);
-    if (used > 1) {
-      float* to = p.part + (((size_t)bh * p.ntile + tile) * p.S + split) * (NW * part_floats(NT)) + wave * part_floats(NT);
+      for (int j = 0; j < HALF; j++) *reinterpret_cast<f32x4*>(give + (j * 64 + lane) * 4) = O[0][J1 + j];
+      give[HALF * 256 + lane] = m[0];
+      give[HALF * 256 + 64 + lane] = l[0];
+      __syncthreads();
+      const float m1 = take[HALF * 256 + lane], l1 = take[HALF * 256 + 64 + lane], mm = fmaxf(m[0], m1);
+      const float f0 = m[0] == -INFINITY ? 0.f : exp2_w(m[0] - mm), f1 = m1 == -INFINITY ? 0.f : exp2_w(m1 - mm);
+      const float sum = cols_sum(l[0] * f0 + l1 * f1);
 #pragma unroll
-      for (int j = 0; j < NT; j++) *reinterpret_cast<f32x4*>(to + (j * 64 + lane) * 4) = O[0][j];
-      const float all = cols_sum(l[0]);
-      if (lane < 16) {
-        to[NT * 256 + lane] = fmaxf(m[0], m1);
-        to[NT * 256 + 16 + lane] = all;
+      for (int j = 0; j < HALF; j++)
+        O[0][J0 + j] = O[0][J0 + j] * f0 + f1 * *reinterpret_cast<const f32x4*>(take + (j * 64 + lane) * 4);
+      if (used > 1) {
+        float* to = p.part + (((size_t)bh * p.ntile + tile) * p.S + split) * (NW * part_floats(NT)) + wave * part_floats(NT);
+#pragma unroll
+        for (int j = J0; j < J0 + HALF; j++) *reinterpret_cast<f32x4*>(to + (j * 64 + lane) * 4) = O[0][j];
+        if (J0 == 0 && lane < 16) {
+          to[NT * 256 + lane] = mm;
+          to[NT * 256 + 16 + lane] = sum;
+        }
+        return;
       }
-      return;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      __syncthreads();
+#pragma unroll
+      for (int j = J0; j < J0 + HALF; j++) put(j, O[0][j] * inv);
+      leave(0, J0, std::integral_constant<int, HALF>{});
+    };
+    if (grp == 0) finish(std::true_type{});
+    else finish(std::false_type{});
+  } else {
+#pragma unroll
+    for (int x = 0; x < QB; x++) {
+      const float sum = cols_sum(l[x]), inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+      for (int j = 0; j < NT; j++) put(j, O[x][j] * inv);
+      leave(x, 0, std::integral_constant<int, NT>{});
     }
-  }
-#pragma unroll
-  for (int x = 0; x < QB; x++) {
-    const int row = row0 + 16 * x + r;
-    const float sum = cols_sum(l[x]), inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (row >= p.Tq) continue;
-    unsigned char* o = p.out + (((size_t)b * p.Tq + row) * p.H + h) * p.hd * 2;
-#pragma unroll
-    for (int j = 0; j < NT; j++)
-      if (16 * j + 4 * q < p.hd)
-        *reinterpret_cast<u32x2*>(o + (16 * j + 4 * q) * 2) =
-            u32x2{pack2<F16>(O[x][j][0] * inv, O[x][j][1] * inv), pack2<F16>(O[x][j][2] * inv, O[x][j][3] * inv)};
   }
 }
 

@@ -212,6 +212,8 @@ __device__ __forceinline__ float cols_max(float v) {
   a = swap32(as_u32(v), as_u32(v));
   return fmaxf(as_f32(a.lo), as_f32(a.hi));
 }
+// Orders a wave's own LDS accesses, where a stage is private to the wave: its LDS instructions run in order.
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 // Value of lane ^ 16 (selected from the swap of x with itself).
 __device__ __forceinline__ unsigned xor16_u32(unsigned x, bool odd_row) {
   const LanePair a = swap16(x, x);

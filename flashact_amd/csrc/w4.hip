@@ -64,9 +64,6 @@ __device__ __forceinline__ u32x2 row_bcast(u32x2 v, int g) {
   return v;
 }
 
-// orders the wave's own LDS accesses (the stage is private to the wave, whose LDS instructions run in order)
-__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
-
 __device__ __forceinline__ void store_out(const Params& p, size_t at, float v) {
   if (p.out_dtype == FA_DTYPE_F32) static_cast<float*>(p.out)[at] = v;
   else if (p.out_dtype == FA_DTYPE_F16) static_cast<_Float16*>(p.out)[at] = (_Float16)v;
