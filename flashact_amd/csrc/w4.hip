@@ -259,21 +259,32 @@ __global__ void __launch_bounds__(256) w4_join_kernel(Params p, int splits) {
   finish(p, m, n, y0, y1);
 }
 
-// How a product is cut: tiles a workgroup, splits of K across workgroups, waves a workgroup.
+// How a product is cut: tiles a workgroup, splits of K across workgroups, waves a workgroup. Times in us of both sides, in
+// turn, group 32, at N x K and rows M.
 struct Cut {
   int nt, splits, waves;
 };
 Cut cut(int M, int N, int K) {
   const int tiles = (N + 15) / 16, nch = (K + 127) / 128;
   Cut c{1, 1, 1};
+  // Four tiles a workgroup share its activations and keep four tiles' codes in flight. That pays where there are workgroups
+  // enough all the same (32768 x 2048: 10.9 instead of 13.3 at M = 5, 11.9 instead of 15.2 at 16) or K is long enough to be
+  // split (2048 x 16384: 10.0 instead of 11.2, 10.4 instead of 12.0); in between it does not (4096 x 16384: 15.1 instead of
+  // 12.9; 2048 x 2048: 6.8 instead of 4.1). More than 16 rows leave registers and LDS for two tiles, more than 32 for one.
   if (M > 32) c.nt = 1;
   else if (M > 16) c.nt = 2;
-  // Four tiles a workgroup share its activations, and hold twice the codes in flight of one tile
-  else if (M > 4 ? tiles >= 64 : tiles >= 1024) c.nt = 4;
+  else if (tiles >= 1024 || (M > 4 && tiles >= 64 && tiles < 256 && nch >= 96)) c.nt = 4;
   const int blocks = (tiles + c.nt - 1) / c.nt, most = M <= 16 && c.nt == 1 ? 16 : 8;
-  if (blocks < 128) c.splits = std::max(1, std::min({256 / blocks, nch / 8, 16}));
+  // Splits cost a second launch, about 2 us. With one tile and few rows 16 waves share K already, and only a handful of
+  // workgroups needs more (64 x 16384: 5.5 instead of 8.0, but 2048 x 8192 in two 7.7 instead of 5.8); else K is split until there is a
+  // workgroup a CU (2048 x 16384: 10.0 instead of 24.3 at M = 5, 14.8 instead of 24.6 at 32, 20.7 instead of 28.7 at 48), in
+  // parts of 2048 columns or more (2048 x 2048 in two at M = 32: 7.7 instead of 6.6).
+  c.splits = std::max(1, std::min({(most == 16 ? 32 : 256) / blocks, nch / 16, 16}));
   const int mine = (nch + c.splits - 1) / c.splits;
-  c.waves = std::max(1, std::min({most, std::max(4, 4096 / (blocks * c.splits)), mine}));
+  // Waves: 4096 in all, with two tiles 2048 (16384 x 2048 at M = 32: 11.4 instead of 13.2), of two chunks each or more
+  // (2560 x 2048: 4.1 instead of 4.7 at M = 5, 3.7 instead of 3.9 at 1), and no fewer than four (32768 x 2048 with four
+  // instead of eight: 12.1 instead of 10.9).
+  c.waves = std::max(1, std::min({most, std::max(4, (c.nt == 2 ? 2048 : 4096) / (blocks * c.splits)), mine, std::max(4, mine / 2)}));
   return c;
 }
 
