@@ -2,6 +2,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <chrono>
 #include <mutex>
 #include <set>
 #include <utility>
@@ -88,6 +89,18 @@ int check_gfx950(const char* who) {
                 prop.gcnArchName);
   g_gfx950[dev].store(1, std::memory_order_relaxed);
   return FA_OK;
+}
+
+uint64_t launch_nonce() {
+  static const uint64_t seed = (uint64_t)std::chrono::steady_clock::now().time_since_epoch().count() ^
+                               reinterpret_cast<uintptr_t>(&g_gfx950);
+  static std::atomic<uint64_t> calls{0};
+  uint64_t x = seed + calls.fetch_add(1, std::memory_order_relaxed);
+  for (int i = 0; i < 2; i++) {  // each step is one to one: an odd factor, the upper bits onto the lower ones
+    x *= 0x9e3779b97f4a7c15ull;
+    x ^= x >> 32;
+  }
+  return x ? x : ~0ull;
 }
 
 int allow_lds(const void* kernel, unsigned lds_bytes, const char* who) {

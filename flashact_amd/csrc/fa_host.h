@@ -3,6 +3,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdarg.h>
+#include <stdint.h>
 #include <stdio.h>
 
 #include "../../include/flashact_mi355x.h"
@@ -36,6 +37,9 @@ int check_device(const void* kernel, int threads, unsigned lds_bytes, int nwg, c
 int check_gfx950(const char* who);
 // Raises a kernel's dynamic-LDS limit to `lds_bytes` (once per device and kernel).
 int allow_lds(const void* kernel, unsigned lds_bytes, const char* who);
+
+// 64 bits that no other launch of this process has and that memory does not hold by chance; never 0.
+uint64_t launch_nonce();
 
 }  // namespace host
 

@@ -10,8 +10,8 @@
 // product wants it: row m of key tile t is key 8 (m / 4) + 4 t + m % 4, so lane quarter q ends with keys 8 q .. 8 q + 7.
 // Each wave copies its blocks to LDS on its own (no registers, no barrier): the keys' next block is asked for as soon as
 // this one's codes are in registers, the values' likewise, so a whole block is on its way at any time. Keys are split
-// over the waves of a workgroup and, where rows are few, over workgroups (the sums then go through the workspace to
-// join_kernel). They are dealt block by block, so that the waves read one contiguous stretch of memory together: with a
+// over the waves of a workgroup and, where rows are few, over workgroups (the sums then meet in
+// the workspace). They are dealt block by block, so that the waves read one contiguous stretch of memory together: with a
 // stretch for each wave, equally far apart, all of them met in the same memory channels (2 x 131072 keys: 35.8 us instead of 33.0).
 //
 // Codes are exact in bf16 and fp16. Q K^T runs in q's type; P is rounded to fp16 (2^-12, half the step of an fp16
@@ -38,7 +38,8 @@ struct AttnArgs {
   const int *lens, *count;
   const float* slopes;
   unsigned char* out;
-  float* part;  // [sample][head][row tile][split] {O[16][hd], m[16], l[16]}
+  float* part;  // [sample][head][row tile][split] {O[16][hd], {m, l}[16]}
+  uint64_t *arrived, nonce;  // [sample][head][row tile][FUSED], where the last workgroup joins the splits
   int B, T, H, G, nblk, RT, RC, S, least, causal;  // RT row tiles of a head, RC of them side by side on an XCD
   float scale, over, cap;  // base 2: scale log2(e); capped, scale / cap and cap log2(e)
 };
@@ -56,6 +57,7 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int b) {
 }
 // Splits that a row tile of nb blocks uses: each wave of each has a.least blocks or more.
 constexpr int MAX_SPLITS = 256;
+constexpr int FUSED = 8;  // up to so many are joined by the last workgroup, more by a kernel with workgroups enough to read them
 __device__ __forceinline__ int splits_used(const AttnArgs& a, int nb, int waves) {
   const unsigned per = waves * a.least;
   return max(1, min(a.S, (int)((nb + per - 1) / per)));
@@ -334,7 +336,8 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) att
 #pragma unroll
   for (int w = 0; w < W; w++) M = fmaxf(M, wm[w * 16 + r]);
   const float mine = m == -INFINITY ? 0.f : exp2_w(m - M);
-  float* part = a.part + (((size_t)bh * a.RT + rt) * a.S + split) * (16 * HD + 32);
+  constexpr int ONE = 16 * HD + 32;
+  const rsrc_t part = make_rsrc(a.part + ((size_t)bh * a.RT + rt) * a.S * ONE, 0xffffffffu);  // the tile's splits
 #pragma unroll
   for (int d0 = 0; d0 < HD; d0 += DC) {
     if (d0) __syncthreads();
@@ -354,11 +357,8 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) att
 #pragma unroll
       for (int w = 1; w < W; w++) o += *reinterpret_cast<const f32x4*>(osum + (w * 16 + row) * PITCH + d);
       if (used > 1) {
-        *reinterpret_cast<f32x4*>(part + row * HD + d0 + d) = o;
-        if (d0 + d == 0) {
-          part[16 * HD + row] = rm;
-          part[16 * HD + 16 + row] = rl;
-        }
+        stb128<kCpSc1>(part, (split * ONE + row * HD + d0 + d) * 4, __builtin_bit_cast(u32x4, o));
+        if (d0 + d == 0) stb64<kCpSc1>(part, (split * ONE + 16 * HD + 2 * row) * 4, __builtin_bit_cast(u32x2, f32x2{rm, rl}));
       } else {
         const int tt = g / a.G;
         if (tt >= sp.n || sp.len - sp.n + tt < 0) o = f32x4{0.f, 0.f, 0.f, 0.f}, rl = 0.f;
@@ -367,9 +367,70 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) att
       }
     }
   }
+  if (used == 1 || a.S > FUSED) return;
+  // The last of the tile's workgroups joins its splits, in their order. Each writes the launch's nonce into its word once its
+  // sums are in memory, and then looks at all words: the last one finds the nonce in each, whatever the workspace held
+  // before. Nobody waits. Two may both find it; they store the same bits. Who joins clears the words, as a captured launch is
+  // replayed with the same nonce. (One token of 983 keys on eight splits: 9.4 us, 9.7 with a second kernel to join, 11.4 with a
+  // counter per tile by compare and exchange, which eight that arrive together retry; 48 requests: 24.1, 26.1 with the kernel.)
+  uint64_t* words = a.arrived + ((size_t)bh * a.RT + rt) * FUSED;
+  unsigned* flag = reinterpret_cast<unsigned*>(wm);
+  __builtin_amdgcn_s_waitcnt(0);  // this wave's sums have arrived
+  __syncthreads();
+  if (wave == 0) {
+    if (lane == 0) __hip_atomic_store(words + split, a.nonce, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __builtin_amdgcn_s_waitcnt(0);
+    const bool there = lane >= used || __hip_atomic_load(words + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.nonce;
+    const bool all = __builtin_amdgcn_ballot_w64(!there) == 0;
+    if (lane == 0) *flag = all;
+    if (all && lane < used) __hip_atomic_store(words + lane, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (*flag == 0) return;
+  f32x2* ml = reinterpret_cast<f32x2*>(lds);
+  static_assert(16 * FUSED <= 64 * W, "a split's row a thread");
+  const int rows = min(16, a.T * a.G - rt * 16), own = threadIdx.x;
+  f32x2 mine_ml = f32x2{-INFINITY, 0.f};
+  if (own < 16 * used) mine_ml = __builtin_bit_cast(f32x2, ldb64<kCpSc1>(part, ((own >> 4) * ONE + 16 * HD + 2 * (own & 15)) * 4));
+  constexpr int PER = HD / 4, EACH = 2;  // quads of dims of a row; of these a thread's at a time
+  for (int base = 0; base < rows * PER; base += EACH * 64 * W) {
+    const int e0 = base + threadIdx.x;
+    f32x4 x[EACH][FUSED];
+#pragma unroll
+    for (int k = 0; k < EACH; k++)
+#pragma unroll
+      for (int s = 0; s < FUSED; s++) {
+        const int e = e0 + k * 64 * W;
+        if (s < used && e < rows * PER)
+          x[k][s] = __builtin_bit_cast(f32x4, ldb128<kCpSc1>(part, (s * ONE + e * 4) * 4));
+      }
+    if (base == 0) {
+      if (own < 16 * FUSED) ml[own] = mine_ml;
+      __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < EACH; k++) {
+      const int e = e0 + k * 64 * W, row = e / PER, g = rt * 16 + row, tt = g / a.G;
+      if (e >= rows * PER) continue;
+      float rm = -INFINITY, rl = 0.f;
+#pragma unroll
+      for (int s = 0; s < FUSED; s++) rm = fmaxf(rm, ml[s * 16 + row][0]);
+      f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < FUSED; s++)
+        if (s < used) {
+          const f32x2 v = ml[s * 16 + row];
+          const float w = v[0] == -INFINITY ? 0.f : exp2_w(v[0] - rm);
+          rl += w * v[1];
+          o += w * x[k][s];
+        }
+      if (tt >= sp.n || sp.len - sp.n + tt < 0) o = f32x4{0.f, 0.f, 0.f, 0.f}, rl = 0.f;
+      store_row4<F16>(a.out, ((size_t)b * a.T + tt) * a.H * a.G * HD + (size_t)(h * a.G + g % a.G) * HD + e % PER * 4, o * inverse(rl));
+    }
+  }
 }
 
-// The splits' sums, in a fixed order. One workgroup: one row; nothing to do where its sample used one split. Threads are
+// The splits' sums, in a fixed order, where there are more than FUSED. One workgroup: one row; nothing to do where its sample used one split. Threads are
 // (hd / 4) dims x groups of splits, so many splits are read side by side.
 template <bool F16, int HD, int W>
 __global__ void __launch_bounds__(256) join_kernel(AttnArgs a) {
@@ -389,8 +450,8 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a) {
   constexpr int ONE = 16 * HD + 32;
   const float* part = a.part + ((size_t)bh * a.RT + rt) * a.S * ONE;
   const int i = threadIdx.x, wave = i >> 6;
-  const float ms = i < used ? part[(size_t)i * ONE + 16 * HD + row] : -INFINITY;
-  const float ls = i < used ? part[(size_t)i * ONE + 16 * HD + 16 + row] : 0.f;
+  const f32x2 ml = i < used ? *reinterpret_cast<const f32x2*>(part + (size_t)i * ONE + 16 * HD + 2 * row) : f32x2{-INFINITY, 0.f};
+  const float ms = ml[0], ls = ml[1];
   float x = wave_max(ms);
   if ((i & 63) == 0) red[wave] = x;
   __syncthreads();
@@ -440,11 +501,13 @@ int splits_for(int batch, int tokens, int heads, int kv_heads, int hd, int block
   return best;
 }
 
+size_t arrived_bytes(size_t tiles) { return (tiles * FUSED * sizeof(uint64_t) + 255) / 256 * 256; }
+
 size_t attn_workspace(int batch, int tokens, int heads, int kv_heads, int hd, int blocks) {
   const int S = splits_for(batch, tokens, heads, kv_heads, hd, blocks);
   if (S == 1) return 0;
   const size_t rt = ((size_t)tokens * (heads / kv_heads) + 15) / 16;
-  return rt * batch * kv_heads * S * (16 * hd + 32) * sizeof(float);
+  return (S <= FUSED ? arrived_bytes(rt * batch * kv_heads) : 0) + rt * batch * kv_heads * S * (16 * hd + 32) * sizeof(float);
 }
 
 template <bool F16, int HD, int W>
@@ -459,7 +522,7 @@ int launch_waves(const AttnArgs& a, hipStream_t s) {
   const int rc = host::allow_lds(reinterpret_cast<const void*>(k), lds, "fa_kv8_attention");
   if (rc != FA_OK) return rc;
   hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * W), lds, s, a);
-  if (a.S > 1)
+  if (a.S > FUSED)
     hipLaunchKernelGGL((join_kernel<F16, HD, W>), dim3((unsigned)(a.B * a.H * a.T * a.G)), dim3(256), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return host::fail(FA_ERR_LAUNCH, "fa_kv8_attention: %s", hipGetErrorString(e));
@@ -529,6 +592,11 @@ extern "C" int fa_kv8_attention(const fa_kv8_attn_args* a, fa_stream_t stream) {
   p.B = a->batch, p.T = a->tokens, p.H = a->kv_heads, p.G = a->heads / a->kv_heads, p.nblk = a->blocks;
   p.RT = (p.T * p.G + 15) / 16;
   p.S = kv8::splits_for(a->batch, a->tokens, a->heads, a->kv_heads, a->head_dim, a->blocks);
+  if (p.S > 1 && p.S <= kv8::FUSED) {
+    p.nonce = host::launch_nonce();
+    p.arrived = static_cast<uint64_t*>(a->workspace);
+    p.part = reinterpret_cast<float*>(static_cast<unsigned char*>(a->workspace) + kv8::arrived_bytes((size_t)p.RT * p.B * p.H));
+  }
   // All row tiles of a (split, sample, head) run on one XCD where these divide evenly over the 8, else in runs short enough
   // that there are 32 or more (200 tokens of 8 heads over 1100 keys of one sample 35 -> 22 us; 18.4 -> 19.2 for 4 samples of 50).
   const int64_t groups = (int64_t)p.B * p.H * p.S, runs = groups % 8 ? std::min<int64_t>((31 + groups) / groups, p.RT) : 1;

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from flashact_amd import kv8, pi05
+from flashact_amd import _lib, kv8, pi05
 from tests import kv8_case as C
 
 pytestmark = pytest.mark.gpu
@@ -316,3 +316,28 @@ def test_shared_memory_is_refused_but_for_q_itself(gpu):
     kv8.load(cache, lens, k=both[:, :, 0], v=both[:, :, 1])
     want = kv8.load(cache, lens, dtype=torch.float32)
     assert torch.equal(both[:, :, 0], want[0][:, :500]) and torch.equal(both[:, :, 1], want[1][:, :500])
+
+
+@pytest.mark.parametrize("b,tokens,h,hkv,hd,length", [(1, 1, 8, 1, 256, 983), (4, 50, 8, 1, 256, 900), (5, 1, 16, 4, 128, 1500)])
+def test_split_sums_in_any_workspace(gpu, monkeypatch, b, tokens, h, hkv, hd, length):
+    """The workgroups that share a row tile count themselves in memory of any contents: ones, random words, an earlier call's."""
+    cache = _filled(gpu, b, length, hkv, hd, seed=hd)
+    q, lens = torch.randn(b, tokens, h, hd, device=gpu).half(), _ints(gpu, *[length - 200 * i for i in range(b)])
+    kc, vc = C.rows_of(cache)
+    ref, bound = C.attend(q, C.values(kc, cache["ks"]).to(gpu), C.values(vc, cache["vs"]).to(gpu), lens.tolist())
+    need = kv8._workspace_bytes(b, tokens, h, hkv, hd, cache["v"].shape[2])
+    assert need
+    ws = torch.full((need,), 255, dtype=torch.uint8, device=gpu)
+    real = _lib.run_on
+
+    def run_on(index, fn, a, what):
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        real(index, fn, a, what)
+
+    monkeypatch.setattr(_lib, "run_on", run_on)
+    out = kv8.attend(q, cache, lens)
+    C.check(out, ref, bound)
+    for i in range(5):
+        if i == 2:
+            ws.copy_(torch.randint(0, 256, ws.shape, dtype=torch.uint8, device=gpu))
+        assert torch.equal(kv8.attend(q, cache, lens), out)

@@ -12,7 +12,7 @@ import math
 import pytest
 import torch
 
-from flashact_amd import w4
+from flashact_amd import _lib, w4
 
 pytestmark = pytest.mark.gpu
 
@@ -133,3 +133,25 @@ def test_refuses_on_the_gpu(gpu):
     ):
         with pytest.raises(err, match=text):
             w4.linear(**{"x": y, "w": w, **kw})
+
+
+def test_split_sums_in_any_workspace(gpu, monkeypatch):
+    """The splits' sums meet in memory of any contents: zeros, ones, random words, an earlier call's."""
+    x, w = torch.randn(7, 16384, device=gpu).bfloat16(), w4.quantize(torch.randn(2048, 16384, device=gpu) * 0.02, 64)
+    ref = w4.linear(x, w)
+    need = w4._workspace_bytes(7, 2048, 16384)
+    ws = torch.zeros(need, dtype=torch.uint8, device=gpu)
+    real = _lib.run_on
+
+    def run_on(index, fn, a, what):
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        real(index, fn, a, what)
+
+    monkeypatch.setattr(_lib, "run_on", run_on)
+    for fill in (None, 0, 255, "random", None, None):
+        if fill == "random":
+            ws.copy_(torch.randint(0, 256, ws.shape, dtype=torch.uint8, device=gpu))
+        elif fill is not None:
+            ws.fill_(fill)
+        for _ in range(3):
+            assert torch.equal(w4.linear(x, w), ref)
