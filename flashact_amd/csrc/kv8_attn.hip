@@ -57,7 +57,9 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int b) {
 }
 // Splits that a row tile of nb blocks uses: each wave of each has a.least blocks or more.
 constexpr int MAX_SPLITS = 256;
-constexpr int FUSED = 8;  // up to so many are joined by the last workgroup, more by a kernel with workgroups enough to read them
+// Up to so many are joined by the last workgroup (32 requests of 50 to 16384 keys on 16 splits: 20.6 us, 22.6 with a kernel), more
+// by a kernel with workgroups enough to read them.
+constexpr int FUSED = 16;
 __device__ __forceinline__ int splits_used(const AttnArgs& a, int nb, int waves) {
   const unsigned per = waves * a.least;
   return max(1, min(a.S, (int)((nb + per - 1) / per)));
@@ -392,52 +394,46 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) att
   const int rows = min(16, a.T * a.G - rt * 16), own = threadIdx.x;
   f32x2 mine_ml = f32x2{-INFINITY, 0.f};
   if (own < 16 * used) mine_ml = __builtin_bit_cast(f32x2, ldb64<kCpSc1>(part, ((own >> 4) * ONE + 16 * HD + 2 * (own & 15)) * 4));
-  constexpr int PER = HD / 4, EACH = 2;  // quads of dims of a row; of these a thread's at a time
-  for (int base = 0; base < rows * PER; base += EACH * 64 * W) {
-    const int e0 = base + threadIdx.x;
-    f32x4 x[EACH][FUSED];
+  constexpr int PER = HD / 4;  // quads of dims of a row
+  for (int base = 0; base < rows * PER; base += 64 * W) {
+    const int e = base + threadIdx.x, row = e / PER, g = rt * 16 + row, tt = g / a.G;
+    const bool there = e < rows * PER;
+    f32x4 x[FUSED];
 #pragma unroll
-    for (int k = 0; k < EACH; k++)
-#pragma unroll
-      for (int s = 0; s < FUSED; s++) {
-        const int e = e0 + k * 64 * W;
-        if (s < used && e < rows * PER)
-          x[k][s] = __builtin_bit_cast(f32x4, ldb128<kCpSc1>(part, (s * ONE + e * 4) * 4));
-      }
+    for (int s = 0; s < FUSED; s++)
+      if (s < used && there) x[s] = __builtin_bit_cast(f32x4, ldb128<kCpSc1>(part, (s * ONE + e * 4) * 4));
     if (base == 0) {
       if (own < 16 * FUSED) ml[own] = mine_ml;
       __syncthreads();
     }
+    if (!there) continue;
+    float rm = -INFINITY, rl = 0.f;
 #pragma unroll
-    for (int k = 0; k < EACH; k++) {
-      const int e = e0 + k * 64 * W, row = e / PER, g = rt * 16 + row, tt = g / a.G;
-      if (e >= rows * PER) continue;
-      float rm = -INFINITY, rl = 0.f;
+    for (int s = 0; s < FUSED; s++) rm = fmaxf(rm, ml[s * 16 + row][0]);
+    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int s = 0; s < FUSED; s++) rm = fmaxf(rm, ml[s * 16 + row][0]);
-      f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < FUSED; s++)
-        if (s < used) {
-          const f32x2 v = ml[s * 16 + row];
-          const float w = v[0] == -INFINITY ? 0.f : exp2_w(v[0] - rm);
-          rl += w * v[1];
-          o += w * x[k][s];
-        }
-      if (tt >= sp.n || sp.len - sp.n + tt < 0) o = f32x4{0.f, 0.f, 0.f, 0.f}, rl = 0.f;
-      store_row4<F16>(a.out, ((size_t)b * a.T + tt) * a.H * a.G * HD + (size_t)(h * a.G + g % a.G) * HD + e % PER * 4, o * inverse(rl));
-    }
+    for (int s = 0; s < FUSED; s++)
+      if (s < used) {
+        const f32x2 v = ml[s * 16 + row];
+        const float w = v[0] == -INFINITY ? 0.f : exp2_w(v[0] - rm);
+        rl += w * v[1];
+        o += w * x[s];
+      }
+    if (tt >= sp.n || sp.len - sp.n + tt < 0) o = f32x4{0.f, 0.f, 0.f, 0.f}, rl = 0.f;
+    store_row4<F16>(a.out, ((size_t)b * a.T + tt) * a.H * a.G * HD + (size_t)(h * a.G + g % a.G) * HD + e % PER * 4, o * inverse(rl));
   }
 }
 
-// The splits' sums, in a fixed order, where there are more than FUSED. One workgroup: one row; nothing to do where its sample used one split. Threads are
-// (hd / 4) dims x groups of splits, so many splits are read side by side.
+// The splits' sums, in a fixed order, where there are more than FUSED. One workgroup: 64 dims (96) of
+// one row; nothing to do where its sample used one split. Threads are quads of dims x groups of splits, so that 16 splits are
+// read side by side (2 x 131072 keys on 128 splits: 32.3 us, 32.8 with all 256 dims in one workgroup).
 template <bool F16, int HD, int W>
 __global__ void __launch_bounds__(256) join_kernel(AttnArgs a) {
-  constexpr int SLOTS = HD / 4, GROUPS = 256 / SLOTS;
+  constexpr int DIMS = HD % 64 == 0 ? 64 : HD, SLOTS = DIMS / 4, GROUPS = 256 / SLOTS, RUNS = HD / DIMS;
   __shared__ float wt[MAX_SPLITS], red[8];
   __shared__ f32x4 sums[GROUPS][SLOTS];
-  const int rows = a.T * a.G, g = blockIdx.x % rows, bh = blockIdx.x / rows, h = bh % a.H, b = bh / a.H;
+  const int rows = a.T * a.G, unit = blockIdx.x / RUNS, run = blockIdx.x % RUNS;
+  const int g = unit % rows, bh = unit / rows, h = bh % a.H, b = bh / a.H;
   const int rt = g >> 4, row = g & 15, t = g / a.G;
   const Span sp = span_of(a, b);
   int hi = 0;  // as the attention found it: the keys that the tile's last row sees
@@ -462,7 +458,7 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a) {
   if ((i & 63) == 0) red[4 + wave] = x;
   __syncthreads();
   float L = red[4] + red[5] + red[6] + red[7];
-  const int d = (i % SLOTS) * 4, grp = i / SLOTS;
+  const int d = run * DIMS + (i % SLOTS) * 4, grp = i / SLOTS;
   f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
   if (grp < GROUPS) {
 #pragma unroll 8
@@ -523,7 +519,7 @@ int launch_waves(const AttnArgs& a, hipStream_t s) {
   if (rc != FA_OK) return rc;
   hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * W), lds, s, a);
   if (a.S > FUSED)
-    hipLaunchKernelGGL((join_kernel<F16, HD, W>), dim3((unsigned)(a.B * a.H * a.T * a.G)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((join_kernel<F16, HD, W>), dim3((unsigned)(a.B * a.H * a.T * a.G * (HD % 64 == 0 ? HD / 64 : 1))), dim3(256), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return host::fail(FA_ERR_LAUNCH, "fa_kv8_attention: %s", hipGetErrorString(e));
   return FA_OK;
