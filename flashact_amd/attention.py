@@ -3,7 +3,7 @@
 The prompt's form of attention for what the prefill's fused kernel does not take: prompts of different lengths packed one
 behind the other, a prefix that all of a document sees with causal tokens behind it (the attention pattern of PaliGemma's
 prompts, where images and instruction see each other and the answer is causal), capped scores, a distance bias, rows that
-are padding. One HIP launch (C ABI ``fa_span_attention``); a second joins the parts where few queries see many keys.
+are padding. One HIP launch (C ABI ``fa_span_attention``); a second joins the parts where few queries see very many keys.
 """
 from __future__ import annotations
 

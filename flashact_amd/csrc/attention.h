@@ -8,7 +8,7 @@
 // a wave see whole skip the masks. S^T = K Q^T and O^T += V^T P^T on the 16x16x32 MFMA: a lane holds one query's column, the
 // softmax needs two cross-lane steps, and P^T is already the second product's operand (slot 8 q + j of a 32-key step is key
 // 4 q + j of its first 16 for j < 4, key 16 + 4 q + j - 4 beyond), which the values' transposing LDS read matches.
-// Where that leaves CUs idle, the keys are split over workgroups too, whose sums go through a workspace to join_kernel.
+// Where that leaves CUs idle, the keys are split over workgroups too, whose sums meet in a workspace.
 // Keys and values of the next tiles are copied to LDS (no registers) while this one is worked on, one barrier a tile. With
 // many queries the MFMAs are the bound, next to the LDS reads that feed them (each operand of 1 KB serves 16 or 32 queries)
 // and, capped, the three exponentials a score; with few it is one wave's chain of a tile's steps, about 3000 cycles.
@@ -44,10 +44,14 @@ struct Params {
   int S, least;
   int* used;
   float* part;
+  uint64_t *arrived, nonce;  // [tile, sample, head][FUSED], where the last workgroup joins the parts
 };
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MAX_SPLITS = 256, LEAST = 8;
+// Up to so many parts are joined by the last workgroup (1024 queries over 4096 keys 43 -> 37 us, 50 over 1018 with 256 dims 24 -> 23),
+// more by a kernel with workgroups enough to read them.
+constexpr int FUSED = 4;
 
 // Chunk c (16 bytes) of row `row` lies in LDS slot c ^ turn of the row's CH slots: the same chunk of 16 rows (a key operand)
 // and the same pair of chunks of 8 rows (a value operand) meet in different banks.
@@ -500,19 +504,43 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
       __syncthreads();
       const float m1 = take[HALF * 256 + lane], l1 = take[HALF * 256 + 64 + lane], mm = fmaxf(m[0], m1);
       const float f0 = m[0] == -INFINITY ? 0.f : exp2_w(m[0] - mm), f1 = m1 == -INFINITY ? 0.f : exp2_w(m1 - mm);
-      const float sum = cols_sum(l[0] * f0 + l1 * f1);
+      float sum = cols_sum(l[0] * f0 + l1 * f1);
 #pragma unroll
       for (int j = 0; j < HALF; j++)
         O[0][J0 + j] = O[0][J0 + j] * f0 + f1 * *reinterpret_cast<const f32x4*>(take + (j * 64 + lane) * 4);
       if (used > 1) {
-        float* to = p.part + (((size_t)bh * p.ntile + tile) * p.S + split) * (NW * part_floats(NT)) + wave * part_floats(NT);
+        constexpr unsigned PART = NW * part_floats(NT) * 4;  // bytes
+        const size_t unit = (size_t)bh * p.ntile + tile;
+        const rsrc_t parts = make_rsrc(reinterpret_cast<unsigned char*>(p.part) + unit * p.S * PART, 0xffffffffu);
+        const unsigned mine = wave * (part_floats(NT) * 4);
 #pragma unroll
-        for (int j = J0; j < J0 + HALF; j++) *reinterpret_cast<f32x4*>(to + (j * 64 + lane) * 4) = O[0][j];
-        if (J0 == 0 && lane < 16) {
-          to[NT * 256 + lane] = mm;
-          to[NT * 256 + 16 + lane] = sum;
+        for (int j = J0; j < J0 + HALF; j++) {
+          const f32x4 o = O[0][j];
+          stb128<kCpSc1>(parts, split * PART + mine + (j * 64 + lane) * 16, __builtin_bit_cast(u32x4, o));
         }
-        return;
+        if (J0 == 0 && lane < 16)
+          stb64<kCpSc1>(parts, split * PART + mine + NT * 1024 + lane * 8, __builtin_bit_cast(u32x2, f32x2{mm, sum}));
+        if (p.S > FUSED || !arrived_last(p.arrived + unit * FUSED, p.nonce, split, used, ext)) return;
+        f32x2 ml[FUSED];
+        float top = -INFINITY;
+#pragma unroll
+        for (int s = 0; s < FUSED; s++) {
+          ml[s] = f32x2{-INFINITY, 0.f};
+          if (s < used) ml[s] = __builtin_bit_cast(f32x2, ldb64<kCpSc1>(parts, s * PART + mine + NT * 1024 + r * 8));
+          top = fmaxf(top, ml[s][0]);
+        }
+        sum = 0.f;
+#pragma unroll
+        for (int j = J0; j < J0 + HALF; j++) O[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < FUSED; s++)
+          if (s < used) {
+            const float w = ml[s][0] == -INFINITY ? 0.f : exp2_w(ml[s][0] - top);
+            sum += w * ml[s][1];
+#pragma unroll
+            for (int j = J0; j < J0 + HALF; j++)
+              O[0][j] += w * __builtin_bit_cast(f32x4, ldb128<kCpSc1>(parts, s * PART + mine + (j * 64 + lane) * 16));
+          }
       }
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       __syncthreads();
@@ -544,10 +572,10 @@ __global__ void __launch_bounds__(256) join_kernel(Params p) {
   const float* from = p.part + (size_t)unit * p.S * (4 * part_floats(NT)) + rows * part_floats(NT);
   const int stride = 4 * part_floats(NT), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, q = lane >> 4;
   float mm = -INFINITY;
-  for (int s = 0; s < used; s++) mm = fmaxf(mm, from[(size_t)s * stride + NT * 256 + r]);
+  for (int s = 0; s < used; s++) mm = fmaxf(mm, from[(size_t)s * stride + NT * 256 + 2 * r]);
   float sum = 0.f;
   for (int s = 0; s < used; s++) {
-    const float m = from[(size_t)s * stride + NT * 256 + r], l = from[(size_t)s * stride + NT * 256 + 16 + r];
+    const float m = from[(size_t)s * stride + NT * 256 + 2 * r], l = from[(size_t)s * stride + NT * 256 + 2 * r + 1];
     const float w = m == -INFINITY ? 0.f : exp2_w(m - mm);
     sum += w * l;
     if (tid < 16) wt[s][r] = w;
@@ -579,8 +607,8 @@ __global__ void __launch_bounds__(256) join_kernel(Params p) {
 
 // Parts that keys are split into, for workgroups of 64 queries with two groups of waves: the least of (rounds of
 // workgroups) x (steps of each, and two for its beginning and end), joining taken as three. A workgroup whose queries see
-// fewer keys makes fewer parts, of LEAST steps or more (packed prompts of 2604 tokens: 60 us with 8, 68 with 4, 62 with 16).
-// 64 queries over 65536 keys of 256 dims 1521 -> 107 us, one over 131072 of 128 dims 1534 -> 128, 1024 over 4096 56 -> 40;
+// fewer keys makes fewer parts, of LEAST steps or more (packed prompts of 2604 tokens: 59 us with 8, 64 with 4, 61 with 16).
+// 64 queries over 65536 keys of 256 dims 1521 -> 107 us, one over 131072 of 128 dims 1534 -> 126, 1024 over 4096 56 -> 36;
 // of the counts 1 .. 16 the rule's was within 8 % of the best in all of 14 shapes between.
 inline int splits_for(int64_t units, int keys, int hd) {
   const int step = hd > 128 ? 64 : 128;
@@ -596,10 +624,12 @@ inline int splits_for(int64_t units, int keys, int hd) {
 inline int64_t units_of(int batch, int queries, int heads) { return ((int64_t)queries + 63) / 64 * batch * heads; }
 // Few queries: see launch_dims.
 inline bool few(int64_t units, int hd) { return units <= (hd > 128 ? 384 : 256); }
+inline size_t used_bytes(int64_t units) { return ((size_t)units * 4 + 255) / 256 * 256; }
+inline size_t arrived_bytes(int64_t units) { return ((size_t)units * FUSED * 8 + 255) / 256 * 256; }
 inline size_t workspace(int batch, int queries, int keys, int heads, int hd) {
   const int64_t units = units_of(batch, queries, heads);
   const int S = few(units, hd) ? splits_for(units, keys, hd) : 1, nt = (hd <= 64 ? 64 : hd <= 96 ? 96 : hd <= 128 ? 128 : 256) / 16;
-  return S == 1 ? 0 : ((size_t)units * 4 + 255) / 256 * 256 + (size_t)units * S * 4 * part_floats(nt) * 4;
+  return S == 1 ? 0 : used_bytes(units) + arrived_bytes(units) + (size_t)units * S * 4 * part_floats(nt) * 4;
 }
 
 template <bool F16, int HD, int QB, int NW, int SP>
@@ -620,7 +650,7 @@ int launch(Params p, hipStream_t s) {
   const int rc = host::allow_lds(reinterpret_cast<const void*>(k), lds, "fa_span_attention");
   if (rc != FA_OK) return rc;
   hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * NW * SP), lds, s, p);
-  if (SP > 1 && p.S > 1) hipLaunchKernelGGL((join_kernel<F16, HD>), dim3((unsigned)(4 * units)), dim3(256), 0, s, p);
+  if (SP > 1 && p.S > FUSED) hipLaunchKernelGGL((join_kernel<F16, HD>), dim3((unsigned)(4 * units)), dim3(256), 0, s, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return host::fail(FA_ERR_LAUNCH, "fa_span_attention: %s", hipGetErrorString(e));
   return FA_OK;

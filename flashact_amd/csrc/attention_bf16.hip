@@ -63,7 +63,9 @@ extern "C" int fa_span_attention(const fa_span_args* a, fa_stream_t stream) {
     p.S = attn::splits_for(units, a->keys, a->head_dim);
     p.least = attn::LEAST;
     p.used = static_cast<int*>(a->workspace);
-    p.part = reinterpret_cast<float*>(static_cast<unsigned char*>(a->workspace) + (units * 4 + 255) / 256 * 256);
+    p.arrived = reinterpret_cast<uint64_t*>(static_cast<unsigned char*>(a->workspace) + attn::used_bytes(units));
+    p.part = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(p.arrived) + attn::arrived_bytes(units));
+    p.nonce = p.S <= attn::FUSED ? host::launch_nonce() : 0;
   }
   const int rc = host::check_gfx950(who);
   if (rc != FA_OK) return rc;

@@ -212,6 +212,27 @@ __device__ __forceinline__ float cols_max(float v) {
   a = swap32(as_u32(v), as_u32(v));
   return fmaxf(as_f32(a.lo), as_f32(a.hi));
 }
+// For `n` <= 64 workgroups whose sums, stored with sc1, meet in a workspace that needs no initial contents: whether this one,
+// number `i` of them, is the last to arrive, so that all sums can be read with sc1 loads. Each writes the launch's nonce into its
+// word once its sums are in memory, and then looks at all words: the last one finds the nonce in each, whatever the memory held
+// before. Nobody waits. Two may both find it, and must then store the same bits. Who does clears the words, as a captured launch
+// is replayed with the same nonce. Called by all threads; flag: in LDS, not in use.
+__device__ __forceinline__ bool arrived_last(uint64_t* words, uint64_t nonce, int i, int n, int* flag) {
+  __builtin_amdgcn_s_waitcnt(0);  // this wave's sums have arrived
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x;
+    if (lane == 0) __hip_atomic_store(words + i, nonce, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __builtin_amdgcn_s_waitcnt(0);
+    const bool there = lane >= n || __hip_atomic_load(words + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nonce;
+    const bool all = __builtin_amdgcn_ballot_w64(!there) == 0;
+    if (lane == 0) *flag = all;
+    if (all && lane < n) __hip_atomic_store(words + lane, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  return *flag != 0;
+}
+
 // Orders a wave's own LDS accesses, where a stage is private to the wave: its LDS instructions run in order.
 __device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 // Value of lane ^ 16 (selected from the swap of x with itself).

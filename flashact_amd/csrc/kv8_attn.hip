@@ -370,25 +370,10 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) att
     }
   }
   if (used == 1 || a.S > FUSED) return;
-  // The last of the tile's workgroups joins its splits, in their order. Each writes the launch's nonce into its word once its
-  // sums are in memory, and then looks at all words: the last one finds the nonce in each, whatever the workspace held
-  // before. Nobody waits. Two may both find it; they store the same bits. Who joins clears the words, as a captured launch is
-  // replayed with the same nonce. (One token of 983 keys on eight splits: 9.4 us, 9.7 with a second kernel to join, 11.4 with a
-  // counter per tile by compare and exchange, which eight that arrive together retry; 48 requests: 24.1, 26.1 with the kernel.)
-  uint64_t* words = a.arrived + ((size_t)bh * a.RT + rt) * FUSED;
-  unsigned* flag = reinterpret_cast<unsigned*>(wm);
-  __builtin_amdgcn_s_waitcnt(0);  // this wave's sums have arrived
-  __syncthreads();
-  if (wave == 0) {
-    if (lane == 0) __hip_atomic_store(words + split, a.nonce, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __builtin_amdgcn_s_waitcnt(0);
-    const bool there = lane >= used || __hip_atomic_load(words + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.nonce;
-    const bool all = __builtin_amdgcn_ballot_w64(!there) == 0;
-    if (lane == 0) *flag = all;
-    if (all && lane < used) __hip_atomic_store(words + lane, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  __syncthreads();
-  if (*flag == 0) return;
+  // The last of the tile's workgroups joins its splits, in their order. (One token of 983 keys on eight splits: 9.4 us, 9.7 with
+  // a second kernel to join, 11.4 with a counter per tile by compare and exchange, which eight that arrive together retry; 48
+  // requests: 24.1, 26.1 with the kernel.)
+  if (!arrived_last(a.arrived + ((size_t)bh * a.RT + rt) * FUSED, a.nonce, split, used, reinterpret_cast<int*>(wm))) return;
   f32x2* ml = reinterpret_cast<f32x2*>(lds);
   static_assert(16 * FUSED <= 64 * W, "a split's row a thread");
   const int rows = min(16, a.T * a.G - rt * 16), own = threadIdx.x;

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from flashact_amd import attention
+from flashact_amd import _lib, attention
 from tests import span_case as C
 
 pytestmark = pytest.mark.gpu
@@ -260,3 +260,28 @@ def test_out_is_q_or_apart_from_it(gpu, tk):
     with pytest.raises(ValueError, match="share memory"):
         attention.attend(q.view(1, 4, 40, 64).transpose(1, 2), k, v, out=q)
     assert attention.attend(q, k, v, out=q) is q and torch.equal(q, ref)
+
+
+@pytest.mark.parametrize("tq,tk,h,hkv,hd,kind", [(1100, 2100, 8, 1, 256, "causal"), (1000, 4000, 8, 2, 64, "random"),
+                                                 (2300, 2300, 8, 1, 256, "documents")])
+def test_parts_in_any_workspace(gpu, monkeypatch, tq, tk, h, hkv, hd, kind):
+    """The workgroups that share a tile count themselves in memory of any contents: ones, random words, an earlier call's."""
+    q, k, v = _qkv(gpu, 1, tq, tk, h, hkv, hd, torch.float16, seed=tk)
+    spans = _spans(gpu, kind, 1, tq, tk)
+    ref, bound = C.attend(q, k, v, spans)
+    need = attention._workspace_bytes(1, tq, tk, h, hd)
+    assert need
+    ws = torch.full((need,), 255, dtype=torch.uint8, device=gpu)
+    real = _lib.run_on
+
+    def run_on(index, fn, a, what):
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        real(index, fn, a, what)
+
+    monkeypatch.setattr(_lib, "run_on", run_on)
+    out = attention.attend(q, k, v, spans)
+    C.check(out, ref, bound)
+    for i in range(5):
+        if i == 2:
+            ws.copy_(torch.randint(0, 256, ws.shape, dtype=torch.uint8, device=gpu))
+        assert torch.equal(attention.attend(q, k, v, spans), out)
