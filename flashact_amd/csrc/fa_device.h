@@ -215,9 +215,10 @@ __device__ __forceinline__ float cols_max(float v) {
 // For `n` <= 64 workgroups whose sums, stored with sc1, meet in a workspace that needs no initial contents: whether this one,
 // number `i` of them, is the last to arrive, so that all sums can be read with sc1 loads. Each writes the launch's nonce into its
 // word once its sums are in memory, and then looks at all words: the last one finds the nonce in each, whatever the memory held
-// before. Nobody waits. Two may both find it, and must then store the same bits. Who does clears the words, as a captured launch
-// is replayed with the same nonce. Called by all threads; flag: in LDS, not in use.
-__device__ __forceinline__ bool arrived_last(uint64_t* words, uint64_t nonce, int i, int n, int* flag) {
+// before. Nobody waits. Two may both find it, and must then store the same bits, or, where they cannot, give a `claim`: a word
+// that number 0 has set to 0 in its first wave before the call, and that the first of the two takes. Who finds the nonce in all
+// clears the words, as a captured launch is replayed with the same nonce. Called by all threads; flag: in LDS, not in use.
+__device__ __forceinline__ bool arrived_last(uint64_t* words, uint64_t nonce, int i, int n, int* flag, uint64_t* claim = nullptr) {
   __builtin_amdgcn_s_waitcnt(0);  // this wave's sums have arrived
   __syncthreads();
   if (threadIdx.x < 64) {
@@ -226,7 +227,8 @@ __device__ __forceinline__ bool arrived_last(uint64_t* words, uint64_t nonce, in
     __builtin_amdgcn_s_waitcnt(0);
     const bool there = lane >= n || __hip_atomic_load(words + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nonce;
     const bool all = __builtin_amdgcn_ballot_w64(!there) == 0;
-    if (lane == 0) *flag = all;
+    if (lane == 0)
+      *flag = all && (!claim || __hip_atomic_exchange(claim, nonce, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != nonce);
     if (all && lane < n) __hip_atomic_store(words + lane, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();

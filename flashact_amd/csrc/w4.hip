@@ -35,7 +35,8 @@ struct Params {
   const float* bias;
   const float* residual;
   void* out;
-  float* part;  // [split][M][N padded to 16] where K is split across workgroups
+  float* part;  // [workgroup's tiles][split][pair of outputs][2] where K is split across workgroups
+  uint64_t *arrived, nonce;  // [workgroup's tiles][WORDS]: a word a split, and the claim
   int M, N, K, nch, out_dtype, gate;
 };
 
@@ -93,6 +94,7 @@ __device__ __forceinline__ void finish(const Params& p, int m, int n, float y0, 
   }
 }
 
+constexpr int MAX_SPLITS = 16, WORDS = MAX_SPLITS + 1;
 constexpr int max_waves(int MR, int NT) { return MR <= 16 && NT == 1 ? 16 : 8; }  // of a workgroup at most, by registers and LDS
 
 // MR: rows of x the LDS stage holds (1, 4, 16, 32 or 64); XC: chunks a stage; NT: weight tiles a workgroup; RUN:
@@ -108,7 +110,9 @@ struct Shape {
   static_assert(RUN % XC == 0 && RUN * GC <= 16, "a run is whole stages, its scales one row of lanes");
 };
 
-template <bool F16, int GROUP, int MR, int XC, int NT, int RUN>
+// SPLIT: K is split across workgroups (blockIdx.y). A kernel of its own: with the join behind it, the unsplit one of four tiles a
+// workgroup, whose loop has all registers, ran 32768 x 2048 in 11.4 us instead of 9.6.
+template <bool F16, int GROUP, int MR, int XC, int NT, int RUN, bool SPLIT>
 __global__ void __launch_bounds__(64 * max_waves(MR, NT)) w4_kernel(Params p) {
   using S = Shape<GROUP, MR, XC, NT, RUN>;
   constexpr int MB = S::MB, GC = S::GC;
@@ -118,7 +122,7 @@ __global__ void __launch_bounds__(64 * max_waves(MR, NT)) w4_kernel(Params p) {
   const int ntile = (p.N + 15) >> 4;
   const int t0 = blockIdx.x * NT;
   unsigned char* xl = lds + wave * S::XBYTES;
-  const int part = blockIdx.y * W + wave, parts = gridDim.y * W;  // of K: contiguous ranges of chunks
+  const int part = SPLIT ? blockIdx.y * W + wave : wave, parts = SPLIT ? gridDim.y * W : W;  // of K: contiguous ranges of chunks
   const int cb = (int)((int64_t)p.nch * part / parts), ce = (int)((int64_t)p.nch * (part + 1) / parts);
 
   f32x4 acc[NT][MB];
@@ -225,38 +229,49 @@ __global__ void __launch_bounds__(64 * max_waves(MR, NT)) w4_kernel(Params p) {
       *reinterpret_cast<f32x4*>(lds + (((wave * NT + t) * MB + b) * 64 + lane) * 16) = acc[t][b];
   __syncthreads();
   // one thread per output pair (rows 2f, 2f + 1 of the tile) and row of x
-  for (int e = threadIdx.x; e < NT * MB * 128; e += blockDim.x) {
-    const int tb = e >> 7, pr = e & 7, col = (e >> 3) & 15;  // tile and block, pair, row of x within the block
-    const int m = (tb % MB) * 16 + col, n = (t0 + tb / MB) * 16 + 2 * pr;
-    if (m >= p.M || n >= p.N) continue;
+  constexpr int PAIRS = NT * MB * 128;
+  auto pairs = [&](auto&& each) {
+    for (int e = threadIdx.x; e < PAIRS; e += blockDim.x) {
+      const int tb = e >> 7, pr = e & 7, col = (e >> 3) & 15;  // tile and block, pair, row of x within the block
+      const int m = (tb % MB) * 16 + col, n = (t0 + tb / MB) * 16 + 2 * pr;
+      if (m < p.M && n < p.N) each(e, tb, pr, col, m, n);
+    }
+  };
+  auto sum = [&](int tb, int pr, int col) {
     const float* s = reinterpret_cast<const float*>(lds) + (tb * 64 + (pr >> 1) * 16 + col) * 4 + (pr & 1) * 2;
-    float y0 = 0.f, y1 = 0.f;
+    f32x2 y = f32x2{0.f, 0.f};
     for (int w = 0; w < W; w++) {
-      y0 += s[w * NT * MB * 256];
-      y1 += s[w * NT * MB * 256 + 1];
+      y[0] += s[w * NT * MB * 256];
+      y[1] += s[w * NT * MB * 256 + 1];
     }
-    if (gridDim.y > 1) {  // w4_join_kernel adds the splits and finishes
-      *reinterpret_cast<f32x2*>(p.part + ((size_t)blockIdx.y * p.M + m) * ntile * 16 + n) = f32x2{y0, y1};
-      continue;
-    }
-    finish(p, m, n, y0, y1);
-  }
-}
-
-// The splits' sums, in their order, and what follows the product.
-__global__ void __launch_bounds__(256) w4_join_kernel(Params p, int splits) {
-  const int pairs = (p.N + 1) >> 1, i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= pairs * p.M) return;
-  const int m = i / pairs, n = 2 * (i - m * pairs);
-  const size_t row = (size_t)((p.N + 15) >> 4) * 16;
-  float y0 = 0.f, y1 = 0.f;
+    return y;
+  };
+  if constexpr (!SPLIT) {
+    pairs([&](int, int tb, int pr, int col, int m, int n) {
+      const f32x2 y = sum(tb, pr, col);
+      finish(p, m, n, y[0], y[1]);
+    });
+  } else {
+    // The last of the splits' workgroups adds them in their order and finishes: once, as the result may lie over the residual.
+    uint64_t* words = p.arrived + (size_t)blockIdx.x * WORDS;
+    if (blockIdx.y == 0 && threadIdx.x == 0)
+      __hip_atomic_store(words + MAX_SPLITS, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const rsrc_t sums = make_rsrc(p.part + (size_t)blockIdx.x * gridDim.y * PAIRS * 2, 0xffffffffu);
+    pairs([&](int e, int tb, int pr, int col, int, int) {
+      stb64<kCpSc1>(sums, (blockIdx.y * PAIRS + e) * 8, __builtin_bit_cast(u32x2, sum(tb, pr, col)));
+    });
+    if (!arrived_last(words, p.nonce, blockIdx.y, gridDim.y, reinterpret_cast<int*>(lds), words + MAX_SPLITS)) return;
+    pairs([&](int e, int, int, int, int m, int n) {
+      float y0 = 0.f, y1 = 0.f;
 #pragma unroll 8
-  for (int s = 0; s < splits; s++) {
-    const f32x2 v = *reinterpret_cast<const f32x2*>(p.part + ((size_t)s * p.M + m) * row + n);
-    y0 += v[0];
-    y1 += v[1];
+      for (unsigned s = 0; s < gridDim.y; s++) {
+        const f32x2 v = __builtin_bit_cast(f32x2, ldb64<kCpSc1>(sums, (s * PAIRS + e) * 8));
+        y0 += v[0];
+        y1 += v[1];
+      }
+      finish(p, m, n, y0, y1);
+    });
   }
-  finish(p, m, n, y0, y1);
 }
 
 // How a product is cut: tiles a workgroup, splits of K across workgroups, waves a workgroup. Times in us of both sides, in
@@ -275,11 +290,11 @@ Cut cut(int M, int N, int K) {
   else if (M > 16) c.nt = 2;
   else if (tiles >= 1024 || (M > 4 && tiles >= 64 && tiles < 256 && nch >= 96)) c.nt = 4;
   const int blocks = (tiles + c.nt - 1) / c.nt, most = M <= 16 && c.nt == 1 ? 16 : 8;
-  // Splits cost a second launch, about 2 us. With one tile and few rows 16 waves share K already, and only a handful of
+  // Splits cost the join of the last workgroup, about 2 us. With one tile and few rows 16 waves share K already, and only a handful of
   // workgroups needs more (64 x 16384: 5.5 instead of 8.0, but 2048 x 8192 in two 7.7 instead of 5.8); else K is split until there is a
   // workgroup a CU (2048 x 16384: 10.0 instead of 24.3 at M = 5, 14.8 instead of 24.6 at 32, 20.7 instead of 28.7 at 48), in
   // parts of 2048 columns or more (2048 x 2048 in two at M = 32: 7.7 instead of 6.6).
-  c.splits = std::max(1, std::min({(most == 16 ? 32 : 256) / blocks, nch / 16, 16}));
+  c.splits = std::max(1, std::min({(most == 16 ? 32 : 256) / blocks, nch / 16, MAX_SPLITS}));
   const int mine = (nch + c.splits - 1) / c.splits;
   // Waves: 4096 in all, with two tiles 2048 (16384 x 2048 at M = 32: 11.4 instead of 13.2), of two chunks each or more
   // (2560 x 2048: 4.1 instead of 4.7 at M = 5, 3.7 instead of 3.9 at 1), and no fewer than four (32768 x 2048 with four
@@ -288,19 +303,18 @@ Cut cut(int M, int N, int K) {
   return c;
 }
 
-template <bool F16, int GROUP, int MR, int XC, int NT, int RUN>
+template <bool F16, int GROUP, int MR, int XC, int NT, int RUN, bool SPLIT = false>
 int launch_shape(const Params& p, const Cut& c, hipStream_t stream) {
+  if constexpr (!SPLIT && !(MR <= 4 && NT == 4))  // these have workgroups enough
+    if (c.splits > 1) return launch_shape<F16, GROUP, MR, XC, NT, RUN, true>(p, c, stream);
   using S = Shape<GROUP, MR, XC, NT, RUN>;
   const int blocks = ((p.N + 15) / 16 + NT - 1) / NT;
   const unsigned lds = (unsigned)(c.waves * S::XBYTES);
-  const void* k = reinterpret_cast<const void*>(&w4_kernel<F16, GROUP, MR, XC, NT, RUN>);
+  const void* k = reinterpret_cast<const void*>(&w4_kernel<F16, GROUP, MR, XC, NT, RUN, SPLIT>);
   int rc = host::allow_lds(k, max_waves(MR, NT) * S::XBYTES, "fa_w4_linear");
   if (rc != FA_OK) return rc;
-  hipLaunchKernelGGL((w4_kernel<F16, GROUP, MR, XC, NT, RUN>), dim3(blocks, c.splits), dim3(64 * c.waves), lds, stream,
+  hipLaunchKernelGGL((w4_kernel<F16, GROUP, MR, XC, NT, RUN, SPLIT>), dim3(blocks, c.splits), dim3(64 * c.waves), lds, stream,
                      p);
-  if (c.splits > 1)
-    hipLaunchKernelGGL(w4_join_kernel, dim3((unsigned)(((size_t)(p.N + 1) / 2 * p.M + 255) / 256)), dim3(256), 0, stream,
-                       p, c.splits);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return host::fail(FA_ERR_LAUNCH, "fa_w4_linear: %s", hipGetErrorString(e));
   return FA_OK;
@@ -325,8 +339,12 @@ int launch_group(const Params& p, const Cut& c, int group, hipStream_t s) {
   return launch_rows<F16, 128>(p, c, s);
 }
 
+size_t blocks_of(const Cut& c, int N) { return ((N + 15) / 16 + c.nt - 1) / c.nt; }
+size_t arrived_bytes(const Cut& c, int N) { return (blocks_of(c, N) * WORDS * sizeof(uint64_t) + 255) / 256 * 256; }
 size_t part_bytes(const Cut& c, int M, int N) {
-  return c.splits > 1 ? (size_t)c.splits * M * ((N + 15) / 16 * 16) * sizeof(float) : 0;
+  if (c.splits == 1) return 0;
+  const int rows = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+  return arrived_bytes(c, N) + blocks_of(c, N) * c.splits * c.nt * rows * 16 * sizeof(float);
 }
 
 }  // namespace w4
@@ -379,7 +397,9 @@ extern "C" int fa_w4_linear(const fa_w4_args* a, fa_stream_t stream) {
                a->bias,
                a->residual,
                a->out,
-               static_cast<float*>(a->workspace),
+               need ? reinterpret_cast<float*>(static_cast<unsigned char*>(a->workspace) + w4::arrived_bytes(c, a->n)) : nullptr,
+               static_cast<uint64_t*>(a->workspace),
+               need ? host::launch_nonce() : 0,
                a->rows,
                a->n,
                a->k,

@@ -155,3 +155,15 @@ def test_split_sums_in_any_workspace(gpu, monkeypatch):
             ws.fill_(fill)
         for _ in range(3):
             assert torch.equal(w4.linear(x, w), ref)
+
+
+@pytest.mark.parametrize("rows,n,k", [(7, 2048, 16384), (1, 64, 16384), (40, 1024, 8192), (20, 512, 4096)])
+def test_split_sums_over_the_residual(gpu, rows, n, k):
+    """The result takes the residual's place: it is added once, whichever workgroup joins the splits."""
+    assert w4._workspace_bytes(rows, n, k) > 0
+    x, w = torch.randn(rows, k, device=gpu).bfloat16(), w4.quantize(torch.randn(n, k, device=gpu) * 0.02, 32)
+    r = torch.randn(rows, n, device=gpu)
+    ref = w4.linear(x, w, residual=r)
+    for _ in range(20):
+        out = r.clone()
+        assert w4.linear(x, w, residual=out, out=out) is out and torch.equal(out, ref)
