@@ -285,3 +285,15 @@ def test_parts_in_any_workspace(gpu, monkeypatch, tq, tk, h, hkv, hd, kind):
         if i == 2:
             ws.copy_(torch.randint(0, 256, ws.shape, dtype=torch.uint8, device=gpu))
         assert torch.equal(attention.attend(q, k, v, spans), out)
+
+
+def test_parts_of_inputs_in_turn(gpu):
+    """Calls that reuse one another's workspace take no sum of an earlier one."""
+    _, k, v = _qkv(gpu, 1, 1, 4096, 8, 1, 128, torch.bfloat16)
+    qs = [torch.randn(1, 1024, 8, 128, device=gpu).bfloat16() for _ in range(3)]
+    refs = [attention.attend(q, k, v) for q in qs]
+    bad = torch.zeros((), dtype=torch.int64, device=gpu)
+    for i in range(600):
+        j = (i * 7 + i // 5) % 3
+        bad += (attention.attend(qs[j], k, v) != refs[j]).any()
+    assert not torch.equal(refs[0], refs[1]) and bad.item() == 0

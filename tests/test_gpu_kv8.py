@@ -341,3 +341,15 @@ def test_split_sums_in_any_workspace(gpu, monkeypatch, b, tokens, h, hkv, hd, le
         if i == 2:
             ws.copy_(torch.randint(0, 256, ws.shape, dtype=torch.uint8, device=gpu))
         assert torch.equal(kv8.attend(q, cache, lens), out)
+
+
+def test_split_sums_of_inputs_in_turn(gpu):
+    """Calls that reuse one another's workspace take no sum of an earlier one."""
+    cache, lens = _filled(gpu, 3, 1000, 1, 256, seed=2), _ints(gpu, 1000, 777, 40)
+    qs = [torch.randn(3, 5, 8, 256, device=gpu).bfloat16() for _ in range(3)]
+    refs = [kv8.attend(q, cache, lens) for q in qs]
+    bad = torch.zeros((), dtype=torch.int64, device=gpu)
+    for i in range(600):
+        j = (i * 7 + i // 5) % 3
+        bad += (kv8.attend(qs[j], cache, lens) != refs[j]).any()
+    assert not torch.equal(refs[0], refs[1]) and bad.item() == 0

@@ -167,3 +167,15 @@ def test_split_sums_over_the_residual(gpu, rows, n, k):
     for _ in range(20):
         out = r.clone()
         assert w4.linear(x, w, residual=out, out=out) is out and torch.equal(out, ref)
+
+
+def test_split_sums_of_inputs_in_turn(gpu):
+    """Calls that reuse one another's workspace take no sum of an earlier one."""
+    w = w4.quantize(torch.randn(2048, 16384, device=gpu) * 0.02, 32)
+    xs = [torch.randn(9, 16384, device=gpu).bfloat16() for _ in range(3)]
+    refs = [w4.linear(x, w) for x in xs]
+    bad = torch.zeros((), dtype=torch.int64, device=gpu)
+    for i in range(600):
+        j = (i * 7 + i // 5) % 3
+        bad += (w4.linear(xs[j], w) != refs[j]).any()
+    assert not torch.equal(refs[0], refs[1]) and bad.item() == 0
