@@ -62,14 +62,6 @@ __device__ __forceinline__ int turn(int row) {
   else return ((row & 7) << 1) | ((row >> 3) & 1);
 }
 
-__device__ __forceinline__ void copy16(const unsigned char* base, unsigned off, unsigned lds) {
-  unsigned saved;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-               : "=&s"(saved)
-               : "v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds))
-               : "memory");
-}
-
 #define ATTN_VMCNT(n) (((n) & 15) | (((n) >> 4) << 14) | (7 << 4) | (15 << 8))
 // Waits until at most n (wave-uniform: 2, 4, 6, 8, 12, 16, or else 0) copies or loads of this wave are outstanding.
 __device__ __forceinline__ void vm_wait(int n) {
@@ -238,8 +230,8 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
 #pragma unroll
       for (int n = 0; n < PER; n++) {
         if (COPIES % NW && n * NW + wave >= COPIES) break;
-        copy16(kp, koff[n], to + n * NW * 1024);
-        copy16(vp, voff[n], to + n * NW * 1024 + TILE);
+        copy_to_lds(kp, koff[n], to + n * NW * 1024);
+        copy_to_lds(vp, voff[n], to + n * NW * 1024 + TILE);
       }
       return;
     }
@@ -251,8 +243,8 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
       const int slot = (n * NW + wave) * 64 + ln, row = slot / CH, c = (slot % CH) ^ turn<CH>(row);
       const unsigned at = min(row, p.Tk - 1 - key);
       if (c * 8 < p.hd) {
-        copy16(kp, at * (unsigned)(p.kt * 2) + c * 16, to + n * NW * 1024);
-        copy16(vp, at * (unsigned)(p.vt * 2) + c * 16, to + n * NW * 1024 + TILE);
+        copy_to_lds(kp, at * (unsigned)(p.kt * 2) + c * 16, to + n * NW * 1024);
+        copy_to_lds(vp, at * (unsigned)(p.vt * 2) + c * 16, to + n * NW * 1024 + TILE);
       }
     }
   };

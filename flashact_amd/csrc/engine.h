@@ -83,38 +83,11 @@ __device__ __forceinline__ int vwg() {
 }
 
 // ---------------------------------------------------------------- global <-> LDS copies
-// global_load_lds_dwordx4: lane i copies 16 bytes from its address to LDS m0 + 16 i, so one
-// instruction lands one 1 KB MFMA fragment in lane order. m0 is saved and restored.
-template <bool SC1>
-__device__ __forceinline__ void dma16(const void* g, uint32_t lds_addr) {
-  unsigned saved;
-  if (SC1)
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off sc1\n\ts_mov_b32 m0, %0"
-                 : "=&s"(saved)
-                 : "v"(g), "s"(__builtin_amdgcn_readfirstlane(lds_addr))
-                 : "memory");
-  else
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-                 : "=&s"(saved)
-                 : "v"(g), "s"(__builtin_amdgcn_readfirstlane(lds_addr))
-                 : "memory");
-}
-
 #define FA_ENG_VMCNT(n) (((n) & 15) | (((n) >> 4) << 14) | (7 << 4) | (15 << 8))
 template <int N>
 __device__ __forceinline__ void vm_wait() {
   __builtin_amdgcn_s_waitcnt(FA_ENG_VMCNT(N));
   asm volatile("" ::: "memory");
-}
-
-// The same copy with a wave-uniform 64-bit base in SGPRs and a 32-bit per-lane byte offset (one VGPR
-// per copy address instead of two).
-__device__ __forceinline__ void dma16s(const void* base, uint32_t voff, uint32_t lds_addr) {
-  unsigned saved;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-               : "=&s"(saved)
-               : "v"(voff), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds_addr))
-               : "memory");
 }
 
 __device__ __forceinline__ uint32_t lds_addr(uint32_t off) { return (uint32_t)(uintptr_t)lds + off; }
@@ -290,9 +263,9 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int m0, int n0, int
     for (int j = 0; j < S::IPW; j++) {
       const int f = w + NWAVE * j;
       if (f < S::NA)
-        dma16<true>(src[j] + (AF ? 4096 : 256) * s, lds_addr(base + f * S::PITCH));
+        copy_to_lds<true>(src[j] + (AF ? 4096 : 256) * s, lds_addr(base + f * S::PITCH));
       else
-        dma16<false>(src[j] + 256 * s, lds_addr(base + f * S::PITCH));
+        copy_to_lds(src[j] + 256 * s, lds_addr(base + f * S::PITCH));
     }
   };
   f32x4 acc[WN][WM];
@@ -541,7 +514,7 @@ __device__ __forceinline__ void gemm_tile_d(const GemmArgsF& g, int m0, int n0, 
   u32x4 a[NA];  // [WM ks + i]: token block tb0 + i, k-step ks of the current 128-k step
   auto issue_w = [&](int s, int j) {
     const int f = w + NWAVE * j;
-    dma16s(wbase, wlane + (uint32_t)((64 * (f >> 4) + (f & 15)) * g.ldw * 2 + 256 * s),
+    copy_to_lds(wbase, wlane + (uint32_t)((64 * (f >> 4) + (f & 15)) * g.ldw * 2 + 256 * s),
            lds_addr((uint32_t)(s & 3) * TALL_ST + f * 1040));
   };
   // Token blocks past M read zeros (the descriptor's bound) and their MFMAs run on them: no branch

@@ -212,6 +212,34 @@ __device__ __forceinline__ float cols_max(float v) {
   a = swap32(as_u32(v), as_u32(v));
   return fmaxf(as_f32(a.lo), as_f32(a.hi));
 }
+// 1 KB from global memory to LDS without registers (global_load_lds_dwordx4): lane i's 16 bytes land at lds + 16 i, so one
+// instruction brings an MFMA fragment in lane order. Inline asm, as the compiler drains the builtin's copies at waits that it inserts
+// for other memory operations; m0, which it reserves, is saved and restored. What it would see to between its own instructions is
+// in the string: a copy needs one wait state behind the scalar write of m0, and five behind a vector instruction
+// (readfirstlane) that wrote its scalar base, of which the two moves are two.
+template <bool SC1 = false>
+__device__ __forceinline__ void copy_to_lds(const void* from, unsigned lds) {  // each lane from its own address
+  unsigned saved;
+  if constexpr (SC1)
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off sc1\n\ts_mov_b32 m0, %0"
+                 : "=&s"(saved)
+                 : "v"(from), "s"(__builtin_amdgcn_readfirstlane(lds))
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(saved)
+                 : "v"(from), "s"(__builtin_amdgcn_readfirstlane(lds))
+                 : "memory");
+}
+// base: the same in all lanes; off: bytes from there, each lane's own (one register an address instead of two)
+__device__ __forceinline__ void copy_to_lds(const void* base, unsigned off, unsigned lds) {
+  unsigned saved;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 2\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+               : "=&s"(saved)
+               : "v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds))
+               : "memory");
+}
+
 // For `n` <= 64 workgroups whose sums, stored with sc1, meet in a workspace that needs no initial contents: whether this one,
 // number `i` of them, is the last to arrive, so that all sums can be read with sc1 loads. Each writes the launch's nonce into its
 // word once its sums are in memory, and then looks at all words: the last one finds the nonce in each, whatever the memory held

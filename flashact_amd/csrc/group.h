@@ -158,18 +158,13 @@ __device__ __forceinline__ void page_release(const Ctx& c, int upto) {
   if (c.lane == 0) ctl_st<K>(2 + c.wave, (unsigned)upto);
 }
 
-// global_load_lds_dwordx4 with a wave-uniform base and a 32-bit lane offset: lane i copies 16 bytes to
-// LDS m0 + 16 i (fragments in the order of copy_row / copy_chunk).
+// A copy to LDS from a wave-uniform base and a 32-bit lane offset (fragments in the order of copy_row / copy_chunk).
 __device__ __forceinline__ void dma16(const unsigned char* base, uint32_t voff, uint32_t lds) {
-  unsigned saved;
   // (each half is cast to uint32_t before widening: readfirstlane returns int)
   const uint64_t a = reinterpret_cast<uint64_t>(base);
   const uint64_t u = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)) << 32 |
                      (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a);
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-               : "=&s"(saved)
-               : "v"(voff), "s"(u), "s"(__builtin_amdgcn_readfirstlane(lds))
-               : "memory");
+  copy_to_lds(reinterpret_cast<const void*>(u), voff, lds);
 }
 
 #define FA_PG_VMCNT(n) (((n) & 15) | (((n) >> 4) << 14) | (7 << 4) | (15 << 8))

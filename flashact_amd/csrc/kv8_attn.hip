@@ -96,15 +96,7 @@ __device__ __forceinline__ void store_row4(unsigned char* out, size_t at, f32x4 
 // 1 / l of a row: no keys give zeros, NaN stays.
 __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
-// 1 KB from global memory to LDS: lane i brings 16 bytes from base + 16 i to lds + 16 i. Inline asm, so that the compiler
-// does not drain these copies at waits of its own; vm_wait<N> waits until at most N are outstanding.
-__device__ __forceinline__ void copy1k(const unsigned char* base, unsigned lane16, unsigned lds) {
-  unsigned saved;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-               : "=&s"(saved)
-               : "v"(lane16), "s"(base), "s"(lds)
-               : "memory");
-}
+// Waits until at most N copies to LDS (or loads) of this wave are outstanding.
 template <int N>
 __device__ __forceinline__ void vm_wait() {
   __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
@@ -181,7 +173,7 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) att
   auto copy = [&](const unsigned char* from, int blk, unsigned to) {
     const unsigned char* p = from + (unit + blk) * (BT * HD);
 #pragma unroll
-    for (int i = 0; i < NC; i++) copy1k(p + i * 1024, lane * 16, to + i * 1024);
+    for (int i = 0; i < NC; i++) copy_to_lds(p + i * 1024, lane * 16, to + i * 1024);
   };
 
   f32x4 O[NT];

@@ -477,12 +477,12 @@ __device__ __forceinline__ void catt_copy(const Params& p, int l, int it, uint32
       const int kt = f / 3, ks = f - 3 * kt;
       int key = key0 + 32 * (kt >> 1) + 8 * (lr >> 2) + 4 * (kt & 1) + (lr & 3);
       if (key >= p.Lk) key = 0;
-      dma16<false>(kb_ + (size_t)key * D + ks * 32 + 8 * g4, lds_addr(cb + C_K + f * 1024));
+      copy_to_lds(kb_ + (size_t)key * D + ks * 32 + 8 * g4, lds_addr(cb + C_K + f * 1024));
     } else {  // V^T fragment (dim tile dt, span sp)
       const int fv = f - 24, dt = fv >> 2, sp = fv & 3;
       int kg = key0 + 32 * sp + 8 * g4;
       if (kg >= p.Lk) kg = 0;
-      dma16<false>(vb_ + (size_t)(16 * dt + lr) * p.Lkmax + kg, lds_addr(cb + C_V + fv * 1024));
+      copy_to_lds(vb_ + (size_t)(16 * dt + lr) * p.Lkmax + kg, lds_addr(cb + C_V + fv * 1024));
     }
   }
 }

@@ -636,7 +636,7 @@ __device__ __forceinline__ void copy_gu(const Params& p, const Ctx& c, int l) {
 #pragma unroll
   for (int q = 0; q < 24; q++) {  // fragment (wave w2, row tile rt, k-step j) of this wave's half
     const int w2 = 2 * (c.w & 1) + q / 12, rt = (q / 6) & 1, j = q % 6;
-    dma16<false>((rt ? r1 : r0) + 32 * (6 * w2 + j), lds_addr(L_GU + ((w2 * 2 + rt) * 6 + j) * 1024));
+    copy_to_lds((rt ? r1 : r0) + 32 * (6 * w2 + j), lds_addr(L_GU + ((w2 * 2 + rt) * 6 + j) * 1024));
   }
 }
 // 16 weight rows x 768 to LDS [4 waves][6 k-steps][1 KB], by waves W0..3.
@@ -647,7 +647,7 @@ __device__ __forceinline__ void copy16(const Ctx& c, const bf16* W, int row, uin
 #pragma unroll
   for (int q = 0; q < N; q++) {
     const int f = N * (c.w - W0) + q;
-    dma16<false>(r + 32 * f, lds_addr(dst + f * 1024));
+    copy_to_lds(r + 32 * f, lds_addr(dst + f * 1024));
   }
 }
 __device__ __forceinline__ void copy_dn(const Params& p, const Ctx& c, int l) {
@@ -657,7 +657,7 @@ __device__ __forceinline__ void copy_dn(const Params& p, const Ctx& c, int l) {
 #pragma unroll
   for (int q = 0; q < 8; q++) {
     const int f = 8 * (c.w - 1) + q;  // row tile f / 12, k-step f % 12
-    dma16<false>((f >= 12 ? r1 : r0) + 32 * (f >= 12 ? f - 12 : f), lds_addr(L_DN + f * 1024));
+    copy_to_lds((f >= 12 ? r1 : r0) + 32 * (f >= 12 ? f - 12 : f), lds_addr(L_DN + f * 1024));
   }
 }
 

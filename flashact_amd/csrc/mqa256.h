@@ -135,7 +135,7 @@ __device__ __forceinline__ void stage_att(const P& p, rsrc_t ws, int l) {
       const int f = w + NWAVE * j, h = f >> 5, sl = f & 31, kt = sl >> 4, i = sl & 15;
       int key = key0 + 32 * lq + 8 * (i >> 2) + 4 * kt + (i & 3);
       if (key >= Ltot) key = 0;
-      dma16<true>(kb_ + (size_t)key * HD + 128 * h + 8 * lr, lds_addr(f * ATT_PITCH));
+      copy_to_lds<true>(kb_ + (size_t)key * HD + 128 * h + 8 * lr, lds_addr(f * ATT_PITCH));
     }
     load_q(0);
     vm_wait<0>();
@@ -145,7 +145,7 @@ __device__ __forceinline__ void stage_att(const P& p, rsrc_t ws, int l) {
       const int y = w + NWAVE * j;
       int kg = key0 + 8 * lr;
       if (kg >= Ltot) kg = 0;
-      dma16<true>(vb_ + (size_t)(y + 64 * lq) * p.Lmax + kg, lds_addr(ATT_VB + y * ATT_PITCH));
+      copy_to_lds<true>(vb_ + (size_t)(y + 64 * lq) * p.Lmax + kg, lds_addr(ATT_VB + y * ATT_PITCH));
     }
     // two query tiles per pass (qt, qt + NWAVE): every K / V^T fragment read from LDS feeds 2 MFMAs
     constexpr int NPASS = QTG / (2 * NWAVE);

@@ -244,16 +244,6 @@ __device__ __forceinline__ void page_release(const Ctx& c, int upto) {
   if (c.lane == 0) ctl_st(2 + c.wave, (unsigned)upto);
 }
 
-__device__ __forceinline__ void dma16(const void* g, uint32_t lds_addr) {
-  // global_load_lds_dwordx4: lane i copies 16 bytes from g to LDS m0 + 16 i. Inline asm keeps the compiler from draining these copies at waits it
-  // inserts for other memory operations; m0 is saved and restored (the compiler reserves it).
-  unsigned saved;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-               : "=&s"(saved)
-               : "v"(g), "s"(__builtin_amdgcn_readfirstlane(lds_addr))
-               : "memory");
-}
-
 __device__ __forceinline__ int qkv_row(int g, int vr) {
   return vr < 256 ? 256 * g + vr : (vr < 512 ? 2048 + (vr - 256) : 2304 + (vr - 512));
 }
@@ -409,7 +399,7 @@ __device__ void loader_main(const Params& p, const Ctx& c, int lw) {
       const unsigned char* src = L.b[i] + (size_t)l * lstride;
       const uint32_t dst = c.lds_addr + (uint32_t)(pg % RING) * PAGE + lw * 8 * 1024;
 #pragma unroll
-      for (int ff = 0; ff < 8; ff++) dma16(src + (ff & fmask) * fstride, dst + ff * 1024);
+      for (int ff = 0; ff < 8; ff++) copy_to_lds(src + (ff & fmask) * fstride, dst + ff * 1024);
       if (tr && c.lane == 0 && pg >= tpg0 && pg < tpg0 + PPL) tr[2 * (pg - tpg0)] = __builtin_amdgcn_s_memrealtime();
     }
   }
