@@ -39,6 +39,7 @@ struct Params {
   int B, Tq, Tk, H, G, hd, ntile, stages;
   // base 2: scale log2(e); capped, 2 log2(e) scale / cap for tanh_far, scale / cap for tanh_near, and cap log2(e)
   float scale, over, cap;
+  int flat;  // the scale is zero: see where the queries are loaded
   // where keys are split over workgroups: into up to S parts of `least` steps or more; the parts that each (tile, sample,
   // head) was split into, and their sums, 64 rows of {O[hd], m, l} each as a wave's lanes hold them
   int S, least;
@@ -268,6 +269,16 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
   for (int x = 0; x < QB; x++)
 #pragma unroll
     for (int i = 0; i < NK; i++) asm volatile("" : "+v"(qf[x][i]));
+  // A scale of zero would take masked scores (-inf) to NaN as the unit of a tile's scores. It leaves of a query only what is not
+  // finite (0 x inf is NaN), so the query is what is scaled, and the unit becomes one.
+  if (p.flat) {
+#pragma unroll
+    for (int x = 0; x < QB; x++)
+#pragma unroll
+      for (int i = 0; i < NK; i++)
+#pragma unroll
+        for (int n = 0; n < 4; n++) qf[x][i][n] = spread(not_finite<F16>(qf[x][i][n])) & 0x7fff7fffu;
+  }
   int buf = 0, free = p.stages - 1;
   for (int step = k0; step < k1; step += STEP) {
     const int key = step + grp * KT;

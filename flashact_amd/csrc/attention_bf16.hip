@@ -51,6 +51,8 @@ extern "C" int fa_span_attention(const fa_span_args* a, fa_stream_t stream) {
   p.scale = a->softcap > 0.f ? 2.f * attn::LOG2E * a->scale / a->softcap : a->scale * attn::LOG2E;
   p.over = a->softcap > 0.f ? a->scale / a->softcap : 0.f;
   p.cap = a->softcap * attn::LOG2E;
+  p.flat = a->scale == 0.f;
+  if (p.flat) p.scale = 1.f;
   if (!(p.scale < INFINITY) || !(p.cap < INFINITY))
     return host::fail(FA_ERR_INVALID_ARG, "%s: scale=%g over softcap=%g leaves the fp32 range", who, a->scale, a->softcap);
   const size_t need = attn::workspace(a->batch, a->queries, a->keys, a->heads, a->head_dim);

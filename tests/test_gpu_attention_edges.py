@@ -1,0 +1,45 @@
+"""Edges of ``attention.attend`` on the MI355X: a scale of zero."""
+import pytest
+import torch
+
+from flashact_amd import attention
+from tests import span_case as C
+from tests.test_gpu_attention import DTYPES, _qkv, _spans
+
+pytestmark = pytest.mark.gpu
+
+
+ZERO = [
+    # b, tq, tk, heads, kv_heads, hd, spans
+    (1, 130, 130, 2, 1, 128, "causal"),
+    (2, 100, 100, 2, 2, 96, "random"),         # empty, reversed and single-key spans
+    (1, 70, 77, 2, 1, 64, None),               # no spans, the last tile of keys is not whole
+    (1, 1500, 1500, 48, 16, 128, "documents"),
+    (1, 64, 9001, 8, 1, 256, "causal"),        # parts, joined by a kernel
+    (1, 1000, 4000, 8, 2, 64, "random"),       # parts, joined by the last workgroup
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", ZERO, ids=lambda c: "-".join(str(x) for x in c))
+def test_a_scale_of_zero_gives_the_mean(gpu, case, dtype):
+    """Every score is zero: a query gets the mean of the values that it sees, one that sees none zeros."""
+    b, tq, tk, h, hkv, hd, kind = case
+    q, k, v = _qkv(gpu, b, tq, tk, h, hkv, hd, dtype, seed=tq)
+    spans = _spans(gpu, kind, b, tq, tk)
+    for opt in ({}, dict(softcap=5.0), dict(slopes=torch.rand(h, device=gpu) * 0.1)):
+        out = attention.attend(q, k, v, spans, scale=0.0, **opt)
+        C.check(out, *C.attend(q, k, v, spans, scale=0.0, **opt))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_scale_of_zero_keeps_what_is_not_a_number(gpu, dtype):
+    """0 x inf is NaN: a query that is not finite, and those that see such a key, are NaN; the others do not change."""
+    q, k, v = _qkv(gpu, 1, 90, 90, 2, 2, 64, dtype)
+    spans = _spans(gpu, "causal", 1, 90, 90)
+    ref = attention.attend(q, k, v, spans, scale=0.0)
+    q[0, 3, 0, 2], q[0, 4, 0, 7], k[0, 50, 1, 1] = float("inf"), float("nan"), float("-inf")
+    out = attention.attend(q, k, v, spans, scale=0.0)
+    bad = torch.zeros(90, 2, dtype=torch.bool, device=gpu)
+    bad[3:5, 0] = bad[50:, 1] = True
+    assert out[0, bad].isnan().all() and torch.equal(out[0, ~bad], ref[0, ~bad])
