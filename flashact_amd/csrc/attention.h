@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
 #pragma unroll
           for (int t = 0; t < MT; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) s[x][t][i] = tanh_far(s[x][t][i] * p.scale);
+            for (int i = 0; i < 4; i++) s[x][t][i] = tanh_own(s[x][t][i] * p.over, s[x][t][i] * p.scale);
         }
       }
       if constexpr (BIAS) {

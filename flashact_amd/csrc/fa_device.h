@@ -302,7 +302,8 @@ __device__ __forceinline__ float silu(float x) {
 
 // tanh(x) of an attention score's cap, in two forms. Near zero the odd Taylor series up to x^9 (|x| <= kTanhNear: the next term
 // is 2^-22 of x); else 1 - 2 / (1 + e^2x) with e = 2 log2(e) x given, two instructions of about 1 ulp each: an error of 2^-23
-// absolute, which a large cap would multiply where x is small, so a tile takes the series if all its scores allow it.
+// absolute, which a large cap would multiply where x is small. Each score takes the form of its own size (tanh_own), so that no
+// other score changes it; a tile whose scores all lie near zero skips the other form.
 constexpr float kTanhNear = 0.35f;
 __device__ __forceinline__ float tanh_near(float x) {
   const float u = x * x;
@@ -311,6 +312,7 @@ __device__ __forceinline__ float tanh_near(float x) {
 __device__ __forceinline__ float tanh_far(float e) {
   return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(e));
 }
+__device__ __forceinline__ float tanh_own(float x, float e) { return fabsf(x) <= kTanhNear ? tanh_near(x) : tanh_far(e); }
 
 // 2^x as the bare v_exp_f32, for softmax weights and their rescale factors: a result below 2^-126
 // comes out as zero or a flushed value instead of an exact denormal (exp2f adds a range fix-up of

@@ -228,12 +228,17 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) att
           s[x][i] *= ksc * a.over;
           most = fmaxf(most, fabsf(s[x][i]));
         }
-      const bool near = __builtin_amdgcn_ballot_w64(most > kTanhNear) == 0;
+      if (__builtin_amdgcn_ballot_w64(most > kTanhNear) == 0) {
 #pragma unroll
-      for (int x = 0; x < 2; x++)
+        for (int x = 0; x < 2; x++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-          s[x][i] = a.cap * (near ? tanh_near(s[x][i]) : tanh_far(s[x][i] * (2.f * LOG2E)));
+          for (int i = 0; i < 4; i++) s[x][i] = a.cap * tanh_near(s[x][i]);
+      } else {
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) s[x][i] = a.cap * tanh_own(s[x][i], s[x][i] * (2.f * LOG2E));
+      }
     } else {
       const float f = ksc * a.scale;
       s[0] *= f;

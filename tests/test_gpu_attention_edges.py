@@ -1,4 +1,4 @@
-"""Edges of ``attention.attend`` on the MI355X: a scale of zero."""
+"""Edges of ``attention.attend`` on the MI355X: a scale of zero, caps."""
 import pytest
 import torch
 
@@ -43,3 +43,29 @@ def test_a_scale_of_zero_keeps_what_is_not_a_number(gpu, dtype):
     bad = torch.zeros(90, 2, dtype=torch.bool, device=gpu)
     bad[3:5, 0] = bad[50:, 1] = True
     assert out[0, bad].isnan().all() and torch.equal(out[0, ~bad], ref[0, ~bad])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd,n,heads", [(64, 200, 2), (256, 150, 2), (128, 1400, 48)])
+def test_a_cap_is_each_scores_own(gpu, dtype, hd, n, heads):
+    """Large scores of other queries, or of keys that a query does not see, do not change a bit of its result."""
+    q, k, v = _qkv(gpu, 1, n, n, heads, heads, hd, dtype, seed=hd)
+    spans = _spans(gpu, "causal", 1, n, n)
+    for slopes in (None, torch.rand(heads, device=gpu) * 0.1):
+        ref = attention.attend(q, k, v, spans, softcap=50.0, slopes=slopes)
+        k2, q2 = k.clone(), q.clone()
+        k2[0, n - 10:] *= 300
+        assert torch.equal(attention.attend(q, k2, v, spans, softcap=50.0, slopes=slopes)[:, :n - 10], ref[:, :n - 10])
+        q2[0, 17] *= 300
+        out = attention.attend(q2, k, v, spans, softcap=50.0, slopes=slopes)
+        assert torch.equal(out[:, :17], ref[:, :17]) and torch.equal(out[:, 18:], ref[:, 18:])
+
+
+@pytest.mark.parametrize("softcap", [1.0, 8.0, 100.0])
+def test_caps_next_to_the_two_forms_border(gpu, softcap):
+    """Scores on both sides of the border in every tile."""
+    q, k, v = _qkv(gpu, 1, 150, 150, 2, 2, 128, torch.float16, seed=4)
+    for scale in (0.35 * softcap / 128 ** 0.5, 0.05 * softcap):
+        for spans in (None, _spans(gpu, "random", 1, 150, 150)):
+            C.check(attention.attend(q, k, v, spans, scale=scale, softcap=softcap),
+                    *C.attend(q, k, v, spans, scale=scale, softcap=softcap))
