@@ -15,7 +15,9 @@
 // stretch for each wave, equally far apart, all of them met in the same memory channels (2 x 131072 keys: 35.8 us instead of 33.0).
 //
 // Codes are exact in bf16 and fp16. Q K^T runs in q's type; P is rounded to fp16 (2^-12, half the step of an fp16
-// result, a sixteenth of bf16's) for the product with the values' codes; scales, softmax and sums are fp32.
+// result, a sixteenth of bf16's) for the product with the values' codes; scales, softmax and sums are fp32. Weights are taken
+// against a reference 2^15 below the maximum: fp16 then holds those above 2^-29 of the largest with all its bits and the rest to 2^-40
+// of it, where against the maximum itself 131072 keys of 2^-26 each, 2^-9 of the sum, were lost.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -55,6 +57,11 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int b) {
   s.n = a.count ? max(0, min(a.count[b], a.T)) : a.T;
   return s;
 }
+// The reference of weights whose scores (base 2) have the maximum `top`; past 2^22, where the difference would round, itself.
+__device__ __forceinline__ float reference(float top) { return fabsf(top) < 4194304.f ? top - 15.f : top; }
+// Both sums, of weighted values and of weights, are kept times 2^-35. With weights of up to 2^15 a key adds at most 2^-20 of its
+// value: a million keys of the largest values stay in the fp32 range, and those of the smallest scale (2^-100) above its end.
+constexpr float SMALL = 0x1p-35f;
 // Splits that a row tile of nb blocks uses: each wave of each has a.least blocks or more.
 constexpr int MAX_SPLITS = 256;
 // Up to so many are joined by the last workgroup (32 requests of 50 to 16384 keys on 16 splits: 20.6 us, 22.6 with a kernel), more
@@ -202,7 +209,7 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) att
         if (HD % 64 == 0 || 64 * i + 16 * q < HD)
           kc[x][i] = *reinterpret_cast<const u32x4*>(kl + ((4 * i + q) * BT + 8 * (r >> 2) + 4 * x + (r & 3)) * 16);
       }
-    const float ksc = a.ks[unit + blk], vsc = a.vs[unit + blk];
+    const float ksc = a.ks[unit + blk], vsc = a.vs[unit + blk] * SMALL;
     lds_wait();
     if (more) copy(a.k, blk + all, at_k);
     f32x4 s[2];
@@ -263,7 +270,7 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) att
     for (int x = 0; x < 2; x++)
 #pragma unroll
       for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[x][i]);
-    const float mn = fmaxf(m, cols_max(mx));
+    const float mn = fmaxf(m, reference(cols_max(mx)));
     const float ms = mn == -INFINITY ? 0.f : mn;
     if (__builtin_amdgcn_ballot_w64(mn != m)) {
       const float al = exp2_w(m - ms);  // 0 where there was nothing yet
@@ -324,7 +331,7 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) att
   }
 
   // the waves' sums
-  l = cols_sum(l);
+  l = cols_sum(l) * SMALL;
   __syncthreads();  // the blocks in LDS are done with
   if (q == 0) {
     wm[wave * 16 + r] = m;
