@@ -115,6 +115,12 @@ __device__ __forceinline__ int rows_least(int v) {
   return min(v, __builtin_amdgcn_update_dpp(0, v, 0x121, 0xF, 0xF, false));
 }
 
+// The reference of weights whose scores (base 2) have the maximum `top`. In fp16 the largest starts at 2^12 and may grow to 2^15:
+// those above 2^-26 of it keep all their bits and the rest is held to 2^-37 of it, where with the maximum at one 65536 keys of
+// 2^-26 each were lost. Past 2^22, where the difference would round, it is the maximum. bf16 has the range of fp32.
+template <bool F16>
+__device__ __forceinline__ float reference(float top) { return F16 && fabsf(top) < 4194304.f ? top - 12.f : top; }
+
 constexpr int part_floats(int nt) { return nt * 256 + 32; }  // of 16 rows
 
 template <bool F16, int HD, int QB, int NW, int SP, bool CAP, bool BIAS>
@@ -122,6 +128,7 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
   constexpr int KT = HD == 256 ? 32 : 64, CH = HD / 8, NK = HD / 32, NT = HD / 16, MT = KT / 16;
   constexpr int TILE = KT * HD * 2, COPIES = KT * CH / 64, PER = (COPIES + NW - 1) / NW;  // bytes, copies of a tile of keys
   constexpr unsigned ONE = F16 ? 0x3c00u : 0x3f80u;
+  constexpr float PASS = F16 ? 15.f : 8.f;  // how far weights may grow, as powers of two, before the reference follows
   // 4096 for a NaN, 64 for an infinity, 1 for a negative one: the 32 keys of a step sum up without mixing
   constexpr unsigned NANS = (F16 ? 0x6c00u : 0x4580u) * 0x10001u, UPS = (F16 ? 0x5400u : 0x4280u) * 0x10001u;
   constexpr unsigned DOWNS = ONE * 0x10001u;
@@ -384,11 +391,11 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
 #pragma unroll
         for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[x][t][i]);
       mx = cols_max(mx) * post;  // post >= 0
-      // The reference that weights are taken against follows the maximum only where it is passed by more than 2^8: what
+      // The reference that weights are taken against follows the maximum only where they would pass 2^PASS: what
       // counts is that no weight overflows, and most tiles leave the sums as they are.
-      if (__builtin_amdgcn_ballot_w64(mx > m[x] + 8.f)) {
+      if (__builtin_amdgcn_ballot_w64(mx - m[x] > PASS)) {
         // each row's by itself: another's keys do not change its roundings
-        const float mn = mx > m[x] + 8.f ? mx : m[x], al = m[x] == mn ? 1.f : exp2_w(m[x] - mn);  // 0 where there was nothing yet
+        const float mn = mx - m[x] > PASS ? reference<F16>(mx) : m[x], al = m[x] == mn ? 1.f : exp2_w(m[x] - mn);  // 0 where there was nothing yet
         l[x] *= al;
 #pragma unroll
         for (int j = 0; j < NT; j++) O[x][j] *= al;

@@ -1,4 +1,6 @@
-"""Edges of ``attention.attend`` on the MI355X: a scale of zero, caps."""
+"""Edges of ``attention.attend`` on the MI355X: a scale of zero, caps, weights far below the largest."""
+import math
+
 import pytest
 import torch
 
@@ -69,3 +71,20 @@ def test_caps_next_to_the_two_forms_border(gpu, softcap):
         for spans in (None, _spans(gpu, "random", 1, 150, 150)):
             C.check(attention.attend(q, k, v, spans, scale=scale, softcap=softcap),
                     *C.attend(q, k, v, spans, scale=scale, softcap=softcap))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tq,tk,heads", [(1, 65536, 2), (500, 65536, 1), (1500, 16384, 48)])
+def test_many_keys_of_small_weight_count(gpu, dtype, tq, tk, heads):
+    """One key outweighs each of the others by e^18, 2^26: together they are 2^-12 to 2^-10 of the sum, and hold all of its value.
+
+    Rounded: the weights (eps / 2 of the values' type), the result, and, 2^-12 in all, the score of 18 log2(e) (2^-19) and the sums,
+    of at most 2^10 terms a lane (2^-14).
+    """
+    q = torch.ones(1, tq, heads, 64, device=gpu, dtype=dtype)
+    k, v = torch.zeros(1, tk, heads, 64, device=gpu, dtype=dtype), torch.ones(1, tk, heads, 64, device=gpu, dtype=dtype)
+    k[0, 5], v[0, 5] = 2.25, 0.0  # 64 x 2.25 / 8 = 18
+    others = (tk - 1) * math.exp(-18.0)
+    want = others / (1 + others)
+    out = attention.attend(q, k, v).double()
+    assert bool(((out - want).abs() <= want * (torch.finfo(dtype).eps + 2.0 ** -12)).all()), (out.min().item(), out.max().item(), want)
