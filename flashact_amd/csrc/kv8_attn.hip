@@ -464,6 +464,10 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a) {
 }
 
 constexpr int WAVES = 4;  // of a workgroup
+// Splits of all row tiles together: they bound the workspace (68 MB with 256 dims), where whole rounds of workgroups alone would ask
+// for gigabytes beside a small cache. 2049 tokens of 8 heads of 256 dims over 8192 keys 354 us, unbounded (135 MB) 440, over 32768 keys
+// 1360 and 1275; 4152 of 128 dims 244 and 276, 1143 and 1085; 4 x 2080 of 64 dims over 16384 keys 643 and 603.
+constexpr int MAX_PARTS = 4096;
 
 // Splits of the keys across workgroups. A wave takes about 2.3 us for a block of 256 dims that comes from memory (1.2 of 128
 // and less) and one to begin and end, more than one (four) workgroups a CU share its bandwidth, and joining the splits costs
@@ -472,7 +476,7 @@ constexpr int WAVES = 4;  // of a workgroup
 int splits_for(int batch, int tokens, int heads, int kv_heads, int hd, int blocks) {
   const int64_t rt = ((int64_t)tokens * (heads / kv_heads) + 15) / 16, units = rt * batch * kv_heads;
   const double block = hd == 256 ? 2.3 : 1.2, resident = hd == 256 ? 1.0 : 4.0;
-  const int64_t most = std::min<int64_t>((blocks + WAVES - 1) / WAVES, MAX_SPLITS);
+  const int64_t most = std::min<int64_t>({(blocks + WAVES - 1) / WAVES, MAX_SPLITS, std::max<int64_t>(1, MAX_PARTS / units)});
   int best = 1;
   double least = 1e300;
   auto consider = [&](int64_t S) {
