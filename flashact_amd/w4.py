@@ -117,7 +117,8 @@ def linear(x: torch.Tensor, w: dict, *, bias=None, residual=None, gate=None, out
             raise TypeError(f"out must be bfloat16, float16 or float32 and agree with out_dtype, got {t}")
         if out.shape != shape or not out.is_contiguous() or out.get_device() != index:
             raise ValueError(f"out must be contiguous {shape} on x's GPU, got {tuple(out.shape)} on {out.device}")
-        if _lib.overlap(out, x) or (residual is not None and out.data_ptr() != residual.data_ptr() and _lib.overlap(out, residual)):
+        being = residual is not None and out.data_ptr() == residual.data_ptr() and t is torch.float32
+        if _lib.overlap(out, x) or (residual is not None and not being and _lib.overlap(out, residual)):
             raise ValueError("out must not share memory with x, nor with a residual but for being it")
     if rows == 0:
         return out
