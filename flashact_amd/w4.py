@@ -120,6 +120,8 @@ def linear(x: torch.Tensor, w: dict, *, bias=None, residual=None, gate=None, out
         being = residual is not None and out.data_ptr() == residual.data_ptr() and t is torch.float32
         if _lib.overlap(out, x) or (residual is not None and not being and _lib.overlap(out, residual)):
             raise ValueError("out must not share memory with x, nor with a residual but for being it")
+        if _lib.overlap(out, codes) or _lib.overlap(out, scales) or (bias is not None and _lib.overlap(out, bias)):
+            raise ValueError("out must not share memory with the weights or the bias")
     if rows == 0:
         return out
     lib = _lib.lib()
