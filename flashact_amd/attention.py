@@ -98,6 +98,8 @@ def attend(q, k, v, spans=None, *, scale=None, softcap: float = 0.0, slopes=None
     elif (_lib.overlap(out, k) or _lib.overlap(out, v)
           or _lib.overlap(out, q) and (out.data_ptr() != q.data_ptr() or not q.is_contiguous())):
         raise ValueError("out must not share memory with k or v, nor with q but for being it")
+    elif (spans is not None and _lib.overlap(out, spans)) or (slopes is not None and _lib.overlap(out, slopes)):
+        raise ValueError("out must not share memory with spans or slopes")
     need = _workspace_bytes(b, tq, tk, h, hd)
     ws = q.new_empty(need, dtype=torch.uint8) if need else None
     a = _lib.SpanArgs(_lib.DTYPES[t], q.data_ptr(), _S3(*strides[0]), k.data_ptr(), _S3(*strides[1]), v.data_ptr(),

@@ -157,6 +157,8 @@ def attend(q, cache: dict, lens, *, count=None, scale=None, softcap: float = 0.0
         raise ValueError(f"out must be contiguous {q.dtype} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
     elif _lib.overlap(out, q) and (out.data_ptr() != q.data_ptr() or not q.is_contiguous()):
         raise ValueError("out must not share memory with q but for being it")
+    elif any(t is not None and _lib.overlap(out, t) for t in (ck, cv, ks, vs, lens, count, slopes)):
+        raise ValueError("out must not share memory with the cache, lens, count or slopes")
     lib = _lib.lib()
     need = _workspace_bytes(b, tokens, heads, h, hd, nb)
     ws = q.new_empty(need, dtype=torch.uint8) if need else None

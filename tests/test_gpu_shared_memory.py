@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from flashact_amd import w4
+from flashact_amd import attention, kv8, w4
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +34,25 @@ def test_a_product_is_not_written_over_its_bias_or_weights(gpu):
     bias = buf[192:].clone()
     out = w4.linear(x, w, bias=buf[192:], out=buf[:192].view(3, 64))  # beside it
     assert torch.equal(out, w4.linear(x, w, bias=bias, out_dtype=torch.float32))
+
+
+def test_attention_is_not_written_over_spans_or_slopes(gpu):
+    q, k, v = (torch.randn(1, 40, 2, 64, device=gpu).bfloat16() for _ in range(3))
+    out = torch.empty(1, 40, 2, 64, dtype=torch.bfloat16, device=gpu)
+    spans, slopes = out.view(-1).view(torch.int32)[:80].view(40, 2), out.view(-1).view(torch.float32)[2000:2002]
+    for kw in (dict(spans=spans), dict(slopes=slopes)):
+        with pytest.raises(ValueError, match="share memory"):
+            attention.attend(q, k, v, out=out, **kw)
+
+
+def test_attention_is_not_written_over_the_cache_and_its_lengths(gpu):
+    cache, lens = kv8.make_caches(1, 2, 64, 2, 64, gpu)[0], torch.tensor([50, 3], dtype=torch.int32, device=gpu)
+    q, out = torch.randn(2, 5, 4, 64, device=gpu).bfloat16(), torch.zeros(2, 5, 4, 64, dtype=torch.bfloat16, device=gpu)
+    for name in ("k", "v"):
+        with pytest.raises(ValueError, match="share memory"):
+            kv8.attend(q, cache, lens, out=cache[name].view(-1).view(torch.bfloat16)[:2560].view(2, 5, 4, 64))
+    ints = out.view(-1).view(torch.int32)
+    for kw in (dict(lens=ints[:2]), dict(count=ints[7:9]), dict(slopes=out.view(-1).view(torch.float32)[20:24]),
+               dict(cache=dict(cache, ks=out.view(-1).view(torch.float32)[:8].view(2, 2, 2)))):
+        with pytest.raises(ValueError, match="share memory"):
+            kv8.attend(**{"q": q, "cache": cache, "lens": lens, "out": out, **kw})
