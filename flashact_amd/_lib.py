@@ -219,3 +219,47 @@ def overlap(a, b) -> bool:
     a0, a1 = ends(a)
     b0, b1 = ends(b)
     return a0 < b1 and b0 < a1
+
+
+def doubled(t) -> bool:
+    """Whether two elements of a tensor may be one: a stride that does not step over all that smaller strides reach."""
+    reach = 0
+    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if s <= reach:
+            return t.numel() > 0
+        reach += s * (n - 1)
+    return False
+
+
+def meet(a, b) -> bool:
+    """Whether two tensors of one type have an element in common (or may have, where telling would take long)."""
+    if not overlap(a, b):
+        return False
+    apart, odd = divmod(b.data_ptr() - a.data_ptr(), a.element_size())
+    if odd:
+        return True
+    # sum of i * stride over a's dimensions less the same over b's = apart: by stride, the span of its factors
+    spans = {}
+    for t, low, high in ((a, 0, 1), (b, -1, 0)):
+        for s, n in zip(t.stride(), t.shape):
+            was = spans.get(s, (0, 0))
+            spans[s] = (was[0] + low * (n - 1), was[1] + high * (n - 1))
+    terms = sorted(((s, low, high) for s, (low, high) in spans.items() if s and (low or high)), reverse=True)
+    least, most = [0], [0]  # what the terms behind one can add
+    for s, low, high in reversed(terms):
+        least.insert(0, least[0] + s * low)
+        most.insert(0, most[0] + s * high)
+    left = 10000
+
+    def found(i, rest):
+        nonlocal left
+        if i == len(terms):
+            return rest == 0
+        s, low, high = terms[i]
+        for c in range(max(low, -((most[i + 1] - rest) // s)), min(high, (rest - least[i + 1]) // s) + 1):
+            left -= 1
+            if left < 0 or found(i + 1, rest - c * s):
+                return True
+        return False
+
+    return found(0, apart)

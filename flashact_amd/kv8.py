@@ -108,8 +108,7 @@ def load(cache: dict, lens, *, k=None, v=None, dtype=torch.bfloat16):
     if (k is None) != (v is None):
         raise ValueError("pass both of k and v or neither")
     fresh = k is None
-    if not fresh and (k.numel() and k.data_ptr() == v.data_ptr()
-                      or any(s == 0 and n > 1 for t in (k, v) for s, n in zip(t.stride(), t.shape))):
+    if not fresh and (_lib.doubled(k) or _lib.doubled(v) or k.dtype is v.dtype and _lib.meet(k, v)):
         raise ValueError("k and v are written: no two of their elements may be one")
     if fresh:
         if dtype not in _lib.DTYPES:

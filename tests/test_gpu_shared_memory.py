@@ -56,3 +56,20 @@ def test_attention_is_not_written_over_the_cache_and_its_lengths(gpu):
                dict(cache=dict(cache, ks=out.view(-1).view(torch.float32)[:8].view(2, 2, 2)))):
         with pytest.raises(ValueError, match="share memory"):
             kv8.attend(**{"q": q, "cache": cache, "lens": lens, "out": out, **kw})
+
+
+def test_rows_are_not_loaded_over_each_other(gpu):
+    """Keys and values that are shifted into one another, and rows that overlap themselves, would be written twice."""
+    cache, lens = kv8.make_caches(1, 1, 64, 1, 64, gpu)[0], torch.tensor([60], dtype=torch.int32, device=gpu)
+    rows = torch.randn(60, 64, device=gpu)
+    kv8.store(cache, rows[None, :, None], rows[None, :, None] * 2, torch.zeros(1, dtype=torch.int32, device=gpu))
+    buf = torch.zeros(130, 64, device=gpu)
+    part = lambda at: buf[at:at + 60][None, :, None]  # noqa: E731
+    with pytest.raises(ValueError, match="no two"):
+        kv8.load(cache, lens, k=part(0), v=part(59))
+    over = buf.view(-1).as_strided((1, 60, 1, 64), (4096, 32, 64, 1))
+    with pytest.raises(ValueError, match="no two"):
+        kv8.load(cache, lens, k=over, v=part(70))
+    kv8.load(cache, lens, k=part(0), v=part(60))
+    k, v = kv8.load(cache, lens, dtype=torch.float32)
+    assert torch.equal(buf[:60], k[0, :60, 0]) and torch.equal(buf[60:120], v[0, :60, 0]) and not buf[120:].any()
