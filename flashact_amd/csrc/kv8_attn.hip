@@ -596,7 +596,7 @@ extern "C" int fa_kv8_attention(const fa_kv8_attn_args* a, fa_stream_t stream) {
   p.scale = a->scale * kv8::LOG2E;
   p.over = a->softcap > 0.f ? a->scale / a->softcap : 0.f;
   p.cap = a->softcap * kv8::LOG2E;
-  if (!(fabsf(p.over) < INFINITY) || !(p.cap < INFINITY))
+  if (!(fabsf(p.scale) < INFINITY) || !(fabsf(p.over) < INFINITY) || !(p.cap < INFINITY))
     return host::fail(FA_ERR_INVALID_ARG, "%s: scale=%g over softcap=%g leaves the fp32 range", who, a->scale, a->softcap);
   rc = host::check_gfx950(who);
   if (rc != FA_OK) return rc;
