@@ -217,21 +217,22 @@ def extend(weights: list, ln_in, ln_post, x, caches: list, lens, count=None) -> 
 
     weights: ``pack_backbone_w4`` output. x [B][T][2048] fp32: the hidden states entering layer 0, B T <= 64. caches as
     ``prefill_packed`` leaves them; lens int32 [B] on the GPU: tokens cached so far, the positions of the new ones follow
-    them; count int32 [B]: how many of the T are real (None: all, clamped to [0, T]); lens + T must fit the caches, which is
-    not checked (tokens behind their end are dropped). The tokens' keys and values are appended (the caller's
-    lens grow by T or count), each token sees all cached ones and the new ones up to itself. Returns the hidden states
-    leaving the last layer [B][T][2048] fp32 (undefined behind count). Nothing synchronises, and a captured graph serves
-    every length.
+    them; count int32 [B]: how many of the T are real (None: all, clamped to [0, T]); those behind the caches' end are not.
+    The real tokens' keys and values are appended (the caller's lens grow by as many), each token sees all cached ones and the
+    new ones up to itself. Returns the hidden states leaving the last layer [B][T][2048] fp32 (undefined where a token is not
+    real). Nothing synchronises, and a captured graph serves every length.
     """
     _check_backbone(ln_in, ln_post, len(weights), x, caches)
     if x.dim() != 3 or x.shape[0] != caches[0]["v"].shape[0] or x.shape[0] * x.shape[1] > w4.MAX_ROWS:
         raise ValueError(f"x must be [B={caches[0]['v'].shape[0]}][T][{D}] with B T <= {w4.MAX_ROWS}, got {tuple(x.shape)}")
     B, T = int(x.shape[0]), int(x.shape[1])
+    if count is not None and count.shape != lens.shape:
+        raise ValueError(f"count must be [{B}] like lens, got {tuple(count.shape)} and {tuple(lens.shape)}")
     dev = x.device
     rope = _rope(lens[:, None] + torch.arange(T, device=dev), dev)
-    if count is not None:
-        count = count.clamp(0, T)
-    after = lens + (T if count is None else count)
+    room = (caches[0]["v"].shape[2] * kv8.BLOCK - lens).clamp(0, T)
+    count = room if count is None else torch.minimum(count, room).clamp(min=0)
+    after = lens + count
     x = x.reshape(B * T, D)
     for l, w in enumerate(weights):
         q, k, v = _qkv(w4.linear(_norm(x, ln_in[l]), w["wqkv"]).view(B, T, -1), rope)

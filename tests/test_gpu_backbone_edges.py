@@ -1,0 +1,25 @@
+"""Edges of ``prefill.prefill_packed`` and ``prefill.extend`` on the MI355X."""
+import pytest
+import torch
+
+from flashact_amd import kv8, prefill
+from tests.test_gpu_backbone import NL, _ints, _weights
+
+pytestmark = pytest.mark.gpu
+
+
+def test_tokens_behind_the_caches_end_are_not_real(gpu):
+    """Those that fit get what they get alone: positions, keys and cache do not shift."""
+    _, _, w4s, ln = _weights(gpu, seed=6)
+    lens, filled = _ints(gpu, 30, 5, 32), kv8.make_caches(NL, 3, 32, device=gpu)
+    prefill.extend(w4s, *ln, torch.randn(3, 20, 2048, device=gpu), filled, _ints(gpu, 0, 0, 0))
+    x, runs = torch.randn(3, 4, 2048, device=gpu), []
+    for count in (None, (9, 4, 1), (2, 4, 0)):
+        caches = [{n: t.clone() for n, t in c.items()} for c in filled]
+        runs.append((prefill.extend(w4s, *ln, x, caches, lens, None if count is None else _ints(gpu, *count)), caches))
+    with pytest.raises(ValueError, match="count"):
+        prefill.extend(w4s, *ln, x, caches, lens, _ints(gpu, 4))
+    ref, want = runs[-1]
+    for out, caches in runs[:-1]:
+        assert torch.equal(out[0, :2], ref[0, :2]) and torch.equal(out[1], ref[1])
+        assert all(torch.equal(a[n], b[n]) for a, b in zip(caches, want) for n in a)
