@@ -235,7 +235,7 @@ def extend(weights: list, ln_in, ln_post, x, caches: list, lens, count=None) -> 
     after = lens + count
     x = x.reshape(B * T, D)
     for l, w in enumerate(weights):
-        q, k, v = _qkv(w4.linear(_norm(x, ln_in[l]), w["wqkv"]).view(B, T, -1), rope)
+        q, k, v = _qkv(w4.linear(_norm(x, ln_in[l]), w["wqkv"]).view(B, T, (H + 2) * HD), rope)
         kv8.store(caches[l], k, v, lens, count)
         o = kv8.attend(q, caches[l], after, count=count)
         x = w4.linear(o.view(B * T, H * HD), w["wo"], residual=x)

@@ -23,3 +23,9 @@ def test_tokens_behind_the_caches_end_are_not_real(gpu):
     for out, caches in runs[:-1]:
         assert torch.equal(out[0, :2], ref[0, :2]) and torch.equal(out[1], ref[1])
         assert all(torch.equal(a[n], b[n]) for a, b in zip(caches, want) for n in a)
+
+
+def test_no_tokens(gpu):
+    _, _, w4s, ln = _weights(gpu, seed=6)
+    caches = kv8.make_caches(NL, 2, 32, device=gpu)
+    assert prefill.extend(w4s, *ln, torch.zeros(2, 0, 2048, device=gpu), caches, _ints(gpu, 0, 3)).shape == (2, 0, 2048)
