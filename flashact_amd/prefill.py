@@ -166,8 +166,8 @@ def _check_backbone(ln_in, ln_post, layers, x, caches):
     if x.shape[-1] != D or ln_in.shape != (layers, D) or ln_post.shape != (layers, D):
         raise ValueError(f"shapes: x {tuple(x.shape)}, ln_in {tuple(ln_in.shape)}, ln_post {tuple(ln_post.shape)}: need "
                          f"[..][{D}] and [{layers}][{D}]")
-    if len(caches) != layers or any(c["v"].shape[1] != 1 or c["v"].shape[3] != HD for c in caches):
-        raise ValueError(f"caches must be {layers} layers of kv8.make_caches with one K/V head of {HD}")
+    if len(caches) != layers or any(c["v"].shape != caches[0]["v"].shape or c["v"].shape[1] != 1 or c["v"].shape[3] != HD for c in caches):
+        raise ValueError(f"caches must be {layers} equal layers of kv8.make_caches with one K/V head of {HD}")
 
 
 def prefill_packed(packed: dict, ln_in, ln_post, x, lengths, caches: list, prefix=None) -> torch.Tensor:

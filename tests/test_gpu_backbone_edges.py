@@ -29,3 +29,16 @@ def test_no_tokens(gpu):
     _, _, w4s, ln = _weights(gpu, seed=6)
     caches = kv8.make_caches(NL, 2, 32, device=gpu)
     assert prefill.extend(w4s, *ln, torch.zeros(2, 0, 2048, device=gpu), caches, _ints(gpu, 0, 3)).shape == (2, 0, 2048)
+
+
+def test_caches_of_unequal_layers_are_refused(gpu):
+    ln = [torch.zeros(NL, 2048, device=gpu) for _ in range(2)]
+    packed = {k: torch.zeros(NL, n, m, dtype=torch.bfloat16, device=gpu)
+              for k, n, m in (("wqkv", 2560, 2048), ("wo", 2048, 2048), ("wgu", 32768, 2048), ("wdn", 2048, 16384))}
+    full = kv8.make_caches(NL, 2, 64, device=gpu)
+    for other in (kv8.make_caches(1, 2, 32, device=gpu), kv8.make_caches(1, 3, 64, device=gpu)):
+        caches = full[:1] + other
+        with pytest.raises(ValueError, match="caches"):
+            prefill.prefill_packed(packed, *ln, torch.zeros(50, 2048, device=gpu), [40, 10], caches)
+        with pytest.raises(ValueError, match="caches"):
+            prefill.extend([None] * NL, *ln, torch.zeros(2, 1, 2048, device=gpu), caches, _ints(gpu, 0, 0))
