@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from flashact_amd import kv8, prefill
+from flashact_amd import kv8, pi05, prefill
 from tests.test_gpu_backbone import NL, _ints, _weights
 
 pytestmark = pytest.mark.gpu
@@ -42,3 +42,25 @@ def test_caches_of_unequal_layers_are_refused(gpu):
             prefill.prefill_packed(packed, *ln, torch.zeros(50, 2048, device=gpu), [40, 10], caches)
         with pytest.raises(ValueError, match="caches"):
             prefill.extend([None] * NL, *ln, torch.zeros(2, 1, 2048, device=gpu), caches, _ints(gpu, 0, 0))
+
+
+def test_two_samples_from_prompts_to_the_denoise_loops_caches(gpu):
+    """Packed prompts, answers, and each sample's rows into its own caches of the denoise loop."""
+    _, packed, w4s, ln = _weights(gpu, seed=7)
+    lengths, cap = [20, 9], 40
+    caches = kv8.make_caches(NL, batch=2, max_tokens=cap, device=gpu)
+    prefill.prefill_packed(packed, *ln, torch.randn(sum(lengths), 2048, device=gpu), lengths, caches, prefix=[12, 9])
+    lens = _ints(gpu, *lengths)
+    for _ in range(3):
+        prefill.extend(w4s, *ln, torch.randn(2, 1, 2048, device=gpu), caches, lens)
+        lens += 1
+    Lmax = pi05.lmax_for(cap, 50)
+    kcache = torch.zeros(2, NL, Lmax, 256, dtype=torch.bfloat16, device=gpu)
+    vtcache = torch.zeros(2, NL, 256, Lmax, dtype=torch.bfloat16, device=gpu)
+    for l in range(NL):
+        kv8.load(caches[l], lens, k=kcache[:, l, :, None], v=vtcache[:, l].transpose(1, 2)[:, :, None])
+    for l in range(NL):
+        k, v = kv8.load(caches[l], lens)
+        for b, n in enumerate(lens.tolist()):
+            assert torch.equal(kcache[b, l, :n], k[b, :n, 0]) and not kcache[b, l, n:].any()
+            assert torch.equal(vtcache[b, l, :, :n].t(), v[b, :n, 0]) and not vtcache[b, l, :, n:].any()
