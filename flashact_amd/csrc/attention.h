@@ -63,16 +63,10 @@ __device__ __forceinline__ int turn(int row) {
   else return ((row & 7) << 1) | ((row >> 3) & 1);
 }
 
-#define ATTN_VMCNT(n) (((n) & 15) | (((n) >> 4) << 14) | (7 << 4) | (15 << 8))
-// Waits until at most n (wave-uniform: 2, 4, 6, 8, 12, 16, or else 0) copies or loads of this wave are outstanding.
-__device__ __forceinline__ void vm_wait(int n) {
-  if (n == 16) __builtin_amdgcn_s_waitcnt(ATTN_VMCNT(16));
-  else if (n == 12) __builtin_amdgcn_s_waitcnt(ATTN_VMCNT(12));
-  else if (n == 8) __builtin_amdgcn_s_waitcnt(ATTN_VMCNT(8));
-  else if (n == 6) __builtin_amdgcn_s_waitcnt(ATTN_VMCNT(6));
-  else if (n == 4) __builtin_amdgcn_s_waitcnt(ATTN_VMCNT(4));
-  else if (n == 2) __builtin_amdgcn_s_waitcnt(ATTN_VMCNT(2));
-  else __builtin_amdgcn_s_waitcnt(ATTN_VMCNT(0));
+// Waits until at most N copies or loads of this wave are outstanding.
+template <int N>
+__device__ __forceinline__ void vm_wait() {
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
   asm volatile("" ::: "memory");
 }
 
@@ -126,13 +120,13 @@ constexpr int part_floats(int nt) { return nt * 256 + 32; }  // of 16 rows
 template <bool F16, int HD, int QB, int NW, int SP, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
   constexpr int KT = HD == 256 ? 32 : 64, CH = HD / 8, NK = HD / 32, NT = HD / 16, MT = KT / 16;
-  constexpr int TILE = KT * HD * 2, COPIES = KT * CH / 64, PER = (COPIES + NW - 1) / NW;  // bytes, copies of a tile of keys
+  constexpr int TILE = KT * HD * 2, COPIES = KT * CH / 64, PER = COPIES / NW;  // bytes, copies of a tile of keys: all, a wave's
   constexpr unsigned ONE = F16 ? 0x3c00u : 0x3f80u;
   constexpr float PASS = F16 ? 15.f : 8.f;  // how far weights may grow, as powers of two, before the reference follows
   // 4096 for a NaN, 64 for an infinity, 1 for a negative one: the 32 keys of a step sum up without mixing
   constexpr unsigned NANS = (F16 ? 0x6c00u : 0x4580u) * 0x10001u, UPS = (F16 ? 0x5400u : 0x4280u) * 0x10001u;
   constexpr unsigned DOWNS = ONE * 0x10001u;
-  static_assert(KT * CH % 64 == 0, "whole copies");
+  static_assert(KT * CH % 64 == 0 && COPIES % NW == 0, "whole copies, as many of each wave");
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // p.stages buffers of {keys, values}
   const int lane = threadIdx.x & 63, all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wave = SP > 1 ? all_waves % NW : all_waves, grp = SP > 1 ? all_waves / NW : 0;  // grp: whose tiles of keys
@@ -237,7 +231,6 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
     if (p.hd == HD && key + KT <= p.Tk) {
 #pragma unroll
       for (int n = 0; n < PER; n++) {
-        if (COPIES % NW && n * NW + wave >= COPIES) break;
         copy_to_lds(kp, koff[n], to + n * NW * 1024);
         copy_to_lds(vp, voff[n], to + n * NW * 1024 + TILE);
       }
@@ -247,7 +240,6 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
     asm volatile("" : "+v"(ln));  // worked out here each time: no registers to keep it in
 #pragma unroll
     for (int n = 0; n < PER; n++) {
-      if (COPIES % NW && n * NW + wave >= COPIES) break;
       const int slot = (n * NW + wave) * 64 + ln, row = slot / CH, c = (slot % CH) ^ turn<CH>(row);
       const unsigned at = min(row, p.Tk - 1 - key);
       if (c * 8 < p.hd) {
@@ -268,7 +260,7 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
 
   // p.stages - 1 tiles are on their way
   constexpr int STEP = KT * SP;
-  const int ahead = (p.stages - 1) * STEP, mine = (COPIES - wave + NW - 1) / NW;
+  const int ahead = (p.stages - 1) * STEP;
   for (int i = 0; i < p.stages - 1; i++)
     if (k0 + i * STEP + grp * KT < k1) copy_tile(k0 + i * STEP + grp * KT, i);
   // The queries are waited for here: left to the compiler, that wait (for everything under way) stands in the loop.
@@ -290,7 +282,9 @@ __global__ void __launch_bounds__(64 * NW * SP, 2) span_kernel(Params p) {
   for (int step = k0; step < k1; step += STEP) {
     const int key = step + grp * KT;
     const int later = min(p.stages - 2, max(k1 - 1 - key, 0) / STEP);  // tiles behind this one that are on their way
-    vm_wait(later * 2 * mine);  // this wave's share of this one has landed
+    if (later == 2) vm_wait<4 * PER>();  // this wave's share of this one has landed
+    else if (later == 1) vm_wait<2 * PER>();
+    else vm_wait<0>();
     __syncthreads();  // everyone's has, and the tile before is no longer read
     if (key + ahead < k1) copy_tile(key + ahead, free);
     const unsigned char* kl = lds + (buf * SP + grp) * 2 * TILE;

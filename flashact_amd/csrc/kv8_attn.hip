@@ -62,13 +62,14 @@ __device__ __forceinline__ float reference(float top) { return fabsf(top) < 4194
 // Both sums, of weighted values and of weights, are kept times 2^-35. With weights of up to 2^15 a key adds at most 2^-20 of its
 // value: a million keys of the largest values stay in the fp32 range, and those of the smallest scale (2^-100) above its end.
 constexpr float SMALL = 0x1p-35f;
+constexpr int W = 4;  // waves of a workgroup
 // Splits that a row tile of nb blocks uses: each wave of each has a.least blocks or more.
 constexpr int MAX_SPLITS = 256;
 // Up to so many are joined by the last workgroup (32 requests of 50 to 16384 keys on 16 splits: 20.6 us, 22.6 with a kernel), more
 // by a kernel with workgroups enough to read them.
 constexpr int FUSED = 16;
-__device__ __forceinline__ int splits_used(const AttnArgs& a, int nb, int waves) {
-  const unsigned per = waves * a.least;
+__device__ __forceinline__ int splits_used(const AttnArgs& a, int nb) {
+  const unsigned per = W * a.least;
   return max(1, min(a.S, (int)((nb + per - 1) / per)));
 }
 
@@ -112,21 +113,21 @@ __device__ __forceinline__ void vm_wait() {
 // this wave's LDS reads have returned
 __device__ __forceinline__ void lds_wait() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-template <int HD, int W>
+template <int HD>
 struct Lds {
-  static constexpr int DC = W == 4 || HD < 128 ? HD : 128, PITCH = DC + 4;  // dims a round of the waves' sum
+  static constexpr int PITCH = HD + 4;                               // of the waves' sums
   static constexpr int WAVE = 2 * BT * HD;                           // a block of keys and one of values
   static constexpr int SUM = W * 16 * PITCH * 4 > W * WAVE ? W * 16 * PITCH * 4 : W * WAVE;
   static constexpr int BYTES = SUM + 2 * W * 16 * 4;
 };
 
-template <bool F16, int HD, int W, bool CAP, bool BIAS>
+template <bool F16, int HD, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) attn_kernel(AttnArgs a) {
   constexpr int KS = (HD + 63) / 64, NT = HD / 16, NC = BT * HD / 1024;  // NC: copies of a block
-  constexpr int DC = Lds<HD, W>::DC, PITCH = Lds<HD, W>::PITCH;
+  constexpr int PITCH = Lds<HD>::PITCH;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   float* osum = reinterpret_cast<float*>(lds);
-  float* wm = reinterpret_cast<float*>(lds + Lds<HD, W>::SUM);
+  float* wm = reinterpret_cast<float*>(lds + Lds<HD>::SUM);
   float* wl = wm + W * 16;
 
   // Row tiles of one (split, sample, head) share their keys: RC neighbours on one XCD. Splits are the slowest index: samples
@@ -157,7 +158,7 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) att
   lo = __builtin_amdgcn_readfirstlane(lo);  // keys that every row sees (rows that are not there do not count)
   if (!valid) limit = hi;
   const int nb = (hi + BT - 1) / BT;
-  const int used = splits_used(a, nb, W);
+  const int used = splits_used(a, nb);
   if (split >= used) return;
   const int at = split * W + wave, all = used * W;
 
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) att
   const float slope = BIAS && valid ? a.slopes[head] * LOG2E : 0.f;
 
   const size_t unit = ((size_t)b * a.H + h) * a.nblk;
-  unsigned char* kl = lds + wave * Lds<HD, W>::WAVE;
+  unsigned char* kl = lds + wave * Lds<HD>::WAVE;
   unsigned char* vl = kl + BT * HD;
   const unsigned at_k = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)kl), at_v = at_k + BT * HD;
   auto copy = [&](const unsigned char* from, int blk, unsigned to) {
@@ -345,32 +346,28 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) att
   constexpr int ONE = 16 * HD + 32;
   const rsrc_t part = make_rsrc(a.part + ((size_t)bh * a.RT + rt) * a.S * ONE, 0xffffffffu);  // the tile's splits
 #pragma unroll
-  for (int d0 = 0; d0 < HD; d0 += DC) {
-    if (d0) __syncthreads();
+  for (int j = 0; j < NT; j++)
+    *reinterpret_cast<f32x4*>(osum + (wave * 16 + r) * PITCH + 16 * j + 4 * q) = mine * O[j];
+  __syncthreads();
+  for (int e = threadIdx.x; e < 16 * HD / 4; e += 64 * W) {
+    const int row = e / (HD / 4), d = e % (HD / 4) * 4, g = rt * 16 + row;
+    if (g >= a.T * a.G) continue;
+    float rm = -INFINITY, rl = 0.f;
 #pragma unroll
-    for (int j = d0 / 16; j < (d0 + DC) / 16; j++)
-      *reinterpret_cast<f32x4*>(osum + (wave * 16 + r) * PITCH + 16 * j - d0 + 4 * q) = mine * O[j];
-    __syncthreads();
-    for (int e = threadIdx.x; e < 16 * DC / 4; e += 64 * W) {
-      const int row = e / (DC / 4), d = e % (DC / 4) * 4, g = rt * 16 + row;
-      if (g >= a.T * a.G) continue;
-      float rm = -INFINITY, rl = 0.f;
+    for (int w = 0; w < W; w++) rm = fmaxf(rm, wm[w * 16 + row]);
 #pragma unroll
-      for (int w = 0; w < W; w++) rm = fmaxf(rm, wm[w * 16 + row]);
+    for (int w = 0; w < W; w++) rl += wm[w * 16 + row] == -INFINITY ? 0.f : wl[w * 16 + row] * exp2_w(wm[w * 16 + row] - rm);
+    f32x4 o = *reinterpret_cast<const f32x4*>(osum + row * PITCH + d);
 #pragma unroll
-      for (int w = 0; w < W; w++) rl += wm[w * 16 + row] == -INFINITY ? 0.f : wl[w * 16 + row] * exp2_w(wm[w * 16 + row] - rm);
-      f32x4 o = *reinterpret_cast<const f32x4*>(osum + row * PITCH + d);
-#pragma unroll
-      for (int w = 1; w < W; w++) o += *reinterpret_cast<const f32x4*>(osum + (w * 16 + row) * PITCH + d);
-      if (used > 1) {
-        stb128<kCpSc1>(part, (split * ONE + row * HD + d0 + d) * 4, __builtin_bit_cast(u32x4, o));
-        if (d0 + d == 0) stb64<kCpSc1>(part, (split * ONE + 16 * HD + 2 * row) * 4, __builtin_bit_cast(u32x2, f32x2{rm, rl}));
-      } else {
-        const int tt = g / a.G;
-        if (tt >= sp.n || sp.len - sp.n + tt < 0) o = f32x4{0.f, 0.f, 0.f, 0.f}, rl = 0.f;
-        store_row4<F16>(a.out, ((size_t)b * a.T + tt) * a.H * a.G * HD + (size_t)(h * a.G + g % a.G) * HD + d0 + d,
-                        o * inverse(rl));
-      }
+    for (int w = 1; w < W; w++) o += *reinterpret_cast<const f32x4*>(osum + (w * 16 + row) * PITCH + d);
+    if (used > 1) {
+      stb128<kCpSc1>(part, (split * ONE + row * HD + d) * 4, __builtin_bit_cast(u32x4, o));
+      if (d == 0) stb64<kCpSc1>(part, (split * ONE + 16 * HD + 2 * row) * 4, __builtin_bit_cast(u32x2, f32x2{rm, rl}));
+    } else {
+      const int tt = g / a.G;
+      if (tt >= sp.n || sp.len - sp.n + tt < 0) o = f32x4{0.f, 0.f, 0.f, 0.f}, rl = 0.f;
+      store_row4<F16>(a.out, ((size_t)b * a.T + tt) * a.H * a.G * HD + (size_t)(h * a.G + g % a.G) * HD + d,
+                      o * inverse(rl));
     }
   }
   if (used == 1 || a.S > FUSED) return;
@@ -416,7 +413,7 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 2 : HD == 128 ? 3 : 4) att
 // The splits' sums, in a fixed order, where there are more than FUSED. One workgroup: 64 dims (96) of
 // one row; nothing to do where its sample used one split. Threads are quads of dims x groups of splits, so that 16 splits are
 // read side by side (2 x 131072 keys on 128 splits: 32.3 us, 32.8 with all 256 dims in one workgroup).
-template <bool F16, int HD, int W>
+template <bool F16, int HD>
 __global__ void __launch_bounds__(256) join_kernel(AttnArgs a) {
   constexpr int DIMS = HD % 64 == 0 ? 64 : HD, SLOTS = DIMS / 4, GROUPS = 256 / SLOTS, RUNS = HD / DIMS;
   __shared__ float wt[MAX_SPLITS], red[8];
@@ -430,7 +427,7 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a) {
     const int last = min(min(rt * 16 + 15, rows - 1) / a.G, sp.n - 1), pos = sp.len - sp.n + last;
     hi = pos < 0 ? 0 : a.causal ? pos + 1 : sp.len;
   }
-  const int used = splits_used(a, (hi + BT - 1) / BT, W);
+  const int used = splits_used(a, (hi + BT - 1) / BT);
   if (used == 1) return;
   constexpr int ONE = 16 * HD + 32;
   const float* part = a.part + ((size_t)bh * a.RT + rt) * a.S * ONE;
@@ -463,7 +460,6 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a) {
   store_row4<F16>(a.out, ((size_t)b * a.T + t) * a.H * a.G * HD + (size_t)(h * a.G + g % a.G) * HD + d, o * inverse(L));
 }
 
-constexpr int WAVES = 4;  // of a workgroup
 // Splits of all row tiles together: they bound the workspace (68 MB with 256 dims), where whole rounds of workgroups alone would ask
 // for gigabytes beside a small cache. 2049 tokens of 8 heads of 256 dims over 8192 keys 354 us, unbounded (135 MB) 440, over 32768 keys
 // 1360 and 1275; 4152 of 128 dims 244 and 276, 1143 and 1085; 4 x 2080 of 64 dims over 16384 keys 643 and 603.
@@ -476,12 +472,12 @@ constexpr int MAX_PARTS = 4096;
 int splits_for(int batch, int tokens, int heads, int kv_heads, int hd, int blocks) {
   const int64_t rt = ((int64_t)tokens * (heads / kv_heads) + 15) / 16, units = rt * batch * kv_heads;
   const double block = hd == 256 ? 2.3 : 1.2, resident = hd == 256 ? 1.0 : 4.0;
-  const int64_t most = std::min<int64_t>({(blocks + WAVES - 1) / WAVES, MAX_SPLITS, std::max<int64_t>(1, MAX_PARTS / units)});
+  const int64_t most = std::min<int64_t>({(blocks + W - 1) / W, MAX_SPLITS, std::max<int64_t>(1, MAX_PARTS / units)});
   int best = 1;
   double least = 1e300;
   auto consider = [&](int64_t S) {
     if (S < 1 || S > most) return;
-    const int64_t each = (blocks + WAVES * S - 1) / (WAVES * S);
+    const int64_t each = (blocks + W * S - 1) / (W * S);
     const double t = (block * each + 1.0) * std::max(1.0, (units * S + 255) / 256 / resident) + (S > 1 ? 3.0 : 0.0);
     if (t < least) best = (int)S, least = t;
   };
@@ -499,28 +495,23 @@ size_t attn_workspace(int batch, int tokens, int heads, int kv_heads, int hd, in
   return (S <= FUSED ? arrived_bytes(rt * batch * kv_heads) : 0) + rt * batch * kv_heads * S * (16 * hd + 32) * sizeof(float);
 }
 
-template <bool F16, int HD, int W>
-int launch_waves(const AttnArgs& a, hipStream_t s) {
+template <bool F16, int HD>
+int launch_attn(const AttnArgs& a, hipStream_t s) {
   const int runs = (a.RT + a.RC - 1) / a.RC;
   const int64_t grid = ((int64_t)a.B * a.H * a.S * runs + 7) / 8 * 8 * a.RC;
   if (grid > 0x7fffffff) return host::fail(FA_ERR_INVALID_ARG, "fa_kv8_attention: too many rows for one call");
   const bool cap = a.cap > 0.f, bias = a.slopes != nullptr;
-  void (*k)(AttnArgs) = cap ? (bias ? attn_kernel<F16, HD, W, true, true> : attn_kernel<F16, HD, W, true, false>)
-                            : (bias ? attn_kernel<F16, HD, W, false, true> : attn_kernel<F16, HD, W, false, false>);
-  const unsigned lds = Lds<HD, W>::BYTES;
+  void (*k)(AttnArgs) = cap ? (bias ? attn_kernel<F16, HD, true, true> : attn_kernel<F16, HD, true, false>)
+                            : (bias ? attn_kernel<F16, HD, false, true> : attn_kernel<F16, HD, false, false>);
+  const unsigned lds = Lds<HD>::BYTES;
   const int rc = host::allow_lds(reinterpret_cast<const void*>(k), lds, "fa_kv8_attention");
   if (rc != FA_OK) return rc;
   hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * W), lds, s, a);
   if (a.S > FUSED)
-    hipLaunchKernelGGL((join_kernel<F16, HD, W>), dim3((unsigned)(a.B * a.H * a.T * a.G * (HD % 64 == 0 ? HD / 64 : 1))), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((join_kernel<F16, HD>), dim3((unsigned)(a.B * a.H * a.T * a.G * (HD % 64 == 0 ? HD / 64 : 1))), dim3(256), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return host::fail(FA_ERR_LAUNCH, "fa_kv8_attention: %s", hipGetErrorString(e));
   return FA_OK;
-}
-
-template <bool F16, int HD>
-int launch_attn(const AttnArgs& a, hipStream_t s) {
-  return launch_waves<F16, HD, WAVES>(a, s);
 }
 
 template <bool F16>
