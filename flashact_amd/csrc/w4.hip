@@ -282,23 +282,27 @@ struct Cut {
 Cut cut(int M, int N, int K) {
   const int tiles = (N + 15) / 16, nch = (K + 127) / 128;
   Cut c{1, 1, 1};
-  // Four tiles a workgroup share its activations and keep four tiles' codes in flight. That pays where there are workgroups
-  // enough all the same (32768 x 2048: 10.9 instead of 13.3 at M = 5, 11.9 instead of 15.2 at 16) or K is long enough to be
-  // split (2048 x 16384: 10.0 instead of 11.2, 10.4 instead of 12.0); in between it does not (4096 x 16384: 15.1 instead of
-  // 12.9; 2048 x 2048: 6.8 instead of 4.1). More than 16 rows leave registers and LDS for two tiles, more than 32 for one.
+  // Four tiles a workgroup share its activations and keep four tiles' codes in flight. Tiles x chunks of 128 columns: us with
+  // one tile, with four. 5 to 16 rows: from 1024 tiles on (2048 x 16: 13.2, 10.4 at 5 rows and 14.7, 11.3 at 16; at worst 1250 x 32: 15.0,
+  // 17.1), and from 32 tiles of 112 chunks on, where K is split (32 x 112: 10.0, 9.4 and 12.0, 10.0; 128 x 128: 11.9, 9.8 and 13.3, 10.4;
+  // 300 x 128: 23.1, 15.1; below it 16 x 112: 8.9, 9.3; 32 x 104: 9.8, 10.3) but for 201 to 256 tiles of fewer than 160 chunks, whose workgroups
+  // are one too many for a CU each (200 x 128: 12.4, 12.4; 208 x 128: 12.5, 13.6; 208 x 160: 14.8, 14.7). 1 to 4 rows: only from 2048
+  // tiles of up to 8 chunks on, whose waves have next to nothing to do (4096 x 8, 1 row: 11.2, 10.4; 1500 x 8: 6.3, 6.8;
+  // 3125 x 16: 13.6, 21.1). More than 16 rows leave registers and LDS for two tiles, more than 32 for one.
   if (M > 32) c.nt = 1;
   else if (M > 16) c.nt = 2;
-  else if (tiles >= 1024 || (M > 4 && tiles >= 64 && tiles < 256 && nch >= 96)) c.nt = 4;
+  else if (M > 4) c.nt = tiles >= 1024 || (tiles >= 32 && nch >= 112 && (tiles <= 200 || tiles > 256 || nch >= 160)) ? 4 : 1;
+  else c.nt = tiles >= 2048 && nch <= 8 ? 4 : 1;
   const int blocks = (tiles + c.nt - 1) / c.nt, most = M <= 16 && c.nt == 1 ? 16 : 8;
   // Splits cost the join of the last workgroup, about 2 us. With one tile and few rows 16 waves share K already, and only a handful of
-  // workgroups needs more (64 x 16384: 5.5 instead of 8.0, but 2048 x 8192 in two 7.7 instead of 5.8); else K is split until there is a
-  // workgroup a CU (2048 x 16384: 10.0 instead of 24.3 at M = 5, 14.8 instead of 24.6 at 32, 20.7 instead of 28.7 at 48), in
-  // parts of 2048 columns or more (2048 x 2048 in two at M = 32: 7.7 instead of 6.6).
+  // workgroups needs more (64 x 16384: 5.4 instead of 7.7, but 2048 x 8192 in two 7.0 instead of 5.9); else K is split until there is a
+  // workgroup a CU (2048 x 16384: 9.4 instead of 24.2 at M = 5, 14.2 instead of 24.1 at 32, 20.8 instead of 28.8 at 48), in
+  // parts of 2048 columns or more (2048 x 2048 in two at M = 32: 8.2 instead of 6.2).
   c.splits = std::max(1, std::min({(most == 16 ? 32 : 256) / blocks, nch / 16, MAX_SPLITS}));
   const int mine = (nch + c.splits - 1) / c.splits;
-  // Waves: 4096 in all, with two tiles 2048 (16384 x 2048 at M = 32: 11.4 instead of 13.2), of two chunks each or more
-  // (2560 x 2048: 4.1 instead of 4.7 at M = 5, 3.7 instead of 3.9 at 1), and no fewer than four (32768 x 2048 with four
-  // instead of eight: 12.1 instead of 10.9).
+  // Waves: 4096 in all, with two tiles 2048 (16384 x 2048 at M = 32: 10.9 instead of 12.7), of two chunks each or more
+  // (2560 x 2048: 4.2 instead of 4.5 at M = 5, 3.7 instead of 3.9 at 1), and no fewer than four (32768 x 2048 with four
+  // instead of eight: 11.6 instead of 10.6).
   c.waves = std::max(1, std::min({most, std::max(4, (c.nt == 2 ? 2048 : 4096) / (blocks * c.splits)), mine, std::max(4, mine / 2)}));
   return c;
 }
