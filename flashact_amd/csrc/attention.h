@@ -12,7 +12,7 @@
 // Keys and values of the next tiles are copied to LDS (no registers) while this one is worked on, one barrier a tile. With
 // many queries the MFMAs are the bound, next to the LDS reads that feed them (each operand of 1 KB serves 16 or 32 queries)
 // and, capped, the three exponentials a score; with few it is one wave's chain of a tile's steps, about 3000 cycles.
-// 8191 tokens of 16 heads of 128 dims over 4 K/V heads, causal behind a tenth, capped: 374 us, 742 TFLOP/s.
+// 8191 tokens of 16 heads of 128 dims over 4 K/V heads, causal behind a tenth, capped: 369 us, 752 TFLOP/s.
 //
 // Rounding: the scores' products are exact in fp32, softmax and sums are fp32, P is rounded to the values' type for the
 // second product (bf16 values have a range that fp16 weights times fp16 values would not hold), the result once.
@@ -611,9 +611,9 @@ __global__ void __launch_bounds__(256) join_kernel(Params p) {
 
 // Parts that keys are split into, for workgroups of 64 queries with two groups of waves: the least of (rounds of
 // workgroups) x (steps of each, and two for its beginning and end), joining taken as three. A workgroup whose queries see
-// fewer keys makes fewer parts, of LEAST steps or more (packed prompts of 2604 tokens: 59 us with 8, 64 with 4, 61 with 16).
-// 64 queries over 65536 keys of 256 dims 1521 -> 107 us, one over 131072 of 128 dims 1534 -> 126, 1024 over 4096 56 -> 36;
-// of the counts 1 .. 16 the rule's was within 8 % of the best in all of 14 shapes between.
+// fewer keys makes fewer parts, of LEAST steps or more (packed prompts of 2364 tokens: 60.5 us with 8, 62.6 with 4, 60.7 with 16).
+// 64 queries over 65536 keys of 256 dims 1517 -> 109 us, one over 131072 of 128 dims 1424 -> 103, 1024 over 4096 59 -> 39;
+// of the counts 1 .. 16 the rule's was within 3 % of the best in all of 14 shapes between.
 inline int splits_for(int64_t units, int keys, int hd) {
   const int step = hd > 128 ? 64 : 128;
   const int64_t n = (keys + (int64_t)step - 1) / step, most = std::min<int64_t>({n / LEAST, MAX_SPLITS, 1024 / units});
@@ -663,10 +663,10 @@ int launch(Params p, hipStream_t s) {
 template <bool F16, int HD>
 int launch_dims(const Params& p, hipStream_t s) {
   // Few queries: workgroups of 64 in which two groups of waves share the keys, as a lone wave a SIMD waits for itself most of
-  // the time (2048 tokens of 8 heads of 128 dims 44 -> 33 us; 384 workgroups of 96 dims, though, 40 -> 45; with 256 dims up to
-  // 384, where packed prompts of 2604 tokens gain, 86 -> 60 us, more than whole ones of 3000 lose, 140 -> 143). Many:
+  // the time (2048 tokens of 8 heads of 128 dims 46 -> 35 us; 304 workgroups, though, 66 -> 69, 384 of 96 dims 41 -> 48; with 256 dims up
+  // to 384, where packed prompts of 2364 tokens gain, 83 -> 60 us, more than whole ones of 3000 lose, 140 -> 148). Many, past 512:
   // workgroups of 128 with two blocks a wave, which halve the LDS reads for each product (8192 tokens of 16 heads of 128
-  // dims: 631 us instead of 843). 256 dims leave registers for one (two, at one wave a SIMD: 2374 instead of 1467), and two
+  // dims: 605 us instead of 765; 768 workgroups of 64: 72 instead of 90; 512: 57 instead of 53). 256 dims leave registers for one (two, at one wave a SIMD: 2374 instead of 1467), and two
   // workgroups of 64 on a CU go better than one of 128 (1467 instead of 1511).
   const int64_t small = units_of(p.B, p.Tq, p.H);
   if (few(small, HD)) return launch<F16, HD, 1, 4, 2>(p, s);

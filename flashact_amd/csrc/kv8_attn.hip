@@ -578,7 +578,7 @@ extern "C" int fa_kv8_attention(const fa_kv8_attn_args* a, fa_stream_t stream) {
     p.part = reinterpret_cast<float*>(static_cast<unsigned char*>(a->workspace) + kv8::arrived_bytes((size_t)p.RT * p.B * p.H));
   }
   // All row tiles of a (split, sample, head) run on one XCD where these divide evenly over the 8, else in runs short enough
-  // that there are 32 or more (200 tokens of 8 heads over 1100 keys of one sample 35 -> 22 us; 18.4 -> 19.2 for 4 samples of 50).
+  // that there are 32 or more (200 tokens of 8 heads over 1100 keys of one sample 38 -> 21 us; 17.3 -> 17.5 for 4 samples of 50).
   const int64_t groups = (int64_t)p.B * p.H * p.S, runs = groups % 8 ? std::min<int64_t>((31 + groups) / groups, p.RT) : 1;
   p.RC = (int)((p.RT + runs - 1) / runs);
   p.least = (int64_t)p.RT * p.B * p.H >= 64 ? 4 : 1;

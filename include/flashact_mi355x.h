@@ -397,7 +397,9 @@ size_t fa_kv8_attention_workspace_bytes(int batch, int tokens, int heads, int kv
  * documents of a packed batch, a prefix that all see with causal tokens behind it, windows, rows that see nothing (they
  * become zero). Scores are s = q . k * scale, with softcap > 0 softcap * tanh(s / softcap), less
  * slopes[h] * |i + keys - queries - j| (slopes [heads] fp32 or NULL). Query heads h share K/V head h / (heads / kv_heads).
- * What a query does not see does not reach it, NaN and infinities included.
+ * What a query does not see does not reach it, NaN and infinities included. Weights are held in the values' type, relative to a
+ * reference (fp16: from 2^-26 of the largest on with all bits), sums of weighted values in fp32: bf16 values should stay below
+ * 2^120 over the number of keys. out shares no memory with what is read, but may be q itself where that is contiguous.
  * q [batch][queries][heads][head_dim], k and v [batch][keys][kv_heads][head_dim], bf16 or fp16, head_dim a multiple of 8
  * up to 256, dims contiguous, 16-byte aligned, with strides (sample, token, head) in elements, multiples of 8 (token
  * strides of k and v at most 2^23). out [batch][queries][heads][head_dim] contiguous, of the same type, 16-byte aligned.
