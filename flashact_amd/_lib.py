@@ -6,6 +6,7 @@ no fallback: if the shared library is missing or fails to load, every entry poin
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 import torch
@@ -207,28 +208,27 @@ def strides3(t) -> tuple:
     return (s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
 
 
+@functools.lru_cache(maxsize=1024)
+def _layout(shape, stride) -> tuple:
+    """(elements from the first to behind the last, whether two may be one) of a strided layout."""
+    if 0 in shape:
+        return 0, False
+    reach, twice = 0, False
+    for s, n in sorted((s, n) for s, n in zip(stride, shape) if n > 1):
+        twice = twice or s <= reach
+        reach += s * (n - 1)
+    return reach + 1, twice
+
+
 def overlap(a, b) -> bool:
     """Whether two tensors' memory ranges meet."""
-    def ends(t):
-        at = t.data_ptr()
-        if not t.numel():
-            return at, at
-        low = sum(s * (n - 1) for s, n in zip(t.stride(), t.shape) if s < 0)
-        high = sum(s * (n - 1) for s, n in zip(t.stride(), t.shape) if s > 0)
-        return at + low * t.element_size(), at + (high + 1) * t.element_size()
-    a0, a1 = ends(a)
-    b0, b1 = ends(b)
-    return a0 < b1 and b0 < a1
+    at, bt, na, nb = a.data_ptr(), b.data_ptr(), _layout(a.shape, a.stride())[0], _layout(b.shape, b.stride())[0]
+    return na > 0 and nb > 0 and at < bt + nb * b.element_size() and bt < at + na * a.element_size()
 
 
 def doubled(t) -> bool:
     """Whether two elements of a tensor may be one: a stride that does not step over all that smaller strides reach."""
-    reach = 0
-    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
-        if s <= reach:
-            return t.numel() > 0
-        reach += s * (n - 1)
-    return False
+    return _layout(t.shape, t.stride())[1]
 
 
 def meet(a, b) -> bool:

@@ -50,5 +50,6 @@ def test_ordinary_layouts_pass():
     assert _lib.meet(rows[:60], rows[59:]) and not _lib.meet(rows[:60], rows[60:]) and not _lib.meet(rows[::2], rows[1::2])
     assert not _lib.meet(rows[:0], rows) and not _lib.doubled(rows[:0])
     assert _lib.doubled(torch.zeros(10).unfold(0, 4, 2)) and _lib.doubled(torch.zeros(1).expand(5))
+    assert not _lib.overlap(rows[50:50], rows) and _lib.overlap(rows[50:51], rows) and not _lib.overlap(rows[50:51], rows[51:])
     large = torch.zeros(1).expand(1 << 20, 1 << 10)[:, :0]
     assert not _lib.doubled(large)
