@@ -16,10 +16,10 @@ pytestmark = pytest.mark.gpu
 
 def test_joined_parts_in_a_graph(gpu):
     """Up to four parts, joined by the last workgroup. A replay repeats the launch's number: the words that it leaves must not count."""
-    q, k, v = _qkv(gpu, 1, 1024, 4096, 8, 1, 128, torch.bfloat16)
-    i = torch.arange(1024, device=gpu)
-    spans = torch.stack([torch.zeros_like(i), i + 1 + 3072], -1).to(torch.int32)
-    assert attention._workspace_bytes(1, 1024, 4096, 8, 128) > 0
+    q, k, v = _qkv(gpu, 1, 1000, 4000, 8, 1, 128, torch.bfloat16)
+    i = torch.arange(1000, device=gpu)
+    spans = torch.stack([torch.zeros_like(i), i + 3001], -1).to(torch.int32)
+    assert attention._workspace_bytes(1, 1000, 4000, 8, 128) > 0
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
         y = attention.attend(q, k, v, spans)
@@ -27,7 +27,7 @@ def test_joined_parts_in_a_graph(gpu):
     for n in range(6):
         for x in (q, k, v):
             x.copy_(torch.randn(x.shape, device=gpu))
-        spans[:, 1] = (i + 1 + 3072 - 500 * n).clamp(min=0)
+        spans[:, 1] = (i + 3001 - 500 * n).clamp(min=0)
         g.replay()
         torch.cuda.synchronize()
         want = attention.attend(q, k, v, spans)
