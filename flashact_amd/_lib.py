@@ -126,6 +126,30 @@ class SpanArgs(ctypes.Structure):
     ]
 
 
+class PagedRowsArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int), ("q", ctypes.c_void_p), ("q_stride", ctypes.c_longlong * 3), ("q_out", ctypes.c_void_p),
+        ("k", ctypes.c_void_p), ("k_stride", ctypes.c_longlong * 4), ("v", ctypes.c_void_p), ("v_stride", ctypes.c_longlong * 4),
+        ("pool_k", ctypes.c_void_p), ("pool_v", ctypes.c_void_p), ("table", ctypes.c_void_p), ("table_stride", ctypes.c_longlong),
+        ("start", ctypes.c_void_p), ("count", ctypes.c_void_p), ("freqs", ctypes.c_void_p),
+        ("batch", ctypes.c_int), ("tokens", ctypes.c_int), ("heads", ctypes.c_int), ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int), ("pages", ctypes.c_int), ("table_pages", ctypes.c_int), ("rotary", ctypes.c_int),
+        ("adjacent", ctypes.c_int), ("zero_rest", ctypes.c_int),
+    ]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int), ("q", ctypes.c_void_p), ("q_stride", ctypes.c_longlong * 3),
+        ("pool_k", ctypes.c_void_p), ("pool_v", ctypes.c_void_p), ("table", ctypes.c_void_p), ("table_stride", ctypes.c_longlong),
+        ("lens", ctypes.c_void_p), ("count", ctypes.c_void_p), ("slopes", ctypes.c_void_p),
+        ("batch", ctypes.c_int), ("tokens", ctypes.c_int), ("heads", ctypes.c_int), ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int), ("pages", ctypes.c_int), ("table_pages", ctypes.c_int), ("causal", ctypes.c_int),
+        ("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("out", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class DeviceInfo(ctypes.Structure):
     _fields_ = [("cus", ctypes.c_int), ("xcds", ctypes.c_int), ("lds_bytes", ctypes.c_int),
                 ("coop_launch", ctypes.c_int), ("coop_max_blocks", ctypes.c_int), ("arch", ctypes.c_char * 64)]
@@ -156,6 +180,10 @@ SYMBOLS = [
     ("fa_kv8_attention_workspace_bytes", ctypes.c_size_t, [ctypes.c_int] * 6),
     ("fa_span_attention_workspace_bytes", ctypes.c_size_t, [ctypes.c_int] * 5),
     ("fa_span_attention", ctypes.c_int, [ctypes.POINTER(SpanArgs), ctypes.c_void_p]),
+    ("fa_paged_append", ctypes.c_int, [ctypes.POINTER(PagedRowsArgs), ctypes.c_void_p]),
+    ("fa_paged_load", ctypes.c_int, [ctypes.POINTER(PagedRowsArgs), ctypes.c_void_p]),
+    ("fa_paged_attention", ctypes.c_int, [ctypes.POINTER(PagedAttnArgs), ctypes.c_void_p]),
+    ("fa_paged_attention_workspace_bytes", ctypes.c_size_t, [ctypes.c_int] * 6),
     ("fa_device_query", ctypes.c_int, [ctypes.c_int, ctypes.POINTER(DeviceInfo)]),
     ("fa_last_error", ctypes.c_char_p, []),
     ("fa_abi_version", ctypes.c_int, []),

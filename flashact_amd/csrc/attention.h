@@ -86,11 +86,6 @@ template <bool F16>
 __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
   return F16 ? mfma16h(a, b, c) : mfma16(a, b, c);
 }
-// sign bit of each half that is an infinity or NaN
-template <bool F16>
-__device__ __forceinline__ unsigned not_finite(unsigned x) {
-  return F16 ? ((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u : ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-}
 // sign bit of each half whose fraction is not zero
 template <bool F16>
 __device__ __forceinline__ unsigned fraction(unsigned x) {

@@ -1,0 +1,286 @@
+// Attention of each sample's newest tokens over a paged cache (fa_paged_attention); the pages' layout is in paged.hip.
+//
+// Row (t, h) of sample b is the query of token t < n at position i = len - n + t. It sees keys j < i + 1 (causal)
+// or j < len:  s_j = q . k_j scale, capped to cap tanh(s_j / cap), less slope_h |i - j|;  o = sum_j softmax(s)_j v_j.
+//
+// What bounds it is reading the cache once: 4 hd bytes a key and K/V head. The rows that share a K/V head are the 16 columns of the
+// MFMAs. A wave takes pages on its own with a running maximum and sum: S^T = K Q^T (16x16x32, two tiles of 16 keys), softmax
+// down the columns, O^T += V^T P^T; row m of key tile t is key 8 (m / 4) + 4 t + m % 4, so lane quarter q ends with keys
+// 8 q .. 8 q + 7, the next product's operand. Each wave copies its pages to LDS on its own (no registers, no barrier): the next
+// page's keys are asked for as soon as this one's are in registers, the values' likewise, and the page after it is looked up in
+// the table by a scalar load meanwhile. How pages are dealt to waves and workgroups, and how their sums meet: newest.h.
+//
+// Rounding: scores are exact products summed in fp32, softmax and sums are fp32. bf16: the weights go into the second
+// product as two bf16 (2^-17 of each is lost; its MFMAs are not the bound), and are taken against a reference 2^17 above
+// the maximum, so that 131072 keys cannot leave the fp32 range whatever the values. fp16: the weights are rounded once (2^-12), against a
+// reference 2^15 below the maximum: those above 2^-29 of the largest keep all their bits.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "../../include/flashact_mi355x.h"
+#include "fa_device.h"
+#include "fa_host.h"
+#include "newest.h"
+
+namespace fa {
+namespace paged {
+
+using newest::BT;
+using newest::Place;
+using newest::Span;
+using newest::W;
+using newest::lds_wait;
+using newest::vm_wait;
+
+struct AttnArgs : newest::Args {
+  const unsigned char *k, *v;
+  const int* table;
+  int64_t ts;
+  int pages;
+};
+
+template <bool F16>
+__device__ __forceinline__ float reference(float top) {
+  return fabsf(top) < 4194304.f ? top + (F16 ? -15.f : 17.f) : top;  // past 2^22 the difference would round
+}
+template <bool F16>
+__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+  return F16 ? mfma16h(a, b, c) : mfma16(a, b, c);
+}
+// The halves of words 0 .. 3 (keys 0 .. 7) below n.
+__device__ __forceinline__ u32x4 halves_below(int n) {
+  u32x4 x;
+#pragma unroll
+  for (int j = 0; j < 4; j++) x[j] = n >= 2 * j + 2 ? ~0u : n == 2 * j + 1 ? 0xffffu : 0u;
+  return x;
+}
+
+template <int HD>
+using Lds = newest::Lds<HD, 2 * BT * HD * 2>;  // of a wave: a page of keys and one of values
+
+template <bool F16, int HD, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : HD == 128 ? 2 : HD == 96 ? 3 : 4) attn_kernel(AttnArgs a) {
+  constexpr int KS = HD / 32, NT = HD / 16, PAGE = BT * HD * 2, NC = PAGE / 1024;  // NC: copies of a page
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  const Place here = newest::place_of(a);
+  if (!here.there) return;
+  const int b = here.b, h = here.h, rt = here.rt, split = here.split;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const Span sp = newest::span_of(a, b);
+
+  const int rr = rt * 16 + r, t = rr / a.G, head = h * a.G + rr % a.G, pos = sp.len - sp.n + t;
+  const bool valid = rr < a.T * a.G && t < sp.n && pos >= 0;
+  int limit = valid ? (a.causal ? pos + 1 : sp.len) : 0;
+  int hi = limit, lo = valid ? limit : 0x7fffffff;
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    hi = max(hi, __shfl_xor(hi, o));
+    lo = min(lo, __shfl_xor(lo, o));
+  }
+  hi = __builtin_amdgcn_readfirstlane(hi);  // keys that any row sees
+  lo = __builtin_amdgcn_readfirstlane(lo);  // keys that every row sees (rows that are not there do not count)
+  if (!valid) limit = hi;
+  const int nb = (hi + BT - 1) / BT;
+  const int used = newest::splits_used(a, nb);
+  if (split >= used) return;
+  const int at = split * W + wave, all = used * W;
+
+  u32x4 qf[KS];
+#pragma unroll
+  for (int i = 0; i < KS; i++) {
+    qf[i] = u32x4{0, 0, 0, 0};
+    if (valid) qf[i] = *reinterpret_cast<const u32x4*>(a.q + (b * a.qb + t * a.qt + head * a.qh + 32 * i + 8 * q) * 2);
+  }
+  const float slope = BIAS && valid ? a.slopes[head] * newest::LOG2E : 0.f;
+
+  // The table is constant while the kernel runs: scalar loads.
+  typedef const __attribute__((address_space(4))) int* Table;
+  const Table table = (Table)(uintptr_t)(a.table + b * a.ts);
+  auto page = [&](int blk) { return blk < nb ? table[blk] : 0; };
+  auto there = [&](int pg) { return (unsigned)pg < (unsigned)a.pages; };
+  unsigned char* kl = lds + wave * Lds<HD>::WAVE;
+  unsigned char* vl = kl + PAGE;
+  const unsigned at_k = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)kl), at_v = at_k + PAGE;
+  auto copy = [&](const unsigned char* from, int pg, unsigned to) {  // of a page that is not there, the first one
+    const unsigned char* p = from + ((size_t)(there(pg) ? pg : 0) * a.H + h) * PAGE;
+#pragma unroll
+    for (int i = 0; i < NC; i++) copy_to_lds(p + i * 1024, lane * 16, to + i * 1024);
+  };
+
+  f32x4 O[NT];
+#pragma unroll
+  for (int j = 0; j < NT; j++) O[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;  // l: this lane's keys only
+  int pg = page(at), next = page(at + all);
+  if (at < nb) {
+    copy(a.k, pg, at_k);
+    copy(a.v, pg, at_v);
+  }
+  // The queries are waited for here: left to the compiler, that wait (for everything under way) stands in the loop.
+#pragma unroll
+  for (int i = 0; i < KS; i++) asm volatile("" : "+v"(qf[i]));
+  for (int blk = at; blk < nb; blk += all) {
+    const bool more = blk + all < nb;
+    const int later = page(blk + 2 * all);
+    vm_wait<NC>();  // the keys; the values are still on their way
+    u32x4 kc[2][KS];
+#pragma unroll
+    for (int i = 0; i < KS; i++)
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+        kc[x][i] = *reinterpret_cast<const u32x4*>(kl + ((4 * i + q) * BT + 8 * (r >> 2) + 4 * x + (r & 3)) * 16);
+    lds_wait();
+    if (more) copy(a.k, next, at_k);
+    f32x4 s[2];
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      s[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KS; i++) s[x] = mma<F16>(kc[x][i], qf[i], s[x]);
+    }
+    const bool gone = !there(pg);  // nobody sees a key of no page
+    const int key0 = blk * BT + 8 * q, lo_b = gone ? 0 : lo, hi_b = gone ? 0 : hi, own = gone ? 0 : limit;
+    const bool mixed = blk * BT + BT > lo_b;
+    const float mx = newest::scores<CAP, BIAS>(a, s, 1.f, key0, mixed, own, slope, pos);
+    const float mn = fmaxf(m, reference<F16>(cols_max(mx)));
+    const float ms = mn == -INFINITY ? 0.f : mn;
+    if (__builtin_amdgcn_ballot_w64(mn != m)) {
+      const float al = exp2_w(m - ms);  // 0 where there was nothing yet
+      l *= al;
+#pragma unroll
+      for (int j = 0; j < NT; j++) O[j] *= al;
+      m = mn;
+    }
+    u32x4 P, R;  // R: what P's rounding left, bf16 only
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        s[x][i] = exp2_w(s[x][i] - ms);
+        l += s[x][i];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        if constexpr (F16) {
+          P[2 * x + i] = pack_f16x2(s[x][2 * i], s[x][2 * i + 1]);
+        } else {
+          const unsigned p = pack_bf16x2(s[x][2 * i], s[x][2 * i + 1]);
+          P[2 * x + i] = p;
+          R[2 * x + i] = pack_bf16x2(s[x][2 * i] - bf_lo(p), s[x][2 * i + 1] - bf_hi(p));
+        }
+      }
+    }
+    if (more) vm_wait<NC>();
+    else vm_wait<0>();
+    u32x4 vc[NT];  // keys key0 .. key0 + 7 of dim 16 j + r
+#pragma unroll
+    for (int j = 0; j < NT; j++) vc[j] = *reinterpret_cast<const u32x4*>(vl + (q * HD + 16 * j + r) * 16);
+    lds_wait();
+    if (more) copy(a.v, next, at_v);
+    // Values of keys that a row does not see must not reach it: its P is 0 there, but 0 x NaN is NaN. Those behind the
+    // last key that any row sees are cleared; where one between lo and hi is not finite, each column has its own product.
+    bool apart = false;
+    if (mixed) {
+      const u32x4 some = halves_below(hi_b - key0), each = halves_below(lo_b - key0);
+      unsigned bad = 0;
+#pragma unroll
+      for (int j = 0; j < NT; j++) {
+        vc[j] &= some;
+#pragma unroll
+        for (int i = 0; i < 4; i++) bad |= not_finite<F16>(vc[j][i]) & ~each[i];
+      }
+      apart = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+    }
+    if (!apart) {
+#pragma unroll
+      for (int j = 0; j < NT; j++) {
+        O[j] = mma<F16>(vc[j], P, O[j]);
+        if constexpr (!F16) O[j] = mma<F16>(vc[j], R, O[j]);
+      }
+    } else {
+#pragma unroll 1
+      for (int c = 0; c < 16; c++) {
+        const u32x4 mine = halves_below(__builtin_amdgcn_readlane(own, c) - key0);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+          f32x4 o = mma<F16>(vc[j] & mine, P, O[j]);
+          if constexpr (!F16) o = mma<F16>(vc[j] & mine, R, o);
+          if (r == c) O[j] = o;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+    pg = next, next = later;
+  }
+  newest::meet<F16, HD, Lds<HD>>(a, here, sp, used, lds, O, m, cols_sum(l));
+}
+
+template <bool F16, int HD>
+__global__ void __launch_bounds__(256) join_kernel(AttnArgs a) {
+  newest::join<F16, HD>(a);
+}
+
+// Estimates of a wave's time for a page, and of the workgroups whose waves do not share bandwidth.
+int splits_for(int batch, int tokens, int heads, int kv_heads, int hd, int pages) {
+  return newest::splits_for(batch, tokens, heads, kv_heads, pages, hd == 256 ? 2.3 : 1.2, hd == 256 ? 1.0 : 2.0);
+}
+
+template <bool F16, int HD>
+int launch_attn(const AttnArgs& a, hipStream_t s) {
+  const unsigned grid = newest::grid_of(a);
+  if (!grid) return host::fail(FA_ERR_INVALID_ARG, "fa_paged_attention: too many rows for one call");
+  const bool cap = a.cap > 0.f, bias = a.slopes != nullptr;
+  void (*k)(AttnArgs) = cap ? (bias ? attn_kernel<F16, HD, true, true> : attn_kernel<F16, HD, true, false>)
+                            : (bias ? attn_kernel<F16, HD, false, true> : attn_kernel<F16, HD, false, false>);
+  const unsigned lds = Lds<HD>::BYTES;
+  const int rc = host::allow_lds(reinterpret_cast<const void*>(k), lds, "fa_paged_attention");
+  if (rc != FA_OK) return rc;
+  hipLaunchKernelGGL(k, dim3(grid), dim3(64 * W), lds, s, a);
+  if (a.S > newest::FUSED) hipLaunchKernelGGL((join_kernel<F16, HD>), dim3(newest::join_grid(a, HD)), dim3(256), 0, s, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return host::fail(FA_ERR_LAUNCH, "fa_paged_attention: %s", hipGetErrorString(e));
+  return FA_OK;
+}
+
+template <bool F16>
+int launch_attn(const AttnArgs& a, int hd, hipStream_t s) {
+  if (hd == 64) return launch_attn<F16, 64>(a, s);
+  if (hd == 96) return launch_attn<F16, 96>(a, s);
+  if (hd == 128) return launch_attn<F16, 128>(a, s);
+  return launch_attn<F16, 256>(a, s);
+}
+
+int check_pool(const void* k, const void* v, const int* table, int batch, int heads, int hd, int pages, int width, int64_t stride,
+               const char* who);  // paged.hip
+
+}  // namespace paged
+}  // namespace fa
+
+extern "C" size_t fa_paged_attention_workspace_bytes(int batch, int tokens, int heads, int kv_heads, int head_dim, int table_pages) {
+  if (batch < 1 || tokens < 1 || kv_heads < 1 || heads < kv_heads || heads % kv_heads || head_dim < 1 || table_pages < 1) return 0;
+  return fa::newest::workspace(fa::paged::splits_for(batch, tokens, heads, kv_heads, head_dim, table_pages), batch, tokens, heads,
+                               kv_heads, head_dim);
+}
+
+extern "C" int fa_paged_attention(const fa_paged_attn_args* a, fa_stream_t stream) {
+  using namespace fa;
+  const char* who = "fa_paged_attention";
+  if (!a) return host::fail(FA_ERR_INVALID_ARG, "%s: args is NULL", who);
+  int rc = paged::check_pool(a->pool_k, a->pool_v, a->table, a->batch, a->kv_heads, a->head_dim, a->pages, a->table_pages,
+                             a->table_stride, who);
+  if (rc != FA_OK) return rc;
+  rc = newest::check_call(a, who);
+  if (rc != FA_OK || a->tokens == 0) return rc;
+  paged::AttnArgs p{};
+  p.k = static_cast<const unsigned char*>(a->pool_k), p.v = static_cast<const unsigned char*>(a->pool_v);
+  p.table = a->table, p.ts = a->table_stride, p.pages = a->pages;
+  rc = newest::set_up(p, a, a->table_pages, paged::splits_for(a->batch, a->tokens, a->heads, a->kv_heads, a->head_dim, a->table_pages),
+                      who);
+  if (rc != FA_OK) return rc;
+  rc = host::check_gfx950(who);
+  if (rc != FA_OK) return rc;
+  return a->dtype == FA_DTYPE_F16 ? paged::launch_attn<true>(p, a->head_dim, (hipStream_t)stream)
+                                  : paged::launch_attn<false>(p, a->head_dim, (hipStream_t)stream);
+}

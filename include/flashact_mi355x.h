@@ -392,6 +392,81 @@ typedef struct fa_kv8_attn_args {
 int fa_kv8_attention(const fa_kv8_attn_args* args, fa_stream_t stream);
 size_t fa_kv8_attention_workspace_bytes(int batch, int tokens, int heads, int kv_heads, int head_dim, int blocks);
 
+/* ---------------------------------------------------------------- paged K/V cache
+ * A pool of `pages` pages of 32 tokens, one layer's, that a table deals to the samples; 16-bit, contiguous, 16-byte aligned:
+ *   pool_k [pages][kv_heads][head_dim / 8][32 tokens][8 dims] and pool_v [pages][kv_heads][4][head_dim][8 tokens]
+ * (token 8 i + j of a page is [i][dim][j]), head_dim 64, 96, 128 or 256. Tokens 32 i .. 32 i + 31 of sample b are in page
+ * table[b][i], i < table_pages (rows table_stride elements apart). A page may be named more than once (shared prefixes);
+ * one outside [0, pages) holds nothing: what is stored there is dropped, what is read there is not seen (loaded: zeros).
+ * fa_paged_append puts row i < count[b] (tokens where count is NULL) of sample b at token p = start[b] + i and turns the first
+ * `rotary` dims of its key (a multiple of 16; 0: none) by the angles p freqs[j], j < rotary / 2, radians, taken in 64 bits: the pairs
+ * (j, j + rotary / 2), or (2 j, 2 j + 1) with `adjacent`, which are stored as (j, j + rotary / 2) too. Rows of queries, if
+ * q is given, are turned alike into q_out [batch][tokens][heads][head_dim], contiguous; those that are not real become zero. Rows
+ * behind the table's end are dropped (queries are turned there too), as is a sample with a negative start.
+ * fa_paged_load writes tokens i < min(count[b], tokens) to row i of k and v; rows behind them become zero with zero_rest, else
+ * they are left as they are.
+ * Rows have the pool's type and strides (sample, token, head, dim) in elements: for append multiples of 8, dims contiguous,
+ * 16-byte aligned; for load any. Rows, q_out and the pool share no memory.
+ */
+typedef struct fa_paged_rows_args {
+  int dtype; /* FA_DTYPE_BF16 or FA_DTYPE_F16 */
+  const void* q; /* append only, or NULL */
+  long long q_stride[3];
+  void* q_out;
+  void* k;
+  long long k_stride[4];
+  void* v;
+  long long v_stride[4];
+  void* pool_k;
+  void* pool_v;
+  const int* table;
+  long long table_stride;
+  const int* start; /* [batch], append only */
+  const int* count; /* [batch] */
+  const double* freqs; /* [rotary / 2], append only */
+  int batch;
+  int tokens;
+  int heads; /* of q */
+  int kv_heads;
+  int head_dim;
+  int pages;
+  int table_pages;
+  int rotary;
+  int adjacent;
+  int zero_rest; /* load only */
+} fa_paged_rows_args;
+int fa_paged_append(const fa_paged_rows_args* args, fa_stream_t stream);
+int fa_paged_load(const fa_paged_rows_args* args, fa_stream_t stream);
+
+/* fa_kv8_attention's attention over the pages: see there. lens beyond the table count as its end; tokens of no page are not seen. */
+typedef struct fa_paged_attn_args {
+  int dtype; /* of q, the pool and out */
+  const void* q;
+  long long q_stride[3];
+  const void* pool_k;
+  const void* pool_v;
+  const int* table;
+  long long table_stride;
+  const int* lens;  /* [batch] */
+  const int* count; /* [batch] or NULL */
+  const float* slopes;
+  int batch;
+  int tokens;
+  int heads;
+  int kv_heads;
+  int head_dim;
+  int pages;
+  int table_pages;
+  int causal;
+  float scale;
+  float softcap;
+  void* out;
+  void* workspace;
+  size_t workspace_bytes;
+} fa_paged_attn_args;
+int fa_paged_attention(const fa_paged_attn_args* args, fa_stream_t stream);
+size_t fa_paged_attention_workspace_bytes(int batch, int tokens, int heads, int kv_heads, int head_dim, int table_pages);
+
 /* ---------------------------------------------------------------- attention over spans of keys
  * Query i of sample b sees the keys spans[b][i][0] <= j < spans[b][i][1] (clamped to [0, keys); spans NULL: all): the
  * documents of a packed batch, a prefix that all see with causal tokens behind it, windows, rows that see nothing (they
