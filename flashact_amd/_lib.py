@@ -150,6 +150,25 @@ class PagedAttnArgs(ctypes.Structure):
     ]
 
 
+class LoraArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int), ("y_dtype", ctypes.c_int), ("x", ctypes.c_void_p), ("x_stride", ctypes.c_longlong),
+        ("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("index", ctypes.c_void_p),
+        ("rows", ctypes.c_int), ("n", ctypes.c_int), ("k", ctypes.c_int), ("rank", ctypes.c_int), ("adapters", ctypes.c_int),
+        ("gate", ctypes.c_int), ("y", ctypes.c_void_p), ("out", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class TokenLogprobsArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int), ("logits", ctypes.c_void_p), ("stride", ctypes.c_longlong), ("tokens", ctypes.c_void_p),
+        ("wide_tokens", ctypes.c_int), ("scale", ctypes.c_float), ("rows", ctypes.c_int), ("vocabulary", ctypes.c_int),
+        ("top", ctypes.c_int), ("logprob", ctypes.c_void_p), ("entropy", ctypes.c_void_p), ("top_tokens", ctypes.c_void_p),
+        ("top_logprobs", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class DeviceInfo(ctypes.Structure):
     _fields_ = [("cus", ctypes.c_int), ("xcds", ctypes.c_int), ("lds_bytes", ctypes.c_int),
                 ("coop_launch", ctypes.c_int), ("coop_max_blocks", ctypes.c_int), ("arch", ctypes.c_char * 64)]
@@ -184,6 +203,10 @@ SYMBOLS = [
     ("fa_paged_load", ctypes.c_int, [ctypes.POINTER(PagedRowsArgs), ctypes.c_void_p]),
     ("fa_paged_attention", ctypes.c_int, [ctypes.POINTER(PagedAttnArgs), ctypes.c_void_p]),
     ("fa_paged_attention_workspace_bytes", ctypes.c_size_t, [ctypes.c_int] * 6),
+    ("fa_lora_add", ctypes.c_int, [ctypes.POINTER(LoraArgs), ctypes.c_void_p]),
+    ("fa_lora_workspace_bytes", ctypes.c_size_t, [ctypes.c_int] * 3),
+    ("fa_token_logprobs", ctypes.c_int, [ctypes.POINTER(TokenLogprobsArgs), ctypes.c_void_p]),
+    ("fa_token_logprobs_workspace_bytes", ctypes.c_size_t, [ctypes.c_int] * 4),
     ("fa_device_query", ctypes.c_int, [ctypes.c_int, ctypes.POINTER(DeviceInfo)]),
     ("fa_last_error", ctypes.c_char_p, []),
     ("fa_abi_version", ctypes.c_int, []),

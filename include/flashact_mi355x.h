@@ -467,6 +467,70 @@ typedef struct fa_paged_attn_args {
 int fa_paged_attention(const fa_paged_attn_args* args, fa_stream_t stream);
 size_t fa_paged_attention_workspace_bytes(int batch, int tokens, int heads, int kv_heads, int head_dim, int table_pages);
 
+/* ---------------------------------------------------------------- low-rank adapters of many requests
+ * out[m] = y[m] + scale[i] b_i (a_i x[m]), i = index[m] (outside [0, adapters): out[m] = y[m]), m < rows. a_i [rank][k] and b_i [n][rank]
+ * are x's type, bf16 or fp16, finite, k and rank multiples of 8, rank <= 128 (adapters of lower rank are padded with zeros), laid out as
+ *   a [adapters][k / 8][rank][8] and b [adapters][rank / 8][n][8], 16-byte aligned; scale [adapters] fp32.
+ * x [rows][k] with a row stride of x_stride elements (a multiple of 8), 16-byte aligned; y and out [rows][n] contiguous, fp32 or x's type;
+ * out may be y itself and shares no other memory with what is read. gate != 0: columns 2f, 2f + 1 of the sum are a gate and its
+ * input, out[m][f] = gelu_tanh(sum[2f]) sum[2f + 1], [rows][n / 2] of x's type, which shares no memory with y.
+ * Sums are fp32. workspace: fa_lora_workspace_bytes(rows, k, rank) bytes, 16-byte aligned; it needs no initialisation and holds
+ * nothing between calls.
+ */
+typedef struct fa_lora_args {
+  int dtype;   /* of x, a, b: FA_DTYPE_BF16 or FA_DTYPE_F16 */
+  int y_dtype; /* FA_DTYPE_F32 or dtype */
+  const void* x;
+  long long x_stride;
+  const void* a;
+  const void* b;
+  const float* scale;
+  const int* index;
+  int rows;
+  int n;
+  int k;
+  int rank;
+  int adapters;
+  int gate;
+  const void* y;
+  void* out;
+  void* workspace;
+  size_t workspace_bytes;
+} fa_lora_args;
+int fa_lora_add(const fa_lora_args* args, fa_stream_t stream);
+size_t fa_lora_workspace_bytes(int rows, int k, int rank);
+
+/* ---------------------------------------------------------------- log probabilities of tokens
+ * With z = scale * logits[row] (scale > 0, an inverse temperature) and p = softmax(z): logprob[row] = log p[tokens[row]], entropy[row] =
+ * -sum p log p (in nats, terms with p = 0 are 0), and the `top` largest logits' indices, equal ones by ascending index, with their
+ * log p. logits bf16, fp16 or fp32, rows `stride` elements apart, of any alignment; sums are fp32. A logit of -inf is a token that
+ * is ruled out (log p = -inf); a row of nothing else has log p = -inf throughout and entropy 0. tokens are int, or long long with
+ * wide_tokens; one outside [0, vocabulary) has log p = -inf. A row with a NaN or +inf has log p and entropy NaN; NaN is never among
+ * the largest (where fewer than `top` others are left: token -1).
+ * workspace: fa_token_logprobs_workspace_bytes(...) bytes, 16-byte aligned (0: may be NULL); it needs no initialisation and holds
+ * nothing between calls, but calls that may overlap need one each.
+ */
+#define FA_TOKENS_MAX_TOP 32
+typedef struct fa_token_logprobs_args {
+  int dtype;
+  const void* logits;
+  long long stride;
+  const void* tokens;
+  int wide_tokens;
+  float scale;
+  int rows;
+  int vocabulary;
+  int top; /* 0 .. FA_TOKENS_MAX_TOP */
+  float* logprob;      /* [rows] */
+  float* entropy;      /* [rows] */
+  int* top_tokens;     /* [rows][top] */
+  float* top_logprobs; /* [rows][top] */
+  void* workspace;
+  size_t workspace_bytes;
+} fa_token_logprobs_args;
+int fa_token_logprobs(const fa_token_logprobs_args* args, fa_stream_t stream);
+size_t fa_token_logprobs_workspace_bytes(int dtype, int rows, int vocabulary, int top);
+
 /* ---------------------------------------------------------------- attention over spans of keys
  * Query i of sample b sees the keys spans[b][i][0] <= j < spans[b][i][1] (clamped to [0, keys); spans NULL: all): the
  * documents of a packed batch, a prefix that all see with causal tokens behind it, windows, rows that see nothing (they
