@@ -3,13 +3,16 @@
 //   z = scale x;  m = max z, s = sum e^(z - m), t = sum (z - m) e^(z - m):
 //   log p_i = z_i - m - log s,  entropy = log s - t / s,  alternatives by (x descending, index ascending).
 //
-// Bound by reading the logits. A workgroup takes a part of a row, 16 values a thread at a time; every lane keeps its own running
-// maximum (of x, exact) and sums. The alternatives are a sorted list in the lanes of each wave, lane i the i-th best. Against it
-// each batch costs one comparison of the lane's maximum, which the running maximum needs anyway; only where that passes the list's
-// last are the single values looked at, and those that pass are inserted one by one. A wave's first batch is filtered by
-// a bound under which k values lie: the k-th largest of the lanes' maxima, by bisection of their upper 16 bits. Behind it a
-// batch of n values after N has k n / N that pass.
-// Few rows are split over up to 64 workgroups, whose sums and lists the last one to arrive joins.
+// Bound by reading the logits, once. A workgroup takes a part of a row, 16 values a thread at a time; every thread keeps its own
+// running maximum (of x, exact) and sums. Few rows are split over up to 32 workgroups, whose sums the last one to arrive joins.
+//
+// The alternatives cost the pass over the row nothing: they are found behind it, from the threads' maxima. The k-th largest maximum of 64
+// groups of threads is a bound that at least k values reach, and few more (24 for k = 20, whatever the row's length). The
+// threads whose maximum reaches it read their values again, those that do are put side by side, and each counts how many are before it.
+// Where ties leave too many (a row of equal values), the k-th largest value is found exactly by four counts of eight bits
+// over the whole row, and equal ones are taken in the row's order.
+// (Sorted lists kept by each wave during the pass, with insertions one by one, took 16 us instead of 9 for 8 of 262144 bf16 logits, and
+// 35 instead of 14 for 20 of 48 rows of 99991: every step from a comparison to a scalar and back costs some 50 cycles.)
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -22,8 +25,8 @@ namespace fa {
 namespace tokens {
 
 constexpr int W = 4;  // waves of a workgroup
-constexpr int MAX_SPLITS = 64;
-constexpr int NONE = 0x7fffffff;  // index of an alternative that is not there
+constexpr int MAX_SPLITS = 32;
+constexpr int MOST = 512;  // threads that look again, and values that they may find, for the short way
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float LEAST = -1e30f;  // for -inf where it is multiplied by a weight of 0
 
@@ -33,14 +36,14 @@ struct Params {
   const void* tokens;
   int wide;  // tokens are 64-bit
   float scale, c;  // c: scale log2(e)
-  int rows, V, top, S;
+  int rows, V, top, S, per;  // per: vectors of a split
   float *logprob, *entropy;
   int* top_tokens;
   float* top_logprobs;
-  float* part;  // [row][split] {m, s, t, 0, {x, index}[top]}
+  float* part;  // [row][split] {m, s, t, 0, maximum[threads]}; without alternatives the first four
   uint64_t *arrived, nonce;  // [row][split]
 };
-__host__ __device__ constexpr int part_floats(int top) { return 4 + 2 * top; }
+__host__ __device__ constexpr int part_floats(bool top) { return top ? 4 + 64 * W : 4; }
 
 template <int DT>
 struct Vec {
@@ -61,52 +64,13 @@ __device__ __forceinline__ float value_at(const unsigned char* row, int i) {
   else return as_f32((unsigned)reinterpret_cast<const unsigned short*>(row)[i] << 16);
 }
 
-// A wave's best alternatives: lane i < k holds the i-th.
-struct Best {
-  float v;
-  int i;
-  float last_v;  // the k-th
-  int last_i, k;
-
-  __device__ __forceinline__ void clear(int top) { v = last_v = -INFINITY, i = last_i = NONE, k = top; }
-  __device__ __forceinline__ bool passes(float x, int at) const { return x > last_v || (x == last_v && at < last_i); }
-  __device__ __forceinline__ void insert(float x, int at) {
-    const bool before = v > x || (v == x && i < at);  // a prefix of the lanes
-    const int place = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before)), lane = threadIdx.x & 63;
-    const float up_v = __shfl_up(v, 1);
-    const int up_i = __shfl_up(i, 1);
-    v = lane < place ? v : lane == place ? x : up_v;
-    i = lane < place ? i : lane == place ? at : up_i;
-    last_v = as_f32(__builtin_amdgcn_readlane(as_u32(v), k - 1));
-    last_i = __builtin_amdgcn_readlane(i, k - 1);
-  }
-  // Each lane offers one value; whether any passed.
-  __device__ __forceinline__ bool offer(float x, int at, bool there) {
-    uint64_t todo = __builtin_amdgcn_ballot_w64(there && passes(x, at));
-    if (!todo) return false;
-    do {
-      const int l = __builtin_ctzll(todo);
-      insert(as_f32(__builtin_amdgcn_readlane(as_u32(x), l)), __builtin_amdgcn_readlane(at, l));
-      todo &= todo - 1;
-      todo &= __builtin_amdgcn_ballot_w64(passes(x, at));
-    } while (todo);
-    return true;
-  }
-};
-
-// A bound that at least k of the lanes' values x reach: their k-th largest, its lower 16 bits cleared downwards.
-__device__ __forceinline__ float kth_bound(float x, int k) {
-  const unsigned u = as_u32(x), key = (u >> 31 ? ~u : u | 0x80000000u) >> 16;  // ordered as the values are
-  unsigned p = 0;
-#pragma unroll
-  for (int bit = 15; bit >= 0; bit--) {
-    const unsigned next = p | 1u << bit;
-    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(key >= next)) >= k) p = next;
-  }
-  if (p <= 0x007fu) return -INFINITY;  // the key of -inf
-  const unsigned b = p << 16;
-  return as_f32(b >> 31 ? b & 0x7fffffffu : ~b);
+// Unsigned numbers in the values' order (-0 as 0), and back. NaN is above all: it is sorted out by itself.
+__device__ __forceinline__ unsigned ordered(float x) {
+  const unsigned u = as_u32(x + 0.f);
+  return u >> 31 ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float unordered(unsigned u) { return as_f32(u >> 31 ? u & 0x7fffffffu : ~u); }
+constexpr unsigned NOTHING = 0x007fffffu;  // ordered(-inf)
 
 struct Sums {
   float m, s, t;
@@ -116,65 +80,271 @@ __device__ __forceinline__ Sums sum_lanes(Sums x, float c) {
   Sums y;
   y.m = wave_max(x.m);
   const float d = fmaxf((x.m - (y.m == -INFINITY ? 0.f : y.m)) * c, LEAST), a = exp2_w(d);
-  y.s = wave_sum(a * x.s);
-  y.t = wave_sum(a * (x.t + d * x.s));
+  // lane 0's: a fused product and sum in the first step may leave the lanes a last bit apart
+  y.s = as_f32(__builtin_amdgcn_readfirstlane(as_u32(wave_sum(a * x.s))));
+  y.t = as_f32(__builtin_amdgcn_readfirstlane(as_u32(wave_sum(a * (x.t + d * x.s)))));
   return y;
+}
+
+// Where a row lies: vectors of 16 aligned bytes, of which [whole_b, whole_e) lie in it whole. Up to 2 (E - 1) values at its ends do not
+// belong to one of these.
+template <int DT>
+struct Row {
+  static constexpr int E = Vec<DT>::E;
+  const unsigned char* x;
+  const u32x4* base;
+  int off, V, whole_b, whole_e;
+
+  __device__ __forceinline__ Row(const Params& p, int row) {
+    x = p.x + (int64_t)row * p.xs * Vec<DT>::BYTES;
+    off = (int)(reinterpret_cast<uintptr_t>(x) & 15) / Vec<DT>::BYTES;
+    V = p.V;
+    base = reinterpret_cast<const u32x4*>(x - off * Vec<DT>::BYTES);
+    whole_b = off ? 1 : 0, whole_e = (off + V) / E;
+  }
+  __device__ __forceinline__ int index(int v, int i) const { return v * E - off + i; }  // of value i of vector v
+  // Index of the i-th value at the ends, or -1: i < E those before the whole vectors, i < 2 E those behind them.
+  __device__ __forceinline__ int end(int i) const {
+    const int before = off ? min(E - off, V) : 0, at = i < E ? i : max(whole_e * E - off, before) + i - E;
+    return i < E ? (i < before ? i : -1) : i < 2 * E && at < V ? at : -1;
+  }
+  // Vector v of all that hold one of the row's values; what is not in the row reads as -inf.
+  __device__ __forceinline__ int vectors() const { return (off + V + E - 1) / E; }
+  __device__ __forceinline__ u32x4 any(int v) const {
+    u32x4 y = u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+      const int at = index(v, i);
+      const unsigned low = DT == FA_DTYPE_F32 ? 0xff800000u : DT == FA_DTYPE_F16 ? 0xfc00u : 0xff80u;
+      unsigned u = low;
+      if (at >= 0 && at < V) u = DT == FA_DTYPE_F32 ? reinterpret_cast<const unsigned*>(x)[at] : reinterpret_cast<const unsigned short*>(x)[at];
+      if constexpr (DT == FA_DTYPE_F32) y[i] = u;
+      else y[i >> 1] |= u << (16 * (i & 1));
+    }
+    return y;
+  }
+};
+
+struct Shared {
+  Sums sums[W];
+  float maxima[W][64];
+  unsigned items, found, digit, above;
+  unsigned item[MOST];
+  uint64_t key[MOST];
+  unsigned count[256];
+  int flag;
+};
+
+// The workgroup's threads count their values' next eight bits, of those whose upper bits are `prefix`'s; four times, and the k-th
+// largest value is known. Returns it (ordered) and how many are above it.
+template <int DT>
+__device__ __forceinline__ unsigned kth_of_row(const Row<DT>& r, int k, Shared& sh, int& above) {
+  static_assert(64 * W == 256, "a thread a count");
+  unsigned prefix = 0;
+  above = 0;
+#pragma unroll 1
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    sh.count[threadIdx.x] = 0;
+    __syncthreads();
+    for (int v = threadIdx.x; v < r.vectors(); v += 64 * W) {
+      const u32x4 y = r.any(v);
+#pragma unroll
+      for (int i = 0; i < Vec<DT>::E; i++) {
+        const float x = value<DT>(y, i);
+        const unsigned u = ordered(x);
+        if (x > -INFINITY && (shift == 24 || u >> (shift + 8) == prefix >> (shift + 8))) atomicAdd(&sh.count[u >> shift & 255], 1u);
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int d = 255;
+      for (; d > 0 && above + (int)sh.count[d] < k; d--) above += sh.count[d];
+      sh.digit = d, sh.above = above;
+    }
+    __syncthreads();
+    prefix |= sh.digit << shift;
+    above = sh.above;
+  }
+  return prefix;
+}
+
+// The best `top` of a row, by the workgroup's threads. Maxima of the row's threads (thread t of split s has taken the whole vectors t + 256 i
+// of the split's): this one's `own`, or, where there are splits, a share of all of them. m, logs: as the log probabilities need them.
+// Loops stay loops: code that runs once costs its fetch.
+template <int DT>
+__device__ __forceinline__ void alternatives(const Params& p, const Row<DT>& r, int row, Shared& sh, float m, float logs, float own_max,
+                                             const f32x4* maxima) {
+  constexpr int E = Vec<DT>::E, T = 64 * W, QUADS = MAX_SPLITS / 4;
+  const int t = threadIdx.x, lane = t & 63, k = p.top, edge = r.end(t);
+  float high[QUADS], most = own_max;
+  if (p.S > 1) {
+    most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < QUADS; i++) {
+      high[i] = fmaxf(fmaxf(maxima[i][0], maxima[i][1]), fmaxf(maxima[i][2], maxima[i][3]));
+      most = fmaxf(most, high[i]);
+    }
+  }
+  sh.maxima[t >> 6][lane] = most;
+  if (t == 0) sh.items = sh.found = 0;
+  __syncthreads();
+  float g = sh.maxima[0][lane];
+#pragma unroll
+  for (int w = 1; w < W; w++) g = fmaxf(g, sh.maxima[w][lane]);
+  // the largest group's maximum that k of them reach
+  int reach = 0;
+#pragma unroll 4
+  for (int j = 0; j < 64; j++) reach += as_f32(__builtin_amdgcn_readlane(as_u32(g), j)) >= g;
+  const float bound = wave_max(reach >= k ? g : -INFINITY);
+  auto reaches = [&](float x) { return x >= bound && x > -INFINITY; };
+  // who has to look again: threads, or four neighbours of a split
+  auto look = [&](float x, int who) {
+    if (reaches(x)) {
+      const unsigned at = atomicAdd(&sh.items, 1u);
+      if (at < MOST) sh.item[at] = who;
+    }
+  };
+  const int side = p.S > 1 ? 4 : 1;
+  if (p.S == 1) {
+    look(own_max, t);
+  } else {
+#pragma unroll
+    for (int i = 0; i < QUADS; i++) look(high[i], (4 * i + (t >> 6)) * 64 + lane);
+  }
+  auto found = [&](float x, int index) {
+    if (reaches(x)) {
+      const unsigned at = atomicAdd(&sh.found, 1u);
+      if (at < MOST) sh.key[at] = (uint64_t)ordered(x) << 32 | ~(unsigned)index;
+    }
+  };
+  if (edge >= 0) found(value_at<DT>(r.x, edge), edge);
+  __syncthreads();
+  const int items = sh.items, nv = r.vectors(), each = side * ((p.per + T - 1) / T);  // vectors of an item, at most
+  unsigned floor = ordered(bound);
+  int n = MOST + 1, fill = 0;  // values found, and further ones that equal `floor`
+  if (items <= MOST) {
+#pragma unroll 1
+    for (unsigned e = t; e < (unsigned)(items * each); e += T) {
+      const unsigned i = e / (unsigned)each, rest = e - i * each, who = sh.item[i] * side, s = who / T;
+      const int v = max(s * p.per, (unsigned)r.whole_b) + who % T + rest % side + T * (rest / side);
+      if (v >= min((int)(s + 1) * p.per, r.whole_e)) continue;
+      const u32x4 y = r.base[v];
+#pragma unroll
+      for (int j = 0; j < E; j++) found(value<DT>(y, j), r.index(v, j));
+    }
+    __syncthreads();
+    n = sh.found;
+    if (n < k) floor = NOTHING, fill = k - n;  // all others are ruled out
+  }
+  if (n > MOST) {
+    int above;
+    floor = kth_of_row(r, k, sh, above);
+    fill = k - above, n = above;
+    if (t == 0) sh.found = 0;
+    __syncthreads();
+    for (int v = t; v < nv; v += T) {
+      const u32x4 y = r.any(v);
+#pragma unroll
+      for (int j = 0; j < E; j++) {
+        const float x = value<DT>(y, j);
+        if (x > -INFINITY && ordered(x) > floor) sh.key[atomicAdd(&sh.found, 1u)] = (uint64_t)ordered(x) << 32 | ~(unsigned)r.index(v, j);
+      }
+    }
+    __syncthreads();
+  }
+  int* const tokens = p.top_tokens + (size_t)row * k;
+  float* const logprobs = p.top_logprobs + (size_t)row * k;
+  for (int c = t; c < n; c += T) {
+    const uint64_t own = sh.key[c];
+    int before = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; j++) before += sh.key[j] > own;
+    if (before < k) {
+      tokens[before] = (int)~(unsigned)own;
+      logprobs[before] = (unordered((unsigned)(own >> 32)) - m) * p.scale - logs;
+    }
+  }
+  // those that equal `floor`, in the row's order; where there are not enough (NaN), token -1
+  if (fill == 0) return;
+  int have = 0;
+#pragma unroll 1
+  for (int v0 = 0; v0 < nv && have < fill; v0 += T) {
+    const int v = v0 + t;
+    unsigned hits = 0;
+    if (v < nv) {
+      const u32x4 y = r.any(v);
+#pragma unroll
+      for (int i = 0; i < E; i++) {
+        const float x = value<DT>(y, i);
+        const int at = r.index(v, i);
+        if (x == x && ordered(x) == floor && at >= 0 && at < p.V) hits |= 1u << i;
+      }
+    }
+    int before = have, all = 0;  // of lower lanes, of the wave
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+      const uint64_t b = __builtin_amdgcn_ballot_w64(hits >> i & 1);
+      before += __builtin_amdgcn_mbcnt_hi((unsigned)(b >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)b, 0));
+      all += __builtin_popcountll(b);
+    }
+    if (lane == 0) sh.count[t >> 6] = all;
+    __syncthreads();
+    for (int w = 0; w < W; w++) {
+      if (w < t >> 6) before += sh.count[w];
+      have += sh.count[w];
+    }
+    for (; hits; hits &= hits - 1, before++)
+      if (before < fill) {
+        tokens[n + before] = r.index(v, __builtin_ctz(hits));
+        logprobs[n + before] = (unordered(floor) - m) * p.scale - logs;
+      }
+    __syncthreads();
+  }
+  for (int i = n + have + t; i < k; i += T) tokens[i] = -1, logprobs[i] = -INFINITY - logs;
 }
 
 template <int DT, bool TOP>
 __global__ void __launch_bounds__(64 * W) logprobs_kernel(Params p) {
-  constexpr int E = Vec<DT>::E, U = Vec<DT>::U, BYTES = Vec<DT>::BYTES;
-  __shared__ Sums sums[W];
-  __shared__ float list_v[W][FA_TOKENS_MAX_TOP];
-  __shared__ int list_i[W][FA_TOKENS_MAX_TOP], flag;
+  constexpr int E = Vec<DT>::E, U = Vec<DT>::U, STEP = U * W * 64, QUADS = MAX_SPLITS / 4;
+  __shared__ Shared sh;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = blockIdx.x / p.S, split = blockIdx.x - row * p.S;
-  const unsigned char* x = p.x + (int64_t)row * p.xs * BYTES;
-  // vectors of 16 aligned bytes; the first may begin before the row and the last end behind it
-  const int off = (int)(reinterpret_cast<uintptr_t>(x) & 15) / BYTES;
-  const int nv = (int)(((int64_t)off + p.V + E - 1) / E);
-  const int vb = (int)((int64_t)nv * split / p.S), ve = (int)((int64_t)nv * (split + 1) / p.S);
-  const int whole_b = off ? 1 : 0, whole_e = (int)(((int64_t)off + p.V) / E);  // vectors that lie in the row
-  const u32x4* base = reinterpret_cast<const u32x4*>(x - off * BYTES);
+  const Row<DT> r(p, row);
+  const int vb = max(split * p.per, r.whole_b), ve = min((split + 1) * p.per, r.whole_e);
   const unsigned low = DT == FA_DTYPE_F32 ? 0xff800000u : DT == FA_DTYPE_F16 ? 0xfc00fc00u : 0xff80ff80u;  // -inf
 
-  Sums a{-INFINITY, 0.f, 0.f};
-  Best best;
-  if constexpr (TOP) best.clear(p.top);
-  bool fresh = true;
-  for (int v0 = vb; v0 < ve; v0 += U * W * 64) {
-    u32x4 raw[U];
-    if (v0 >= whole_b && v0 + U * W * 64 <= min(ve, whole_e)) {
+  u32x4 raw[U], next[U];
+  auto fetch = [&](int v0) {
+    const int v1 = v0 + threadIdx.x;
+    if (v0 + STEP <= ve) {
 #pragma unroll
-      for (int u = 0; u < U; u++) raw[u] = __builtin_nontemporal_load(base + v0 + (u * W + wave) * 64 + lane);
+      for (int u = 0; u < U; u++) next[u] = __builtin_nontemporal_load(r.base + v1 + u * W * 64);
     } else {
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        const int v = v0 + (u * W + wave) * 64 + lane;
-        raw[u] = u32x4{low, low, low, low};
-        if (v >= ve) continue;
-        if (v >= whole_b && v < whole_e) {
-          raw[u] = __builtin_nontemporal_load(base + v);
-        } else {
-#pragma unroll
-          for (int i = 0; i < E; i++) {
-            const int64_t at = (int64_t)v * E - off + i;
-            if (at < 0 || at >= p.V) continue;
-            if constexpr (DT == FA_DTYPE_F32) {
-              raw[u][i] = reinterpret_cast<const unsigned*>(x)[at];
-            } else {
-              const unsigned w = reinterpret_cast<const unsigned short*>(x)[at];
-              raw[u][i >> 1] = i & 1 ? (raw[u][i >> 1] & 0xffffu) | w << 16 : (raw[u][i >> 1] & 0xffff0000u) | w;
-            }
-          }
-        }
+        next[u] = u32x4{low, low, low, low};
+        if (v1 + u * W * 64 < ve) next[u] = __builtin_nontemporal_load(r.base + v1 + u * W * 64);
       }
     }
+  };
+  Sums a{-INFINITY, 0.f, 0.f};
+  if (split == 0 && r.end(threadIdx.x) >= 0) {
+    const float x = value_at<DT>(r.x, r.end(threadIdx.x));
+    a = Sums{x == x ? x : -INFINITY, x > -INFINITY ? 1.f : x == x ? 0.f : x, 0.f};
+    if (x == INFINITY) a.s = NAN;
+  }
+  if (vb < ve) fetch(vb);
+  float own = -INFINITY;  // the maximum of this thread's whole vectors
+  for (int v0 = vb; v0 < ve; v0 += STEP) {
+#pragma unroll
+    for (int u = 0; u < U; u++) raw[u] = next[u];
+    if (v0 + STEP < ve) fetch(v0 + STEP);
     float most = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
       for (int i = 0; i < E; i++) most = fmaxf(most, value<DT>(raw[u], i));
+    own = fmaxf(own, most);
     const float m = fmaxf(a.m, most), ms = m == -INFINITY ? 0.f : m;
     const float down = fmaxf((a.m - ms) * p.c, LEAST), w = exp2_w(down);
     a.t = w * (a.t + down * a.s);
@@ -188,87 +358,51 @@ __global__ void __launch_bounds__(64 * W) logprobs_kernel(Params p) {
         a.s += e;
         a.t += fmaxf(d, LEAST) * e;
       }
-    if constexpr (TOP) {
-      float bound = best.last_v;
-      if (fresh) bound = kth_bound(most, p.top);
-      fresh = false;
-      if (__builtin_amdgcn_ballot_w64(most >= bound)) {
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-          for (int i = 0; i < E; i++) {
-            const int64_t at = ((int64_t)v0 + (u * W + wave) * 64 + lane) * E - off + i;
-            const float y = value<DT>(raw[u], i);
-            best.offer(y, (int)at, y >= bound && at >= 0 && at < p.V && v0 + (u * W + wave) * 64 + lane < ve);
-          }
-      }
-    }
   }
   a = sum_lanes(a, p.c);
-  if (lane == 0) sums[wave] = a;
-  if constexpr (TOP) {
-    if (lane < p.top) list_v[wave][lane] = best.v, list_i[wave][lane] = best.i;
-  }
+  if (lane == 0) sh.sums[wave] = a;
   __syncthreads();
-  if (wave == 0) {
-    a = sum_lanes(lane < W ? sums[lane] : Sums{-INFINITY, 0.f, 0.f}, p.c);
-    if constexpr (TOP) {
-      constexpr int PER = 64 / FA_TOKENS_MAX_TOP;  // lists side by side
-#pragma unroll
-      for (int w0 = 1; w0 < W; w0 += PER) {  // the other waves'
-        const int w = w0 + lane / FA_TOKENS_MAX_TOP, j = lane % FA_TOKENS_MAX_TOP;
-        best.offer(list_v[min(w, W - 1)][j], list_i[min(w, W - 1)][j], w < W && j < p.top);
-      }
-    }
-  }
+  a = sum_lanes(lane < W ? sh.sums[lane] : Sums{-INFINITY, 0.f, 0.f}, p.c);
+  f32x4 maxima[TOP ? QUADS : 1];  // the threads' of all splits: quad i of this thread is of split 4 i + wave, threads 4 lane ..
   if (p.S > 1) {
-    const int one = part_floats(TOP ? p.top : 0);
+    constexpr int one = part_floats(TOP);
     const rsrc_t parts = make_rsrc(p.part + (size_t)row * p.S * one, (uint32_t)(p.S * one * 4));
-    if (wave == 0) {
-      if (lane == 0)
-        stb128<kCpSc1>(parts, split * one * 4, u32x4{as_u32(a.m), as_u32(a.s), as_u32(a.t), 0});
-      if constexpr (TOP)
-        if (lane < p.top) stb64<kCpSc1>(parts, (split * one + 4 + 2 * lane) * 4, u32x2{as_u32(best.v), (unsigned)best.i});
-    }
-    if (!arrived_last(p.arrived + (size_t)row * p.S, p.nonce, split, p.S, &flag)) return;
-    if (wave == 0) {
-      const u32x4 s = lane < p.S ? ldb128<kCpSc1>(parts, lane * one * 4) : u32x4{as_u32(-INFINITY), 0, 0, 0};
-      a = sum_lanes(Sums{as_f32(s[0]), as_f32(s[1]), as_f32(s[2])}, p.c);
-      if constexpr (TOP) {
-        best.clear(p.top);
-        for (int j = 0; j < p.top; j++) {  // the lists are sorted: once no split's j-th passes, none does
-          const u32x2 e = lane < p.S ? ldb64<kCpSc1>(parts, (lane * one + 4 + 2 * j) * 4) : u32x2{as_u32(-INFINITY), (unsigned)NONE};
-          if (!best.offer(as_f32(e[0]), (int)e[1], lane < p.S)) break;
-        }
+    if (threadIdx.x == 0) stb128<kCpSc1>(parts, split * one * 4, u32x4{as_u32(a.m), as_u32(a.s), as_u32(a.t), 0});
+    if constexpr (TOP) __builtin_amdgcn_raw_buffer_store_b32(as_u32(own), parts, (split * one + 4 + threadIdx.x) * 4, 0, kCpSc1);
+    if (!arrived_last(p.arrived + (size_t)row * p.S, p.nonce, split, p.S, &sh.flag)) return;
+    const u32x4 x = ldb128<kCpSc1>(parts, lane < p.S ? lane * one * 4 : 0);
+    if constexpr (TOP) {
+#pragma unroll
+      for (int i = 0; i < QUADS; i++) {
+        maxima[i] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (4 * i + wave < p.S) maxima[i] = as_f32x4(ldb128<kCpSc1>(parts, ((4 * i + wave) * one + 4 + 4 * lane) * 4));
       }
     }
+    a = sum_lanes(lane < p.S ? Sums{as_f32(x[0]), as_f32(x[1]), as_f32(x[2])} : Sums{-INFINITY, 0.f, 0.f}, p.c);
   }
-  if (wave != 0) return;
   const bool nothing = a.m == -INFINITY && a.s == 0.f;
   const float logs = nothing ? 0.f : logf(a.s), m = nothing ? 0.f : a.m;
-  if (lane == 0) {
+  if (threadIdx.x == 0) {
     const int64_t token = p.wide ? static_cast<const int64_t*>(p.tokens)[row] : static_cast<const int*>(p.tokens)[row];
     float z = -INFINITY;
-    if (token >= 0 && token < p.V) z = value_at<DT>(x, (int)token);
+    if (token >= 0 && token < p.V) z = value_at<DT>(r.x, (int)token);
     p.logprob[row] = (z - m) * p.scale - logs;
     p.entropy[row] = nothing ? 0.f : logs - a.t / a.s * LN2;
   }
-  if constexpr (TOP) {
-    if (lane < p.top) {
-      p.top_tokens[(size_t)row * p.top + lane] = best.i == NONE ? -1 : best.i;
-      p.top_logprobs[(size_t)row * p.top + lane] = (best.v - m) * p.scale - logs;
-    }
-  }
+  if constexpr (TOP) alternatives<DT>(p, r, row, sh, m, logs, own, maxima);
 }
 
-// Workgroups of a row: the chip full, each with a batch of every thread or more.
-int splits_for(int rows, int V, int dtype) {
-  const int batches = (int)(((int64_t)V + 64 * W * 16 - 1) / (64 * W * 16));
-  return std::max(1, std::min({MAX_SPLITS, batches, 1024 / std::min(rows, 1024)}));
+// Workgroups of a row: the chip full, each with a batch of every thread or more. `per`: vectors of each.
+int splits_for(int rows, int V, int dtype, int* per = nullptr) {
+  const int e = dtype == FA_DTYPE_F32 ? 4 : 8, nv = V / e + 2, batch = 64 * W * 16 / e;
+  const int most = std::max(1, std::min({MAX_SPLITS, (nv + batch - 1) / batch, 1024 / std::min(rows, 1024)}));
+  const int each = (nv + most - 1) / most;
+  if (per) *per = each;
+  return (nv + each - 1) / each;
 }
 size_t arrived_bytes(int rows, int S) { return ((size_t)rows * S * sizeof(uint64_t) + 255) / 256 * 256; }
 size_t workspace(int rows, int S, int top) {
-  return S == 1 ? 0 : arrived_bytes(rows, S) + (size_t)rows * S * part_floats(top) * sizeof(float);
+  return S == 1 ? 0 : arrived_bytes(rows, S) + (size_t)rows * S * part_floats(top > 0) * sizeof(float);
 }
 
 template <int DT>
@@ -313,7 +447,8 @@ extern "C" int fa_token_logprobs(const fa_token_logprobs_args* a, fa_stream_t st
     if (t.need && !t.p) return host::fail(FA_ERR_INVALID_ARG, "%s: %s is NULL", who, t.name);
     if (reinterpret_cast<uintptr_t>(t.p) % t.align) return host::fail(FA_ERR_INVALID_ARG, "%s: %s is not %u-byte aligned", who, t.name, t.align);
   }
-  const int S = tokens::splits_for(a->rows, a->vocabulary, a->dtype);
+  int per = 0;
+  const int S = tokens::splits_for(a->rows, a->vocabulary, a->dtype, &per);
   const size_t need = tokens::workspace(a->rows, S, a->top);
   if (need && (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16))
     return host::fail(FA_ERR_INVALID_ARG, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, need,
@@ -322,7 +457,7 @@ extern "C" int fa_token_logprobs(const fa_token_logprobs_args* a, fa_stream_t st
   if (rc != FA_OK) return rc;
   tokens::Params p{};
   p.x = static_cast<const unsigned char*>(a->logits), p.xs = a->stride, p.tokens = a->tokens, p.wide = a->wide_tokens;
-  p.scale = a->scale, p.c = a->scale * tokens::LOG2E, p.rows = a->rows, p.V = a->vocabulary, p.top = a->top, p.S = S;
+  p.scale = a->scale, p.c = a->scale * tokens::LOG2E, p.rows = a->rows, p.V = a->vocabulary, p.top = a->top, p.S = S, p.per = per;
   p.logprob = a->logprob, p.entropy = a->entropy, p.top_tokens = a->top_tokens, p.top_logprobs = a->top_logprobs;
   if (S > 1) {
     p.arrived = static_cast<uint64_t*>(a->workspace), p.nonce = host::launch_nonce();
