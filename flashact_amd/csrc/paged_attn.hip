@@ -7,11 +7,16 @@
 // MFMAs. A wave takes pages on its own with a running maximum and sum: S^T = K Q^T (16x16x32, two tiles of 16 keys), softmax
 // down the columns, O^T += V^T P^T; row m of key tile t is key 8 (m / 4) + 4 t + m % 4, so lane quarter q ends with keys
 // 8 q .. 8 q + 7, the next product's operand. Each wave copies its pages to LDS on its own (no registers, no barrier): the next
-// page's keys are asked for as soon as this one's are in registers, the values' likewise, and the page after it is looked up in
-// the table by a scalar load meanwhile. How pages are dealt to waves and workgroups, and how their sums meet: newest.h.
+// page's keys are asked for as soon as this one's are in registers, the values' likewise. How pages are dealt to waves and
+// workgroups, and how their sums meet: newest.h.
+//
+// With many rows (a piece of a prompt) each workgroup of 16 takes its pages from the L2 again, at what a CU copies from there (110 GB/s),
+// and the chain of a page's step is about 1500 cycles a wave. Workgroups of 64 rows, whose waves walk together over pages that are copied once,
+// were no better: 293 tokens x 8 heads over up to 4011 keys 38 us so, 52 with four splits and 117 unsplit the other way; 1024
+// tokens of 32 heads over 8192 keys 328 and 306 us; 4 x 256 of 8 heads of 256 dims over 4096 keys 143 and 183.
 //
 // Rounding: scores are exact products summed in fp32, softmax and sums are fp32. bf16: the weights go into the second
-// product as two bf16 (2^-17 of each is lost; its MFMAs are not the bound), and are taken against a reference 2^17 above
+// product as two bf16 (2^-16 of each is lost; its MFMAs are not the bound), and are taken against a reference 2^17 above
 // the maximum, so that 131072 keys cannot leave the fp32 range whatever the values. fp16: the weights are rounded once (2^-12), against a
 // reference 2^15 below the maximum: those above 2^-29 of the largest keep all their bits.
 #include <hip/hip_runtime.h>
@@ -56,94 +61,97 @@ __device__ __forceinline__ u32x4 halves_below(int n) {
   return x;
 }
 
-template <int HD>
-using Lds = newest::Lds<HD, 2 * BT * HD * 2>;  // of a wave: a page of keys and one of values
+// A page of keys lies in LDS with its tokens in the order in which the two MFMAs' rows take them (16 lanes read 256 bytes in one run;
+// in the page's own order they met in half of the banks): slot 16 x + m holds token 8 (m / 4) + 4 x + m % 4. A copy's lane i
+// fetches what belongs into slot i of its 1 KB, four neighbours 64 bytes in one run.
+__device__ __forceinline__ unsigned key_offset(int lane) {
+  return (lane >> 5) * 512 + (8 * ((lane & 15) >> 2) + 4 * ((lane >> 4) & 1) + (lane & 3)) * 16;
+}
 
+// What a wave keeps of its tile of 16 rows: row r is column r of the MFMAs, lane r + 16 q.
 template <bool F16, int HD, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : HD == 128 ? 2 : HD == 96 ? 3 : 4) attn_kernel(AttnArgs a) {
-  constexpr int KS = HD / 32, NT = HD / 16, PAGE = BT * HD * 2, NC = PAGE / 1024;  // NC: copies of a page
-  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-  const Place here = newest::place_of(a);
-  if (!here.there) return;
-  const int b = here.b, h = here.h, rt = here.rt, split = here.split;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r = lane & 15, q = lane >> 4;
-  const Span sp = newest::span_of(a, b);
-
-  const int rr = rt * 16 + r, t = rr / a.G, head = h * a.G + rr % a.G, pos = sp.len - sp.n + t;
-  const bool valid = rr < a.T * a.G && t < sp.n && pos >= 0;
-  int limit = valid ? (a.causal ? pos + 1 : sp.len) : 0;
-  int hi = limit, lo = valid ? limit : 0x7fffffff;
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) {
-    hi = max(hi, __shfl_xor(hi, o));
-    lo = min(lo, __shfl_xor(lo, o));
-  }
-  hi = __builtin_amdgcn_readfirstlane(hi);  // keys that any row sees
-  lo = __builtin_amdgcn_readfirstlane(lo);  // keys that every row sees (rows that are not there do not count)
-  if (!valid) limit = hi;
-  const int nb = (hi + BT - 1) / BT;
-  const int used = newest::splits_used(a, nb);
-  if (split >= used) return;
-  const int at = split * W + wave, all = used * W;
-
-  u32x4 qf[KS];
-#pragma unroll
-  for (int i = 0; i < KS; i++) {
-    qf[i] = u32x4{0, 0, 0, 0};
-    if (valid) qf[i] = *reinterpret_cast<const u32x4*>(a.q + (b * a.qb + t * a.qt + head * a.qh + 32 * i + 8 * q) * 2);
-  }
-  const float slope = BIAS && valid ? a.slopes[head] * newest::LOG2E : 0.f;
-
-  // The table is constant while the kernel runs: scalar loads.
-  typedef const __attribute__((address_space(4))) int* Table;
-  const Table table = (Table)(uintptr_t)(a.table + b * a.ts);
-  auto page = [&](int blk) { return blk < nb ? table[blk] : 0; };
-  auto there = [&](int pg) { return (unsigned)pg < (unsigned)a.pages; };
-  unsigned char* kl = lds + wave * Lds<HD>::WAVE;
-  unsigned char* vl = kl + PAGE;
-  const unsigned at_k = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)kl), at_v = at_k + PAGE;
-  auto copy = [&](const unsigned char* from, int pg, unsigned to) {  // of a page that is not there, the first one
-    const unsigned char* p = from + ((size_t)(there(pg) ? pg : 0) * a.H + h) * PAGE;
-#pragma unroll
-    for (int i = 0; i < NC; i++) copy_to_lds(p + i * 1024, lane * 16, to + i * 1024);
-  };
-
+struct Tile {
+  static constexpr int KS = HD / 32, NT = HD / 16;
+  int pos, limit, lo, hi;  // keys that the row sees, that every row does (those that are not there do not count), that any does
+  float slope, m, l;       // m: the weights' reference; l: their sum over this lane's keys
+  u32x4 q[KS];
   f32x4 O[NT];
+
+  __device__ __forceinline__ void begin(const AttnArgs& a, const Place& at, const Span& sp) {
+    const int lane = threadIdx.x & 63, row = at.rt * 16 + (lane & 15), t = row / a.G, head = at.h * a.G + row % a.G;
+    pos = sp.len - sp.n + t;
+    const bool valid = row < a.T * a.G && t < sp.n && pos >= 0;
+    limit = valid ? (a.causal ? pos + 1 : sp.len) : 0;
+    hi = limit, lo = valid ? limit : 0x7fffffff;
 #pragma unroll
-  for (int j = 0; j < NT; j++) O[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;  // l: this lane's keys only
-  int pg = page(at), next = page(at + all);
-  if (at < nb) {
-    copy(a.k, pg, at_k);
-    copy(a.v, pg, at_v);
+    for (int o = 1; o < 16; o <<= 1) {
+      hi = max(hi, __shfl_xor(hi, o));
+      lo = min(lo, __shfl_xor(lo, o));
+    }
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    if (!valid) limit = hi;
+#pragma unroll
+    for (int i = 0; i < KS; i++) {
+      q[i] = u32x4{0, 0, 0, 0};
+      if (valid)
+        q[i] = *reinterpret_cast<const u32x4*>(a.q + (at.b * a.qb + t * a.qt + head * a.qh + 32 * i + 8 * (lane >> 4)) * 2);
+    }
+    slope = BIAS && valid ? a.slopes[head] * newest::LOG2E : 0.f;
+    m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int j = 0; j < NT; j++) O[j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  // The queries are waited for here: left to the compiler, that wait (for everything under way) stands in the loop.
+  // Waits for the queries: left to the compiler, that wait (for everything under way) stands in the loop.
+  __device__ __forceinline__ void arrive() {
 #pragma unroll
-  for (int i = 0; i < KS; i++) asm volatile("" : "+v"(qf[i]));
-  for (int blk = at; blk < nb; blk += all) {
-    const bool more = blk + all < nb;
-    const int later = page(blk + 2 * all);
-    vm_wait<NC>();  // the keys; the values are still on their way
+    for (int i = 0; i < KS; i++) asm volatile("" : "+v"(q[i]));
+    asm volatile("" : "+v"(slope));
+  }
+
+  // Page `blk` of the sample, its keys and values at kl and vl in LDS; gone: it is no page, and nobody sees its keys. keys_read and
+  // values_read run once the one and the other are in registers, values_there before these are read.
+  template <class A, class B, class C>
+  __device__ __forceinline__ void step(const AttnArgs& a, const unsigned char* kl, const unsigned char* vl, int blk, bool gone,
+                                       A&& keys_read, B&& values_there, C&& values_read) {
+    const int lane = threadIdx.x & 63, r = lane & 15, qq = lane >> 4;
     u32x4 kc[2][KS];
 #pragma unroll
     for (int i = 0; i < KS; i++)
 #pragma unroll
-      for (int x = 0; x < 2; x++)
-        kc[x][i] = *reinterpret_cast<const u32x4*>(kl + ((4 * i + q) * BT + 8 * (r >> 2) + 4 * x + (r & 3)) * 16);
-    lds_wait();
-    if (more) copy(a.k, next, at_k);
+      for (int x = 0; x < 2; x++) kc[x][i] = *reinterpret_cast<const u32x4*>(kl + ((4 * i + qq) * BT + 16 * x + r) * 16);
+    keys_read();
     f32x4 s[2];
 #pragma unroll
     for (int x = 0; x < 2; x++) {
       s[x] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < KS; i++) s[x] = mma<F16>(kc[x][i], qf[i], s[x]);
+      for (int i = 0; i < KS; i++) s[x] = mma<F16>(kc[x][i], q[i], s[x]);
     }
-    const bool gone = !there(pg);  // nobody sees a key of no page
-    const int key0 = blk * BT + 8 * q, lo_b = gone ? 0 : lo, hi_b = gone ? 0 : hi, own = gone ? 0 : limit;
-    const bool mixed = blk * BT + BT > lo_b;
-    const float mx = newest::scores<CAP, BIAS>(a, s, 1.f, key0, mixed, own, slope, pos);
+    const int key0 = blk * BT + 8 * qq, low = gone ? 0 : lo, high = gone ? 0 : hi;
+    const bool mixed = blk * BT + BT > low;
+    u32x4 P, R;  // R: what P left off, bf16 only
+    const int own = gone ? 0 : limit;
+    float mx, f = 1.f;  // scores are s f
+    if (!CAP && !BIAS && a.scale > 0.f) {
+      f = a.scale;  // goes into the exponent's one instruction
+      if (mixed) {
+        asm volatile("");  // a branch: as selects the masks cost every block
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (key0 + 4 * x + i >= own) s[x][i] = -INFINITY;
+      }
+      mx = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[x][i]);
+      mx *= f;
+    } else {
+      mx = newest::scores<CAP, BIAS>(a, s, 1.f, key0, mixed, own, slope, pos);
+    }
     const float mn = fmaxf(m, reference<F16>(cols_max(mx)));
     const float ms = mn == -INFINITY ? 0.f : mn;
     if (__builtin_amdgcn_ballot_w64(mn != m)) {
@@ -153,37 +161,34 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : HD == 128 ? 2 : HD == 
       for (int j = 0; j < NT; j++) O[j] *= al;
       m = mn;
     }
-    u32x4 P, R;  // R: what P's rounding left, bf16 only
 #pragma unroll
     for (int x = 0; x < 2; x++) {
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        s[x][i] = exp2_w(s[x][i] - ms);
+        s[x][i] = exp2_w(!CAP && !BIAS ? fmaf(s[x][i], f, -ms) : s[x][i] - ms);
         l += s[x][i];
       }
 #pragma unroll
       for (int i = 0; i < 2; i++) {
+        const float p0 = s[x][2 * i], p1 = s[x][2 * i + 1];
         if constexpr (F16) {
-          P[2 * x + i] = pack_f16x2(s[x][2 * i], s[x][2 * i + 1]);
-        } else {
-          const unsigned p = pack_bf16x2(s[x][2 * i], s[x][2 * i + 1]);
-          P[2 * x + i] = p;
-          R[2 * x + i] = pack_bf16x2(s[x][2 * i] - bf_lo(p), s[x][2 * i + 1] - bf_hi(p));
+          P[2 * x + i] = pack_f16x2(p0, p1);
+        } else {  // the upper halves as they are, and the rest
+          P[2 * x + i] = __builtin_amdgcn_perm(as_u32(p1), as_u32(p0), 0x07060302u);
+          R[2 * x + i] = pack_bf16x2(p0 - as_f32(as_u32(p0) & 0xffff0000u), p1 - as_f32(as_u32(p1) & 0xffff0000u));
         }
       }
     }
-    if (more) vm_wait<NC>();
-    else vm_wait<0>();
+    values_there();
     u32x4 vc[NT];  // keys key0 .. key0 + 7 of dim 16 j + r
 #pragma unroll
-    for (int j = 0; j < NT; j++) vc[j] = *reinterpret_cast<const u32x4*>(vl + (q * HD + 16 * j + r) * 16);
-    lds_wait();
-    if (more) copy(a.v, next, at_v);
+    for (int j = 0; j < NT; j++) vc[j] = *reinterpret_cast<const u32x4*>(vl + (qq * HD + 16 * j + r) * 16);
+    values_read();
     // Values of keys that a row does not see must not reach it: its P is 0 there, but 0 x NaN is NaN. Those behind the
-    // last key that any row sees are cleared; where one between lo and hi is not finite, each column has its own product.
+    // last key that any row sees are cleared; where one between low and high is not finite, each column has its own product.
     bool apart = false;
     if (mixed) {
-      const u32x4 some = halves_below(hi_b - key0), each = halves_below(lo_b - key0);
+      const u32x4 some = halves_below(high - key0), each = halves_below(low - key0);
       unsigned bad = 0;
 #pragma unroll
       for (int j = 0; j < NT; j++) {
@@ -212,9 +217,85 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : HD == 128 ? 2 : HD == 
         }
       }
     }
-    pg = next, next = later;
   }
-  newest::meet<F16, HD, Lds<HD>>(a, here, sp, used, lds, O, m, cols_sum(l));
+};
+
+// The pages of a sample that a wave goes over, blk, blk + step, .., one after the other: 64 are held in the lanes (looked up one by one, by
+// scalar loads, each step waited for the one of the step after it: LDS reads and scalar loads share a counter).
+struct Pages {
+  const int* table;
+  int pages, nb, blk, step, left, held;
+  __device__ __forceinline__ Pages(const AttnArgs& a, int b, int nb, int first, int step)
+      : table(a.table + b * a.ts), pages(a.pages), nb(nb), blk(first), step(step), left(0), held(0) {}
+  // The next one's number, 0 behind the last; where there are no more in the lanes, all copies under way are waited for.
+  __device__ __forceinline__ int next() {
+    if (left == 0) {
+      const int64_t mine = blk + (int64_t)step * (threadIdx.x & 63);
+      held = mine < nb ? table[mine] : 0;
+      asm volatile("" : "+v"(held));
+      left = 64;
+    }
+    blk += step;
+    return __builtin_amdgcn_readlane(held, 64 - left--);
+  }
+  __device__ __forceinline__ bool there(int pg) const { return (unsigned)pg < (unsigned)pages; }
+  __device__ __forceinline__ size_t read(int pg) const { return there(pg) ? pg : 0; }  // the first one, where there is none
+};
+
+template <int HD>
+using Lds = newest::Lds<HD, 2 * BT * HD * 2>;  // of a wave: a page of keys and one of values
+
+template <bool F16, int HD, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : HD == 128 ? 2 : HD == 96 ? 3 : 4) attn_kernel(AttnArgs a) {
+  constexpr int PAGE = BT * HD * 2, NC = PAGE / 1024;  // NC: copies of a page
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  const Place here = newest::place_of(a);
+  if (!here.there) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Span sp = newest::span_of(a, here.b);
+  Tile<F16, HD, CAP, BIAS> tile;
+  tile.begin(a, here, sp);
+  const int nb = (tile.hi + BT - 1) / BT;
+  const int used = newest::splits_used(a, nb);
+  if (here.split >= used) return;
+  const int at = here.split * W + wave, all = used * W;
+  Pages pages(a, here.b, nb, at, all);
+  unsigned char* kl = lds + wave * Lds<HD>::WAVE;
+  unsigned char* vl = kl + PAGE;
+  const unsigned at_k = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)kl), at_v = at_k + PAGE;
+  const unsigned keys_at = key_offset(lane), values_at = lane * 16;
+  auto copy = [&](const unsigned char* from, int pg, unsigned to, unsigned off) {
+    const unsigned char* p = from + (pages.read(pg) * a.H + here.h) * PAGE;
+#pragma unroll
+    for (int i = 0; i < NC; i++) copy_to_lds(p + i * 1024, off, to + i * 1024);
+  };
+  int pg = pages.next();
+  if (at < nb) {
+    copy(a.k, pg, at_k, keys_at);
+    copy(a.v, pg, at_v, values_at);
+  }
+  tile.arrive();
+  for (int blk = at; blk < nb; blk += all) {
+    const bool more = blk + all < nb;
+    const int next = more ? pages.next() : 0;
+    vm_wait<NC>();  // the keys; the values are still on their way
+    tile.step(
+        a, kl, vl, blk, !pages.there(pg),
+        [&] {
+          lds_wait();
+          if (more) copy(a.k, next, at_k, keys_at);
+        },
+        [&] {
+          if (more) vm_wait<NC>();
+          else vm_wait<0>();
+        },
+        [&] {
+          lds_wait();
+          if (more) copy(a.v, next, at_v, values_at);
+        });
+    pg = next;
+  }
+  newest::meet<F16, HD, Lds<HD>>(a, here, sp, used, lds, tile.O, tile.m, cols_sum(tile.l));
 }
 
 template <bool F16, int HD>
@@ -222,9 +303,15 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a) {
   newest::join<F16, HD>(a);
 }
 
-// Estimates of a wave's time for a page, and of the workgroups whose waves do not share bandwidth.
+// A wave takes about 2.3 us for a page of 256 dims (1.2 of 128 and less); more than one workgroup a CU (two) share its bandwidth. That
+// is for samples that fill their tables. Where one tile of rows is all there is (single tokens), samples are of any age, and a
+// full one that takes few splits is waited for: up to 8 splits of 4 pages a wave or more. (48 samples of 1 to 8192 tokens, 4 K/V
+// heads of 128 dims, 3 splits by the estimate: 43 us, 8: 33, 16: 32.5; 48 of 4096 each 75, 78 and 79; of 983 24 all three.)
 int splits_for(int batch, int tokens, int heads, int kv_heads, int hd, int pages) {
-  return newest::splits_for(batch, tokens, heads, kv_heads, pages, hd == 256 ? 2.3 : 1.2, hd == 256 ? 1.0 : 2.0);
+  const int s = newest::splits_for(batch, tokens, heads, kv_heads, pages, hd == 256 ? 2.3 : 1.2, hd == 256 ? 1.0 : 2.0);
+  const int64_t units = (int64_t)batch * kv_heads;
+  if ((int64_t)tokens * (heads / kv_heads) > 16 || units < 64) return s;
+  return (int)std::max<int64_t>(s, std::min<int64_t>({8, (pages + 4 * W - 1) / (4 * W), newest::MAX_PARTS / units}));
 }
 
 template <bool F16, int HD>
