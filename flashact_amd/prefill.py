@@ -9,8 +9,9 @@ straight to ``pi05.launch`` with no copy in between.
 
 ``prefill_packed`` and ``extend`` run the same backbone where that launch does not reach: prompts of different lengths packed
 one behind the other, with tokens that are causal behind a prefix that all see, and further tokens one by one (or a few)
-behind what is cached. They keep keys and values in 8 bits (``kv8``), from where ``kv8.load`` fills the denoise loop's caches;
-``extend`` reads the weights in 4 bits (``w4``).
+behind what is cached. They keep keys and values in 8 bits (``kv8``), from where ``kv8.load`` fills the denoise loop's caches,
+or, given a table, in pages that many requests share (``paged``); ``extend`` reads the weights in 4 bits (``w4``). Each prompt or
+sample may have low-rank adapters of its own (``lora``), and ``answer`` turns hidden states into log probabilities (``tokens``).
 
 Backbone shape: D = 2048, 8 query heads / 1 K/V head of 256, F = 16384 (GeLU-tanh gate), RMSNorm
 eps 1e-6 scaled by (1 + w), RoPE base 10000 at positions 0..Lp-1, no mask inside the prefix.
@@ -21,7 +22,8 @@ import ctypes
 
 import torch
 
-from . import _lib, attention, kv8, pi05, w4
+from . import _lib, attention, kv8, lora, paged, pi05, w4
+from . import tokens as _tokens
 
 D, F, HD, H = 2048, 16384, 256, 8
 
@@ -160,85 +162,176 @@ def _qkv(y, rope):
     return qk[..., :H, :], qk[..., H:, :], y[..., 9 * HD:].unflatten(-1, (1, HD))
 
 
-def _check_backbone(ln_in, ln_post, layers, x, caches):
+def _check_backbone(ln_in, ln_post, layers, x, caches, table=None):
     if x.dtype is not torch.float32 or ln_in.dtype is not torch.float32 or ln_post.dtype is not torch.float32:
         raise TypeError("x, ln_in and ln_post must be float32")
     if x.shape[-1] != D or ln_in.shape != (layers, D) or ln_post.shape != (layers, D):
         raise ValueError(f"shapes: x {tuple(x.shape)}, ln_in {tuple(ln_in.shape)}, ln_post {tuple(ln_post.shape)}: need "
                          f"[..][{D}] and [{layers}][{D}]")
     if len(caches) != layers or any(c["v"].shape != caches[0]["v"].shape or c["v"].shape[1] != 1 or c["v"].shape[3] != HD for c in caches):
-        raise ValueError(f"caches must be {layers} equal layers of kv8.make_caches with one K/V head of {HD}")
+        raise ValueError(f"caches must be {layers} equal layers of {'kv8.make_caches' if table is None else 'paged.make_pools'} with one "
+                         f"K/V head of {HD}")
+    if (caches[0]["v"].dtype is not torch.uint8) != (table is not None):
+        raise ValueError("a table belongs to paged.make_pools caches, and kv8.make_caches ones have none")
+    if table is not None and (caches[0]["v"].dtype is not torch.bfloat16 or table.dim() != 2):
+        raise ValueError(f"the pools must be bfloat16 and the table [samples][pages of one], got {caches[0]['v'].dtype} and {tuple(table.shape)}")
 
 
-def prefill_packed(packed: dict, ln_in, ln_post, x, lengths, caches: list, prefix=None) -> torch.Tensor:
-    """Runs the backbone over prompts of different lengths, packed one behind the other, into empty 8-bit caches.
+def _room(caches, table):
+    """Samples, and tokens that each may have."""
+    if table is not None:
+        return int(table.shape[0]), int(table.shape[1]) * paged.PAGE
+    return int(caches[0]["v"].shape[0]), int(caches[0]["v"].shape[2]) * kv8.BLOCK
+
+
+def _check_adapters(adapters, layers, samples):
+    if adapters is None:
+        return [{}] * layers, None
+    banks, index = adapters
+    if len(banks) != layers or any(n not in ("wqkv", "wo", "wgu", "wdn") for bank in banks for n in bank):
+        raise ValueError(f"adapters must be ({layers} dicts of banks for wqkv, wo, wgu or wdn, an index)")
+    if index.dtype is not torch.int32 or index.shape != (samples,):
+        raise ValueError(f"the adapters' index must be int32 [{samples}], got {index.dtype} {tuple(index.shape)}")
+    return banks, index
+
+
+def prefill_packed(packed: dict, ln_in, ln_post, x, lengths, caches: list, prefix=None, *, table=None, adapters=None) -> torch.Tensor:
+    """Runs the backbone over prompts of different lengths, packed one behind the other, into empty 8-bit caches (or pages).
 
     packed: ``pack_backbone`` output. x [T][2048] fp32: the hidden states entering layer 0 of prompt 0, then of prompt 1, and
     so on; lengths: their tokens (whole numbers, on the host; their sum is at most T, rows behind it are padding). prefix:
     how many of its first tokens all of a prompt sees, the others being causal (None: all, no mask in a prompt). caches:
-    ``kv8.make_caches(layers, len(lengths), ...)``, filled from token 0 on. Returns the hidden states leaving the last
-    layer [T][2048] fp32 (undefined in padding). The matrix products are the library's; the attention and the cache are
-    ``attention.attend`` and ``kv8.store``.
+    ``kv8.make_caches(layers, len(lengths), ...)``, filled from token 0 on; with a table (int32 [len(lengths)][n] on the GPU)
+    ``paged.make_pools(layers, ...)``, of which it names each prompt's pages. adapters: (for each layer a dict of ``lora.pack`` banks
+    for any of "wqkv", "wo", "wgu", "wdn", int32 [len(lengths)] on the GPU: each prompt's adapter, -1 for none). Returns the hidden
+    states leaving the last layer [T][2048] fp32 (undefined in padding). The matrix products are the library's; the attention and the
+    cache are ``attention.attend`` and ``kv8.store`` (``paged.append``).
     """
     layers = int(packed["wqkv"].shape[0])
-    _check_backbone(ln_in, ln_post, layers, x, caches)
+    _check_backbone(ln_in, ln_post, layers, x, caches, table)
     lengths = [int(n) for n in lengths]
     prefix = lengths if prefix is None else [int(n) for n in prefix]
     if x.dim() != 2 or min(lengths, default=0) < 0 or sum(lengths) > x.shape[0] or len(prefix) != len(lengths):
         raise ValueError(f"x {tuple(x.shape)} must be [T][{D}] with T >= the sum of lengths {lengths}, and prefix {prefix} "
                          "as long as lengths")
-    cap = caches[0]["v"].shape[2] * kv8.BLOCK
-    if caches[0]["v"].shape[0] != len(lengths) or max(lengths, default=0) > cap:
-        raise ValueError(f"caches of {caches[0]['v'].shape[0]} samples x {cap} tokens do not hold prompts of {lengths}")
+    samples, cap = _room(caches, table)
+    if samples != len(lengths) or max(lengths, default=0) > cap:
+        raise ValueError(f"caches of {samples} samples x {cap} tokens do not hold prompts of {lengths}")
     for k in ("wqkv", "wo", "wgu", "wdn"):
         if packed[k].dtype is not torch.bfloat16:
             raise TypeError(f"packed[{k!r}] must be bfloat16")
+    banks, index = _check_adapters(adapters, layers, samples)
     dev, T = x.device, x.shape[0]
     t = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
     spans = attention.prefix_spans(t(lengths), t(prefix), T)
     rope = _rope(torch.arange(T, device=dev) - spans[:, 0], dev)
     zero, at = t([0]), [sum(lengths[:i]) for i in range(len(lengths))]
+    if index is not None:  # of the rows; padding has none
+        doc = torch.repeat_interleave(torch.arange(samples + 1, device=dev), torch.tensor(lengths + [T - sum(lengths)], device=dev), output_size=T)
+        index = torch.cat([index, index.new_full((1,), -1)])[doc]
+
+    def project(l, name, h):
+        y = h @ packed[name][l].t()
+        return lora.add(y, h, banks[l][name], index, out=y) if name in banks[l] else y
+
     for l in range(layers):
-        q, k, v = _qkv(_norm(x, ln_in[l]) @ packed["wqkv"][l].t(), rope)
+        q, k, v = _qkv(project(l, "wqkv", _norm(x, ln_in[l])), rope)
         for b, n in enumerate(lengths):
-            if n:
+            if n and table is None:
                 kv8.store({name: c[b:b + 1] for name, c in caches[l].items()}, k[None, at[b]:at[b] + n],
                           v[None, at[b]:at[b] + n], zero)
+            elif n:
+                paged.append(caches[l], table[b:b + 1], k[None, at[b]:at[b] + n], v[None, at[b]:at[b] + n], zero)
         o = attention.attend(q[None], k[None], v[None], spans)
-        x = x + (o.view(T, H * HD) @ packed["wo"][l].t()).float()
-        y = (_norm(x, ln_post[l]) @ packed["wgu"][l].t()).unflatten(-1, (F, 2)).float()
-        h = (torch.nn.functional.gelu(y[..., 0], approximate="tanh") * y[..., 1]).to(torch.bfloat16)
-        x = x + (h @ packed["wdn"][l].t()).float()
+        x = x + project(l, "wo", o.view(T, H * HD)).float()
+        h = _norm(x, ln_post[l])
+        if "wgu" in banks[l]:
+            h = lora.add(h @ packed["wgu"][l].t(), h, banks[l]["wgu"], index, gate="gelu")
+        else:
+            y = (h @ packed["wgu"][l].t()).unflatten(-1, (F, 2)).float()
+            h = (torch.nn.functional.gelu(y[..., 0], approximate="tanh") * y[..., 1]).to(torch.bfloat16)
+        x = x + project(l, "wdn", h).float()
     return x
 
 
-def extend(weights: list, ln_in, ln_post, x, caches: list, lens, count=None) -> torch.Tensor:
+def extend(weights: list, ln_in, ln_post, x, caches: list, lens, count=None, *, table=None, adapters=None) -> torch.Tensor:
     """Runs the backbone over T further tokens of each sample behind its cached ones (answers token by token: T = 1).
 
-    weights: ``pack_backbone_w4`` output. x [B][T][2048] fp32: the hidden states entering layer 0, B T <= 64. caches as
-    ``prefill_packed`` leaves them; lens int32 [B] on the GPU: tokens cached so far, the positions of the new ones follow
-    them; count int32 [B]: how many of the T are real (None: all, clamped to [0, T]); those behind the caches' end are not.
-    The real tokens' keys and values are appended (the caller's lens grow by as many), each token sees all cached ones and the
+    weights: ``pack_backbone_w4`` output. x [B][T][2048] fp32: the hidden states entering layer 0, B T <= 64. caches, and table
+    where they are pages, as ``prefill_packed`` leaves them; lens int32 [B] on the GPU: tokens cached so far, the positions of the new
+    ones follow them; count int32 [B]: how many of the T are real (None: all, clamped to [0, T]); those behind the caches' (the
+    table's) end are not. adapters: as in ``prefill_packed``, an index for each sample. The real tokens' keys and values are appended (the
+    caller's lens grow by as many, and with a table it names the pages that they go to), each token sees all cached ones and the
     new ones up to itself. Returns the hidden states leaving the last layer [B][T][2048] fp32 (undefined where a token is not
-    real). Nothing synchronises, and a captured graph serves every length.
+    real). Nothing synchronises, and a captured graph serves every length and every table.
     """
-    _check_backbone(ln_in, ln_post, len(weights), x, caches)
-    if x.dim() != 3 or x.shape[0] != caches[0]["v"].shape[0] or x.shape[0] * x.shape[1] > w4.MAX_ROWS:
-        raise ValueError(f"x must be [B={caches[0]['v'].shape[0]}][T][{D}] with B T <= {w4.MAX_ROWS}, got {tuple(x.shape)}")
+    _check_backbone(ln_in, ln_post, len(weights), x, caches, table)
+    samples, cap = _room(caches, table)
+    if x.dim() != 3 or x.shape[0] != samples or x.shape[0] * x.shape[1] > w4.MAX_ROWS:
+        raise ValueError(f"x must be [B={samples}][T][{D}] with B T <= {w4.MAX_ROWS}, got {tuple(x.shape)}")
     B, T = int(x.shape[0]), int(x.shape[1])
     if count is not None and count.shape != lens.shape:
         raise ValueError(f"count must be [{B}] like lens, got {tuple(count.shape)} and {tuple(lens.shape)}")
+    banks, index = _check_adapters(adapters, len(weights), B)
     dev = x.device
-    rope = _rope(lens[:, None] + torch.arange(T, device=dev), dev)
-    room = (caches[0]["v"].shape[2] * kv8.BLOCK - lens).clamp(0, T)
+    if table is None:
+        rope = _rope(lens[:, None] + torch.arange(T, device=dev), dev)
+    else:
+        freqs = paged.frequencies(HD, device=dev)
+    room = (cap - lens).clamp(0, T)
     count = room if count is None else torch.minimum(count, room).clamp(min=0)
     after = lens + count
     x = x.reshape(B * T, D)
+    if index is not None and T > 1:
+        index = index.repeat_interleave(T)
+
+    def project(l, name, h, residual=None):
+        y = w4.linear(h, weights[l][name], residual=residual)
+        return lora.add(y, h, banks[l][name], index, out=y) if name in banks[l] else y
+
     for l, w in enumerate(weights):
-        q, k, v = _qkv(w4.linear(_norm(x, ln_in[l]), w["wqkv"]).view(B, T, (H + 2) * HD), rope)
-        kv8.store(caches[l], k, v, lens, count)
-        o = kv8.attend(q, caches[l], after, count=count)
-        x = w4.linear(o.view(B * T, H * HD), w["wo"], residual=x)
-        h = w4.linear(_norm(x, ln_post[l]), w["wgu"], gate="gelu")
-        x = w4.linear(h, w["wdn"], residual=x)
+        y = project(l, "wqkv", _norm(x, ln_in[l])).view(B, T, (H + 2) * HD)
+        if table is None:
+            q, k, v = _qkv(y, rope)
+            kv8.store(caches[l], k, v, lens, count)
+            o = kv8.attend(q, caches[l], after, count=count)
+        else:
+            q, k, v = y.unflatten(-1, (H + 2, HD)).split((H, 1, 1), 2)
+            q = paged.append(caches[l], table, k, v, lens, count, q=q, freqs=freqs, adjacent=True)
+            o = paged.attend(q, caches[l], table, after, count=count, out=q)
+        x = project(l, "wo", o.view(B * T, H * HD), x)
+        h = _norm(x, ln_post[l])
+        if "wgu" in banks[l]:
+            h = lora.add(w4.linear(h, w["wgu"], out_dtype=torch.float32), h, banks[l]["wgu"], index, gate="gelu")
+        else:
+            h = w4.linear(h, w["wgu"], gate="gelu")
+        x = project(l, "wdn", h, x)
     return x.view(B, T, D)
+
+
+def answer(head, ln_final, x, tokens=None, *, top: int = 1, scale: float = 1.0):
+    """Log probabilities of tokens behind hidden states: the final norm, the head and ``tokens.logprobs``, whose result it returns.
+
+    head: [V][2048] bf16 (often the embedding), whose logits are bf16, or, for up to 64 rows, ``w4.quantize`` of it, whose logits
+    are fp32. ln_final [2048] fp32, applied as (1 + w). x [rows][2048] or [B][T][2048] fp32: the hidden states leaving the last layer. tokens
+    int32 or int64 [rows] or [B][T]: those to score; None: the most probable ones, which are top_tokens[..., 0] (top >= 1). scale: one
+    over the temperature.
+    """
+    if x.dtype is not torch.float32 or ln_final.dtype is not torch.float32:
+        raise TypeError(f"x and ln_final must be float32, got {x.dtype} and {ln_final.dtype}")
+    if x.dim() not in (2, 3) or x.shape[-1] != D or ln_final.shape != (D,):
+        raise ValueError(f"x must be [rows][{D}] or [B][T][{D}] and ln_final [{D}], got {tuple(x.shape)} and {tuple(ln_final.shape)}")
+    if tokens is None and top < 1:
+        raise ValueError("without tokens to score, top must be 1 or more")
+    h = _norm(x.reshape(-1, D), ln_final)
+    if isinstance(head, dict):
+        logits = w4.linear(h, head, out_dtype=torch.float32)
+    else:
+        if head.dtype is not torch.bfloat16 or head.dim() != 2 or head.shape[1] != D:
+            raise ValueError(f"head must be bfloat16 [V][{D}] or a w4.quantize result, got {head.dtype} {tuple(head.shape)}")
+        logits = h @ head.t()
+    given = tokens
+    if tokens is None:
+        tokens = torch.zeros(x.shape[:-1], dtype=torch.int32, device=x.device)
+    r = _tokens.logprobs(logits.view(*x.shape[:-1], -1), tokens, top=top, scale=scale)
+    return r if given is not None else r._replace(logprob=r.top_logprobs[..., 0])
