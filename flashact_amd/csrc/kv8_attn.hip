@@ -289,7 +289,8 @@ extern "C" int fa_kv8_attention(const fa_kv8_attn_args* a, fa_stream_t stream) {
   kv8::AttnArgs p{};
   p.k = static_cast<const unsigned char*>(a->cache_k), p.v = static_cast<const unsigned char*>(a->cache_v);
   p.ks = a->cache_ks, p.vs = a->cache_vs;
-  rc = newest::set_up(p, a, a->blocks, kv8::splits_for(a->batch, a->tokens, a->heads, a->kv_heads, a->head_dim, a->blocks), who);
+  rc = newest::set_up(p, a, a->blocks, kv8::splits_for(a->batch, a->tokens, a->heads, a->kv_heads, a->head_dim, a->blocks), 1,
+                      who);
   if (rc != FA_OK) return rc;
   rc = host::check_gfx950(who);
   if (rc != FA_OK) return rc;

@@ -32,7 +32,7 @@ struct Args {
   unsigned char* out;
   float* part;               // [sample][head][row tile][split] {O[16][hd], {m, l}[16]}
   uint64_t *arrived, nonce;  // [sample][head][row tile][FUSED], where the last workgroup joins the splits
-  int B, T, H, G, nblk, RT, RC, S, least, causal;  // RT row tiles of a head, RC of them side by side on an XCD
+  int B, T, H, G, nblk, RT, RU, RC, S, least, causal;  // RT row tiles of a head in RU workgroups, RC of these side by side on an XCD
   float scale, over, cap;  // base 2: scale log2(e); capped, scale / cap and cap log2(e)
 };
 
@@ -55,7 +55,7 @@ __device__ __forceinline__ int splits_used(const Args& a, int nb) {
 
 // Which row tile of which sample and head, and which split of its keys, a workgroup takes.
 struct Place {
-  int split, bh, b, h, rt;
+  int split, bh, b, h, rt;  // rt: the workgroup's place along the rows, its row tile where it has one
   bool there;
 };
 __device__ __forceinline__ Place place_of(const Args& a) {
@@ -63,14 +63,14 @@ __device__ __forceinline__ Place place_of(const Args& a) {
   // that leave the later ones unused would else leave XCDs unused (64 samples of 1050 keys on 16 splits: 72 us instead
   // of 21); within a split the runs of row tiles are turned, so that the splits of one meet on different XCDs.
   const unsigned xcd = blockIdx.x & 7, y = blockIdx.x >> 3, yr = y / (unsigned)a.RC, u = yr * 8 + xcd;
-  const unsigned runs = (a.RT + a.RC - 1) / a.RC, all_runs = a.B * a.H * runs;
+  const unsigned runs = (a.RU + a.RC - 1) / a.RC, all_runs = a.B * a.H * runs;
   Place p;
   p.split = u / all_runs;
   unsigned turned = u - p.split * all_runs + (all_runs >= 8 ? (p.split * (all_runs - 1)) & 7 : 0);
   if (turned >= all_runs) turned -= all_runs;
   p.bh = turned / runs, p.b = p.bh / (unsigned)a.H, p.h = p.bh - p.b * a.H;
   p.rt = (turned - p.bh * runs) * a.RC + y - yr * a.RC;
-  p.there = p.split < a.S && p.rt < a.RT;
+  p.there = p.split < a.S && p.rt < a.RU;
   return p;
 }
 
@@ -301,9 +301,10 @@ constexpr int MAX_PARTS = 4096;
 // Splits of the keys across workgroups. A wave takes `block` us for a block that comes from memory and one to begin and end, more
 // than `resident` workgroups a CU share its bandwidth, and joining the splits costs 3 us: the number with the least estimate, for
 // samples that fill the cache (their lengths are on the GPU), is taken. Shorter ones use fewer.
-inline int splits_for(int batch, int tokens, int heads, int kv_heads, int blocks, double block, double resident) {
-  const int64_t rt = ((int64_t)tokens * (heads / kv_heads) + 15) / 16, units = rt * batch * kv_heads;
-  const int64_t most = std::min<int64_t>({(blocks + W - 1) / W, MAX_SPLITS, std::max<int64_t>(1, MAX_PARTS / units)});
+inline int splits_for(int batch, int tokens, int heads, int kv_heads, int blocks, double block, double resident,
+                      int tiles = 1) {
+  const int64_t rt = ((int64_t)tokens * (heads / kv_heads) + 16 * tiles - 1) / (16 * tiles), units = rt * batch * kv_heads;
+  const int64_t most = std::min<int64_t>({(blocks + W - 1) / W, MAX_SPLITS, std::max<int64_t>(1, MAX_PARTS / (units * tiles))});
   int best = 1;
   double least = 1e300;
   auto consider = [&](int64_t S) {
@@ -352,7 +353,7 @@ int check_call(const A* a, const char* who) {
 }
 
 template <class A>
-int set_up(Args& p, const A* a, int blocks, int splits, const char* who) {
+int set_up(Args& p, const A* a, int blocks, int splits, int tiles, const char* who) {
   const size_t need = workspace(splits, a->batch, a->tokens, a->heads, a->kv_heads, a->head_dim);
   if (need && (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16))
     return host::fail(FA_ERR_INVALID_ARG, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, need,
@@ -363,6 +364,7 @@ int set_up(Args& p, const A* a, int blocks, int splits, const char* who) {
   p.out = static_cast<unsigned char*>(a->out), p.part = static_cast<float*>(a->workspace);
   p.B = a->batch, p.T = a->tokens, p.H = a->kv_heads, p.G = a->heads / a->kv_heads, p.nblk = blocks;
   p.RT = (p.T * p.G + 15) / 16;
+  p.RU = (p.RT + tiles - 1) / tiles;
   p.S = splits;
   if (p.S > 1 && p.S <= FUSED) {
     p.nonce = host::launch_nonce();
@@ -371,9 +373,9 @@ int set_up(Args& p, const A* a, int blocks, int splits, const char* who) {
   }
   // All row tiles of a (split, sample, head) run on one XCD where these divide evenly over the 8, else in runs short enough
   // that there are 32 or more (200 tokens of 8 heads over 1100 keys of one sample 38 -> 21 us; 17.3 -> 17.5 for 4 samples of 50).
-  const int64_t groups = (int64_t)p.B * p.H * p.S, runs = groups % 8 ? std::min<int64_t>((31 + groups) / groups, p.RT) : 1;
-  p.RC = (int)((p.RT + runs - 1) / runs);
-  p.least = (int64_t)p.RT * p.B * p.H >= 64 ? 4 : 1;
+  const int64_t groups = (int64_t)p.B * p.H * p.S, runs = groups % 8 ? std::min<int64_t>((31 + groups) / groups, p.RU) : 1;
+  p.RC = (int)((p.RU + runs - 1) / runs);
+  p.least = (int64_t)p.RU * p.B * p.H >= 64 ? 4 : 1;
   p.causal = a->causal;
   p.scale = a->scale * LOG2E;
   p.over = a->softcap > 0.f ? a->scale / a->softcap : 0.f;
@@ -385,7 +387,7 @@ int set_up(Args& p, const A* a, int blocks, int splits, const char* who) {
 
 // Workgroups of a launch, or 0 where there are too many.
 inline unsigned grid_of(const Args& a) {
-  const int runs = (a.RT + a.RC - 1) / a.RC;
+  const int runs = (a.RU + a.RC - 1) / a.RC;
   const int64_t grid = ((int64_t)a.B * a.H * a.S * runs + 7) / 8 * 8 * a.RC;
   return grid > 0x7fffffff ? 0 : (unsigned)grid;
 }

@@ -10,10 +10,10 @@
 // page's keys are asked for as soon as this one's are in registers, the values' likewise. How pages are dealt to waves and
 // workgroups, and how their sums meet: newest.h.
 //
-// With many rows (a piece of a prompt) each workgroup of 16 takes its pages from the L2 again, at what a CU copies from there (110 GB/s),
-// and the chain of a page's step is about 1500 cycles a wave. Workgroups of 64 rows, whose waves walk together over pages that are copied once,
-// were no better: 293 tokens x 8 heads over up to 4011 keys 38 us so, 52 with four splits and 117 unsplit the other way; 1024
-// tokens of 32 heads over 8192 keys 328 and 306 us; 4 x 256 of 8 heads of 256 dims over 4096 keys 143 and 183.
+// With many rows (a piece of a prompt) each workgroup takes its pages from the L2 again, at what a CU copies from there (110 GB/s): a wave then
+// has two tiles of rows for each page (tiles_for). Not kept: workgroups of 64 rows whose waves walk together over pages that are copied once
+// (293 tokens x 8 heads over up to 4011 keys 38 us with single tiles, 52 with four splits and 117 unsplit that way; 1024 tokens of 32
+// heads over 8192 keys 306, and 242 with two tiles a wave).
 //
 // Rounding: scores are exact products summed in fp32, softmax and sums are fp32. bf16: the weights go into the second
 // product as two bf16 (2^-16 of each is lost; its MFMAs are not the bound), and are taken against a reference 2^17 above
@@ -77,8 +77,8 @@ struct Tile {
   u32x4 q[KS];
   f32x4 O[NT];
 
-  __device__ __forceinline__ void begin(const AttnArgs& a, const Place& at, const Span& sp) {
-    const int lane = threadIdx.x & 63, row = at.rt * 16 + (lane & 15), t = row / a.G, head = at.h * a.G + row % a.G;
+  __device__ __forceinline__ void begin(const AttnArgs& a, const Place& at, const Span& sp, int rt) {
+    const int lane = threadIdx.x & 63, row = rt * 16 + (lane & 15), t = row / a.G, head = at.h * a.G + row % a.G;
     pos = sp.len - sp.n + t;
     const bool valid = row < a.T * a.G && t < sp.n && pos >= 0;
     limit = valid ? (a.causal ? pos + 1 : sp.len) : 0;
@@ -109,28 +109,10 @@ struct Tile {
     asm volatile("" : "+v"(slope));
   }
 
-  // Page `blk` of the sample, its keys and values at kl and vl in LDS; gone: it is no page, and nobody sees its keys. keys_read and
-  // values_read run once the one and the other are in registers, values_there before these are read.
-  template <class A, class B, class C>
-  __device__ __forceinline__ void step(const AttnArgs& a, const unsigned char* kl, const unsigned char* vl, int blk, bool gone,
-                                       A&& keys_read, B&& values_there, C&& values_read) {
-    const int lane = threadIdx.x & 63, r = lane & 15, qq = lane >> 4;
-    u32x4 kc[2][KS];
-#pragma unroll
-    for (int i = 0; i < KS; i++)
-#pragma unroll
-      for (int x = 0; x < 2; x++) kc[x][i] = *reinterpret_cast<const u32x4*>(kl + ((4 * i + qq) * BT + 16 * x + r) * 16);
-    keys_read();
-    f32x4 s[2];
-#pragma unroll
-    for (int x = 0; x < 2; x++) {
-      s[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < KS; i++) s[x] = mma<F16>(kc[x][i], q[i], s[x]);
-    }
-    const int key0 = blk * BT + 8 * qq, low = gone ? 0 : lo, high = gone ? 0 : hi;
-    const bool mixed = blk * BT + BT > low;
-    u32x4 P, R;  // R: what P left off, bf16 only
+  // The products s of block `blk`'s keys -> its weights P (and what they left off, R; bf16 only) against the new reference.
+  __device__ __forceinline__ void weigh(const AttnArgs& a, f32x4* s, int blk, bool gone, u32x4& P, u32x4& R) {
+    const int key0 = blk * BT + 8 * ((threadIdx.x & 63) >> 4);
+    const bool mixed = blk * BT + BT > (gone ? 0 : lo);
     const int own = gone ? 0 : limit;
     float mx, f = 1.f;  // scores are s f
     if (!CAP && !BIAS && a.scale > 0.f) {
@@ -179,46 +161,115 @@ struct Tile {
         }
       }
     }
-    values_there();
-    u32x4 vc[NT];  // keys key0 .. key0 + 7 of dim 16 j + r
+  }
+};
+
+// Values that are not finite, out of v: where +inf (or NaN) stood, plus is 1, where -inf (or NaN), minus.
+template <bool F16>
+__device__ __forceinline__ u32x4 finite_part(u32x4 v, u32x4& plus, u32x4& minus) {
+  constexpr unsigned INF = F16 ? 0x7c00u : 0x7f80u, ONE = F16 ? 0x3c00u : 0x3f80u, BOTH = 0x10001u;
 #pragma unroll
-    for (int j = 0; j < NT; j++) vc[j] = *reinterpret_cast<const u32x4*>(vl + (qq * HD + 16 * j + r) * 16);
-    values_read();
-    // Values of keys that a row does not see must not reach it: its P is 0 there, but 0 x NaN is NaN. Those behind the
-    // last key that any row sees are cleared; where one between low and high is not finite, each column has its own product.
-    bool apart = false;
-    if (mixed) {
-      const u32x4 some = halves_below(high - key0), each = halves_below(low - key0);
-      unsigned bad = 0;
+  for (int i = 0; i < 4; i++) {
+    const unsigned w = v[i], size = w & 0x7fff7fffu;
+    const unsigned nan = (size + (0x7fffu - INF) * BOTH) & 0x80008000u, inf = (size + (0x8000u - INF) * BOTH) & 0x80008000u;
+    plus[i] = (((inf & ~w) | nan) >> 15) * ONE;
+    minus[i] = (((inf & w) | nan) >> 15) * ONE;
+    v[i] = w & ~((inf >> 15) * 0xffffu);
+  }
+  return v;
+}
+
+// Page `blk` of the sample for a wave's MB tiles, its keys and values at kl and vl in LDS; gone: it is no page, and nobody sees its keys.
+// keys_read and values_read run once the one and the other are in registers, values_there before these are read.
+template <int MB, bool F16, int HD, bool CAP, bool BIAS, class A, class B, class C>
+__device__ __forceinline__ void step(Tile<F16, HD, CAP, BIAS>* t, const AttnArgs& a, const unsigned char* kl, const unsigned char* vl, int blk,
+                                     bool gone, A&& keys_read, B&& values_there, C&& values_read) {
+  constexpr int KS = HD / 32, NT = HD / 16;
+  const int lane = threadIdx.x & 63, r = lane & 15, qq = lane >> 4;
+  u32x4 kc[2][KS];
 #pragma unroll
-      for (int j = 0; j < NT; j++) {
-        vc[j] &= some;
+  for (int i = 0; i < KS; i++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) bad |= not_finite<F16>(vc[j][i]) & ~each[i];
-      }
-      apart = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+    for (int x = 0; x < 2; x++) kc[x][i] = *reinterpret_cast<const u32x4*>(kl + ((4 * i + qq) * BT + 16 * x + r) * 16);
+  keys_read();
+  f32x4 s[MB][2];
+#pragma unroll
+  for (int n = 0; n < MB; n++)
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      s[n][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KS; i++) s[n][x] = mma<F16>(kc[x][i], t[n].q[i], s[n][x]);
     }
-    if (!apart) {
+  u32x4 P[MB], R[MB];
 #pragma unroll
-      for (int j = 0; j < NT; j++) {
-        O[j] = mma<F16>(vc[j], P, O[j]);
-        if constexpr (!F16) O[j] = mma<F16>(vc[j], R, O[j]);
-      }
-    } else {
+  for (int n = 0; n < MB; n++) t[n].weigh(a, s[n], blk, gone, P[n], R[n]);
+  int lo = t[0].lo, hi = t[0].hi;
+#pragma unroll
+  for (int n = 1; n < MB; n++) lo = min(lo, t[n].lo), hi = max(hi, t[n].hi);
+  values_there();
+  u32x4 vc[NT];  // keys key0 .. key0 + 7 of dim 16 j + r
+#pragma unroll
+  for (int j = 0; j < NT; j++) vc[j] = *reinterpret_cast<const u32x4*>(vl + (qq * HD + 16 * j + r) * 16);
+  values_read();
+  // Values of keys that a row does not see must not reach it: its P is 0 there, but 0 x NaN is NaN. Those behind the last key that
+  // any row sees are cleared. Where one between low and high is not finite, the product is taken without such values, and rows that see
+  // them get their infinities: products of ones count these (both for a NaN). With 256 dims each column has a product of its own.
+  const int key0 = blk * BT + 8 * qq, low = gone ? 0 : lo, high = gone ? 0 : hi;
+  bool apart = false;
+  if (blk * BT + BT > low) {
+    const u32x4 some = halves_below(high - key0), each = halves_below(low - key0);
+    unsigned bad = 0;
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+      vc[j] &= some;
+#pragma unroll
+      for (int i = 0; i < 4; i++) bad |= not_finite<F16>(vc[j][i]) & ~each[i];
+    }
+    apart = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+  }
+  if constexpr (HD == 256) {  // (products of ones took registers: 4 x 256 tokens of 8 heads over 4096 keys 154 us, 140 so)
+    static_assert(MB == 1, "one tile of 256 dims");
+    if (apart) {
+      const int own = gone ? 0 : t->limit;
 #pragma unroll 1
       for (int c = 0; c < 16; c++) {
         const u32x4 mine = halves_below(__builtin_amdgcn_readlane(own, c) - key0);
 #pragma unroll
         for (int j = 0; j < NT; j++) {
-          f32x4 o = mma<F16>(vc[j] & mine, P, O[j]);
-          if constexpr (!F16) o = mma<F16>(vc[j] & mine, R, o);
-          if (r == c) O[j] = o;
+          f32x4 o = mma<F16>(vc[j] & mine, P[0], t->O[j]);
+          if constexpr (!F16) o = mma<F16>(vc[j] & mine, R[0], o);
+          if (r == c) t->O[j] = o;
           __builtin_amdgcn_sched_barrier(0);
         }
       }
+      return;
+    }
+  } else if (apart) {
+    u32x4 sees[MB];
+#pragma unroll
+    for (int n = 0; n < MB; n++) sees[n] = halves_below((gone ? 0 : t[n].limit) - key0) & (F16 ? 0x3c003c00u : 0x3f803f80u);
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+      u32x4 plus, minus;
+      vc[j] = finite_part<F16>(vc[j], plus, minus);
+#pragma unroll
+      for (int n = 0; n < MB; n++) {
+        const f32x4 p = mma<F16>(plus, sees[n], f32x4{0.f, 0.f, 0.f, 0.f}), m = mma<F16>(minus, sees[n], f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+        for (int i = 0; i < 4; i++) t[n].O[j][i] += (p[i] > 0.f ? INFINITY : 0.f) + (m[i] > 0.f ? -INFINITY : 0.f);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
-};
+#pragma unroll
+  for (int j = 0; j < NT; j++)
+#pragma unroll
+    for (int n = 0; n < MB; n++) {
+      t[n].O[j] = mma<F16>(vc[j], P[n], t[n].O[j]);
+      if constexpr (!F16) t[n].O[j] = mma<F16>(vc[j], R[n], t[n].O[j]);
+    }
+}
 
 // The pages of a sample that a wave goes over, blk, blk + step, .., one after the other: 64 are held in the lanes (looked up one by one, by
 // scalar loads, each step waited for the one of the step after it: LDS reads and scalar loads share a counter).
@@ -245,17 +296,22 @@ struct Pages {
 template <int HD>
 using Lds = newest::Lds<HD, 2 * BT * HD * 2>;  // of a wave: a page of keys and one of values
 
-template <bool F16, int HD, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : HD == 128 ? 2 : HD == 96 ? 3 : 4) attn_kernel(AttnArgs a) {
+template <bool F16, int HD, bool CAP, bool BIAS, int MB>
+__global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : HD == 128 || MB > 1 ? 2 : HD == 96 ? 3 : 4) attn_kernel(AttnArgs a) {
   constexpr int PAGE = BT * HD * 2, NC = PAGE / 1024;  // NC: copies of a page
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const Place here = newest::place_of(a);
   if (!here.there) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Span sp = newest::span_of(a, here.b);
-  Tile<F16, HD, CAP, BIAS> tile;
-  tile.begin(a, here, sp);
-  const int nb = (tile.hi + BT - 1) / BT;
+  Tile<F16, HD, CAP, BIAS> tile[MB];
+  int hi = 0;
+#pragma unroll
+  for (int n = 0; n < MB; n++) {
+    tile[n].begin(a, here, sp, here.rt * MB + n);
+    hi = max(hi, tile[n].hi);
+  }
+  const int nb = (hi + BT - 1) / BT;
   const int used = newest::splits_used(a, nb);
   if (here.split >= used) return;
   const int at = here.split * W + wave, all = used * W;
@@ -274,13 +330,14 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : HD == 128 ? 2 : HD == 
     copy(a.k, pg, at_k, keys_at);
     copy(a.v, pg, at_v, values_at);
   }
-  tile.arrive();
+#pragma unroll
+  for (int n = 0; n < MB; n++) tile[n].arrive();
   for (int blk = at; blk < nb; blk += all) {
     const bool more = blk + all < nb;
     const int next = more ? pages.next() : 0;
     vm_wait<NC>();  // the keys; the values are still on their way
-    tile.step(
-        a, kl, vl, blk, !pages.there(pg),
+    step<MB>(
+        tile, a, kl, vl, blk, !pages.there(pg),
         [&] {
           lds_wait();
           if (more) copy(a.k, next, at_k, keys_at);
@@ -295,7 +352,12 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : HD == 128 ? 2 : HD == 
         });
     pg = next;
   }
-  newest::meet<F16, HD, Lds<HD>>(a, here, sp, used, lds, tile.O, tile.m, cols_sum(tile.l));
+#pragma unroll
+  for (int n = 0; n < MB; n++) {
+    Place at_n = here;
+    at_n.rt = here.rt * MB + n;
+    if (at_n.rt < a.RT) newest::meet<F16, HD, Lds<HD>>(a, at_n, sp, used, lds, tile[n].O, tile[n].m, cols_sum(tile[n].l));
+  }
 }
 
 template <bool F16, int HD>
@@ -303,11 +365,24 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a) {
   newest::join<F16, HD>(a);
 }
 
+// Row tiles of a wave: two where there are many of them over many pages (us with one and with two; heads / K/V heads, dims): 1024 tokens
+// over 8192 keys, 32 / 8, 128 328 and 242, 96 226 and 184, 64 174 and 157; 512 over 4096, 32 / 8, 128 93 and 70; 1024 over 1024 42 and 37;
+// 128 over 131072, 8 / 1 213 and 139; 8 x 512 over 2048, 16 / 4, 96 126 and 119. Fewer leave CUs idle: 293 over 4011, 1500 and 293, 8 / 1, 128 38
+// and 54; 4 x 50 over 1018 12 and 18; and two to four tiles in all read each page once or twice as it is: 32 x 8 over 4096, 32 / 8 98 and 108. (8 x 512
+// over 1024, 16 / 4, 96, on this side of it, 66 and 69.) 256 dims do not fit into the registers twice.
+int tiles_for(int batch, int tokens, int heads, int kv_heads, int hd, int pages) {
+  const int64_t rt = ((int64_t)tokens * (heads / kv_heads) + 15) / 16;
+  return hd <= 128 && rt >= 8 && rt * batch * kv_heads * pages >= 65536 ? 2 : 1;
+}
+
 // A wave takes about 2.3 us for a page of 256 dims (1.2 of 128 and less); more than one workgroup a CU (two) share its bandwidth. That
 // is for samples that fill their tables. Where one tile of rows is all there is (single tokens), samples are of any age, and a
 // full one that takes few splits is waited for: up to 8 splits of 4 pages a wave or more. (48 samples of 1 to 8192 tokens, 4 K/V
 // heads of 128 dims, 3 splits by the estimate: 43 us, 8: 33, 16: 32.5; 48 of 4096 each 75, 78 and 79; of 983 24 all three.)
 int splits_for(int batch, int tokens, int heads, int kv_heads, int hd, int pages) {
+  const int tiles = tiles_for(batch, tokens, heads, kv_heads, hd, pages);
+  if (tiles > 1)
+    return std::min(newest::FUSED, newest::splits_for(batch, tokens, heads, kv_heads, pages, 1.8, 2.0, tiles));  // a second kernel joins single tiles
   const int s = newest::splits_for(batch, tokens, heads, kv_heads, pages, hd == 256 ? 2.3 : 1.2, hd == 256 ? 1.0 : 2.0);
   const int64_t units = (int64_t)batch * kv_heads;
   if ((int64_t)tokens * (heads / kv_heads) > 16 || units < 64) return s;
@@ -319,8 +394,12 @@ int launch_attn(const AttnArgs& a, hipStream_t s) {
   const unsigned grid = newest::grid_of(a);
   if (!grid) return host::fail(FA_ERR_INVALID_ARG, "fa_paged_attention: too many rows for one call");
   const bool cap = a.cap > 0.f, bias = a.slopes != nullptr;
-  void (*k)(AttnArgs) = cap ? (bias ? attn_kernel<F16, HD, true, true> : attn_kernel<F16, HD, true, false>)
-                            : (bias ? attn_kernel<F16, HD, false, true> : attn_kernel<F16, HD, false, false>);
+  void (*k)(AttnArgs) = cap ? (bias ? attn_kernel<F16, HD, true, true, 1> : attn_kernel<F16, HD, true, false, 1>)
+                            : (bias ? attn_kernel<F16, HD, false, true, 1> : attn_kernel<F16, HD, false, false, 1>);
+  if constexpr (HD <= 128)
+    if (a.RU < a.RT)
+      k = cap ? (bias ? attn_kernel<F16, HD, true, true, 2> : attn_kernel<F16, HD, true, false, 2>)
+              : (bias ? attn_kernel<F16, HD, false, true, 2> : attn_kernel<F16, HD, false, false, 2>);
   const unsigned lds = Lds<HD>::BYTES;
   const int rc = host::allow_lds(reinterpret_cast<const void*>(k), lds, "fa_paged_attention");
   if (rc != FA_OK) return rc;
@@ -364,7 +443,7 @@ extern "C" int fa_paged_attention(const fa_paged_attn_args* a, fa_stream_t strea
   p.k = static_cast<const unsigned char*>(a->pool_k), p.v = static_cast<const unsigned char*>(a->pool_v);
   p.table = a->table, p.ts = a->table_stride, p.pages = a->pages;
   rc = newest::set_up(p, a, a->table_pages, paged::splits_for(a->batch, a->tokens, a->heads, a->kv_heads, a->head_dim, a->table_pages),
-                      who);
+                      paged::tiles_for(a->batch, a->tokens, a->heads, a->kv_heads, a->head_dim, a->table_pages), who);
   if (rc != FA_OK) return rc;
   rc = host::check_gfx950(who);
   if (rc != FA_OK) return rc;

@@ -175,7 +175,8 @@ def attend(q, pool: dict, table, lens, *, count=None, scale=None, softcap: float
     [B]: cached tokens (those behind the table's end do not count); count int32 [B]: how many of the T are real (None: all). Query
     t < n is at position i = lens - n + t and sees keys j <= i, or all of the cached ones with causal=False; keys of no page are
     not seen. Scores are q . k * scale (default hd^-1/2), capped to softcap * tanh(s / softcap) where softcap > 0, less
-    slopes[h] |i - j| where slopes (fp32 [H]) are given. Rows without keys become zero. Returns [B][T][H][hd] of q's type, in
+    slopes[h] |i - j| where slopes (fp32 [H]) are given. Rows without keys become zero; what a row does not see never reaches it, and
+    an infinite value that it sees leaves that dim infinite or NaN. Returns [B][T][H][hd] of q's type, in
     `out` where it is given (q itself may be).
     """
     pk, pv, pages, h, hd, index, b, width, stride = _pool(pool, table)
