@@ -253,6 +253,26 @@ def run_on(index: int, fn, args, what: str) -> None:
         check(rc, what)
 
 
+def layout(t) -> tuple:
+    """(type, shape, strides): what a call's checks depend on and their answers may be kept by."""
+    return t.dtype, t.shape, t.stride()
+
+
+def contiguous(lay) -> bool:
+    """Whether a tensor of this ``layout`` is contiguous."""
+    reach = 1
+    for n, s in zip(reversed(lay[1]), reversed(lay[2])):
+        if n > 1 and s != reach:
+            return 0 in lay[1]
+        reach *= n
+    return True
+
+
+def steps3(lay) -> tuple:
+    """Strides of a ``layout``'s first three dimensions; those of size one, which are never stepped, as 0."""
+    return tuple(s if n > 1 else 0 for n, s in zip(lay[1][:3], lay[2]))
+
+
 def strides3(t) -> tuple:
     """Strides of a tensor's first three dimensions; those of size one, which are never stepped, as 0."""
     n, s = t.shape, t.stride()
@@ -275,6 +295,20 @@ def overlap(a, b) -> bool:
     """Whether two tensors' memory ranges meet."""
     at, bt, na, nb = a.data_ptr(), b.data_ptr(), _layout(a.shape, a.stride())[0], _layout(b.shape, b.stride())[0]
     return na > 0 and nb > 0 and at < bt + nb * b.element_size() and bt < at + na * a.element_size()
+
+
+def overlaps(a, others) -> bool:
+    """Whether a's memory range meets one of the others' (None: none)."""
+    at = a.data_ptr()
+    end = at + _layout(a.shape, a.stride())[0] * a.element_size()
+    if at == end:
+        return False
+    for b in others:
+        if b is not None:
+            bt = b.data_ptr()
+            if bt < end and bt + _layout(b.shape, b.stride())[0] * b.element_size() > at:
+                return True
+    return False
 
 
 def doubled(t) -> bool:

@@ -52,6 +52,40 @@ def unpack(bank: dict) -> list:
     return [(a.transpose(0, 1).flatten(1), b.transpose(0, 1).flatten(1), s) for a, b, s in zip(bank["a"], bank["b"], bank["scale"].tolist())]
 
 
+@functools.lru_cache(maxsize=1024)
+def _add_of(y, x, a, b, scale, index, gate):
+    """(the struct's types, the result's shape and type, x's row stride, the struct's sizes, the workspace's bytes, 0 without rows) of
+    layouts (``_lib.layout``), checked: done once for each of them."""
+    t, sx, stx = x
+    if t is not torch.bfloat16 and t is not torch.float16:
+        raise TypeError(f"x must be bfloat16 or float16, got {t}")
+    if a[0] is not t or b[0] is not t or scale[0] is not torch.float32:
+        raise TypeError(f"the bank's a and b must be {t} like x and scale float32, got {a[0]}, {b[0]} and {scale[0]}")
+    if y[0] is not t and y[0] is not torch.float32:
+        raise TypeError(f"y must be float32 or {t} like x, got {y[0]}")
+    sa, sb = a[1], b[1]
+    if (len(sa) != 4 or len(sb) != 4 or sa[3] != 8 or sb[3] != 8 or sa[0] != sb[0] or sa[2] != 8 * sb[1] or not 0 < sa[2] <= MAX_RANK
+            or not sa[0] * sa[1] * sb[2] or scale[1] != sa[:1]):
+        raise ValueError(f"the bank must be a [adapters][K / 8][rank][8], b [adapters][rank / 8][N][8] and scale [adapters] with ranks up "
+                         f"to {MAX_RANK}, got {tuple(sa)}, {tuple(sb)} and {tuple(scale[1])}")
+    if not (_lib.contiguous(a) and _lib.contiguous(b) and _lib.contiguous(scale)):
+        raise ValueError("the bank's tensors must be contiguous")
+    k, n, rank = 8 * sa[1], sb[2], sa[2]
+    rows = sx[0] if len(sx) == 2 else -1
+    if rows < 0 or sx[1] != k or y[1] != (rows, n) or index[1] != (rows,):
+        raise ValueError(f"x must be [rows][K={k}], y [rows][N={n}] and index [rows], got {tuple(sx)}, {tuple(y[1])} and {tuple(index[1])}")
+    if index[0] is not torch.int32 or not _lib.contiguous(index) or not _lib.contiguous(y):
+        raise ValueError(f"index must be contiguous int32 and y contiguous, got {index[0]} and strides {y[2]}")
+    if gate is not None and (gate != "gelu" or n % 2):
+        raise ValueError(f"gate must be None or 'gelu' (with an even N), got {gate!r} and N={n}")
+    stride = stx[0] if rows > 1 else k
+    if stx[1] != 1 or stride % 8 or stride < k:
+        raise ValueError(f"x must have contiguous rows that do not overlap, strides multiples of 8, got strides {stx}")
+    shape, dt = ((rows, n), y[0]) if gate is None else ((rows, n // 2), t)
+    return ((_DT[t], _DT[y[0]]), shape, dt, stride, (rows, n, k, rank, sa[0], 0 if gate is None else 1),
+            _workspace_bytes(rows, k, rank) if rows else 0)
+
+
 def add(y: torch.Tensor, x: torch.Tensor, bank: dict, index: torch.Tensor, *, gate=None, out=None) -> torch.Tensor:
     """y + scale[i] B_i A_i x, row by row with i = index[row]; rows whose index is no adapter's (-1) keep y. On the current stream.
 
@@ -61,49 +95,26 @@ def add(y: torch.Tensor, x: torch.Tensor, bank: dict, index: torch.Tensor, *, ga
     type. Else it is like y, in `out` where that is given (y itself may be). An adapter reaches its own rows only.
     """
     a, b, scale = bank["a"], bank["b"], bank["scale"]
-    t = x.dtype
-    if t is not torch.bfloat16 and t is not torch.float16:
-        raise TypeError(f"x must be bfloat16 or float16, got {t}")
-    if a.dtype is not t or b.dtype is not t or scale.dtype is not torch.float32:
-        raise TypeError(f"the bank's a and b must be {t} like x and scale float32, got {a.dtype}, {b.dtype} and {scale.dtype}")
-    if y.dtype is not t and y.dtype is not torch.float32:
-        raise TypeError(f"y must be float32 or {t} like x, got {y.dtype}")
-    sa, sb = a.shape, b.shape
-    if (len(sa) != 4 or len(sb) != 4 or sa[3] != 8 or sb[3] != 8 or sa[0] != sb[0] or sa[2] != 8 * sb[1] or not 0 < sa[2] <= MAX_RANK
-            or not sa[0] * sa[1] * sb[2] or scale.shape != sa[:1]):
-        raise ValueError(f"the bank must be a [adapters][K / 8][rank][8], b [adapters][rank / 8][N][8] and scale [adapters] with ranks up "
-                         f"to {MAX_RANK}, got {tuple(sa)}, {tuple(sb)} and {tuple(scale.shape)}")
-    if not (a.is_contiguous() and b.is_contiguous() and scale.is_contiguous()):
-        raise ValueError("the bank's tensors must be contiguous")
-    k, n, rank = 8 * sa[1], sb[2], sa[2]
-    rows = x.shape[0] if x.dim() == 2 else -1
-    if rows < 0 or x.shape[1] != k or y.shape != (rows, n) or index.shape != (rows,):
-        raise ValueError(f"x must be [rows][K={k}], y [rows][N={n}] and index [rows], got {tuple(x.shape)}, {tuple(y.shape)} and "
-                         f"{tuple(index.shape)}")
-    if index.dtype is not torch.int32 or not index.is_contiguous() or not y.is_contiguous():
-        raise ValueError(f"index must be contiguous int32 and y contiguous, got {index.dtype} and strides {y.stride()}")
-    if gate is not None and (gate != "gelu" or n % 2):
-        raise ValueError(f"gate must be None or 'gelu' (with an even N), got {gate!r} and N={n}")
-    stride = x.stride(0) if rows > 1 else k
-    if x.stride(1) != 1 or stride % 8 or stride < k or x.data_ptr() % 16:
-        raise ValueError(f"x must have contiguous, 16-byte aligned rows that do not overlap, got strides {x.stride()}")
+    lay = _lib.layout
+    dtype, shape, dt, stride, sizes, need = _add_of(lay(y), lay(x), lay(a), lay(b), lay(scale), lay(index), gate)
+    at = x.data_ptr()
+    if at % 16:
+        raise ValueError("x must be 16-byte aligned")
     gpu = x.get_device()
-    if gpu < 0 or any(v.get_device() != gpu for v in (a, b, scale, y, index)):
+    if not gpu == a.get_device() == b.get_device() == scale.get_device() == y.get_device() == index.get_device() or gpu < 0:
         raise ValueError("x, y, index and the bank must be on the same GPU")
-    shape, dt = ((rows, n), y.dtype) if gate is None else ((rows, n // 2), t)
     if out is None:
-        out = x.new_empty(shape, dtype=dt)
+        out = torch.empty_like(y) if gate is None else x.new_empty(shape)
     elif out.dtype is not dt or out.shape != shape or not out.is_contiguous() or out.get_device() != gpu:
         raise ValueError(f"out must be contiguous {dt} {shape} on x's GPU, got {out.dtype} {tuple(out.shape)} on {out.device}")
-    elif _lib.overlap(out, y) and (gate is not None or out.data_ptr() != y.data_ptr()):
+    elif (gate is not None or out is not y) and _lib.overlap(out, y) and (gate is not None or out.data_ptr() != y.data_ptr()):
         raise ValueError("out must not share memory with y but for being it, without a gate")
-    elif any(_lib.overlap(out, v) for v in (x, a, b, scale, index)):
+    elif _lib.overlaps(out, (x, a, b, scale, index)):
         raise ValueError("out must not share memory with x, index or the bank")
-    if rows == 0:
+    if not need:
         return out
-    need = _workspace_bytes(rows, k, rank)
-    ws = x.new_empty(need, dtype=torch.uint8)
-    args = _lib.LoraArgs(_DT[t], _DT[y.dtype], x.data_ptr(), stride, a.data_ptr(), b.data_ptr(), scale.data_ptr(), index.data_ptr(),
-                         rows, n, k, rank, sa[0], 0 if gate is None else 1, y.data_ptr(), out.data_ptr(), ws.data_ptr(), need)
+    ws = x.new_empty(need // 2)
+    args = _lib.LoraArgs(*dtype, at, stride, a.data_ptr(), b.data_ptr(), scale.data_ptr(), index.data_ptr(), *sizes, y.data_ptr(),
+                         out.data_ptr(), ws.data_ptr(), need)
     _lib.run_on(gpu, _lib.lib().fa_lora_add, args, "fa_lora_add")
     return out

@@ -47,52 +47,88 @@ def frequencies(dims: int = 256, base: float = 10000.0, device="cuda") -> torch.
     return base ** (-torch.arange(0, dims, 2, dtype=torch.float64, device=device) / dims)
 
 
-def _pool(pool, table):
-    """(k, v, pages, kv_heads, head_dim, GPU index, samples, pages of a sample, the table's row stride), checked."""
-    k, v = pool["k"], pool["v"]
-    shape = v.shape
+# What of a call's checks depends on types, shapes and strides (``_lib.layout``) is done once for each of them, with what follows from
+# it for the C call; devices and addresses are looked at in every call. (append with queries: 9.6 us a call so, 12.8 with all of it in each.)
+@functools.lru_cache(maxsize=1024)
+def _pool_of(k, v, table):
+    """(pages, kv_heads, head_dim, samples, pages of a sample, the table's row stride) of layouts, checked."""
+    shape = v[1]
     if len(shape) != 5 or shape[2] != PAGE // 8 or shape[4] != 8 or shape[3] not in HEAD_DIMS:
         raise ValueError(f"pool v must be [pages][Hkv][{PAGE // 8}][hd in {HEAD_DIMS}][8], got {tuple(shape)}")
     pages, h, _, hd, _ = shape
-    if k.shape != (pages, h, hd // 8, PAGE, 8):
-        raise ValueError(f"pool k {tuple(k.shape)} does not belong to v {tuple(shape)}")
-    t = k.dtype
-    if (t is not torch.bfloat16 and t is not torch.float16) or v.dtype is not t:
-        raise TypeError(f"pool k and v must both be bfloat16 or float16, got {t} and {v.dtype}")
-    if not (k.is_contiguous() and v.is_contiguous()):
+    if k[1] != (pages, h, hd // 8, PAGE, 8):
+        raise ValueError(f"pool k {tuple(k[1])} does not belong to v {tuple(shape)}")
+    t = k[0]
+    if (t is not torch.bfloat16 and t is not torch.float16) or v[0] is not t:
+        raise TypeError(f"pool k and v must both be bfloat16 or float16, got {t} and {v[0]}")
+    if not (_lib.contiguous(k) and _lib.contiguous(v)):
         raise ValueError("pool tensors must be contiguous")
     if not pages * h:
         raise ValueError(f"the pool is empty: {tuple(shape)}")
-    index = v.get_device()
-    if (table.dtype is not _I32 or table.dim() != 2 or table.get_device() != index or not table.numel()
-            or (table.shape[1] > 1 and table.stride(1) != 1)):
-        raise ValueError(f"table must be int32 [B][pages of a sample], not empty, rows contiguous, on the pool's GPU, got {table.dtype} "
-                         f"{tuple(table.shape)} on {table.device}")
-    if k.get_device() != index:
-        raise ValueError("the pool's tensors must be on one GPU")
-    b, width = table.shape
-    stride = table.stride(0) if b > 1 else width
+    tt, ts, tst = table
+    if tt is not _I32 or len(ts) != 2 or not ts[0] * ts[1] or (ts[1] > 1 and tst[1] != 1):
+        raise ValueError(f"table must be int32 [B][pages of a sample], not empty, rows contiguous, got {tt} {tuple(ts)} with strides {tst}")
+    b, width = ts
+    stride = tst[0] if b > 1 else width
     if stride < width:
-        raise ValueError(f"the table's rows overlap: {tuple(table.shape)} with strides {table.stride()}")
-    return k, v, pages, h, hd, index, b, width, stride
+        raise ValueError(f"the table's rows overlap: {tuple(ts)} with strides {tst}")
+    return pages, h, hd, b, width, stride
 
 
-def _index(name, t, b, index):
-    if t.dtype is not _I32 or t.shape != (b,) or not t.is_contiguous() or t.get_device() != index:
-        raise ValueError(f"{name} must be contiguous int32 [{b}] on the pool's GPU, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
-
-
-def _rows(pk, k, v, b, h, hd, index):
-    """The rows' tokens, checked."""
-    if k.dtype is not pk.dtype or v.dtype is not pk.dtype:
-        raise TypeError(f"k and v must be {pk.dtype} like the pool, got {k.dtype} and {v.dtype}")
-    shape = k.shape
-    if len(shape) != 4 or shape[0] != b or shape[2] != h or shape[3] != hd or v.shape != shape:
-        raise ValueError(f"k and v must be [{b}][tokens][{h}][{hd}], got {tuple(shape)} and {tuple(v.shape)}")
-    if index < 0 or k.get_device() != index or v.get_device() != index:
-        raise ValueError(f"pool, k and v must be on the same GPU, got {k.device} and {v.device}")
+def _rows_of(t, k, v, b, h, hd) -> int:
+    """The tokens of rows' layouts, checked."""
+    if k[0] is not t or v[0] is not t:
+        raise TypeError(f"k and v must be {t} like the pool, got {k[0]} and {v[0]}")
+    shape = k[1]
+    if len(shape) != 4 or shape[0] != b or shape[2] != h or shape[3] != hd or v[1] != shape:
+        raise ValueError(f"k and v must be [{b}][tokens][{h}][{hd}], got {tuple(shape)} and {tuple(v[1])}")
     return shape[1]
+
+
+def _steps(name, lay) -> tuple:
+    """Strides of rows' first three dimensions, for reads of eight dims at once."""
+    s = _lib.steps3(lay)
+    if lay[2][3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8:
+        raise ValueError(f"{name} must have contiguous dims and strides that are multiples of 8, got {lay[2]}")
+    return s
+
+
+def _per_sample(name, lay, b):
+    if lay is not None and (lay[0] is not _I32 or lay[1] != (b,) or not _lib.contiguous(lay)):
+        raise ValueError(f"{name} must be contiguous int32 [{b}], got {lay[0]} {tuple(lay[1])}")
+
+
+def _on_one(*tensors) -> int:
+    """The GPU that all of them (None: none) are on."""
+    index = tensors[0].get_device()
+    for x in tensors:
+        if x is not None and x.get_device() != index:
+            index = -1
+    if index < 0:
+        raise ValueError(f"all tensors must be on one GPU, got {[str(x.device) for x in tensors if x is not None]}")
+    return index
+
+
+@functools.lru_cache(maxsize=1024)
+def _append_of(pk, pv, table, k, v, q, start, count, freqs):
+    """(strides of q, k and v, the table's row stride, the struct's type and last sizes) of layouts, checked."""
+    pages, h, hd, b, width, stride = _pool_of(pk, pv, table)
+    tokens = _rows_of(pk[0], k, v, b, h, hd)
+    sk, sv, sq, heads = _steps("k", k), _steps("v", v), (0, 0, 0), 0
+    if q is not None:
+        if q[0] is not pk[0]:
+            raise TypeError(f"q must be {pk[0]} like the pool, got {q[0]}")
+        if len(q[1]) != 4 or q[1][0] != b or q[1][1] != tokens or q[1][2] < 1 or q[1][3] != hd:
+            raise ValueError(f"q must be [{b}][{tokens}][heads][{hd}], got {tuple(q[1])}")
+        sq, heads = _steps("q", q), q[1][2]
+    _per_sample("start", start, b)
+    _per_sample("count", count, b)
+    rotary = 0
+    if freqs is not None:
+        rotary = 2 * freqs[1][0] if len(freqs[1]) == 1 else -1
+        if freqs[0] is not torch.float64 or not 0 < rotary <= hd or rotary % 16 or not _lib.contiguous(freqs):
+            raise ValueError(f"freqs must be contiguous float64 [a multiple of 8 up to {hd // 2}], got {freqs[0]} {tuple(freqs[1])}")
+    return _S3(*sq), _S4(*sk, 1), _S4(*sv, 1), stride, _lib.DTYPES[pk[0]], (b, tokens, heads, h, hd, pages, width, rotary)
 
 
 def append(pool: dict, table, k, v, start, count=None, *, q=None, freqs=None, adjacent: bool = False):
@@ -106,36 +142,20 @@ def append(pool: dict, table, k, v, start, count=None, *, q=None, freqs=None, ad
     case. Rows behind the table's end or of no page are dropped, as is a sample with a negative start. The result [B][T][H][hd]
     has zeros where a row is not real. Two rows at one token of one page must be ordered by the caller; rows and pool share no memory.
     """
-    pk, pv, pages, h, hd, index, b, width, stride = _pool(pool, table)
-    tokens = _rows(pk, k, v, b, h, hd, index)
-    t = pk.dtype
-    sk, sv, sq, heads, out = _lib.strides3(k), _lib.strides3(v), (0, 0, 0), 0, None
-    for s, x in ((sk, k), (sv, v)):
-        if x.stride(3) != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 or x.data_ptr() % 16:
-            raise ValueError("k and v must have contiguous dims and strides that are multiples of 8, 16-byte aligned, got "
-                             f"{x.stride()}")
+    pk, pv = pool["k"], pool["v"]
+    lay = _lib.layout
+    sq, sk, sv, stride, dtype, sizes = _append_of(lay(pk), lay(pv), lay(table), lay(k), lay(v), None if q is None else lay(q), lay(start),
+                                                  None if count is None else lay(count), None if freqs is None else lay(freqs))
+    index = _on_one(pk, pv, table, k, v, start, count, q, freqs)
+    at_k, at_v, at_q, out, at_out = k.data_ptr(), v.data_ptr(), None, None, None
     if q is not None:
-        if q.dtype is not t:
-            raise TypeError(f"q must be {t} like the pool, got {q.dtype}")
-        if q.dim() != 4 or q.shape[0] != b or q.shape[1] != tokens or q.shape[2] < 1 or q.shape[3] != hd:
-            raise ValueError(f"q must be [{b}][{tokens}][heads][{hd}], got {tuple(q.shape)}")
-        sq, heads = _lib.strides3(q), q.shape[2]
-        if q.stride(3) != 1 or sq[0] % 8 or sq[1] % 8 or sq[2] % 8 or q.data_ptr() % 16 or q.get_device() != index:
-            raise ValueError("q must have contiguous dims and strides that are multiples of 8, 16-byte aligned, on the pool's GPU, got "
-                             f"{q.stride()} on {q.device}")
-        out = q.new_empty((b, tokens, heads, hd))
-    rotary = 0
-    if freqs is not None:
-        rotary = 2 * freqs.shape[0] if freqs.dim() == 1 else -1
-        if (freqs.dtype is not torch.float64 or not 0 < rotary <= hd or rotary % 16 or not freqs.is_contiguous()
-                or freqs.get_device() != index):
-            raise ValueError(f"freqs must be contiguous float64 [a multiple of 8 up to {hd // 2}] on the pool's GPU, got {freqs.dtype} "
-                             f"{tuple(freqs.shape)} on {freqs.device}")
-    a = _lib.PagedRowsArgs(_lib.DTYPES[t], None if q is None else q.data_ptr(), _S3(*sq), None if out is None else out.data_ptr(),
-                           k.data_ptr(), _S4(*sk, 1), v.data_ptr(), _S4(*sv, 1), pk.data_ptr(), pv.data_ptr(), table.data_ptr(),
-                           stride, _index("start", start, b, index), None if count is None else _index("count", count, b, index),
-                           None if freqs is None else freqs.data_ptr(), b, tokens, heads, h, hd, pages, width, rotary,
-                           int(adjacent), 0)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        at_q, at_out = q.data_ptr(), out.data_ptr()
+    if (at_k | at_v | (at_q or 0)) % 16:
+        raise ValueError("k, v and q must be 16-byte aligned")
+    a = _lib.PagedRowsArgs(dtype, at_q, sq, at_out, at_k, sk, at_v, sv, pk.data_ptr(), pv.data_ptr(), table.data_ptr(), stride,
+                           start.data_ptr(), None if count is None else count.data_ptr(), None if freqs is None else freqs.data_ptr(),
+                           *sizes, int(adjacent), 0)
     _lib.run_on(index, _lib.lib().fa_paged_append, a, "fa_paged_append")
     return out
 
@@ -147,24 +167,45 @@ def load(pool: dict, table, lens, *, k=None, v=None):
     written in place up to min(lens[b], T) and left as they are behind it: a view of ``pi05.make_caches`` caches takes a prefix
     to the denoise loop. Tokens of no page are zeros.
     """
-    pk, pv, pages, h, hd, index, b, width, stride = _pool(pool, table)
+    pk, pv = pool["k"], pool["v"]
+    pages, h, hd, b, width, stride = _pool_of(_lib.layout(pk), _lib.layout(pv), _lib.layout(table))
     if (k is None) != (v is None):
         raise ValueError("pass both of k and v or neither")
     fresh = k is None
     if fresh:
         shape = (b, width * PAGE, h, hd)
         k, v = pk.new_empty(shape), pk.new_empty(shape)
-    tokens = _rows(pk, k, v, b, h, hd, index)
+    tokens = _rows_of(pk.dtype, _lib.layout(k), _lib.layout(v), b, h, hd)
+    _per_sample("lens", _lib.layout(lens), b)
+    index = _on_one(pk, pv, table, k, v, lens)
     if not fresh:
         if _lib.doubled(k) or _lib.doubled(v) or _lib.meet(k, v):
             raise ValueError("k and v are written: no two of their elements may be one")
-        if any(_lib.overlap(x, y) for x in (k, v) for y in (pk, pv, table, lens)):
+        if any(_lib.overlaps(x, (pk, pv, table, lens)) for x in (k, v)):
             raise ValueError("k and v must not share memory with the pool, the table or lens")
     a = _lib.PagedRowsArgs(_lib.DTYPES[pk.dtype], None, _S3(0, 0, 0), None, k.data_ptr(), _S4(*k.stride()), v.data_ptr(),
                            _S4(*v.stride()), pk.data_ptr(), pv.data_ptr(), table.data_ptr(), stride, None,
-                           _index("lens", lens, b, index), None, b, tokens, 0, h, hd, pages, width, 0, 0, int(fresh))
+                           lens.data_ptr(), None, b, tokens, 0, h, hd, pages, width, 0, 0, int(fresh))
     _lib.run_on(index, _lib.lib().fa_paged_load, a, "fa_paged_load")
     return k, v
+
+
+@functools.lru_cache(maxsize=1024)
+def _attend_of(pk, pv, table, q, lens, count, slopes):
+    """(the result's shape, strides of q, the table's row stride, the struct's type, its sizes, the workspace's bytes) of layouts, checked."""
+    pages, h, hd, b, width, stride = _pool_of(pk, pv, table)
+    t, shape = q[0], q[1]
+    if t is not pk[0]:
+        raise TypeError(f"q must be {pk[0]} like the pool, got {t}")
+    if len(shape) != 4 or shape[0] != b or shape[3] != hd or shape[2] < 1 or shape[2] % h:
+        raise ValueError(f"q must be [{b}][tokens][a multiple of {h}][{hd}], got {tuple(shape)}")
+    steps = _steps("q", q)
+    _per_sample("lens", lens, b)
+    _per_sample("count", count, b)
+    if slopes is not None and (slopes[0] is not _F32 or slopes[1] != (shape[2],) or not _lib.contiguous(slopes)):
+        raise ValueError(f"slopes must be contiguous float32 [{shape[2]}], got {slopes[0]} {tuple(slopes[1])}")
+    need = _workspace_bytes(b, shape[1], shape[2], h, hd, width)
+    return tuple(shape), _S3(*steps), stride, _lib.DTYPES[t], (b, shape[1], shape[2], h, hd, pages, width), need
 
 
 def attend(q, pool: dict, table, lens, *, count=None, scale=None, softcap: float = 0.0, slopes=None, causal: bool = True,
@@ -179,38 +220,27 @@ def attend(q, pool: dict, table, lens, *, count=None, scale=None, softcap: float
     an infinite value that it sees leaves that dim infinite or NaN. Returns [B][T][H][hd] of q's type, in
     `out` where it is given (q itself may be).
     """
-    pk, pv, pages, h, hd, index, b, width, stride = _pool(pool, table)
-    t = pk.dtype
-    if q.dtype is not t:
-        raise TypeError(f"q must be {t} like the pool, got {q.dtype}")
-    if q.dim() != 4 or q.shape[0] != b or q.shape[3] != hd or q.shape[2] < 1 or q.shape[2] % h:
-        raise ValueError(f"q must be [{b}][tokens][a multiple of {h}][{hd}], got {tuple(q.shape)}")
-    tokens, heads = q.shape[1], q.shape[2]
-    sb, st, sh = _lib.strides3(q)
-    if q.stride(3) != 1 or sb % 8 or st % 8 or sh % 8 or q.data_ptr() % 16:
-        raise ValueError(f"q must have contiguous dims and strides that are multiples of 8, 16-byte aligned, got {q.stride()}")
-    softcap = float(softcap)
+    pk, pv = pool["k"], pool["v"]
+    lay = _lib.layout
+    shape, sq, stride, dtype, sizes, need = _attend_of(lay(pk), lay(pv), lay(table), lay(q), lay(lens), None if count is None else lay(count),
+                                                       None if slopes is None else lay(slopes))
     if not 0.0 <= softcap < float("inf"):
         raise ValueError(f"softcap must be finite and >= 0, got {softcap}")
-    if index < 0 or q.get_device() != index:
-        raise ValueError(f"pool and q must be on the same GPU, got {q.device}")
-    if slopes is not None and (slopes.dtype is not _F32 or slopes.shape != (heads,) or not slopes.is_contiguous()
-                               or slopes.get_device() != index):
-        raise ValueError(f"slopes must be contiguous float32 [{heads}] on q's GPU, got {slopes.dtype} {tuple(slopes.shape)}")
+    index = _on_one(pk, pv, table, q, lens, count, slopes)
+    at = q.data_ptr()
+    if at % 16:
+        raise ValueError("q must be 16-byte aligned")
     if out is None:
-        out = q.new_empty((b, tokens, heads, hd))
-    elif out.dtype is not t or out.shape != q.shape or not out.is_contiguous() or out.get_device() != index or out.data_ptr() % 16:
-        raise ValueError(f"out must be contiguous, 16-byte aligned {t} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
-    elif _lib.overlap(out, q) and (out.data_ptr() != q.data_ptr() or not q.is_contiguous()):
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.dtype is not q.dtype or out.shape != shape or not out.is_contiguous() or out.get_device() != index or out.data_ptr() % 16:
+        raise ValueError(f"out must be contiguous, 16-byte aligned {q.dtype} {shape}, got {out.dtype} {tuple(out.shape)}")
+    elif _lib.overlap(out, q) and (out.data_ptr() != at or not q.is_contiguous()):
         raise ValueError("out must not share memory with q but for being it")
-    elif any(x is not None and _lib.overlap(out, x) for x in (pk, pv, table, lens, count, slopes)):
+    elif _lib.overlaps(out, (pk, pv, table, lens, count, slopes)):
         raise ValueError("out must not share memory with the pool, the table, lens, count or slopes")
-    need = _workspace_bytes(b, tokens, heads, h, hd, width)
-    ws = q.new_empty(need, dtype=torch.uint8) if need else None
-    a = _lib.PagedAttnArgs(_lib.DTYPES[t], q.data_ptr(), _S3(sb, st, sh), pk.data_ptr(), pv.data_ptr(), table.data_ptr(), stride,
-                           _index("lens", lens, b, index), None if count is None else _index("count", count, b, index),
-                           None if slopes is None else slopes.data_ptr(), b, tokens, heads, h, hd, pages, width, int(causal),
-                           hd ** -0.5 if scale is None else scale, softcap, out.data_ptr(), None if ws is None else ws.data_ptr(),
-                           need)
+    ws = q.new_empty(need // 2) if need else None
+    a = _lib.PagedAttnArgs(dtype, at, sq, pk.data_ptr(), pv.data_ptr(), table.data_ptr(), stride, lens.data_ptr(),
+                           None if count is None else count.data_ptr(), None if slopes is None else slopes.data_ptr(), *sizes, int(causal),
+                           shape[3] ** -0.5 if scale is None else scale, softcap, out.data_ptr(), None if ws is None else ws.data_ptr(), need)
     _lib.run_on(index, _lib.lib().fa_paged_attention, a, "fa_paged_attention")
     return out
