@@ -5,8 +5,8 @@
 // Two launches: h[m] = A_a x[m] (`rank` values a row), whose K is split over waves and workgroups, and the way back to N. Bound by
 // bytes: x, y and out once, each adapter in use once (from HBM; row tiles that share one meet it in the L2). Both products
 // run on the 16x16x32 MFMA in tiles of 16 rows: of each adapter that a tile's rows name, the product is taken of the whole tile and kept
-// for its own rows. So a prompt's tile costs one product, a tile of sixteen requests up to sixteen, and nothing of one
-// request's adapter, NaN included, reaches another one's rows.
+// for its own rows (up to rank 16, two of them with one reading of x). So a prompt's tile costs one product, a tile of sixteen requests
+// up to sixteen, and nothing of one request's adapter, NaN included, reaches another one's rows.
 //
 // Layout (laid out once): a[adapter][K / 8][rank][8] and b[adapter][rank / 8][N][8], so that the lanes of an MFMA operand find
 // their 8 inner elements side by side, 16 rank rows or 4 outputs in one run of memory.
@@ -17,6 +17,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/flashact_mi355x.h"
 #include "fa_device.h"
@@ -44,7 +45,9 @@ struct Params {
   const void* y;
   void* out;
   float* h;  // [split][M][rank]
-  int M, N, K, rank, adapters, splits, waves, share;  // share: workgroups that deal a tile's adapters among them
+  int M, N, K, rank, adapters, splits, waves;
+  bool runs;  // neighbouring tiles on one XCD
+  int share;  // workgroups that deal a tile's adapters among them
 };
 
 template <bool F16>
@@ -80,24 +83,36 @@ __global__ void __launch_bounds__(64 * shrink_waves(RT)) shrink_kernel(Params p)
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const int waves = blockDim.x >> 6;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
-  const int m0 = blockIdx.x * 16, split = blockIdx.y, K8 = p.K >> 3, nch = (p.K + 63) >> 6;
+  const int K8 = p.K >> 3, nch = (p.K + 63) >> 6;
+  // Neighbouring tiles, which mostly name the same adapter, on one XCD, where each has eight or more (1993 rows, K 16384, seven adapters: 41.4
+  // us with the way back, 37.5 so; five tiles of 70 rows 37.9 and 43.3).
+  const int tiles = (p.M + 15) >> 4, per = (tiles + 7) >> 3, at = blockIdx.x >> 3;
+  int split, tile;
+  if (p.runs) split = at / per, tile = (blockIdx.x & 7) * per + at - split * per;
+  else split = blockIdx.x / tiles, tile = blockIdx.x - split * tiles;
+  if (tile >= tiles) return;
+  const int m0 = tile * 16;
   // Runs of AHEAD chunks are dealt to the waves one by one, and each tile begins elsewhere: rows are often a power of two apart, and
   // tiles that walk through K side by side meet in the same memory channels.
   const int part = split * waves + wave, parts = p.splits * waves, turns = (nch + parts * AHEAD - 1) / (parts * AHEAD);
   unsigned char* stage = lds + wave * BYTES;
   const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)stage);
   const unsigned short* row = p.x + (int64_t)min(m0 + copy_row(lane), p.M - 1) * p.xs;
-  for_adapters<16>(p, m0, blockIdx.z, p.share, [&](int ad, uint64_t own) {
-    const unsigned short* a = p.a + (size_t)ad * K8 * p.rank * 8;
-    f32x4 acc[RT];
+  // Of one adapter, or of two with one reading of x (a prompt's end inside a tile would else take its workgroup twice as long as the others).
+  auto product = [&](auto two, int ad0, uint64_t own0, int ad1, uint64_t own1) {
+    constexpr int N = decltype(two)::value ? 2 : 1;
+    const unsigned short* a[2] = {p.a + (size_t)ad0 * K8 * p.rank * 8, p.a + (size_t)ad1 * K8 * p.rank * 8};
+    f32x4 acc[N][RT];
 #pragma unroll
-    for (int t = 0; t < RT; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int turn = blockIdx.x % turns;
+    for (int n = 0; n < N; n++)
+#pragma unroll
+      for (int t = 0; t < RT; t++) acc[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int turn = tile % turns;
     for (int i = 0; i < turns; i++) {
       const int c = (turn * parts + part) * AHEAD;
       turn = turn + 1 == turns ? 0 : turn + 1;
       if (c >= nch) continue;
-      u32x4 w[AHEAD][2][RT];
+      u32x4 w[AHEAD][2][N][RT];
 #pragma unroll
       for (int u = 0; u < AHEAD; u++)
 #pragma unroll
@@ -105,8 +120,10 @@ __global__ void __launch_bounds__(64 * shrink_waves(RT)) shrink_kernel(Params p)
           const int k8 = 8 * (c + u) + 4 * s;  // behind the end of K the last group, which meets zeros
           copy_to_lds(row + min(k8 + copy_chunk(lane), K8 - 1) * 8, to + (u * 2 + s) * 1024);
 #pragma unroll
-          for (int t = 0; t < RT; t++)
-            w[u][s][t] = *reinterpret_cast<const u32x4*>(a + ((size_t)min(k8 + q, K8 - 1) * p.rank + min(t * 16 + r, p.rank - 1)) * 8);
+          for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int t = 0; t < RT; t++)
+              w[u][s][n][t] = *reinterpret_cast<const u32x4*>(a[n] + ((size_t)min(k8 + q, K8 - 1) * p.rank + min(t * 16 + r, p.rank - 1)) * 8);
         }
       __builtin_amdgcn_s_waitcnt(0xf70);  // vmcnt(0)
       asm volatile("" ::: "memory");
@@ -117,26 +134,48 @@ __global__ void __launch_bounds__(64 * shrink_waves(RT)) shrink_kernel(Params p)
           u32x4 x = *reinterpret_cast<const u32x4*>(stage + (u * 2 + s) * 1024 + frag_slot(r, q));
           if (8 * (c + u) + 4 * s + q >= K8) x = u32x4{0, 0, 0, 0};
 #pragma unroll
-          for (int t = 0; t < RT; t++) acc[t] = mma<F16>(w[u][s][t], x, acc[t]);
+          for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int t = 0; t < RT; t++) acc[n][t] = mma<F16>(w[u][s][n][t], x, acc[n][t]);
         }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the next copies
     }
-    __syncthreads();
     float* sums = reinterpret_cast<float*>(lds);
 #pragma unroll
-    for (int t = 0; t < RT; t++)
-      *reinterpret_cast<f32x4*>(sums + wave * (BYTES / 4) + r * PITCH + t * 16 + 4 * q) = acc[t];
-    __syncthreads();
-    for (int e = threadIdx.x; e < 16 * p.rank; e += blockDim.x) {
-      const int m = e / p.rank, j = e - m * p.rank;
-      if (!(own >> m & 1)) continue;
-      float v = 0.f;
+    for (int n = 0; n < N; n++) {
+      const uint64_t own = n ? own1 : own0;
+      __syncthreads();
+#pragma unroll
+      for (int t = 0; t < RT; t++)
+        *reinterpret_cast<f32x4*>(sums + wave * (BYTES / 4) + r * PITCH + t * 16 + 4 * q) = acc[n][t];
+      __syncthreads();
+      for (int e = threadIdx.x; e < 16 * p.rank; e += blockDim.x) {
+        const int m = e / p.rank, j = e - m * p.rank;
+        if (!(own >> m & 1)) continue;
+        float v = 0.f;
 #pragma unroll 4
-      for (int w = 0; w < waves; w++) v += sums[w * (BYTES / 4) + m * PITCH + j];
-      p.h[((size_t)split * p.M + m0 + m) * p.rank + j] = v;
+        for (int w = 0; w < waves; w++) v += sums[w * (BYTES / 4) + m * PITCH + j];
+        p.h[((size_t)split * p.M + m0 + m) * p.rank + j] = v;
+      }
     }
     __syncthreads();
+  };
+  int first = -1;
+  uint64_t first_own = 0;
+  for_adapters<16>(p, m0, blockIdx.y, p.share, [&](int ad, uint64_t own) {
+    if constexpr (RT == 1) {  // by registers
+      if (first < 0) {
+        first = ad, first_own = own;
+        return;
+      }
+      product(std::true_type{}, first, first_own, ad, own);
+      first = -1;
+    } else {
+      product(std::false_type{}, ad, own, ad, own);
+    }
   });
+  if constexpr (RT == 1)
+    if (first >= 0) product(std::false_type{}, first, first_own, first, first_own);
 }
 
 template <int DT>
@@ -345,18 +384,29 @@ Cut cut(int M, int K, int rank) {
   return c;
 }
 
+// Workgroups that deal a tile's adapters among them, where all tiles have `workgroups`. Up to 64 rows are tokens of as many requests; more may
+// be those or prompts, of whose tiles most name one adapter: as many as leave no more than 256 in all. (N and K 2048, rank 16, rows of
+// three neighbours an adapter: 70 rows 18.7 us with one, 8.9 so; 300 30.7 and 17.0; 1000 35.5 and 30.8; prompts of 70, 300 and 1000 rows 8.4, 10.2
+// and 13.3 both ways, 8.5, 12.4 and 19.1 with up to 512. Gated, 300 rows to N 32768, 20.5; 50 with more than one there.)
+int share_of(const Params& p, int64_t workgroups) {
+  if (p.M <= 64) return std::min({16, p.M, p.adapters});
+  return (int)std::min<int64_t>({16, p.adapters, std::max<int64_t>(1, 256 / workgroups)});
+}
+
 template <bool F16, int RT>
-int launch_shrink(const Params& p, hipStream_t s) {
+int launch_shrink(Params p, hipStream_t s) {
+  p.share = share_of(p, (int64_t)((p.M + 15) / 16) * p.splits);
   const int rc = host::allow_lds(reinterpret_cast<const void*>(&shrink_kernel<F16, RT>), shrink_waves(RT) * shrink_bytes(RT), "fa_lora_add");
   if (rc != FA_OK) return rc;
-  hipLaunchKernelGGL((shrink_kernel<F16, RT>), dim3((p.M + 15) / 16, p.splits, p.share), dim3(64 * p.waves), p.waves * shrink_bytes(RT), s,
+  hipLaunchKernelGGL((shrink_kernel<F16, RT>), dim3((p.runs ? (p.M + 127) / 128 * 8 : (p.M + 15) / 16) * p.splits, p.share), dim3(64 * p.waves), p.waves * shrink_bytes(RT), s,
                      p);
   return FA_OK;
 }
 
 template <bool F16, int PARTS, int RANK8, int YT, bool GATE>
-void launch_expand(const Params& p, bool quads, hipStream_t s) {
+void launch_expand(Params p, bool quads, hipStream_t s) {
   const int blocks = (p.N + 64 * W - 1) / (64 * W);
+  p.share = share_of(p, (int64_t)blocks * (p.M > 256 ? (p.M + 31) / 32 : (p.M + 15) / 16));
   if (p.M > 256) {
     const dim3 grid(blocks, (p.M + 31) / 32, p.share);
     if (quads) hipLaunchKernelGGL((expand_kernel<F16, PARTS, RANK8, 2, YT, GATE, true>), grid, dim3(64 * W), 0, s, p);
@@ -369,7 +419,7 @@ void launch_expand(const Params& p, bool quads, hipStream_t s) {
 }
 
 template <bool F16, int RANK8>
-void launch_expand(const Params& p, int yt, bool gate, bool quads, hipStream_t s) {
+void launch_expand(Params p, int yt, bool gate, bool quads, hipStream_t s) {
   constexpr int XT = F16 ? FA_DTYPE_F16 : FA_DTYPE_BF16;
   if (yt == FA_DTYPE_F32) {
     if (gate) launch_expand<F16, 2, RANK8, FA_DTYPE_F32, true>(p, quads, s);
@@ -440,8 +490,7 @@ extern "C" int fa_lora_add(const fa_lora_args* a, fa_stream_t stream) {
   const lora::Cut cut = lora::cut(a->rows, a->k, a->rank);
   lora::Params p{static_cast<const unsigned short*>(a->x), a->x_stride, static_cast<const unsigned short*>(a->a),
                  static_cast<const unsigned short*>(a->b), a->scale, a->index, a->y, a->out, static_cast<float*>(a->workspace),
-                 a->rows, a->n, a->k, a->rank, a->adapters, cut.splits, cut.waves,
-                 a->rows > 64 ? 1 : std::min({16, a->rows, a->adapters})};
+                 a->rows, a->n, a->k, a->rank, a->adapters, cut.splits, cut.waves, (a->rows + 15) / 16 >= 64, 1};
   const bool quads = a->n % 4 == 0 && reinterpret_cast<uintptr_t>(a->y) % (4 * yb) == 0 &&
                      reinterpret_cast<uintptr_t>(a->out) % (a->gate ? 4 : 4 * ob) == 0;
   rc = a->dtype == FA_DTYPE_F16 ? lora::launch<true>(p, a->y_dtype, a->gate, quads, (hipStream_t)stream)
