@@ -38,6 +38,9 @@ int check_gfx950(const char* who);
 // Raises a kernel's dynamic-LDS limit to `lds_bytes` (once per device and kernel).
 int allow_lds(const void* kernel, unsigned lds_bytes, const char* who);
 
+// Workgroups of 256 threads in one dimension of a grid: a launch has less than 2^32 threads in each.
+constexpr long long MAX_GRID = (1ll << 24) - 1;
+
 // 64 bits that no other launch of this process has and that memory does not hold by chance; never 0.
 uint64_t launch_nonce();
 

@@ -460,7 +460,7 @@ extern "C" int fa_lora_add(const fa_lora_args* a, fa_stream_t stream) {
     return host::fail(FA_ERR_INVALID_ARG, "%s: dtype %d: x and the adapters are bf16 or fp16", who, a->dtype);
   if (a->y_dtype != FA_DTYPE_F32 && a->y_dtype != a->dtype)
     return host::fail(FA_ERR_INVALID_ARG, "%s: y_dtype %d: y is fp32 or of x's type", who, a->y_dtype);
-  if (a->rows < 0 || a->rows > (1 << 24)) return host::fail(FA_ERR_INVALID_ARG, "%s: rows=%d outside [0, 2^24]", who, a->rows);
+  if (a->rows < 0 || a->rows > (1 << 20)) return host::fail(FA_ERR_INVALID_ARG, "%s: rows=%d outside [0, 2^20]", who, a->rows);
   if (a->n < 1 || a->k < 8 || a->k % 8 || a->n > (1 << 24) || a->k > (1 << 24))
     return host::fail(FA_ERR_INVALID_ARG, "%s: need 1 <= n, k <= 2^24 and k a multiple of 8, got n=%d k=%d", who, a->n, a->k);
   if (a->rank < 8 || a->rank > lora::MAX_RANK || a->rank % 8)

@@ -389,7 +389,7 @@ int set_up(Args& p, const A* a, int blocks, int splits, int tiles, const char* w
 inline unsigned grid_of(const Args& a) {
   const int runs = (a.RU + a.RC - 1) / a.RC;
   const int64_t grid = ((int64_t)a.B * a.H * a.S * runs + 7) / 8 * 8 * a.RC;
-  return grid > 0x7fffffff ? 0 : (unsigned)grid;
+  return grid > host::MAX_GRID ? 0 : (unsigned)grid;
 }
 
 }  // namespace newest

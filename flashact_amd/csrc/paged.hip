@@ -219,7 +219,7 @@ int set_up(RowArgs& p, const fa_paged_rows_args* a, bool append, const char* who
   if (a->dtype != FA_DTYPE_BF16 && a->dtype != FA_DTYPE_F16)
     return host::fail(FA_ERR_INVALID_ARG, "%s: dtype %d: rows and pages are bf16 or fp16", who, a->dtype);
   if (a->tokens < 0 || a->tokens > (1 << 30)) return host::fail(FA_ERR_INVALID_ARG, "%s: tokens=%d", who, a->tokens);
-  if (!a->k || !a->v || (append ? !a->start : !a->count)) return host::fail(FA_ERR_INVALID_ARG, "%s: a pointer is NULL", who);
+  if (a->tokens && (!a->k || !a->v || (append ? !a->start : !a->count))) return host::fail(FA_ERR_INVALID_ARG, "%s: a pointer is NULL", who);
   const unsigned align = append ? 16 : 2;
   if (reinterpret_cast<uintptr_t>(a->k) % align || reinterpret_cast<uintptr_t>(a->v) % align)
     return host::fail(FA_ERR_INVALID_ARG, "%s: k or v is not %u-byte aligned", who, align);
@@ -263,7 +263,7 @@ extern "C" int fa_paged_append(const fa_paged_rows_args* a, fa_stream_t stream) 
   if (a->tokens == 0) return FA_OK;
   const int win = a->tokens >= 8 ? 8 : 1;
   p.windows = (a->tokens + win - 2) / win + 1;  // of any alignment
-  if ((int64_t)p.windows * a->batch > 0x7fffffff) return host::fail(FA_ERR_INVALID_ARG, "%s: too many rows for one call", who);
+  if ((int64_t)p.windows * a->batch > host::MAX_GRID) return host::fail(FA_ERR_INVALID_ARG, "%s: too many rows for one call", who);
   rc = host::check_gfx950(who);
   if (rc != FA_OK) return rc;
   // Workgroups of a window: a thread has up to three pieces (four prompts of 2011 tokens, 16 and 4 heads of 128 dims: 27.4 us in one
@@ -292,7 +292,7 @@ extern "C" int fa_paged_load(const fa_paged_rows_args* a, fa_stream_t stream) {
   if (a->tokens == 0) return FA_OK;
   p.windows = (a->tokens + paged::PT - 1) / paged::PT;
   const int64_t grid = (int64_t)p.windows * p.B * p.H;
-  if (grid > 0x7fffffff) return host::fail(FA_ERR_INVALID_ARG, "%s: too many rows for one call", who);
+  if (grid > host::MAX_GRID) return host::fail(FA_ERR_INVALID_ARG, "%s: too many rows for one call", who);
   rc = host::check_gfx950(who);
   if (rc != FA_OK) return rc;
   auto whole = [](const long long* s, int one, int x, int y, int z, const void* at) {

@@ -426,8 +426,8 @@ extern "C" int fa_token_logprobs(const fa_token_logprobs_args* a, fa_stream_t st
   if (!a) return host::fail(FA_ERR_INVALID_ARG, "%s: args is NULL", who);
   if (a->dtype != FA_DTYPE_BF16 && a->dtype != FA_DTYPE_F16 && a->dtype != FA_DTYPE_F32)
     return host::fail(FA_ERR_INVALID_ARG, "%s: dtype %d: logits are bf16, fp16 or fp32", who, a->dtype);
-  if (a->rows < 0 || a->rows > (1 << 24) || a->vocabulary < 1 || a->vocabulary > (1 << 30))
-    return host::fail(FA_ERR_INVALID_ARG, "%s: rows=%d outside [0, 2^24] or vocabulary=%d outside [1, 2^30]", who, a->rows, a->vocabulary);
+  if (a->rows < 0 || a->rows > (1 << 20) || a->vocabulary < 1 || a->vocabulary > (1 << 30))
+    return host::fail(FA_ERR_INVALID_ARG, "%s: rows=%d outside [0, 2^20] or vocabulary=%d outside [1, 2^30]", who, a->rows, a->vocabulary);
   if (a->top < 0 || a->top > FA_TOKENS_MAX_TOP || a->top > a->vocabulary)
     return host::fail(FA_ERR_INVALID_ARG, "%s: top=%d outside [0, %d] or more than the vocabulary of %d", who, a->top, FA_TOKENS_MAX_TOP,
                       a->vocabulary);

@@ -282,7 +282,7 @@ def extend(weights: list, ln_in, ln_post, x, caches: list, lens, count=None, *, 
     count = room if count is None else torch.minimum(count, room).clamp(min=0)
     after = lens + count
     x = x.reshape(B * T, D)
-    if index is not None and T > 1:
+    if index is not None and T != 1:
         index = index.repeat_interleave(T)
 
     def project(l, name, h, residual=None):
@@ -333,5 +333,5 @@ def answer(head, ln_final, x, tokens=None, *, top: int = 1, scale: float = 1.0):
     given = tokens
     if tokens is None:
         tokens = torch.zeros(x.shape[:-1], dtype=torch.int32, device=x.device)
-    r = _tokens.logprobs(logits.view(*x.shape[:-1], -1), tokens, top=top, scale=scale)
+    r = _tokens.logprobs(logits.view(*x.shape[:-1], logits.shape[-1]), tokens, top=top, scale=scale)
     return r if given is not None else r._replace(logprob=r.top_logprobs[..., 0])

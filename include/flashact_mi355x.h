@@ -468,7 +468,7 @@ int fa_paged_attention(const fa_paged_attn_args* args, fa_stream_t stream);
 size_t fa_paged_attention_workspace_bytes(int batch, int tokens, int heads, int kv_heads, int head_dim, int table_pages);
 
 /* ---------------------------------------------------------------- low-rank adapters of many requests
- * out[m] = y[m] + scale[i] b_i (a_i x[m]), i = index[m] (outside [0, adapters): out[m] = y[m]), m < rows. a_i [rank][k] and b_i [n][rank]
+ * out[m] = y[m] + scale[i] b_i (a_i x[m]), i = index[m] (outside [0, adapters): out[m] = y[m]), m < rows <= 2^20. a_i [rank][k] and b_i [n][rank]
  * are x's type, bf16 or fp16, finite, k and rank multiples of 8, rank <= 128 (adapters of lower rank are padded with zeros), laid out as
  *   a [adapters][k / 8][rank][8] and b [adapters][rank / 8][n][8], 16-byte aligned; scale [adapters] fp32.
  * x [rows][k] with a row stride of x_stride elements (a multiple of 8), 16-byte aligned; y and out [rows][n] contiguous, fp32 or x's type;

@@ -39,3 +39,14 @@ def test_answers_that_are_refused():
                           (dict(head=head.float()), ValueError, "head"), (dict(head=head[:, :8]), ValueError, "head"), (dict(top=0), ValueError, "top")):
         with pytest.raises(err, match=text):
             prefill.answer(**{"head": head, "ln_final": ln, "x": x, **kw})
+
+
+def test_entries_refuse_more_rows_than_a_grid_has():
+    import ctypes
+    from flashact_amd import _lib
+    from tests import test_lora, test_tokens
+    lib = _lib.lib()
+    assert lib.fa_lora_add(ctypes.byref(test_lora._args(rows=(1 << 20) + 1, workspace_bytes=1 << 50)), None) == 1
+    assert "2^20" in lib.fa_last_error().decode()
+    assert lib.fa_token_logprobs(ctypes.byref(test_tokens._args(rows=(1 << 20) + 1, workspace_bytes=1 << 50)), None) == 1
+    assert "2^20" in lib.fa_last_error().decode()
