@@ -304,6 +304,7 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : HD == 128 || MB > 1 ? 
   if (!here.there) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Span sp = newest::span_of(a, here.b);
+  if (here.split > 0 && here.split >= newest::splits_used(a, (sp.len + BT - 1) / BT)) return;  // of a short sample: 48 of 1 to 8192 keys 34.4 us, 32.8 so
   Tile<F16, HD, CAP, BIAS> tile[MB];
   int hi = 0;
 #pragma unroll
