@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a) {
 // over 1024, 16 / 4, 96, on this side of it, 66 and 69.) 256 dims do not fit into the registers twice.
 int tiles_for(int batch, int tokens, int heads, int kv_heads, int hd, int pages) {
   const int64_t rt = ((int64_t)tokens * (heads / kv_heads) + 15) / 16;
-  return hd <= 128 && rt >= 8 && rt * batch * kv_heads * pages >= 65536 ? 2 : 1;
+  return hd <= 128 && rt >= 8 && (double)rt * batch * kv_heads * pages >= 65536.0 ? 2 : 1;  // (past 64 bits at the limits)
 }
 
 // A wave takes about 2.3 us for a page of 256 dims (1.2 of 128 and less); more than one workgroup a CU (two) share its bandwidth. That
