@@ -11,8 +11,8 @@
 // threads whose maximum reaches it read their values again, those that do are put side by side, and each counts how many are before it.
 // Where ties leave too many (a row of equal values), the k-th largest value is found exactly by four counts of eight bits
 // over the whole row, and equal ones are taken in the row's order.
-// (Sorted lists kept by each wave during the pass, with insertions one by one, took 16 us instead of 9 for 8 of 262144 bf16 logits, and
-// 35 instead of 14 for 20 of 48 rows of 99991: every step from a comparison to a scalar and back costs some 50 cycles.)
+// (Sorted lists kept by each wave during the pass, with insertions one by one, took 16 us instead of 9.5 for 8 of 262144 bf16 logits, and
+// 35 instead of 17.6 for 20 of 48 rows of 99991: every step from a comparison to a scalar and back costs some 50 cycles.)
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
