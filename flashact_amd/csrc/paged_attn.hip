@@ -45,9 +45,10 @@ struct AttnArgs : newest::Args {
   int pages;
 };
 
+constexpr float FAR = 4194304.f;  // from here on numbers are half a unit and more apart
 template <bool F16>
 __device__ __forceinline__ float reference(float top) {
-  return fabsf(top) < 4194304.f ? top + (F16 ? -15.f : 17.f) : top;  // past 2^22 the difference would round
+  return fabsf(top) < FAR ? top + (F16 ? -15.f : 17.f) : top;  // past it the difference would round
 }
 template <bool F16>
 __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
@@ -74,6 +75,7 @@ struct Tile {
   static constexpr int KS = HD / 32, NT = HD / 16;
   int pos, limit, lo, hi;  // keys that the row sees, that every row does (those that are not there do not count), that any does
   float slope, m, l;       // m: the weights' reference; l: their sum over this lane's keys
+  uint64_t far;            // lanes of rows whose reference is past FAR
   u32x4 q[KS];
   f32x4 O[NT];
 
@@ -98,7 +100,7 @@ struct Tile {
         q[i] = *reinterpret_cast<const u32x4*>(a.q + (at.b * a.qb + t * a.qt + head * a.qh + 32 * i + 8 * (lane >> 4)) * 2);
     }
     slope = BIAS && valid ? a.slopes[head] * newest::LOG2E : 0.f;
-    m = -INFINITY, l = 0.f;
+    m = -INFINITY, l = 0.f, far = 0;
 #pragma unroll
     for (int j = 0; j < NT; j++) O[j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -135,13 +137,33 @@ struct Tile {
       mx = newest::scores<CAP, BIAS>(a, s, 1.f, key0, mixed, own, slope, pos);
     }
     const float mn = fmaxf(m, reference<F16>(cols_max(mx)));
-    const float ms = mn == -INFINITY ? 0.f : mn;
-    if (__builtin_amdgcn_ballot_w64(mn != m)) {
+    float ms = mn == -INFINITY ? 0.f : mn;
+    if (__builtin_amdgcn_ballot_w64(mn != m) | far) {
       const float al = exp2_w(m - ms);  // 0 where there was nothing yet
       l *= al;
 #pragma unroll
       for (int j = 0; j < NT; j++) O[j] *= al;
       m = mn;
+      // The reference is a rounded product, and what the rounding took off stands in the fused exponents below: up to 2^6 at 2^30, where the
+      // largest weight would vanish or overflow. Of rows past FAR (each by itself: another's scores do not change its roundings) s
+      // becomes the difference of rounded products, 0 for the largest, in units of f. (The test makes pieces of prompts 1 to 4 % longer; no
+      // test here and a second walk over the pages of waves that met such a row cost as much, as the compiler lays it out.)
+      if constexpr (!CAP && !BIAS) {
+        const bool own = fabsf(ms) >= FAR;
+        far = __builtin_amdgcn_ballot_w64(own);
+        if (__builtin_expect(far != 0, 0)) {
+          const float unit = 1.f / f;
+#pragma unroll
+          for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              float product = s[x][i] * f;
+              asm volatile("" : "+v"(product));  // not to be fused with the difference
+              s[x][i] = own ? (product - ms) * unit : s[x][i];
+            }
+          ms = own ? 0.f : ms;
+        }
+      }
     }
 #pragma unroll
     for (int x = 0; x < 2; x++) {
