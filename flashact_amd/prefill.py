@@ -230,8 +230,10 @@ def prefill_packed(packed: dict, ln_in, ln_post, x, lengths, caches: list, prefi
         doc = torch.repeat_interleave(torch.arange(samples + 1, device=dev), torch.tensor(lengths + [T - sum(lengths)], device=dev), output_size=T)
         index = torch.cat([index, index.new_full((1,), -1)])[doc]
 
-    def project(l, name, h):
+    def project(l, name, h, residual=None):
         y = h @ packed[name][l].t()
+        if residual is not None:  # the adapter's sum goes onto the fp32 one, without a rounding to bf16 of its own
+            y = y.float().add_(residual)
         return lora.add(y, h, banks[l][name], index, out=y) if name in banks[l] else y
 
     for l in range(layers):
@@ -243,14 +245,14 @@ def prefill_packed(packed: dict, ln_in, ln_post, x, lengths, caches: list, prefi
             elif n:
                 paged.append(caches[l], table[b:b + 1], k[None, at[b]:at[b] + n], v[None, at[b]:at[b] + n], zero)
         o = attention.attend(q[None], k[None], v[None], spans)
-        x = x + project(l, "wo", o.view(T, H * HD)).float()
+        x = project(l, "wo", o.view(T, H * HD), x)
         h = _norm(x, ln_post[l])
         if "wgu" in banks[l]:
             h = lora.add(h @ packed["wgu"][l].t(), h, banks[l]["wgu"], index, gate="gelu")
         else:
             y = (h @ packed["wgu"][l].t()).unflatten(-1, (F, 2)).float()
             h = (torch.nn.functional.gelu(y[..., 0], approximate="tanh") * y[..., 1]).to(torch.bfloat16)
-        x = x + project(l, "wdn", h).float()
+        x = project(l, "wdn", h, x)
     return x
 
 
