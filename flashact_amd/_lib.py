@@ -291,6 +291,11 @@ def _layout(shape, stride) -> tuple:
     return reach + 1, twice
 
 
+def extent(lay) -> int:
+    """Elements from the first to behind the last of a ``layout``."""
+    return _layout(lay[1], lay[2])[0]
+
+
 def overlap(a, b) -> bool:
     """Whether two tensors' memory ranges meet."""
     at, bt, na, nb = a.data_ptr(), b.data_ptr(), _layout(a.shape, a.stride())[0], _layout(b.shape, b.stride())[0]

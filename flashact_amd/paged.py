@@ -111,7 +111,8 @@ def _on_one(*tensors) -> int:
 
 @functools.lru_cache(maxsize=1024)
 def _append_of(pk, pv, table, k, v, q, start, count, freqs):
-    """(strides of q, k and v, the table's row stride, the struct's type and last sizes) of layouts, checked."""
+    """(strides of q, k and v, the table's row stride, the struct's type and last sizes, the bytes from the first to behind the last
+    element of one of the pool's tensors, of k, v and q) of layouts, checked."""
     pages, h, hd, b, width, stride = _pool_of(pk, pv, table)
     tokens = _rows_of(pk[0], k, v, b, h, hd)
     sk, sv, sq, heads = _steps("k", k), _steps("v", v), (0, 0, 0), 0
@@ -128,7 +129,8 @@ def _append_of(pk, pv, table, k, v, q, start, count, freqs):
         rotary = 2 * freqs[1][0] if len(freqs[1]) == 1 else -1
         if freqs[0] is not torch.float64 or not 0 < rotary <= hd or rotary % 16 or not _lib.contiguous(freqs):
             raise ValueError(f"freqs must be contiguous float64 [a multiple of 8 up to {hd // 2}], got {freqs[0]} {tuple(freqs[1])}")
-    return _S3(*sq), _S4(*sk, 1), _S4(*sv, 1), stride, _lib.DTYPES[pk[0]], (b, tokens, heads, h, hd, pages, width, rotary)
+    reach = tuple(0 if x is None else 2 * _lib.extent(x) for x in (pk, k, v, q))
+    return _S3(*sq), _S4(*sk, 1), _S4(*sv, 1), stride, _lib.DTYPES[pk[0]], (b, tokens, heads, h, hd, pages, width, rotary), reach
 
 
 def append(pool: dict, table, k, v, start, count=None, *, q=None, freqs=None, adjacent: bool = False):
@@ -140,20 +142,26 @@ def append(pool: dict, table, k, v, start, count=None, *, q=None, freqs=None, ad
     angles (start[b] + i) freqs[j] on the way, taken in 64 bits; None: nothing is turned. The pairs are dims (j, j + len(freqs)), or
     (2 j, 2 j + 1) with `adjacent` (the packing of ``prefill.pack_backbone``), and become dims (j, j + len(freqs)) in either
     case. Rows behind the table's end or of no page are dropped, as is a sample with a negative start. The result [B][T][H][hd]
-    has zeros where a row is not real. Two rows at one token of one page must be ordered by the caller; rows and pool share no memory.
+    has zeros where a row is not real. Two rows at one token of one page must be ordered by the caller. k, v and q share no memory with the
+    pool.
     """
     pk, pv = pool["k"], pool["v"]
     lay = _lib.layout
-    sq, sk, sv, stride, dtype, sizes = _append_of(lay(pk), lay(pv), lay(table), lay(k), lay(v), None if q is None else lay(q), lay(start),
-                                                  None if count is None else lay(count), None if freqs is None else lay(freqs))
-    index = _on_one(pk, pv, table, k, v, start, count, q, freqs)
-    at_k, at_v, at_q, out, at_out = k.data_ptr(), v.data_ptr(), None, None, None
-    if q is not None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        at_q, at_out = q.data_ptr(), out.data_ptr()
+    sq, sk, sv, stride, dtype, sizes, reach = _append_of(lay(pk), lay(pv), lay(table), lay(k), lay(v), None if q is None else lay(q),
+                                                         lay(start), None if count is None else lay(count), None if freqs is None else lay(freqs))
+    at_k, at_v, at_q, out, at_out = k.data_ptr(), v.data_ptr(), None if q is None else q.data_ptr(), None, None
+    to_k, to_v = pk.data_ptr(), pv.data_ptr()
+    whole, *rows = reach
+    for at, n in zip((at_k, at_v, at_q or 0), rows):
+        if n and (at - whole < to_k < at + n or at - whole < to_v < at + n):
+            raise ValueError("k, v and q must not share memory with the pool")
     if (at_k | at_v | (at_q or 0)) % 16:
         raise ValueError("k, v and q must be 16-byte aligned")
-    a = _lib.PagedRowsArgs(dtype, at_q, sq, at_out, at_k, sk, at_v, sv, pk.data_ptr(), pv.data_ptr(), table.data_ptr(), stride,
+    index = _on_one(pk, pv, table, k, v, start, count, q, freqs)
+    if q is not None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        at_out = out.data_ptr()
+    a = _lib.PagedRowsArgs(dtype, at_q, sq, at_out, at_k, sk, at_v, sv, to_k, to_v, table.data_ptr(), stride,
                            start.data_ptr(), None if count is None else count.data_ptr(), None if freqs is None else freqs.data_ptr(),
                            *sizes, int(adjacent), 0)
     _lib.run_on(index, _lib.lib().fa_paged_append, a, "fa_paged_append")
