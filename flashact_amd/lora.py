@@ -74,6 +74,8 @@ def _add_of(y, x, a, b, scale, index, gate):
     rows = sx[0] if len(sx) == 2 else -1
     if rows < 0 or sx[1] != k or y[1] != (rows, n) or index[1] != (rows,):
         raise ValueError(f"x must be [rows][K={k}], y [rows][N={n}] and index [rows], got {tuple(sx)}, {tuple(y[1])} and {tuple(index[1])}")
+    if max(n, k) > 1 << 24 or rows > 1 << 20:
+        raise ValueError(f"N={n} and K={k} must be at most 2^24 and rows={rows} at most 2^20")
     if index[0] is not torch.int32 or not _lib.contiguous(index) or not _lib.contiguous(y):
         raise ValueError(f"index must be contiguous int32 and y contiguous, got {index[0]} and strides {y[2]}")
     if gate is not None and (gate != "gelu" or n % 2):
@@ -111,7 +113,7 @@ def add(y: torch.Tensor, x: torch.Tensor, bank: dict, index: torch.Tensor, *, ga
         raise ValueError("out must not share memory with y but for being it, without a gate")
     elif _lib.overlaps(out, (x, a, b, scale, index)):
         raise ValueError("out must not share memory with x, index or the bank")
-    if not need:
+    if not sizes[0]:
         return out
     ws = x.new_empty(need // 2)
     args = _lib.LoraArgs(*dtype, at, stride, a.data_ptr(), b.data_ptr(), scale.data_ptr(), index.data_ptr(), *sizes, y.data_ptr(),
