@@ -291,6 +291,13 @@ def _layout(shape, stride) -> tuple:
     return reach + 1, twice
 
 
+def ints(*sizes) -> tuple:
+    """Sizes that the C structs hold as int, checked: ctypes would cut larger ones off."""
+    if max(sizes) >= 1 << 31:
+        raise ValueError(f"sizes {sizes} must be below 2^31")
+    return sizes
+
+
 def extent(lay) -> int:
     """Elements from the first to behind the last of a ``layout``."""
     return _layout(lay[1], lay[2])[0]

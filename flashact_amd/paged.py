@@ -72,7 +72,7 @@ def _pool_of(k, v, table):
     stride = tst[0] if b > 1 else width
     if stride < width:
         raise ValueError(f"the table's rows overlap: {tuple(ts)} with strides {tst}")
-    return pages, h, hd, b, width, stride
+    return *_lib.ints(pages, h, hd, b, width), stride
 
 
 def _rows_of(t, k, v, b, h, hd) -> int:
@@ -82,7 +82,7 @@ def _rows_of(t, k, v, b, h, hd) -> int:
     shape = k[1]
     if len(shape) != 4 or shape[0] != b or shape[2] != h or shape[3] != hd or v[1] != shape:
         raise ValueError(f"k and v must be [{b}][tokens][{h}][{hd}], got {tuple(shape)} and {tuple(v[1])}")
-    return shape[1]
+    return _lib.ints(shape[1])[0]
 
 
 def _steps(name, lay) -> tuple:
@@ -121,7 +121,7 @@ def _append_of(pk, pv, table, k, v, q, start, count, freqs):
             raise TypeError(f"q must be {pk[0]} like the pool, got {q[0]}")
         if len(q[1]) != 4 or q[1][0] != b or q[1][1] != tokens or q[1][2] < 1 or q[1][3] != hd:
             raise ValueError(f"q must be [{b}][{tokens}][heads][{hd}], got {tuple(q[1])}")
-        sq, heads = _steps("q", q), q[1][2]
+        sq, heads = _steps("q", q), _lib.ints(q[1][2])[0]
     _per_sample("start", start, b)
     _per_sample("count", count, b)
     rotary = 0
@@ -212,8 +212,9 @@ def _attend_of(pk, pv, table, q, lens, count, slopes):
     _per_sample("count", count, b)
     if slopes is not None and (slopes[0] is not _F32 or slopes[1] != (shape[2],) or not _lib.contiguous(slopes)):
         raise ValueError(f"slopes must be contiguous float32 [{shape[2]}], got {slopes[0]} {tuple(slopes[1])}")
+    sizes = _lib.ints(b, shape[1], shape[2], h, hd, pages, width)
     need = _workspace_bytes(b, shape[1], shape[2], h, hd, width)
-    return tuple(shape), _S3(*steps), stride, _lib.DTYPES[t], (b, shape[1], shape[2], h, hd, pages, width), need
+    return tuple(shape), _S3(*steps), stride, _lib.DTYPES[t], sizes, need
 
 
 def attend(q, pool: dict, table, lens, *, count=None, scale=None, softcap: float = 0.0, slopes=None, causal: bool = True,

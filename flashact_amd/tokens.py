@@ -46,6 +46,8 @@ def _logprobs_of(logits, tokens, top):
     if vocabulary < 1 or logits[2][-1] != 1 or not _lib.contiguous(tokens):
         raise ValueError(f"logits must have contiguous rows that are not empty and tokens be contiguous, got {tuple(logits[1])} with "
                          f"strides {logits[2]} and {tokens[2]}")
+    if rows > 1 << 20 or vocabulary > 1 << 30:
+        raise ValueError(f"rows={rows} must be at most 2^20 and the vocabulary of {vocabulary} at most 2^30")
     if not 0 <= top <= min(MAX_TOP, vocabulary):
         raise ValueError(f"top must be in [0, {min(MAX_TOP, vocabulary)}], got {top}")
     return (t, logits[2][0] if dim == 2 else vocabulary, int(tokens[0] is torch.int64), rows, vocabulary,
