@@ -384,13 +384,15 @@ Cut cut(int M, int K, int rank) {
   return c;
 }
 
-// Workgroups that deal a tile's adapters among them, where all tiles have `workgroups`. Up to 64 rows are tokens of as many requests; more may
-// be those or prompts, of whose tiles most name one adapter: as many as leave no more than 256 in all. (N and K 2048, rank 16, rows of
+// Workgroups that deal a tile's adapters among them, where all tiles have `workgroups`. Up to 64 rows are tokens of as many requests, or a
+// prompt: as many as leave no more than 1024 in all, those without an adapter among them (gated, N 32768, K 2048, rank 32, a bank of 16, us with
+// up to 1024 and with one for each: 64 rows of one adapter 12.5 and 31.2, of 16 19.2 and 37.4; 16 rows of one 9.9 and 12.4, of 16 17.3 and 21.0;
+// up to 256 takes 8.6 to 19.9 there, and for 5 rows of 5 11.9 instead of 10.8). More may be those or prompts, of whose tiles most name one
+// adapter: no more than 256. (N and K 2048, rank 16, rows of
 // three neighbours an adapter: 70 rows 18.7 us with one, 8.9 so; 300 30.7 and 17.0; 1000 35.5 and 30.8; prompts of 70, 300 and 1000 rows 8.4, 10.2
 // and 13.3 both ways, 8.5, 12.4 and 19.1 with up to 512. Gated, 300 rows to N 32768, 20.5; 50 with more than one there.)
 int share_of(const Params& p, int64_t workgroups) {
-  if (p.M <= 64) return std::min({16, p.M, p.adapters});
-  return (int)std::min<int64_t>({16, p.adapters, std::max<int64_t>(1, 256 / workgroups)});
+  return (int)std::min<int64_t>({16, p.M, p.adapters, std::max<int64_t>(1, (p.M <= 64 ? 1024 : 256) / workgroups)});
 }
 
 template <bool F16, int RT>
