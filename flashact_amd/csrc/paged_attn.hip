@@ -16,9 +16,12 @@
 // heads over 8192 keys 306, and 242 with two tiles a wave).
 //
 // Rounding: scores are exact products summed in fp32, softmax and sums are fp32. bf16: the weights go into the second
-// product as two bf16 (2^-16 of each is lost; its MFMAs are not the bound), and are taken against a reference 2^17 above
+// product as two bf16 (2^-16 of each is lost; as one, 2^-9), and are taken against a reference 2^17 above
 // the maximum, so that 131072 keys cannot leave the fp32 range whatever the values. fp16: the weights are rounded once (2^-12), against a
-// reference 2^15 below the maximum: those above 2^-29 of the largest keep all their bits.
+// reference 2^15 below the maximum: those above 2^-29 of the largest keep all their bits. The result's own rounding is 2^-12 as well: of
+// the 2-norm 1.8e-4 to 2.1e-4 are off by it alone, 2.0e-4 to 2.6e-4 with the weights'. A second part takes its time in pieces of prompts, whose
+// MFMAs count: 1024 tokens over 8192 keys 245 us in bf16, 220 in fp16; in fp16 with two parts 293 tokens over up to 4011 keys 37.4 -> 40.8 us,
+// 4 x 256 of 256 dims over 4096 137 -> 146, 48 single tokens over up to 8192 28.7 -> 28.8, capped and biased 29.0 -> 30.0.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -400,8 +403,10 @@ int tiles_for(int batch, int tokens, int heads, int kv_heads, int hd, int pages)
 
 // A wave takes about 2.3 us for a page of 256 dims (1.2 of 128 and less); more than one workgroup a CU (two) share its bandwidth. That
 // is for samples that fill their tables. Where one tile of rows is all there is (single tokens), samples are of any age, and a
-// full one that takes few splits is waited for: up to 8 splits of 4 pages a wave or more. (48 samples of 1 to 8192 tokens, 4 K/V
-// heads of 128 dims, 3 splits by the estimate: 43 us, 8: 33, 16: 32.5; 48 of 4096 each 75, 78 and 79; of 983 24 all three.)
+// full one that takes few splits is waited for: up to 8 splits of 4 pages a wave or more. (Samples of 1 to 8192 tokens by the estimate and so, then
+// of 4096 each, us; samples x K/V heads, 4 of 128 dims: 384 64 and 47, 141 and 153; 256 74 and 37, 96 and 103; 192 38 and 29, 75 and 79; 128
+// 28.6 and 21.5, 52 and 54; 256 dims: 64 42 and 33, 54 and 59; 48 36 and 27, 44 and 49. Past 64, where shorter samples are enough to fill the
+// chip, the one gains more than the other loses; 32 and fewer take as many by the estimate. 16 splits for 192 32.5 instead of 33.)
 int splits_for(int batch, int tokens, int heads, int kv_heads, int hd, int pages) {
   const int tiles = tiles_for(batch, tokens, heads, kv_heads, hd, pages);
   if (tiles > 1)
