@@ -12,7 +12,7 @@
 // Keys and values of the next tiles are copied to LDS (no registers) while this one is worked on, one barrier a tile. With
 // many queries the MFMAs are the bound, next to the LDS reads that feed them (each operand of 1 KB serves 16 or 32 queries)
 // and, capped, the three exponentials a score; with few it is one wave's chain of a tile's steps, about 3000 cycles.
-// 8191 tokens of 16 heads of 128 dims over 4 K/V heads, causal behind a tenth, capped: 369 us, 752 TFLOP/s.
+// 8191 tokens of 16 heads of 128 dims over 4 K/V heads, causal behind a tenth, capped: 373 us, 745 TFLOP/s.
 //
 // Rounding: the scores' products are exact in fp32, softmax and sums are fp32, P is rounded to the values' type for the
 // second product (bf16 values have a range that fp16 weights times fp16 values would not hold), the result once.

@@ -13,7 +13,7 @@
 // With many rows (a piece of a prompt) each workgroup takes its pages from the L2 again, at what a CU copies from there (110 GB/s): a wave then
 // has two tiles of rows for each page (tiles_for). Not kept: workgroups of 64 rows whose waves walk together over pages that are copied once
 // (293 tokens x 8 heads over up to 4011 keys 38 us with single tiles, 52 with four splits and 117 unsplit that way; 1024 tokens of 32
-// heads over 8192 keys 306, and 242 with two tiles a wave).
+// heads over 8192 keys 306, and 239 with two tiles a wave).
 //
 // Rounding: scores are exact products summed in fp32, softmax and sums are fp32. bf16: the weights go into the second
 // product as two bf16 (2^-16 of each is lost; as one, 2^-9), and are taken against a reference 2^17 above
@@ -392,10 +392,10 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a) {
 }
 
 // Row tiles of a wave: two where there are many of them over many pages (us with one and with two; heads / K/V heads, dims): 1024 tokens
-// over 8192 keys, 32 / 8, 128 328 and 242, 96 226 and 184, 64 174 and 157; 512 over 4096, 32 / 8, 128 93 and 70; 1024 over 1024 42 and 37;
-// 128 over 131072, 8 / 1 213 and 139; 8 x 512 over 2048, 16 / 4, 96 126 and 119. Fewer leave CUs idle: 293 over 4011, 1500 and 293, 8 / 1, 128 38
-// and 54; 4 x 50 over 1018 12 and 18; and two to four tiles in all read each page once or twice as it is: 32 x 8 over 4096, 32 / 8 98 and 108. (8 x 512
-// over 1024, 16 / 4, 96, on this side of it, 66 and 69.) 256 dims do not fit into the registers twice.
+// over 8192 keys, 32 / 8, 128 319 and 239 (fp16 296 and 214), 96 234 and 205, 64 172 and 160; 512 over 4096, 32 / 8, 128 88 and 69; 1024 over 1024
+// 44 and 39; 128 over 131072, 8 / 1 173 and 136; 8 x 512 over 2048, 16 / 4, 96 123.5 and 122.9. Fewer leave CUs idle: 293 over 4011, 1500 and 293, 8 / 1,
+// 128 39 and 58; 4 x 50 over 1018 12 and 18; and two to four tiles in all read each page once or twice as it is: 32 x 8 over 4096, 32 / 8 98 and 107.
+// (8 x 512 over 1024, 16 / 4, 96, on this side of it, 69 and 74.5.) 256 dims do not fit into the registers twice.
 int tiles_for(int batch, int tokens, int heads, int kv_heads, int hd, int pages) {
   const int64_t rt = ((int64_t)tokens * (heads / kv_heads) + 15) / 16;
   return hd <= 128 && rt >= 8 && (double)rt * batch * kv_heads * pages >= 65536.0 ? 2 : 1;  // (past 64 bits at the limits)
